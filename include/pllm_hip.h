@@ -454,6 +454,65 @@ int pllm_moe_route_rmsnorm(const void* x, int x_dtype, const float* norm_weight,
 int pllm_fp8_act_quant(const void* x, int x_dtype, int64_t rows, int64_t k, uint8_t* codes, float* scales,
                        float eps, int round_scale_pow2, void* stream);
 
+/*
+ * Residual addition, RMS normalisation and E4M3 quantization of activation rows in one launch; no counterpart in the reference, whose FP8 linears take
+ * the normalized rows through blockfp8_act_quant (src/kernels/ops.py:501-516).
+ *     total = round(x + residual);  n = total * rsqrt(mean(total^2) + eps) * weight;  codes, scales of n as pllm_fp8_act_quant makes them
+ *   x, residual, total  [rows, dim] of dtype (float32, fp16, bf16), 16-byte aligned; residual may be null (n is x's, total unused); total may be
+ *             residual or x itself
+ *   weight    [dim] float32;  codes [rows, dim] E4M3;  scales [rows, dim / 128] float32;  dim a multiple of 128, up to 32768
+ * A block of 128 with an infinity or a NaN has NaN codes and a NaN scale.
+ */
+int pllm_fused_add_rms_norm_fp8(const void* x, const void* residual, int dtype, const float* weight, void* total, uint8_t* codes, float* scales,
+                                int64_t rows, int64_t dim, float eps, float quant_eps, int round_scale_pow2, void* stream);
+
+/*
+ * The paged E4M3 key/value cache; no counterpart in the reference, whose caches are dense 16-bit tensors of one length
+ * (src/models/minimax_m2/architecture.py:158-266).
+ *   key_pages    [pool, kv_heads, page_tokens, head_dim] E4M3    value_pages  [pool, kv_heads, head_dim, page_tokens] E4M3 (tokens innermost)
+ *   key_scales, value_scales  [pool, kv_heads] float32, powers of two (pllm_paged_kv_append makes them)
+ *   block_table  [seqs, table_width] int32, rows table_stride apart: the pages of every sequence in order
+ *   lengths      [seqs] int32: positions of every sequence, this call's new tokens among them
+ *   cu_steps     [seqs + 1] int32, from 0 on: sequence s has the rows cu_steps[s] .. cu_steps[s + 1] - 1, the last of which is position
+ *                lengths[s] - 1; null: every sequence has rows / seqs of them
+ * page_tokens 16, 32, 64 or 128; head_dim 64 or 128; 16-bit types; pages, rows and tables on 16 (scales, tables on 4) bytes.  Table entries outside
+ * the pool and positions outside the table have no page: nothing is stored there and no key is seen there.  No two sequences of a call may write
+ * into one page; full pages may be shared.
+ *
+ * Appends: keys turned by the rotary rows of their positions (cos_table, sin_table float32 [table_positions, head_dim], half-split pairs, sin carrying
+ * the sign, as one position's rows of pllm_attention_decode; table_positions >= table_width * page_tokens; rope_dim a multiple of 16, 0: none) and
+ * values go into their pages as E4M3(x / scale).  The scale of a page and head is the least power of two with amax / scale <= 448; where new tokens raise that
+ * of a page that holds older ones, their codes are scaled down with it.  Values that are not finite become NaN codes.  q [rows, heads * head_dim]
+ * (may be null) leaves turned in q_out, contiguous; rows without a position in the table leave as zeros.  Strides in elements.
+ */
+int pllm_paged_kv_append(const void* q, int64_t q_stride, const void* k_new, int64_t k_stride, const void* v_new, int64_t v_stride, int dtype, void* q_out,
+                         uint8_t* key_pages, uint8_t* value_pages, float* key_scales, float* value_scales, int64_t pool, int64_t page_tokens,
+                         const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* lengths, const int32_t* cu_steps,
+                         const float* cos_table, const float* sin_table, int64_t table_positions, int64_t rope_dim, int64_t rows, int64_t seqs,
+                         int64_t heads, int64_t kv_heads, int64_t head_dim, void* stream);
+
+/*
+ * Attention of `steps` new tokens per sequence (one, or a few drafted ones) over the paged cache that already holds them; no counterpart in the
+ * reference (its decode attention: src/models/minimax_m2/architecture.py:158-266).  q [seqs, steps, heads * head_dim], tokens q_stride elements apart; out
+ * contiguous, of q's type: softmax(scale * q K^T) V over the positions up to each token's own, zeros for tokens that see no key.  A sequence's outputs do not
+ * depend on the batch.  workspace: pllm_paged_attention_decode_workspace_bytes(..., table_width * page_tokens) bytes.
+ */
+size_t pllm_paged_attention_decode_workspace_bytes(int64_t seqs, int64_t steps, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions);
+int pllm_paged_attention_decode(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pages, const uint8_t* value_pages, const float* key_scales,
+                                const float* value_scales, int64_t pool, int64_t page_tokens, const int32_t* block_table, int64_t table_stride,
+                                int64_t table_width, const int32_t* lengths, int64_t seqs, int64_t steps, int64_t heads, int64_t kv_heads,
+                                int64_t head_dim, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The same for many new tokens per sequence, ragged by cu_steps (required): prompts, with or without a past; no counterpart in the reference (its prompt
+ * attention: src/models/minimax_m2/architecture.py:158-266).  q [tokens, heads * head_dim]; out contiguous; rows behind the last sequence are zeros.
+ */
+int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pages, const uint8_t* value_pages, const float* key_scales,
+                                const float* value_scales, int64_t pool, int64_t page_tokens, const int32_t* block_table, int64_t table_stride,
+                                int64_t table_width, const int32_t* lengths, const int32_t* cu_steps, int64_t tokens, int64_t seqs, int64_t heads,
+                                int64_t kv_heads, int64_t head_dim, float scale, void* out, void* stream);
+
+
 #ifdef __cplusplus
 }
 #endif

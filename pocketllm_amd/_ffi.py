@@ -77,6 +77,15 @@ SIGNATURES = {
     "pllm_moe_route_rmsnorm": (_int, [_c_void_p, _int, _c_void_p, ctypes.c_float, _c_void_p, _int, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _int,
                                       _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "pllm_fp8_act_quant": (_int, [_c_void_p, _int, _i64, _i64, _c_void_p, _c_void_p, ctypes.c_float, _int, _c_void_p]),
+    "pllm_fused_add_rms_norm_fp8": (_int, [_c_void_p, _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, ctypes.c_float,
+                                           ctypes.c_float, _int, _c_void_p]),
+    "pllm_paged_kv_append": (_int, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64,
+                                    _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p]),
+    "pllm_paged_attention_decode_workspace_bytes": (_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "pllm_paged_attention_decode": (_int, [_c_void_p, _i64, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p,
+                                           _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _c_void_p, _c_void_p, _size_t, _c_void_p]),
+    "pllm_paged_attention_prompt": (_int, [_c_void_p, _i64, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p,
+                                           _c_void_p, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _c_void_p, _c_void_p]),
 }
 
 _LIB = None

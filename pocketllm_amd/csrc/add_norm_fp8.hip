@@ -1,0 +1,189 @@
+// Residual addition, RMS normalisation and E4M3 quantization of activation rows in one pass: what stands between a projection's output and the
+// next FP8 projection (fp8_gemm).
+//     t = round(x + residual);  n = t * rsqrt(mean(t^2) + eps) * weight;  per 128 values s = max(amax |n|, quant_eps) / 448 (a power of two
+//     when asked for), code = E4M3(n / s)
+// The sum leaves rounded to the stream's type, and what is normalized is that rounded value, so the operator says what the three separate ones
+// say; the normalized values stay in float32 until they become codes (the separate operators round them to 16 bits in between).
+#include "pllm_device.h"
+#include "pllm_internal.h"
+
+namespace pllm {
+namespace {
+
+struct NormArgs {
+    const void* x; const void* residual; const float* weight;
+    void* total; uint8_t* codes; float* scales;
+    int rows, dim, pow2;
+    float eps, quant_eps;
+};
+
+template <int DT> struct Eight { uint4 a[DT == PLLM_F32 ? 2 : 1]; };
+template <int DT> __device__ __forceinline__ Eight<DT> load_eight(const void* p, size_t at) {
+    Eight<DT> e;
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(p) + at * (DT == PLLM_F32 ? 4 : 2));
+#pragma unroll
+    for (int i = 0; i < (DT == PLLM_F32 ? 2 : 1); ++i) e.a[i] = src[i];
+    return e;
+}
+template <int DT> __device__ __forceinline__ float eight_value(const Eight<DT>& e, int i) {
+    if constexpr (DT == PLLM_F32) {
+        const uint4 w = e.a[i >> 2];
+        return __uint_as_float((i & 3) == 0 ? w.x : (i & 3) == 1 ? w.y : (i & 3) == 2 ? w.z : w.w);
+    } else {
+        const uint32_t w = i < 2 ? e.a[0].x : i < 4 ? e.a[0].y : i < 6 ? e.a[0].z : e.a[0].w, h = (i & 1) ? w >> 16 : w & 0xffffu;
+        return DT == PLLM_BF16 ? __uint_as_float(h << 16) : f16_bits_to_float(h);
+    }
+}
+template <int DT> __device__ __forceinline__ uint32_t type_bits(float v) {
+    if constexpr (DT == PLLM_BF16) return from_float<bf16_t>(v).bits;
+    else {
+        union { _Float16 h; uint16_t u; } c;
+        c.h = static_cast<_Float16>(v);
+        return c.u;
+    }
+}
+// eight sums rounded to the type, as they are stored
+template <int DT> __device__ __forceinline__ Eight<DT> pack_eight(const float v[8]) {
+    Eight<DT> e;
+    if constexpr (DT == PLLM_F32) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            e.a[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = type_bits<DT>(v[2 * i]) | (type_bits<DT>(v[2 * i + 1]) << 16);
+        e.a[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return e;
+}
+
+// WAVES waves share a row (one: four rows to a workgroup), PIECES pieces of eight values per lane; the whole row stays in registers.  Sixteen
+// neighbouring lanes hold the 128 values of one scale.
+template <int DT, int WAVES, int PIECES>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void add_norm_fp8_kernel(const NormArgs a) {
+    __shared__ float red[WAVES == 1 ? 4 : WAVES];
+    const int tid = WAVES == 1 ? static_cast<int>(threadIdx.x & 63) : static_cast<int>(threadIdx.x);
+    const int row = WAVES == 1 ? static_cast<int>(blockIdx.x * 4 + (threadIdx.x >> 6)) : static_cast<int>(blockIdx.x);
+    if (WAVES == 1 && row >= a.rows) return;                                  // (no barrier below where a wave has a row of its own)
+    const size_t base = static_cast<size_t>(row) * a.dim;
+    Eight<DT> xv[PIECES], rv[PIECES];
+    Eight<PLLM_F32> g[PIECES];
+    int e0[PIECES];
+    bool inside[PIECES];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+        e0[j] = 8 * (tid + 64 * WAVES * j);
+        inside[j] = e0[j] < a.dim;
+        const int at = inside[j] ? e0[j] : 0;                                 // beyond the row: its first values, not counted
+        xv[j] = load_eight<DT>(a.x, base + at);
+        if (a.residual) rv[j] = load_eight<DT>(a.residual, base + at);
+        g[j] = load_eight<PLLM_F32>(a.weight, at);
+    }
+    float v[PIECES][8], ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+        if (a.residual) {
+            float t[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = eight_value(xv[j], i) + eight_value(rv[j], i);
+            xv[j] = pack_eight<DT>(t);
+            if (inside[j]) {
+                uint4* dst = reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.total) + (base + e0[j]) * (DT == PLLM_F32 ? 4 : 2));
+#pragma unroll
+                for (int i = 0; i < (DT == PLLM_F32 ? 2 : 1); ++i) dst[i] = xv[j].a[i];
+            }
+        }
+        float part = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[j][i] = eight_value(xv[j], i);
+            part = __builtin_fmaf(v[j][i], v[j][i], part);
+        }
+        ss += inside[j] ? part : 0.0f;
+    }
+    ss = group_sum<64>(ss);
+    if constexpr (WAVES > 1) {
+        if ((tid & 63) == 0) red[tid >> 6] = ss;
+        __syncthreads();
+        ss = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) ss += red[w];
+    }
+    const float rstd = rsqrtf(ss / static_cast<float>(a.dim) + a.eps);
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+        uint32_t top = 0;                                                     // magnitudes as integers: in the order of their values, NaN above all
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[j][i] = v[j][i] * rstd * eight_value(g[j], i);
+            top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
+        }
+        top = max(top, __float_as_uint(butterfly_peer<1>(__uint_as_float(top))));
+        top = max(top, __float_as_uint(butterfly_peer<2>(__uint_as_float(top))));
+        top = max(top, __float_as_uint(butterfly_peer<4>(__uint_as_float(top))));
+        top = max(top, __float_as_uint(butterfly_peer<8>(__uint_as_float(top))));
+        const float amax = __uint_as_float(top);
+        float s = fmaxf(amax, a.quant_eps) / 448.0f;
+        if (a.pow2) {
+            int e;
+            const float m = frexpf(fmaxf(s, 1.17549435e-38f), &e);            // s = m * 2^e, m in [0.5, 1)
+            s = ldexpf(1.0f, m == 0.5f ? e - 1 : e);
+        }
+        uint32_t lo, hi;
+        if (top < 0x7f800000u) {
+            float c[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = fminf(fmaxf(v[j][i] / s, -448.0f), 448.0f);
+            int l = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false), h = __builtin_amdgcn_cvt_pk_fp8_f32(c[4], c[5], 0, false);
+            lo = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], l, true));
+            hi = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c[6], c[7], h, true));
+        } else {                                                              // infinities and NaN: E4M3 has only NaN for them, and so has the whole block
+            s = __uint_as_float(0x7fc00000u);
+            lo = hi = 0x7f7f7f7fu;
+        }
+        if (inside[j]) {
+            *reinterpret_cast<uint2*>(a.codes + base + e0[j]) = make_uint2(lo, hi);
+            if ((tid & 15) == 0) a.scales[(base + e0[j]) / 128] = s;
+        }
+    }
+}
+
+template <int DT, int WAVES, int PIECES>
+void launch(const NormArgs& a, hipStream_t stream) {
+    const unsigned blocks = WAVES == 1 ? (static_cast<unsigned>(a.rows) + 3) / 4 : static_cast<unsigned>(a.rows);
+    hipLaunchKernelGGL((add_norm_fp8_kernel<DT, WAVES, PIECES>), dim3(blocks), dim3(WAVES == 1 ? 256 : 64 * WAVES), 0, stream, a);
+}
+
+template <int DT>
+void launch_rows(const NormArgs& a, hipStream_t stream) {
+    if (a.dim <= 512) launch<DT, 1, 1>(a, stream);
+    else if (a.dim <= 2048) launch<DT, 4, 1>(a, stream);
+    else if (a.dim <= 4096) launch<DT, 4, 2>(a, stream);
+    else if (a.dim <= 8192) launch<DT, 4, 4>(a, stream);
+    else if (a.dim <= 16384) launch<DT, 16, 2>(a, stream);
+    else launch<DT, 16, 4>(a, stream);
+}
+
+constexpr int64_t kWidestRow = 32768;           // four pieces of eight values for each of 1024 lanes
+
+}  // namespace
+}  // namespace pllm
+
+extern "C" int pllm_fused_add_rms_norm_fp8(const void* x, const void* residual, int dtype, const float* weight, void* total, uint8_t* codes,
+                                           float* scales, int64_t rows, int64_t dim, float eps, float quant_eps, int round_scale_pow2, void* stream) {
+    using namespace pllm;
+    if (!x || !weight || !codes || !scales || (residual && !total) || rows <= 0 || dim <= 0 || dim % 128 != 0 || !(quant_eps > 0.0f))
+        return PLLM_ERR_INVALID_ARGUMENT;
+    if (dtype != PLLM_F32 && dtype != PLLM_F16 && dtype != PLLM_BF16) return PLLM_ERR_INVALID_ARGUMENT;
+    const uintptr_t wide = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(weight) |
+                           reinterpret_cast<uintptr_t>(total);
+    if ((wide & 15u) || (reinterpret_cast<uintptr_t>(codes) & 7u) || (reinterpret_cast<uintptr_t>(scales) & 3u)) return PLLM_ERR_INVALID_ARGUMENT;
+    if (rows > 0x3fffff || dim > kWidestRow) return PLLM_ERR_UNSUPPORTED;     // (a launch counts its threads in 32 bits)
+    const NormArgs a{x, residual, weight, total, codes, scales, static_cast<int>(rows), static_cast<int>(dim), round_scale_pow2 != 0, eps, quant_eps};
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dtype == PLLM_F32) launch_rows<PLLM_F32>(a, st);
+    else if (dtype == PLLM_F16) launch_rows<PLLM_F16>(a, st);
+    else launch_rows<PLLM_BF16>(a, st);
+    return hipGetLastError() == hipSuccess ? PLLM_OK : PLLM_ERR_LAUNCH;
+}

@@ -1,0 +1,362 @@
+// Attention of one or a few new tokens per sequence over a paged E4M3 cache, the sequences of a batch at any lengths:
+//     out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - m),  k_j, v_j = code * scale of the page and head, j up to the query's position.
+// Two launches: runs of keys with a running maximum each, then the runs of a row together (one launch where no sequence can have two runs).
+//
+// A workgroup has a run of one sequence's keys for one key/value head and up to 16 query rows (the heads that share it, times the new tokens).  Its
+// four waves take 64 keys at a time each, with statistics of their own, and meet in LDS once, at the end.  A wave forms S^T = K Q^T
+// (v_mfma_f32_16x16x32: matrix rows are keys, columns queries), whose accumulator layout, rounded to 16 bits, is what O^T = V^T P^T wants as its
+// second operand if row 4 g + i of score tile t is key 16 g + 4 t + i: then a lane of group g has the 16 neighbouring keys 16 g .. + 15, and its
+// values are 16 neighbouring bytes of a value page.  16 neighbouring keys share a page, so a lane needs one page number for its keys' rows, one for
+// its values and two scales, whatever the page size.  Codes become 16-bit values in registers: E4M3 is exact in both types; the keys' scale goes on the
+// scores, the values' scale (halved, so that fp16 holds every value that rounds up from its largest) into the conversion, both exact.
+// Bound: bytes, 2 * length * D codes per head, once for each 16 rows.
+#include "paged_device.h"
+#include "pllm_internal.h"
+
+#include <cfloat>
+
+namespace pllm {
+namespace {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kRows = 16;                       // query rows of a workgroup
+constexpr int kStep = 64;                       // keys that a wave takes at a time
+
+struct DecodeArgs {
+    const uint16_t* q; size_t q_stride;         // elements between tokens
+    const uint8_t* key_pages; const uint8_t* value_pages;
+    const float* key_scales; const float* value_scales;
+    const int32_t* table; size_t table_stride;
+    const int32_t* lengths;
+    float* sums;                                // [rows][runs_bound][D], null: outputs are written at once
+    float2* stats;                              // [rows][runs_bound]: maximum (base 2), sum of weights
+    uint16_t* out;
+    float scale;                                // base 2
+    int seqs, steps, heads, kv_heads, page_shift, pool, width, runs_bound, row_tiles;
+};
+
+// row of a workgroup's tile -> new token and head; rows of one key/value head: token * group + head in the group
+template <bool BF16, int D>
+__global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const DecodeArgs a) {
+    constexpr int kPieces = D / 64;             // 16-byte pieces of a key row per lane
+    constexpr int kTiles = D / 16;              // output tiles
+    constexpr int kPitch = D + 4;
+    __shared__ __align__(16) float sums[kWaves][kRows * kPitch];
+    __shared__ float2 stats[kWaves][kRows];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const int run = blockIdx.x / a.row_tiles, tile = blockIdx.x % a.row_tiles, kvh = blockIdx.y, s = blockIdx.z;
+    const int group = a.heads / a.kv_heads, rows = a.steps * group;
+    const int given = a.lengths[s], length = paged_length(given, a.width, a.page_shift);
+    const int run_keys = paged_run_keys(length, a.kv_heads), begin = run * run_keys, end = min(begin + run_keys, length);
+    if (run > 0 && begin >= length) return;
+    const int32_t* table = a.table + static_cast<size_t>(s) * a.table_stride;
+
+    // the column's query row and how many keys it sees
+    const int r = kRows * tile + col, token = r / group;
+    const bool row_real = r < rows;
+    const int64_t sees = static_cast<int64_t>(given) - a.steps + token + 1;
+    const int limit = row_real ? static_cast<int>(sees < 0 ? 0 : (sees > length ? length : sees)) : 0x7fffffff;
+    uint4 qf[2 * kPieces];
+    {
+        const uint16_t* q = a.q + (static_cast<size_t>(s) * a.steps + (row_real ? token : 0)) * a.q_stride + (kvh * group + (row_real ? r % group : 0)) * D + 16 * g;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            qf[2 * i] = *reinterpret_cast<const uint4*>(q + 64 * i);
+            qf[2 * i + 1] = *reinterpret_cast<const uint4*>(q + 64 * i + 8);
+        }
+    }
+    // bf16 queries so large that products with codes could pass the largest float, where the scaled score need not: a power of two off, on again behind
+    float late = 1.0f;
+    if constexpr (BF16) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * kPieces; ++i) {
+            float v[8];
+            half_eight<true>(qf[i], v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+        }
+        if (__any(top >= 0x1p60f)) {
+            late = 0x1p64f;
+#pragma unroll
+            for (int i = 0; i < 2 * kPieces; ++i) {
+                float v[8];
+                half_eight<true>(qf[i], v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] *= 0x1p-64f;
+                qf[i] = half_pack<true>(v);
+            }
+        }
+    }
+
+    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    v4f o[kTiles];
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) o[i] = zero;
+    float m = -FLT_MAX, l = 0.0f;               // of the column; l over the lane's own keys
+    const size_t head_bytes = static_cast<size_t>(D) << a.page_shift, page_mask = (size_t{1} << a.page_shift) - 1;
+    // page numbers of the lane's key rows (chunk col / 4 of the step) and of its values and scales (chunk g)
+    auto pages = [&](int j0, int& key_page, int& value_page) {
+        key_page = paged_page(table, min(j0 + 16 * (col >> 2), length - 1), a.width, a.page_shift, a.pool);
+        value_page = j0 + 16 * g < length ? paged_page(table, j0 + 16 * g, a.width, a.page_shift, a.pool) : -1;
+    };
+    for (int j0 = begin + kStep * wave; j0 < end; j0 += kStep * kWaves) {
+        int key_page, value_page;
+        pages(j0, key_page, value_page);
+        const size_t key_at = (static_cast<size_t>(max(key_page, 0)) * a.kv_heads + kvh) * head_bytes + ((j0 + 16 * (col >> 2)) & page_mask) * D;
+        const size_t value_at = (static_cast<size_t>(max(value_page, 0)) * a.kv_heads + kvh) * head_bytes + ((j0 + 16 * g) & page_mask);
+        uint4 kf[4][kPieces], vf[kTiles];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) kf[t][i] = *reinterpret_cast<const uint4*>(a.key_pages + key_at + (4 * t + (col & 3)) * D + 64 * i + 16 * g);
+        const size_t scale_at = static_cast<size_t>(max(value_page, 0)) * a.kv_heads + kvh;
+        const float key_factor = a.key_scales[scale_at] * a.scale, value_scale = value_page >= 0 ? 0.5f * a.value_scales[scale_at] : 1.0f;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) vf[i] = *reinterpret_cast<const uint4*>(a.value_pages + value_at + (static_cast<size_t>(16 * i + col) << a.page_shift));
+
+        v4f sc[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            sc[t] = zero;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                sc[t] = half_mfma16<BF16>(half_from_codes<BF16>(kf[t][i].x, kf[t][i].y, 1.0f), qf[2 * i], sc[t]);
+                sc[t] = half_mfma16<BF16>(half_from_codes<BF16>(kf[t][i].z, kf[t][i].w, 1.0f), qf[2 * i + 1], sc[t]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[t][i] *= key_factor;
+        }
+        if constexpr (BF16) {
+            if (late != 1.0f)
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[t][i] *= late;
+        }
+        const int first = j0 + 16 * g, seen = value_page >= 0 ? limit - first : 0;          // the lane's keys that its column sees
+        bool unseen_nan = false;
+        if (!__all(seen >= 16)) {
+            const int stored = value_page >= 0 ? length - first : 0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[t][i] = 4 * t + i < seen ? sc[t][i] : -INFINITY;
+            // what lies behind the last key may be anything, NaN codes too, and zero times NaN is NaN
+            const uint32_t keep[4] = {first_bytes(stored), first_bytes(stored - 4), first_bytes(stored - 8), first_bytes(stored - 12)};
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                vf[i].x &= keep[0]; vf[i].y &= keep[1]; vf[i].z &= keep[2]; vf[i].w &= keep[3];
+                unseen_nan |= any_nan_code(vf[i].x) | any_nan_code(vf[i].y) | any_nan_code(vf[i].z) | any_nan_code(vf[i].w);
+            }
+        }
+        float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+#pragma unroll
+        for (int t = 1; t < 4; ++t) top = fmaxf(top, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])));
+        float x, y;
+        swapped_pair<16>(top, x, y);
+        swapped_pair<32>(fmaxf(x, y), x, y);
+        const float m_new = fmaxf(m, fmaxf(x, y));
+        if (__any(m_new > m)) {
+            const float back = __builtin_amdgcn_exp2f(m - m_new);
+            l *= back;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[i][j] *= back;
+            m = m_new;
+        }
+        uint4 p[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(sc[2 * u + (j >> 2)][j & 3] - m);
+            l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+            p[u] = half_pack<BF16>(e);
+        }
+        if (__any(unseen_nan)) {
+            // NaN values of a key that some of the rows do not see: zeros for the product, and counted for the rows that see them
+            uint4 sees_key[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float e[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) e[j] = 8 * u + j < seen ? 1.0f : 0.0f;
+                sees_key[u] = half_pack<BF16>(e);
+            }
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                uint32_t w[4] = {vf[i].x, vf[i].y, vf[i].z, vf[i].w}, bad[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t high = ((w[j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;       // 0x80 where the code is NaN
+                    bad[j] = (high >> 7) * 0x38u;                                                   // 1.0 there
+                    w[j] &= ~((high >> 7) * 0xffu);
+                }
+                vf[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                v4f count = zero;
+                count = half_mfma16<BF16>(half_from_codes<BF16>(bad[0], bad[1], 1.0f), sees_key[0], count);
+                count = half_mfma16<BF16>(half_from_codes<BF16>(bad[2], bad[3], 1.0f), sees_key[1], count);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (count[j] > 0.0f) o[i][j] = __uint_as_float(0x7fc00000u);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            o[i] = half_mfma16<BF16>(half_from_codes<BF16>(vf[i].x, vf[i].y, value_scale), p[0], o[i]);
+            o[i] = half_mfma16<BF16>(half_from_codes<BF16>(vf[i].z, vf[i].w, value_scale), p[1], o[i]);
+        }
+    }
+    {
+        float x, y;
+        swapped_pair<16>(l, x, y);
+        swapped_pair<32>(x + y, x, y);
+        if (g == 0) stats[wave][col] = make_float2(m, x + y);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) *reinterpret_cast<v4f*>(&sums[wave][col * kPitch + 16 * i + 4 * g]) = o[i];
+    }
+    __syncthreads();
+    // the waves together, in their order
+#pragma unroll
+    for (int i = 0; i < kRows * D / 4 / kThreads; ++i) {
+        const int e = tid + kThreads * i, c = e / (D / 4), d = 4 * (e % (D / 4)), row = kRows * tile + c;
+        if (row >= rows) continue;
+        float top = stats[0][c].x;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, stats[w][c].x);
+        float den = 0.0f;
+        v4f total = zero;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(stats[w][c].x - top);
+            den = __builtin_fmaf(stats[w][c].y, f, den);
+            const v4f part = *reinterpret_cast<const v4f*>(&sums[w][c * kPitch + d]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) total[j] = __builtin_fmaf(part[j], f, total[j]);
+        }
+        if (a.sums) {
+            const size_t at = ((static_cast<size_t>(s) * a.kv_heads + kvh) * rows + row) * a.runs_bound + run;
+            *reinterpret_cast<v4f*>(a.sums + at * D + d) = total;
+            if (d == 0) a.stats[at] = make_float2(top, den);
+        } else {
+            const float inv = den == 0.0f ? 0.0f : 2.0f / den;                 // (twice: the values went in halved)
+            const size_t at = ((static_cast<size_t>(s) * a.steps + row / group) * a.heads + kvh * group + row % group) * D + d;
+            *reinterpret_cast<uint2*>(a.out + at) = make_uint2(half_pair<BF16>(total[0] * inv, total[1] * inv), half_pair<BF16>(total[2] * inv, total[3] * inv));
+        }
+    }
+}
+
+// A wave per query row: its runs together, in their order.
+template <bool BF16, int D>
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(const DecodeArgs a) {
+    constexpr int kPer = D / 64;
+    const int lane = threadIdx.x & 63, group = a.heads / a.kv_heads, rows = a.steps * group;
+    const int64_t index = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+    if (index >= static_cast<int64_t>(a.seqs) * a.kv_heads * rows) return;
+    const int row = static_cast<int>(index % rows), kvh = static_cast<int>(index / rows % a.kv_heads), s = static_cast<int>(index / rows / a.kv_heads);
+    const int runs = max(1, paged_runs(paged_length(a.lengths[s], a.width, a.page_shift), a.kv_heads));
+    const float2* stats = a.stats + index * a.runs_bound;
+    const float* sums = a.sums + index * a.runs_bound * D + kPer * lane;
+    float top = -FLT_MAX;
+    for (int i = lane; i < runs; i += 64) top = fmaxf(top, stats[i].x);
+    top = group_max<64>(top);
+    float den = 0.0f, total[kPer] = {};
+    for (int base = 0; base < runs; base += 64) {
+        const float2 mine = base + lane < runs ? stats[base + lane] : make_float2(-FLT_MAX, 0.0f);
+        const float factor = __builtin_amdgcn_exp2f(mine.x - top);
+        const float weight = mine.y * factor;
+        const int here = min(64, runs - base);
+        for (int i0 = 0; i0 < here; i0 += 8) {
+            float v[8][kPer];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) v[i][j] = sums[static_cast<size_t>(base + min(i0 + i, here - 1)) * D + j];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (i0 + i >= here) break;
+                const float f = __shfl(factor, i0 + i), w = __shfl(weight, i0 + i);
+                den += w;
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) total[j] = __builtin_fmaf(v[i][j], f, total[j]);
+            }
+        }
+    }
+    const float inv = den == 0.0f ? 0.0f : 2.0f / den;
+    uint16_t* out = a.out + ((static_cast<size_t>(s) * a.steps + row / group) * a.heads + kvh * group + row % group) * D + kPer * lane;
+    if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(out) = half_pair<BF16>(total[0] * inv, total[1] * inv);
+    else *out = static_cast<uint16_t>(half_pair<BF16>(total[0] * inv, 0.0f));
+}
+
+template <bool BF16, int D>
+int launch(const DecodeArgs& a, hipStream_t stream) {
+    hipLaunchKernelGGL((paged_decode_kernel<BF16, D>), dim3(a.runs_bound * a.row_tiles, a.kv_heads, a.seqs), dim3(kThreads), 0, stream, a);
+    if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
+    if (a.sums) {
+        const int64_t rows = static_cast<int64_t>(a.seqs) * a.steps * a.heads;
+        hipLaunchKernelGGL((paged_merge_kernel<BF16, D>), dim3(static_cast<unsigned>((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
+        if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
+    }
+    return PLLM_OK;
+}
+
+}  // namespace
+}  // namespace pllm
+
+extern "C" {
+
+size_t pllm_paged_attention_decode_workspace_bytes(int64_t seqs, int64_t steps, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
+    if (seqs <= 0 || steps <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || positions <= 0 || seqs > 65535 || steps > 4096 || heads > 1024 || kv_heads > heads ||
+        head_dim > 256)
+        return 0;
+    const size_t runs = static_cast<size_t>(pllm::paged_runs_bound(positions, static_cast<int>(kv_heads)));
+    if (runs == 1) return 0;
+    const size_t parts = static_cast<size_t>(seqs) * steps * heads * runs;
+    return pllm::align256(parts * head_dim * sizeof(float)) + pllm::align256(parts * sizeof(float2));
+}
+
+int pllm_paged_attention_decode(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pages, const uint8_t* value_pages, const float* key_scales,
+                                const float* value_scales, int64_t pool, int64_t page_tokens, const int32_t* block_table, int64_t table_stride,
+                                int64_t table_width, const int32_t* lengths, int64_t seqs, int64_t steps, int64_t heads, int64_t kv_heads,
+                                int64_t head_dim, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace pllm;
+    if (!q || !key_pages || !value_pages || !key_scales || !value_scales || !block_table || !lengths || !out) return PLLM_ERR_INVALID_ARGUMENT;
+    if (dtype != PLLM_F16 && dtype != PLLM_BF16) return PLLM_ERR_INVALID_ARGUMENT;
+    if (seqs <= 0 || steps <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || pool <= 0 || table_width <= 0 || table_stride < table_width ||
+        q_stride < heads * head_dim)
+        return PLLM_ERR_INVALID_ARGUMENT;
+    if ((head_dim != 64 && head_dim != 128) || (page_tokens != 16 && page_tokens != 32 && page_tokens != 64 && page_tokens != 128)) return PLLM_ERR_UNSUPPORTED;
+    // pages and positions in 32 bits, one grid row per head and sequence
+    if (seqs > 65535 || heads > 1024 || steps * (heads / kv_heads) > 4096 || seqs * steps * heads > 0x3ffffff || pool > 0x7fffffff || table_width > 0x3fffffff / page_tokens) return PLLM_ERR_UNSUPPORTED;
+    const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) |
+                           reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace);
+    const uintptr_t narrow = reinterpret_cast<uintptr_t>(key_scales) | reinterpret_cast<uintptr_t>(value_scales) | reinterpret_cast<uintptr_t>(block_table) |
+                             reinterpret_cast<uintptr_t>(lengths);
+    if ((wide & 15u) || (narrow & 3u) || q_stride % 8) return PLLM_ERR_INVALID_ARGUMENT;
+    const int64_t positions = table_width * page_tokens;
+    const size_t need = pllm_paged_attention_decode_workspace_bytes(seqs, steps, heads, kv_heads, head_dim, positions);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return PLLM_ERR_WORKSPACE;
+    DecodeArgs a{};
+    a.q = static_cast<const uint16_t*>(q); a.q_stride = static_cast<size_t>(q_stride);
+    a.key_pages = key_pages; a.value_pages = value_pages; a.key_scales = key_scales; a.value_scales = value_scales;
+    a.table = block_table; a.table_stride = static_cast<size_t>(table_stride); a.lengths = lengths;
+    a.out = static_cast<uint16_t*>(out);
+    a.scale = scale * 1.4426950408889634f;
+    a.seqs = static_cast<int>(seqs); a.steps = static_cast<int>(steps); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
+    a.page_shift = page_tokens == 16 ? 4 : page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7;
+    a.pool = static_cast<int>(pool); a.width = static_cast<int>(table_width);
+    a.runs_bound = paged_runs_bound(positions, a.kv_heads);
+    a.row_tiles = (a.steps * (a.heads / a.kv_heads) + kRows - 1) / kRows;
+    if (need > 0) {
+        a.sums = static_cast<float*>(workspace);
+        a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + align256(static_cast<size_t>(seqs) * steps * heads * a.runs_bound * head_dim * sizeof(float)));
+    }
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (head_dim == 128) return dtype == PLLM_BF16 ? launch<true, 128>(a, st) : launch<false, 128>(a, st);
+    return dtype == PLLM_BF16 ? launch<true, 64>(a, st) : launch<false, 64>(a, st);
+}
+
+}  // extern "C"

@@ -604,6 +604,191 @@ def fp8_act_quant_forward(x: torch.Tensor, eps: float = 1e-4, round_scale_pow2: 
     return codes.view(torch.float8_e4m3fn), scales
 
 
+def _aligned16(t: torch.Tensor) -> torch.Tensor:
+    """t, contiguous and on a 16-byte address (a view may begin anywhere)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def fused_add_rms_norm_fp8_forward(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float, *, quant_eps: float = 1e-4,
+                                   round_scale_pow2: bool = False, in_place: bool = False):
+    """The step from one projection to the next FP8 one (fp8_gemm_forward) in one launch: total = x + residual rounded to their type,
+    fp8_act_quant_forward of fused_rms_norm_forward(total, weight, eps) with the normalized values kept in float32 in between.  x and residual
+    [..., dim] of one type, dim a multiple of 128 (up to 32768); without a residual total is x.  in_place: total is written into residual.
+    Returns (codes float8_e4m3fn [..., dim], scales float32 [..., dim / 128], total).  A block of 128 with an infinity or a NaN has NaN codes."""
+    _check(x.dim() >= 1, "add_rms_norm_fp8: x must have shape [..., dim]")
+    dim = x.size(-1)
+    _check_x(x)
+    _check(dim > 0 and dim % 128 == 0 and dim <= 32768, "add_rms_norm_fp8: the last dimension must be a multiple of 128, at most 32768")
+    _check(weight.dim() == 1 and weight.size(0) == dim and weight.dtype == torch.float32, "add_rms_norm_fp8: weight must be fp32 [dim]")
+    _check(x.is_cuda and weight.device == x.device, "add_rms_norm_fp8: tensors must be on one CUDA device")
+    _check(float(quant_eps) > 0.0, "add_rms_norm_fp8: quant_eps must be positive")
+    _check(not in_place or residual is not None, "add_rms_norm_fp8: in_place needs a residual")
+    if residual is not None:
+        _check(residual.shape == x.shape and residual.dtype == x.dtype and residual.device == x.device, "add_rms_norm_fp8: residual must match x")
+        _check(not in_place or (residual.is_contiguous() and residual.data_ptr() % 16 == 0), "add_rms_norm_fp8: in_place needs a contiguous residual on 16 bytes")
+    x, weight = _aligned16(x), _aligned16(weight)
+    codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty(*x.shape[:-1], dim // 128, dtype=torch.float32, device=x.device)
+    total = x
+    if residual is not None:
+        residual = _aligned16(residual)
+        total = residual if in_place else torch.empty_like(x)
+    rows = x.numel() // dim
+    if rows == 0:
+        return codes, scales, total
+    with _on_device(x.device):
+        st = _lib().pllm_fused_add_rms_norm_fp8(x.data_ptr(), None if residual is None else residual.data_ptr(), _DTYPE_CODE[x.dtype], weight.data_ptr(),
+                                                None if residual is None else total.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, dim, float(eps),
+                                                float(quant_eps), int(bool(round_scale_pow2)), _stream(x.device))
+    _ffi.check(st, "fused_add_rms_norm_fp8_forward")
+    return codes, scales, total
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t [tokens, width] as rows that the kernels can read: values side by side, every row on 16 bytes (slices of a wider projection pass as they are)."""
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.size(1) and t.data_ptr() % 16 == 0:
+        return t
+    return _aligned16(t)
+
+
+def _paged_cache(what: str, like: torch.Tensor, key_pages, value_pages, key_scales, value_scales, block_table, lengths):
+    """Checks of a paged cache and its tables; returns (pool, kv_heads, page_tokens, head_dim)."""
+    _check(like.dtype in (torch.float16, torch.bfloat16), f"{what}: float16 or bfloat16 only")
+    _check(key_pages.dim() == 4 and value_pages.dim() == 4, f"{what}: pages must be [pool, kv_heads, page, head_dim] and [pool, kv_heads, head_dim, page]")
+    pool, kv_heads, page, dim = key_pages.shape
+    _check(tuple(value_pages.shape) == (pool, kv_heads, dim, page), f"{what}: pages must be [pool, kv_heads, page, head_dim] and [pool, kv_heads, head_dim, page]")
+    _check(key_pages.dtype in (torch.float8_e4m3fn, torch.uint8) and value_pages.dtype == key_pages.dtype, f"{what}: pages must be float8_e4m3fn (or uint8 codes)")
+    _check(page in (16, 32, 64, 128) and dim in (64, 128), f"{what}: pages of 16, 32, 64 or 128 tokens, heads of 64 or 128 values")
+    _check(pool > 0 and kv_heads > 0, f"{what}: the pool is empty")
+    for s in (key_scales, value_scales):
+        _check(s.dtype == torch.float32 and tuple(s.shape) == (pool, kv_heads) and s.is_contiguous(), f"{what}: scales must be fp32 [pool, kv_heads]")
+    _check(block_table.dim() == 2 and block_table.dtype == torch.int32 and block_table.size(1) > 0 and block_table.stride(1) == 1 and
+           (block_table.size(0) <= 1 or block_table.stride(0) >= block_table.size(1)), f"{what}: block_table must be int32 [seqs, pages], rows side by side")
+    _check(lengths.dtype == torch.int32 and tuple(lengths.shape) == (block_table.size(0),) and lengths.is_contiguous(), f"{what}: lengths must be int32 [seqs]")
+    tensors = (like, key_pages, value_pages, key_scales, value_scales, block_table, lengths)
+    _check(all(t.is_cuda and t.device == like.device for t in tensors), f"{what}: tensors must be on one CUDA device")
+    _check(key_pages.is_contiguous() and value_pages.is_contiguous() and key_pages.data_ptr() % 16 == 0 and value_pages.data_ptr() % 16 == 0,
+           f"{what}: pages must be contiguous, on 16 bytes")
+    return pool, kv_heads, page, dim
+
+
+def _paged_offsets(what: str, cu_steps: torch.Tensor, seqs: int, device: torch.device) -> None:
+    _check(cu_steps.dtype == torch.int32 and tuple(cu_steps.shape) == (seqs + 1,) and cu_steps.is_contiguous() and cu_steps.device == device,
+           f"{what}: cu_steps must be int32 [seqs + 1]")
+
+
+def _table_stride(block_table: torch.Tensor) -> int:
+    return block_table.stride(0) if block_table.size(0) > 1 else block_table.size(1)
+
+
+def paged_kv_append_forward(q: torch.Tensor | None, k_new: torch.Tensor, v_new: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+                            key_scales: torch.Tensor, value_scales: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, *,
+                            cu_steps: torch.Tensor | None = None, cos_table: torch.Tensor | None = None, sin_table: torch.Tensor | None = None,
+                            rope_dim: int = 0) -> torch.Tensor | None:
+    """New keys and values of a batch of sequences into a paged E4M3 cache, rotary phases on the way; the queries beside them turned too and
+    returned (rope_dim 0: q itself; no q: None).
+
+    q [tokens, heads * head_dim], k_new / v_new [tokens, kv_heads * head_dim], float16 or bfloat16, rows may be slices of a wider projection; the tokens of
+    sequence s are rows cu_steps[s] .. cu_steps[s + 1] - 1 (int32, from 0 on; None: tokens / seqs each), the last of them at position lengths[s] - 1.
+    key_pages [pool, kv_heads, page, head_dim], value_pages [pool, kv_heads, head_dim, page] float8_e4m3fn, key_scales / value_scales float32
+    [pool, kv_heads], block_table int32 [seqs, pages]: written in place.  cos_table / sin_table float32 [positions, head_dim] as RotaryTable keeps them, rows for
+    every position that the table can name; rope_dim a multiple of 16.
+    The scale of a page and head is the least power of two with amax / scale <= 448; when it has to grow, the page's older codes are scaled
+    down with it.  Rows without a position in the table store nothing, their queries leave as zeros.  No two sequences may write into one page."""
+    what = "paged_kv_append"
+    pool, kv_heads, page, dim = _paged_cache(what, k_new, key_pages, value_pages, key_scales, value_scales, block_table, lengths)
+    _check(k_new.dim() == 2 and k_new.size(1) == kv_heads * dim and v_new.shape == k_new.shape, f"{what}: k_new and v_new must be [tokens, kv_heads * head_dim]")
+    _check(v_new.dtype == k_new.dtype and v_new.device == k_new.device, f"{what}: k_new and v_new must have one dtype and device")
+    tokens, seqs, width, rope_dim = k_new.size(0), block_table.size(0), block_table.size(1), int(rope_dim)
+    _check(0 <= rope_dim <= dim and rope_dim % 16 == 0, f"{what}: rope_dim must be a multiple of 16 up to head_dim")
+    if rope_dim:
+        for r in (cos_table, sin_table):
+            _check(r is not None and r.dim() == 2 and r.size(1) == dim and r.dtype == torch.float32 and r.is_contiguous() and r.device == k_new.device,
+                   f"{what}: cos_table / sin_table must be contiguous fp32 [positions, head_dim]")
+            _check(r.size(0) >= width * page, f"{what}: cos_table / sin_table must cover the {width * page} positions of the table")
+            _check(r.data_ptr() % 16 == 0, f"{what}: cos_table / sin_table must be on 16 bytes")
+    heads = 0
+    if q is not None:
+        _check(q.dim() == 2 and q.size(0) == tokens and q.size(1) % dim == 0 and q.size(1) > 0, f"{what}: q must be [tokens, heads * head_dim]")
+        _check(q.dtype == k_new.dtype and q.device == k_new.device, f"{what}: q must have the keys' dtype and device")
+        heads = q.size(1) // dim
+    if cu_steps is not None:
+        _paged_offsets(what, cu_steps, seqs, k_new.device)
+    else:
+        _check(tokens == 0 or (seqs > 0 and tokens % seqs == 0), f"{what}: without cu_steps every sequence has the same number of tokens")
+    if tokens == 0 or seqs == 0:
+        return q if q is None or not rope_dim else torch.zeros_like(q, memory_format=torch.contiguous_format)
+    k_new, v_new = _rows16(k_new), _rows16(v_new)
+    turned = None
+    if q is not None and rope_dim:
+        q = _rows16(q)
+        turned = torch.empty(tokens, heads * dim, dtype=q.dtype, device=q.device)
+    with _on_device(k_new.device):
+        st = _lib().pllm_paged_kv_append(
+            None if turned is None else q.data_ptr(), 0 if turned is None else q.stride(0), k_new.data_ptr(), k_new.stride(0), v_new.data_ptr(), v_new.stride(0),
+            _DTYPE_CODE[k_new.dtype], None if turned is None else turned.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(),
+            value_scales.data_ptr(), pool, page, block_table.data_ptr(), _table_stride(block_table), width, lengths.data_ptr(),
+            None if cu_steps is None else cu_steps.data_ptr(), cos_table.data_ptr() if rope_dim else None, sin_table.data_ptr() if rope_dim else None,
+            cos_table.size(0) if rope_dim else 0, rope_dim, tokens, seqs, heads, kv_heads, dim, _stream(k_new.device))
+    _ffi.check(st, "paged_kv_append_forward")
+    return turned if rope_dim else q
+
+
+def paged_attention_decode_forward(q: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor,
+                                   block_table: torch.Tensor, lengths: torch.Tensor, *, scale: float | None = None) -> torch.Tensor:
+    """Grouped-query attention of one or a few new tokens per sequence over a paged E4M3 cache that holds them already (paged_kv_append_forward): q
+    [seqs, steps, heads * head_dim] (or [seqs, heads * head_dim]), token i of `steps` at position lengths[s] - steps + i, seeing the positions up to its own.
+    scale: head_dim ** -0.5 by default.  Returns q's shape and dtype; tokens that see no key get zeros.  The table's width bounds the work that is
+    dealt out: pass a narrower view, block_table[:, :n], where no sequence is longer."""
+    what = "paged_attention_decode"
+    _check(q.dim() in (2, 3), f"{what}: q must be [seqs, steps, heads * head_dim] or [seqs, heads * head_dim]")
+    pool, kv_heads, page, dim = _paged_cache(what, q, key_pages, value_pages, key_scales, value_scales, block_table, lengths)
+    seqs, steps, width = q.size(0), q.size(1) if q.dim() == 3 else 1, q.size(-1)
+    _check(seqs == block_table.size(0), f"{what}: q and block_table must have the same sequences")
+    _check(width % dim == 0 and width > 0 and (width // dim) % kv_heads == 0, f"{what}: heads must be a multiple of the cache's key/value heads")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.numel() == 0:
+        return out
+    rows = _rows16(q.reshape(seqs * steps, width))
+    lib = _lib()
+    heads = width // dim
+    need = lib.pllm_paged_attention_decode_workspace_bytes(seqs, steps, heads, kv_heads, dim, block_table.size(1) * page)
+    with _on_device(q.device):
+        ws = _workspace(need, q.device) if need else None
+        st = lib.pllm_paged_attention_decode(rows.data_ptr(), rows.stride(0), _DTYPE_CODE[q.dtype], key_pages.data_ptr(), value_pages.data_ptr(),
+                                             key_scales.data_ptr(), value_scales.data_ptr(), pool, page, block_table.data_ptr(), _table_stride(block_table),
+                                             block_table.size(1), lengths.data_ptr(), seqs, steps, heads, kv_heads, dim,
+                                             float(dim ** -0.5 if scale is None else scale), out.data_ptr(), None if ws is None else ws.data_ptr(), need,
+                                             _stream(q.device))
+    _ffi.check(st, "paged_attention_decode_forward")
+    return out
+
+
+def paged_attention_prompt_forward(q: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor,
+                                   block_table: torch.Tensor, lengths: torch.Tensor, cu_steps: torch.Tensor, *, scale: float | None = None) -> torch.Tensor:
+    """paged_attention_decode_forward for many new tokens per sequence (prompts, with or without a past, any mix of lengths): q
+    [tokens, heads * head_dim], the tokens of sequence s in rows cu_steps[s] .. cu_steps[s + 1] - 1 (int32 [seqs + 1], from 0 on).  Rows behind the last sequence
+    are zeros.  Sequences of one or a few new tokens behind a long past are the decode form's work."""
+    what = "paged_attention_prompt"
+    _check(q.dim() == 2, f"{what}: q must be [tokens, heads * head_dim]")
+    pool, kv_heads, page, dim = _paged_cache(what, q, key_pages, value_pages, key_scales, value_scales, block_table, lengths)
+    tokens, width, seqs = q.size(0), q.size(1), block_table.size(0)
+    _paged_offsets(what, cu_steps, seqs, q.device)
+    _check(width % dim == 0 and width > 0 and (width // dim) % kv_heads == 0, f"{what}: heads must be a multiple of the cache's key/value heads")
+    if tokens == 0 or seqs == 0:
+        return torch.zeros(tokens, width, dtype=q.dtype, device=q.device)
+    out = torch.empty(tokens, width, dtype=q.dtype, device=q.device)
+    rows = _rows16(q)
+    with _on_device(q.device):
+        st = _lib().pllm_paged_attention_prompt(rows.data_ptr(), rows.stride(0), _DTYPE_CODE[q.dtype], key_pages.data_ptr(), value_pages.data_ptr(),
+                                                key_scales.data_ptr(), value_scales.data_ptr(), pool, page, block_table.data_ptr(), _table_stride(block_table),
+                                                block_table.size(1), lengths.data_ptr(), cu_steps.data_ptr(), tokens, seqs, width // dim, kv_heads, dim,
+                                                float(dim ** -0.5 if scale is None else scale), out.data_ptr(), _stream(q.device))
+    _ffi.check(st, "paged_attention_prompt_forward")
+    return out
+
+
 def gguf_quant_gemm_pair_forward(x, blocks0, row_elems0, type_id0, blocks1, row_elems1, type_id1, signed_grid, *,
                                  out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """src/csrc/cuda_kernel.cpp:615-666: returns the stack [2, ..., N]."""
