@@ -14,11 +14,12 @@
 #include "pllm_internal.h"
 
 #include <cfloat>
+#include <type_traits>
 
 namespace pllm {
 namespace {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves, kBlockRows = 32 * kWaves;
+constexpr int kWaves = 8, kThreads = 64 * kWaves, kBlockRows = 32 * kWaves;
 constexpr int kTile = 64;                       // keys per step
 
 struct PagedPromptArgs {
@@ -34,18 +35,18 @@ struct PagedPromptArgs {
 
 template <bool BF16, int D>
 __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPromptArgs a) {
-    constexpr int kKeyBytes = kTile * D * 2, kTileBytes = 2 * kKeyBytes;      // keys [64][D], then values [D][64]
-    constexpr int kDimTiles = D / 32;
-    constexpr int kLoads = kTile * D / 16 / kThreads;                         // 16-byte pieces of codes per thread, keys and values each
+    constexpr int kKeyBytes = kTile * D * 2, kTileBytes = 2 * kKeyBytes;      // keys [64][D], values [D][64]
+    constexpr int kDimTiles = D / 32, kSteps = D / 16;
     extern __shared__ __align__(1024) unsigned char smem[];                   // [2][kTileBytes]
-    __shared__ __align__(16) float factors[2][4];                             // the keys' scales of a tile's chunks of 16, times `scale`
-    __shared__ int notes[3];                                                  // of tile t at t % 3; bits 0 - 3: chunks whose page is missing, bit 4: a NaN value code
+    __shared__ __align__(16) float factors[4][8];                             // of tile t at t % 4: per chunk the keys' scale times `scale`, and 0 or -inf
+    __shared__ int nan_values[4];                                             // of tile t at t % 4 (masked tiles): some value code is NaN,
+    __shared__ float unread[64 + 4 * 8];
+    __shared__ __align__(8) uint16_t nan_keys[2][D][4];                       // which ones: a bit per key and dimension, of tile t at t % 2
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.x, group = a.heads / a.kv_heads;
     const int64_t slot = a.slots - 1 - static_cast<int64_t>(blockIdx.y);
     // rows of one key/value head: token * group + head in the group; the tokens behind the last sequence are one more, without keys
-    const int64_t rows_all = static_cast<int64_t>(a.tokens) * group;
     int s = 0;
     {
         int owners = 0;
@@ -63,94 +64,164 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     const int64_t row_first = (slot - paged_first_slot(static_cast<int64_t>(offset) * group, s, kBlockRows, 1)) * kBlockRows;
     const int64_t seq_rows = static_cast<int64_t>(n) * group;
     if (n <= 0 || row_first < 0 || row_first >= seq_rows) return;
-    const int row0 = static_cast<int>(row_first), rows = static_cast<int>(min(seq_rows, rows_all));
+    const int row0 = static_cast<int>(row_first), rows = static_cast<int>(seq_rows);
     const int given = tail ? 0 : a.lengths[s], length = paged_length(given, a.width, a.page_shift);
     // keys that a row sees: up to its token's position
     auto visible = [&](int row) {
         const int64_t v = static_cast<int64_t>(given) - n + row / group + 1;
         return tail ? 0 : static_cast<int>(v < 0 ? 0 : (v > length ? length : v));
     };
-    const int last_row = min(rows, row0 + kBlockRows) - 1;
-    const int tiles = (visible(last_row) + kTile - 1) / kTile;
+    const int tiles = (visible(min(rows, row0 + kBlockRows) - 1) + kTile - 1) / kTile;
+    const int full = visible(row0) / kTile;                                   // tiles that every row of the workgroup sees whole
     const int w0 = row0 + 32 * wave, my_row = min(w0 + r, rows - 1);
     const int limit = visible(my_row);
-    const int wave_end = w0 < rows ? visible(min(rows, w0 + 32) - 1) : 0, wave_full = visible(min(w0, rows - 1));   // keys that some / all rows of the wave see
+    const int wave_end = w0 < rows ? visible(min(rows, w0 + 32) - 1) : 0;     // keys that one of the wave's rows sees
     const int32_t* table = a.table + static_cast<size_t>(tail ? 0 : s) * a.table_stride;
-    const size_t head_bytes = static_cast<size_t>(D) << a.page_shift;
-    const int page_mask = (1 << a.page_shift) - 1;
 
-    // staging: a thread's pieces of 16 codes of the tile's keys and values
-    uint4 kraw[kLoads], vraw[kLoads];
-    float vscale[kLoads], factor = 0.0f;
-    bool missing = false;
-    auto fetch = [&](int t) {
-        const int j0 = kTile * t;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int e = tid + kThreads * i, key = e / (D / 16), piece = e % (D / 16);
-            const int page = paged_page(table, min(j0 + key, length - 1), a.width, a.page_shift, a.pool);
-            const uint8_t* src = a.key_pages + (static_cast<size_t>(max(page, 0)) * a.kv_heads + kvh) * head_bytes + ((j0 + key) & page_mask) * D + 16 * piece;
-            kraw[i] = *reinterpret_cast<const uint4*>(src);
-        }
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int e = tid + kThreads * i, d = e >> 2, chunk = e & 3, first = j0 + 16 * chunk;
-            const int page = first < length ? paged_page(table, first, a.width, a.page_shift, a.pool) : -1;
-            const size_t at = static_cast<size_t>(max(page, 0)) * a.kv_heads + kvh;
-            vraw[i] = *reinterpret_cast<const uint4*>(a.value_pages + at * head_bytes + (static_cast<size_t>(d) << a.page_shift) + (first & page_mask));
-            vscale[i] = page >= 0 ? 0.5f * a.value_scales[at] : 1.0f;
-            if (i == 0) { factor = page >= 0 ? a.key_scales[at] * a.scale : 0.0f; missing = page < 0; }
-        }
-    };
-    auto store = [&](int t, int buf, int* noted) {
-        unsigned char* kt = smem + buf * kTileBytes;
-        unsigned char* vt = kt + kKeyBytes;
-        const int j0 = kTile * t;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int e = tid + kThreads * i, key = e / (D / 16), piece = e % (D / 16), turn = key & (D / 8 - 1);
-            unsigned char* row = kt + key * (2 * D);
-            *reinterpret_cast<uint4*>(row + (((2 * piece) ^ turn) << 4)) = half_from_codes<BF16>(kraw[i].x, kraw[i].y, 1.0f);
-            *reinterpret_cast<uint4*>(row + (((2 * piece + 1) ^ turn) << 4)) = half_from_codes<BF16>(kraw[i].z, kraw[i].w, 1.0f);
-        }
-        bool nan = false;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int e = tid + kThreads * i, d = e >> 2, chunk = e & 3, turn = (d >> 1) & 7;
-            if (j0 + kTile > length || missing) {                             // what lies behind the last key may be anything, NaN codes too
-                const int stored = missing ? 0 : length - j0 - 16 * chunk;
-                vraw[i].x &= first_bytes(stored); vraw[i].y &= first_bytes(stored - 4); vraw[i].z &= first_bytes(stored - 8); vraw[i].w &= first_bytes(stored - 12);
-            }
-            nan |= any_nan_code(vraw[i].x) | any_nan_code(vraw[i].y) | any_nan_code(vraw[i].z) | any_nan_code(vraw[i].w);
-            unsigned char* row = vt + d * (2 * kTile);
-            *reinterpret_cast<uint4*>(row + (((2 * chunk) ^ turn) << 4)) = half_from_codes<BF16>(vraw[i].x, vraw[i].z, vscale[i]);
-            *reinterpret_cast<uint4*>(row + (((2 * chunk + 1) ^ turn) << 4)) = half_from_codes<BF16>(vraw[i].y, vraw[i].w, vscale[i]);
-        }
-        if (tid < 4) factors[buf][tid] = factor;
-        if (nan) atomicOr(noted, 16);
-        if (tid < 4 && missing) atomicOr(noted, 1 << tid);
-    };
-    if (tid < 3) notes[tid] = 0;
-    if (tiles > 0) fetch(0);
-    uint4 qf[D / 16];
+    uint4 qf[kSteps];
     float late = 1.0f;
     {
         const uint16_t* q = a.q + (static_cast<size_t>(offset) + my_row / group) * a.q_stride + (kvh * group + my_row % group) * D + 8 * h;
-        float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            qf[i] = *reinterpret_cast<const uint4*>(q + 16 * i);
-            float v[8];
-            half_eight<BF16>(qf[i], v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+        for (int i = 0; i < kSteps; ++i) qf[i] = *reinterpret_cast<const uint4*>(q + 16 * i);
+    }
+
+    // Staging: a lane copies 16 codes of a tile's keys and 16 of its values, of 64-wide heads the one or the other.  All of a wave's are of one chunk of
+    // 16 keys, so the page and the scales are the wave's.
+    const int chunk = wave >> 1, part = wave & 1;
+    const bool copies_keys = D == 128 || part == 0, copies_values = D == 128 || part == 1;
+    const int piece = D == 128 ? 64 * part + lane : lane;                     // of the chunk
+    const int key_row = 16 * chunk + piece / (D / 16), key_piece = piece % (D / 16), value_row = piece;
+    const uint32_t key_lane = static_cast<uint32_t>((key_row & 15) * D + 16 * key_piece), value_lane = static_cast<uint32_t>(value_row) << a.page_shift;
+    const int page_mask = (1 << a.page_shift) - 1;
+    const size_t head_bytes = static_cast<size_t>(D) << a.page_shift;
+    struct Place { size_t at; bool here; };                                   // number of a page and head in the pool; whether the table has one
+    auto first_key = [&](int t) { return kTile * t + 16 * chunk; };
+    auto entry = [&](int t) { return table[min(first_key(t) >> a.page_shift, a.width - 1)]; };            // the wave's page of tile t, unchecked
+    auto checked = [&](int t, int page) {
+        page = __builtin_amdgcn_readfirstlane(page);
+                const bool here = page >= 0 && page < a.pool && first_key(t) < length;     // (no branch: the step is one block)
+        return Place{static_cast<size_t>(here ? page : 0) * a.kv_heads + kvh, here};
+    };
+    auto load_keys = [&](int t, const Place& p) { return *reinterpret_cast<const uint4*>(a.key_pages + p.at * head_bytes + (first_key(t) & page_mask) * D + key_lane); };
+    auto load_values = [&](int t, const Place& p) { return *reinterpret_cast<const uint4*>(a.value_pages + p.at * head_bytes + (first_key(t) & page_mask) + value_lane); };
+    // (one lane writes the factors; the others have a place of their own to write to, which costs less than a branch)
+    float* const factor_at = lane == 0 && part == 0 ? &factors[0][chunk] : &unread[lane];
+    unsigned char* const key_dst = smem + key_row * (2 * D);
+    unsigned char* const value_dst = smem + kKeyBytes + value_row * (2 * kTile);
+    const int key_turn = key_row & (D / 8 - 1), value_turn = (value_row >> 1) & 7;
+    auto blank = [](uint4 raw, bool here) {
+        const uint32_t keep = here ? 0xffffffffu : 0u;
+        return make_uint4(raw.x & keep, raw.y & keep, raw.z & keep, raw.w & keep);
+    };
+    // `half`: the tile's place in LDS, t % 2
+    auto store_keys = [&](int t, int half, bool here, uint4 raw, float key_scale) {
+        if (copies_keys) {
+            raw = blank(raw, here);                                           // (NaN codes would outlive the minus infinity below)
+            unsigned char* row = key_dst + half * kTileBytes;
+            *reinterpret_cast<uint4*>(row + (((2 * key_piece) ^ key_turn) << 4)) = half_from_codes<BF16>(raw.x, raw.y, 1.0f);
+            *reinterpret_cast<uint4*>(row + (((2 * key_piece + 1) ^ key_turn) << 4)) = half_from_codes<BF16>(raw.z, raw.w, 1.0f);
         }
+        // a chunk without a page: any finite factor, and minus infinity behind it
+        factor_at[8 * (t & 3)] = here ? fminf(key_scale * a.scale * late, FLT_MAX) : 1.0f;
+        factor_at[8 * (t & 3) + 4] = here ? 0.0f : -INFINITY;
+    };
+    // PLAIN: a tile that every row sees whole
+    auto store_values = [&](auto plain, int t, int half, bool here, uint4 raw, float value_scale) {
+        if (!copies_values) return;
+        raw = blank(raw, here);
+        if constexpr (!decltype(plain)::value) {
+            const int stored = length - first_key(t);                         // what lies behind the last key may be anything, NaN codes too
+            raw.x &= first_bytes(stored); raw.y &= first_bytes(stored - 4); raw.z &= first_bytes(stored - 8); raw.w &= first_bytes(stored - 12);
+            if (t >= full) {                                                  // a key that not every row sees: no NaN into the product, zero times NaN is NaN
+                const uint32_t bits = nan_codes(raw.x) | (nan_codes(raw.y) << 4) | (nan_codes(raw.z) << 8) | (nan_codes(raw.w) << 12);
+                nan_keys[half][value_row][chunk] = static_cast<uint16_t>(bits);
+                if (bits) nan_values[t & 3] = 1;
+                raw.x = without_nan(raw.x); raw.y = without_nan(raw.y); raw.z = without_nan(raw.z); raw.w = without_nan(raw.w);
+            }
+        }
+        const float scale = here ? 0.5f * value_scale : 1.0f;
+        unsigned char* row = value_dst + half * kTileBytes;
+        *reinterpret_cast<uint4*>(row + (((2 * chunk) ^ value_turn) << 4)) = half_from_codes<BF16>(raw.x, raw.z, scale);
+        *reinterpret_cast<uint4*>(row + (((2 * chunk + 1) ^ value_turn) << 4)) = half_from_codes<BF16>(raw.y, raw.w, scale);
+    };
+
+    const v16f zero = {};
+    v16f o[kDimTiles], sa[2], sb[2];
+#pragma unroll
+    for (int i = 0; i < kDimTiles; ++i) o[i] = zero;
+    float m = -FLT_MAX, l = 0.0f;                                             // of the lane's query; l over its half of the keys
+    // S^T of the tile in one half of LDS
+    auto scores = [&](int half, v16f (&sc)[2]) {
+        const unsigned char* kt = smem + half * kTileBytes;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint4 kf = *reinterpret_cast<const uint4*>(kt + (32 * u + r) * (2 * D) + (((2 * i + h) ^ (r & (D / 8 - 1))) << 4));
+                sc[u] = half_mfma32<BF16>(kf, qf[i], i == 0 ? zero : sc[u]);
+            }
+    };
+
+    // the largest score of the lane's row, in the exponent's units
+    auto row_top = [&](const v16f (&sc)[2], const float (&f)[4], const float (&b)[4]) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            // (a maximum that hands NaN on takes three operands in one instruction and needs no quieting of them; a NaN score is its row's end either way)
+            float x = sc[c >> 1][8 * (c & 1)];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) x = __builtin_elementwise_maximum(x, sc[c >> 1][8 * (c & 1) + i]);
+            most = __builtin_elementwise_maximum(most, __builtin_fmaf(x, f[c], b[c]));
+        }
+        float lower, upper;
+        swapped_pair<32>(most, lower, upper);
+        return __builtin_elementwise_maximum(lower, upper);
+    };
+    auto load_factors = [&](int t, float (&f)[4], float (&b)[4]) {
+        const float4 f4 = *reinterpret_cast<const float4*>(factors[t & 3]), b4 = *reinterpret_cast<const float4*>(factors[t & 3] + 4);
+        f[0] = f4.x; f[1] = f4.y; f[2] = f4.z; f[3] = f4.w;
+        b[0] = b4.x; b[1] = b4.y; b[2] = b4.z; b[3] = b4.w;
+    };
+    float f[4] = {}, b[4] = {}, top = -INFINITY;                              // of the tile whose scores are there
+
+    // what is on its way: codes of keys two tiles ahead of the products, of values one, page numbers and scales ahead of them
+    uint4 key_raw, value_raw;
+    bool values_here = false;                                                 // of value_raw's tile
+    Place keys_at{0, false}, next_at{0, false};                               // of key_raw's tile, of the one behind
+    int entry_next = 0;                                                       // of the one behind that
+    float key_scale = 0.0f, value_scale = 0.0f, value_scale_keys = 0.0f;      // of key_raw's tile; of value_raw's; of key_raw's tile again
+    const int last = tiles - 1;
+    if (tiles > 0) {
+        if (tid < 4) nan_values[tid] = 0;
+        const int e0 = entry(0), e1 = entry(min(1, last)), e2 = entry(min(2, last)), e3 = entry(min(3, last));
+        const Place p0 = checked(0, e0), p1 = checked(min(1, last), e1);
+        keys_at = checked(min(2, last), e2);
+        next_at = checked(min(3, last), e3);
+        values_here = p1.here;
+        const uint4 k0 = load_keys(0, p0), v0 = load_values(0, p0), k1 = load_keys(min(1, last), p1);
+        const float ks0 = a.key_scales[p0.at], vs0 = a.value_scales[p0.at], ks1 = a.key_scales[p1.at];
+        value_scale = a.value_scales[p1.at];
+        key_scale = a.key_scales[keys_at.at];
+        value_scale_keys = a.value_scales[keys_at.at];
+        key_raw = load_keys(min(2, last), keys_at);
+        value_raw = load_values(min(1, last), p1);
+        entry_next = entry(min(4, last));
         // bf16 queries so large that products with codes could pass the largest float, where the scaled score need not: a power of two off, on again behind
         if constexpr (BF16) {
-            if (__any(top >= 0x1p60f)) {
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                float v[8];
+                half_eight<true>(qf[i], v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
+            }
+            // (all waves alike: the factors are the workgroup's)
+            if (__syncthreads_or(top >= 0x1p60f)) {
                 late = 0x1p64f;
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
+                for (int i = 0; i < kSteps; ++i) {
                     float v[8];
                     half_eight<true>(qf[i], v);
 #pragma unroll
@@ -158,129 +229,138 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
                     qf[i] = half_pack<true>(v);
                 }
             }
-        }
+        } else __syncthreads();
+        store_keys(0, 0, p0.here, k0, ks0);
+        store_values(std::false_type{}, 0, 0, p0.here, v0, vs0);
+        store_keys(1, 1, p1.here, k1, ks1);                                   // (one tile only: the same again, in the other half)
+        __syncthreads();
+        scores(0, sa);
+        load_factors(0, f, b);
+        top = row_top(sa, f, b);
     }
-    const v16f zero = {};
-    v16f o[kDimTiles];
-#pragma unroll
-    for (int i = 0; i < kDimTiles; ++i) o[i] = zero;
-    float m = -FLT_MAX, l = 0.0f;                                             // of the lane's query; l over its half of the keys
-    __syncthreads();
-    if (tiles > 0) store(0, 0, &notes[0]);
-    if (tiles > 1) fetch(1);
-    __syncthreads();
-    for (int t = 0, now = 0; t < tiles; ++t) {
-        const int buf = t & 1, j0 = kTile * t, next = now == 2 ? 0 : now + 1;
-        if (tid == 0) notes[next == 2 ? 0 : next + 1] = 0;                    // read before the last barrier, written behind the next
-        const unsigned char* kt = smem + buf * kTileBytes;
-        const unsigned char* vt = kt + kKeyBytes;
-        const bool active = j0 < wave_end;
-        uint4 p[4];
-        int seen = 0, note = 0;
-        if (active) {
-            v16f sc[2];
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint4 kf = *reinterpret_cast<const uint4*>(kt + (32 * u + r) * (2 * D) + (((2 * i + h) ^ (r & (D / 8 - 1))) << 4));
-                    sc[u] = half_mfma32<BF16>(kf, qf[i], i == 0 ? zero : sc[u]);
-                }
-            const float4 f4 = *reinterpret_cast<const float4*>(factors[buf]);
-            const float f[4] = {f4.x, f4.y, f4.z, f4.w};
-            note = notes[now];
+
+    // One tile: its softmax weights beside the next tile's scores, its value product beside the copies of the tiles behind.
+    auto step = [&](auto masked, int t, int half, v16f (&cur)[2], v16f (&next)[2]) {
+        constexpr bool MASKED = decltype(masked)::value;
+        // the copies: keys two tiles ahead take the place of this tile's, values of the next tile that of the one before (behind the last tile: its
+        // codes again, which nobody reads)
+        auto copies = [&]() {
+            if (MASKED && tid == 0) nan_values[(t + 2) & 3] = 0;              // read two steps ago, written in the next
+            store_keys(t + 2, half, keys_at.here, key_raw, key_scale);
+            store_values(std::integral_constant<bool, !MASKED>{}, t + 1, half ^ 1, values_here, value_raw, value_scale);
+            value_raw = load_values(min(t + 2, last), keys_at);
+            key_raw = load_keys(min(t + 3, last), next_at);
+            key_scale = a.key_scales[next_at.at];
+            value_scale = value_scale_keys;
+            value_scale_keys = a.value_scales[next_at.at];
+            values_here = keys_at.here;
+            keys_at = next_at;
+            next_at = checked(min(t + 4, last), entry_next);
+            entry_next = entry(min(t + 5, last));
+        };
+        const int seen = limit - kTile * t - 4 * h;
+        auto hidden = [&](int u, int v) { return MASKED && 32 * u + 8 * (v >> 2) + (v & 3) >= seen; };
+        if constexpr (MASKED) {
+            top = -INFINITY;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) sc[u][v] *= f[2 * u + (v >> 3)];
-            if (BF16 && late != 1.0f)
+                for (int v = 0; v < 16; ++v) {
+                    const float x = __builtin_fmaf(cur[u][v], f[2 * u + (v >> 3)], b[2 * u + (v >> 3)]);
+                    top = __builtin_elementwise_maximum(top, hidden(u, v) ? -INFINITY : x);
+                }
+            float lower, upper;
+            swapped_pair<32>(top, lower, upper);
+            top = __builtin_elementwise_maximum(lower, upper);
+        }
+        // The maximum follows when a row's weights would pass 2^8: what it is exactly falls out of the quotient.
+        if (__any(top > m + 8.0f)) {
+            const float m_new = top > m + 8.0f ? top : m, back = __builtin_amdgcn_exp2f(m - m_new);
+            l *= back;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+            for (int i = 0; i < kDimTiles; ++i)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) sc[u][v] *= late;
-            if (j0 + kTile > wave_full || (note & 15)) {                      // keys behind a query, or without a page
-                seen = limit - j0 - 4 * h;
+                for (int v = 0; v < 16; ++v) o[i][v] *= back;
+            m = m_new;
+        }
+        // The fused product below keeps the bits that the maximum's rounding lost: up to 2^-25 of it, the same factor in every weight of a
+        // row, but past the exponent's range from 2^31 on.  Scores that far out are multiplied and rounded first.
+        if (__any(fabsf(m) > 0x1p20f)) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        if (32 * u + 8 * (v >> 2) + (v & 3) >= seen || ((note >> (2 * u + (v >> 3))) & 1)) sc[u][v] = -INFINITY;
-            } else seen = kTile;
-            float top = fmaxf(sc[0][0], sc[1][0]);
+                for (int v = 0; v < 16; ++v) cur[u][v] = __builtin_fmaf(cur[u][v], f[2 * u + (v >> 3)], b[2 * u + (v >> 3)]);
 #pragma unroll
-            for (int v = 1; v < 16; ++v) top = fmaxf(top, fmaxf(sc[0][v], sc[1][v]));
-            float x, y;
-            swapped_pair<32>(top, x, y);
-            const float m_new = fmaxf(m, fmaxf(x, y));
-            if (__any(m_new > m)) {
-                const float back = __builtin_amdgcn_exp2f(m - m_new);
-                l *= back;
+            for (int c = 0; c < 4; ++c) { f[c] = 1.0f; b[c] = 0.0f; }
+        }
+        copies();
+        scores(half ^ 1, next);
+        uint4 p[4];
 #pragma unroll
-                for (int i = 0; i < kDimTiles; ++i)
+        for (int c = 0; c < 4; ++c) {
+            float e[8];
+            const float behind = b[c] - m;
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) o[i][v] *= back;
-                m = m_new;
+            for (int j = 0; j < 8; ++j) {
+                const int v = 8 * (c & 1) + j;
+                const float x = __builtin_fmaf(cur[c >> 1][v], f[c], behind);
+                e[j] = __builtin_amdgcn_exp2f(hidden(c >> 1, v) ? -INFINITY : x);
+            }
+            p[c] = half_pack<BF16>(e);
+            l = half_pair_sum<BF16>(p[c].x, half_pair_sum<BF16>(p[c].y, half_pair_sum<BF16>(p[c].z, half_pair_sum<BF16>(p[c].w, l))));
+        }
+        load_factors(t + 1, f, b);
+        const unsigned char* vt = smem + half * kTileBytes + kKeyBytes;
+        auto value_piece = [&](int u, int c) { return *reinterpret_cast<const uint4*>(vt + (32 * u + r) * (2 * kTile) + (((2 * c + h) ^ ((r >> 1) & 7)) << 4)); };
+        if (!MASKED || kTile * t < wave_end) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int u = 0; u < kDimTiles; ++u) o[u] = half_mfma32<BF16>(value_piece(u, c), p[c], o[u]);
+        }
+        top = row_top(next, f, b);
+        if constexpr (!MASKED) {
+            // the order that this stretch is issued in: operands a few instructions ahead, a share of the exponentials behind every matrix instruction
+            __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * kSteps; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float e[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(sc[i >> 1][8 * (i & 1) + j] - m);
-                l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-                p[i] = half_pack<BF16>(e);
+            for (int i = 0; i < 4 * kDimTiles; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
             }
         }
-        if (t + 1 < tiles) store(t + 1, buf ^ 1, &notes[next]);
-        if (t + 2 < tiles) fetch(t + 2);
-        if (active) {
-            if ((note & 16) && j0 + kTile > wave_full) {
-                // NaN values in a tile whose keys not every row sees: counted for the rows that see them, zeros for the product (zero times NaN is NaN)
-                uint4 sees[4];
+        if (MASKED && nan_values[t & 3]) {
+            // NaN values were left out of the product: they are the end of the sums of the rows that see them
+            const int keys = limit - kTile * t;
+            const uint64_t sees = keys >= 64 ? ~0ull : (keys <= 0 ? 0ull : (1ull << keys) - 1);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float e[8];
+            for (int u = 0; u < kDimTiles; ++u)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) e[j] = 16 * i + 8 * (j >> 2) + (j & 3) < seen ? 1.0f : 0.0f;
-                    sees[i] = half_pack<BF16>(e);
-                }
-#pragma unroll
-                for (int u = 0; u < kDimTiles; ++u) {
-                    v16f count = zero;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint4 vf = *reinterpret_cast<const uint4*>(vt + (32 * u + r) * (2 * kTile) + (((2 * i + h) ^ ((r >> 1) & 7)) << 4));
-                        float e[8], bad[8];
-                        half_eight<BF16>(vf, e);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            bad[j] = e[j] != e[j] ? 1.0f : 0.0f;
-                            e[j] = e[j] != e[j] ? 0.0f : e[j];
-                        }
-                        o[u] = half_mfma32<BF16>(half_pack<BF16>(e), p[i], o[u]);
-                        count = half_mfma32<BF16>(half_pack<BF16>(bad), sees[i], count);
-                    }
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        if (count[v] > 0.0f) o[u][v] = __uint_as_float(0x7fc00000u);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int u = 0; u < kDimTiles; ++u) {
-                        const uint4 vf = *reinterpret_cast<const uint4*>(vt + (32 * u + r) * (2 * kTile) + (((2 * i + h) ^ ((r >> 1) & 7)) << 4));
-                        o[u] = half_mfma32<BF16>(vf, p[i], o[u]);
-                    }
-            }
+                for (int v = 0; v < 16; ++v)
+                    if (*reinterpret_cast<const uint64_t*>(nan_keys[half][32 * u + 8 * (v >> 2) + 4 * h + (v & 3)]) & sees) o[u][v] = __uint_as_float(0x7fc00000u);
         }
-        __syncthreads();                                                      // the next tile is there, this one has been read
-        now = next;
+        __syncthreads();
+    };
+    int t = 0;
+    for (; t + 3 <= full; t += 2) {                                           // (both steps copy values of tiles that every row sees whole)
+        step(std::false_type{}, t, 0, sa, sb);
+        step(std::false_type{}, t + 1, 1, sb, sa);
     }
-    float x, y;
-    swapped_pair<32>(l, x, y);
-    const float den = x + y, inv = den == 0.0f ? 0.0f : 2.0f / den;           // (twice: the values went in halved)
+    for (; t < tiles; ++t) {
+        step(std::true_type{}, t, t & 1, sa, sb);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) sa[u] = sb[u];
+    }
+    float lower, upper;
+    swapped_pair<32>(l, lower, upper);
+    const float den = lower + upper, inv = den == 0.0f ? 0.0f : 2.0f / den;   // (twice: the values went in halved)
     // lane: query r, dimensions 32 u + 8 (v / 4) + 4 h + v % 4; through the wave's own part of LDS to whole rows
-    __syncthreads();
     unsigned char* turn = smem + wave * (32 * 2 * D);
 #pragma unroll
     for (int u = 0; u < kDimTiles; ++u)
@@ -303,8 +383,8 @@ template <bool BF16, int D>
 int launch(const PagedPromptArgs& a, hipStream_t stream) {
     static SmemGrant granted;
     const size_t smem = 2 * 2 * kTile * D * 2;
-    // (with the kernel's own kilobyte beside it, 128-wide heads pass 64 KB)
-    if (!grant_dynamic_smem(reinterpret_cast<const void*>(paged_prompt_kernel<BF16, D>), smem + 1024, granted)) return PLLM_ERR_LAUNCH;
+    // (with the kernel's own arrays beside it, 128-wide heads pass 64 KB)
+    if (!grant_dynamic_smem(reinterpret_cast<const void*>(paged_prompt_kernel<BF16, D>), smem + 4096, granted)) return PLLM_ERR_LAUNCH;
     hipLaunchKernelGGL((paged_prompt_kernel<BF16, D>), dim3(a.kv_heads, a.slots), dim3(kThreads), smem, stream, a);
     return hipGetLastError() == hipSuccess ? PLLM_OK : PLLM_ERR_LAUNCH;
 }

@@ -60,8 +60,28 @@ template <bool BF16> __device__ __forceinline__ v16f half_mfma32(const uint4& a,
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
+// sum + both 16-bit values of a pair
+template <bool BF16> __device__ __forceinline__ float half_pair_sum(uint32_t pair, float sum) {
+    if constexpr (BF16) {
+        const v2b ones = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, pair), ones, sum, false);
+    } else {
+        const v2h ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, pair), ones, sum, false);
+    }
+}
+
 // whether one of four E4M3 codes is NaN (0x7f or 0xff)
 __device__ __forceinline__ bool any_nan_code(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
+// which of them are: bit i for byte i; the codes with zeros in their place
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) {
+    const uint32_t high = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    return ((high >> 7) * 0x10204080u) >> 28;
+}
+__device__ __forceinline__ uint32_t without_nan(uint32_t w) {
+    const uint32_t high = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    return w & ~((high >> 7) * 0xffu);
+}
 // bytes below `count` of a word of four, as a mask
 __device__ __forceinline__ uint32_t first_bytes(int count) { return count >= 4 ? 0xffffffffu : (count <= 0 ? 0u : (1u << (8 * count)) - 1u); }
 

@@ -58,14 +58,15 @@ def queries(tokens, heads, dim, dtype, seed=0, size=1.0):
 def close(got, want, note, dtype):
     """Every output within what its roundings can add up to.
 
-    u = half a step of the type.  Softmax weights are rounded to the type once (u of the weighted mean of |v|), the output once (u of itself).  A
+    u = half a step of the type.  Softmax weights are rounded to the type once, above the division (u of the weighted mean of |v|) and below it (u of
+    the output), the output once (u of itself).  A
     score is a float32 sum of dim exact products (matrix instructions add four or more at a time: below dim + 8 roundings of 2^-24 of the sum of
     magnitudes), scaled twice and turned to base 2 (4 roundings); as an exponent its error is one of the weight.  exp2, the running maximum's and the runs'
     factors: 16 units; the sums of weights and of products: below (keys / 16 + 64) roundings one after the other.  Weights and their error appear above and
     below the division: twice.  fp16 weights below 2^-14 and halved values lose up to 2^-25 each."""
     u = torch.finfo(dtype).eps / 2
     f32 = (note["score"] * (note["spread"].shape[-1] + 12) + 16 + note["keys"] / 16 + 64) * 2.0 ** -24
-    bound = u * (note["spread"] + np.abs(want)) * (1 + 2 * u) + 2 * f32 * (note["spread"] + np.abs(want))
+    bound = u * (note["spread"] + 2 * np.abs(want)) * (1 + 3 * u) + 2 * f32 * (note["spread"] + np.abs(want))
     if dtype == torch.float16:
         bound = bound + 2.0 ** -25 * (note["keys"] * note["top"] + 4)
     got = got.detach().cpu().double().numpy().reshape(want.shape)
