@@ -37,15 +37,19 @@ struct DecodeArgs {
 
 // row of a workgroup's tile -> new token and head; rows of one key/value head: token * group + head in the group
 template <bool BF16, int D>
-__global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const DecodeArgs a) {
+__global__ __launch_bounds__(kThreads, 3) void paged_decode_kernel(const DecodeArgs a) {
     constexpr int kPieces = D / 64;             // 16-byte pieces of a key row per lane
     constexpr int kTiles = D / 16;              // output tiles
     constexpr int kPitch = D + 4;
     __shared__ __align__(16) float sums[kWaves][kRows * kPitch];
     __shared__ float2 stats[kWaves][kRows];
+    __shared__ __align__(16) uint16_t queries[kRows][D + 8];                  // (in registers they cost the third workgroup of a compute unit)
+    __shared__ __align__(8) uint16_t nan_keys[kWaves][D][4];                  // keys of a wave's step whose value is NaN, a bit each, per dimension
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int run = blockIdx.x / a.row_tiles, tile = blockIdx.x % a.row_tiles, kvh = blockIdx.y, s = blockIdx.z;
+    // Neighbouring workgroups run on different XCDs: heads first, and the runs of every sequence from another one on, or the XCDs of the first runs, which
+    // every sequence has, would do the most (64 sequences of 1 to 8192 positions, run numbers first: TODO us).
+    const int tile = blockIdx.x % a.row_tiles, kvh = blockIdx.x / a.row_tiles, s = blockIdx.z, run = (blockIdx.y + blockIdx.z) % a.runs_bound;
     const int group = a.heads / a.kv_heads, rows = a.steps * group;
     const int given = a.lengths[s], length = paged_length(given, a.width, a.page_shift);
     const int run_keys = paged_run_keys(length, a.kv_heads), begin = run * run_keys, end = min(begin + run_keys, length);
@@ -57,65 +61,40 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const DecodeA
     const bool row_real = r < rows;
     const int64_t sees = static_cast<int64_t>(given) - a.steps + token + 1;
     const int limit = row_real ? static_cast<int>(sees < 0 ? 0 : (sees > length ? length : sees)) : 0x7fffffff;
-    uint4 qf[2 * kPieces];
-    {
-        const uint16_t* q = a.q + (static_cast<size_t>(s) * a.steps + (row_real ? token : 0)) * a.q_stride + (kvh * group + (row_real ? r % group : 0)) * D + 16 * g;
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            qf[2 * i] = *reinterpret_cast<const uint4*>(q + 64 * i);
-            qf[2 * i + 1] = *reinterpret_cast<const uint4*>(q + 64 * i + 8);
-        }
-    }
-    // bf16 queries so large that products with codes could pass the largest float, where the scaled score need not: a power of two off, on again behind
-    float late = 1.0f;
-    if constexpr (BF16) {
-        float top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 2 * kPieces; ++i) {
-            float v[8];
-            half_eight<true>(qf[i], v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
-        }
-        if (__any(top >= 0x1p60f)) {
-            late = 0x1p64f;
-#pragma unroll
-            for (int i = 0; i < 2 * kPieces; ++i) {
-                float v[8];
-                half_eight<true>(qf[i], v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] *= 0x1p-64f;
-                qf[i] = half_pack<true>(v);
-            }
-        }
-    }
-
     const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
     v4f o[kTiles];
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) o[i] = zero;
-    float m = -FLT_MAX, l = 0.0f;               // of the column; l over the lane's own keys
+    float m = -FLT_MAX, l = 0.0f, late = 1.0f;  // of the column; l over the lane's own keys
     const size_t head_bytes = static_cast<size_t>(D) << a.page_shift, page_mask = (size_t{1} << a.page_shift) - 1;
     // page numbers of the lane's key rows (chunk col / 4 of the step) and of its values and scales (chunk g)
     auto pages = [&](int j0, int& key_page, int& value_page) {
         key_page = paged_page(table, min(j0 + 16 * (col >> 2), length - 1), a.width, a.page_shift, a.pool);
         value_page = j0 + 16 * g < length ? paged_page(table, j0 + 16 * g, a.width, a.page_shift, a.pool) : -1;
     };
-    for (int j0 = begin + kStep * wave; j0 < end; j0 += kStep * kWaves) {
-        int key_page, value_page;
-        pages(j0, key_page, value_page);
+    // What is on its way: the codes and scales of a step while the one before is worked on, its page numbers a step before that.
+    struct Step { uint4 keys[4][kPieces], values[kTiles]; float key_scale, value_scale; bool here; };
+    auto request = [&](Step& x, int j0, int key_page, int value_page) {
         const size_t key_at = (static_cast<size_t>(max(key_page, 0)) * a.kv_heads + kvh) * head_bytes + ((j0 + 16 * (col >> 2)) & page_mask) * D;
         const size_t value_at = (static_cast<size_t>(max(value_page, 0)) * a.kv_heads + kvh) * head_bytes + ((j0 + 16 * g) & page_mask);
-        uint4 kf[4][kPieces], vf[kTiles];
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) kf[t][i] = *reinterpret_cast<const uint4*>(a.key_pages + key_at + (4 * t + (col & 3)) * D + 64 * i + 16 * g);
+            for (int i = 0; i < kPieces; ++i) x.keys[t][i] = *reinterpret_cast<const uint4*>(a.key_pages + key_at + (4 * t + (col & 3)) * D + 64 * i + 16 * g);
         const size_t scale_at = static_cast<size_t>(max(value_page, 0)) * a.kv_heads + kvh;
-        const float key_factor = a.key_scales[scale_at] * a.scale, value_scale = value_page >= 0 ? 0.5f * a.value_scales[scale_at] : 1.0f;
+        x.key_scale = a.key_scales[scale_at];
+        x.value_scale = a.value_scales[scale_at];
+        x.here = value_page >= 0;
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) vf[i] = *reinterpret_cast<const uint4*>(a.value_pages + value_at + (static_cast<size_t>(16 * i + col) << a.page_shift));
-
+        for (int i = 0; i < kTiles; ++i) x.values[i] = *reinterpret_cast<const uint4*>(a.value_pages + value_at + (static_cast<size_t>(16 * i + col) << a.page_shift));
+    };
+    auto work = [&](Step& x, int j0) {
+        auto& kf = x.keys;
+        auto& vf = x.values;
+        const float key_factor = x.key_scale * a.scale, value_scale = x.here ? 0.5f * x.value_scale : 1.0f;
+        uint4 qf[2 * kPieces];
+#pragma unroll
+        for (int i = 0; i < 2 * kPieces; ++i) qf[i] = *reinterpret_cast<const uint4*>(&queries[col][64 * (i >> 1) + 16 * g + 8 * (i & 1)]);
         v4f sc[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -135,10 +114,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const DecodeA
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sc[t][i] *= late;
         }
-        const int first = j0 + 16 * g, seen = value_page >= 0 ? limit - first : 0;          // the lane's keys that its column sees
-        bool unseen_nan = false;
+        const int first = j0 + 16 * g, seen = x.here ? limit - first : 0;          // the lane's keys that its column sees
+        bool unseen_nan = false, some_nan = false;
         if (!__all(seen >= 16)) {
-            const int stored = value_page >= 0 ? length - first : 0;
+            const int stored = x.here ? length - first : 0;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -150,14 +129,22 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const DecodeA
                 vf[i].x &= keep[0]; vf[i].y &= keep[1]; vf[i].z &= keep[2]; vf[i].w &= keep[3];
                 unseen_nan |= any_nan_code(vf[i].x) | any_nan_code(vf[i].y) | any_nan_code(vf[i].z) | any_nan_code(vf[i].w);
             }
+            some_nan = __any(unseen_nan);
+            if (some_nan)                                                     // of keys that not every row sees: none into the product, where zero times NaN is NaN
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i) {
+                    nan_keys[wave][16 * i + col][g] =
+                        static_cast<uint16_t>(nan_codes(vf[i].x) | (nan_codes(vf[i].y) << 4) | (nan_codes(vf[i].z) << 8) | (nan_codes(vf[i].w) << 12));
+                    vf[i].x = without_nan(vf[i].x); vf[i].y = without_nan(vf[i].y); vf[i].z = without_nan(vf[i].z); vf[i].w = without_nan(vf[i].w);
+                }
         }
         float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
 #pragma unroll
         for (int t = 1; t < 4; ++t) top = fmaxf(top, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])));
-        float x, y;
-        swapped_pair<16>(top, x, y);
-        swapped_pair<32>(fmaxf(x, y), x, y);
-        const float m_new = fmaxf(m, fmaxf(x, y));
+        float lower, upper;
+        swapped_pair<16>(top, lower, upper);
+        swapped_pair<32>(fmaxf(lower, upper), lower, upper);
+        const float m_new = fmaxf(m, fmaxf(lower, upper));
         if (__any(m_new > m)) {
             const float back = __builtin_amdgcn_exp2f(m - m_new);
             l *= back;
@@ -176,39 +163,58 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const DecodeA
             l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
             p[u] = half_pack<BF16>(e);
         }
-        if (__any(unseen_nan)) {
-            // NaN values of a key that some of the rows do not see: zeros for the product, and counted for the rows that see them
-            uint4 sees_key[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float e[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = 8 * u + j < seen ? 1.0f : 0.0f;
-                sees_key[u] = half_pack<BF16>(e);
-            }
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i) {
-                uint32_t w[4] = {vf[i].x, vf[i].y, vf[i].z, vf[i].w}, bad[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t high = ((w[j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;       // 0x80 where the code is NaN
-                    bad[j] = (high >> 7) * 0x38u;                                                   // 1.0 there
-                    w[j] &= ~((high >> 7) * 0xffu);
-                }
-                vf[i] = make_uint4(w[0], w[1], w[2], w[3]);
-                v4f count = zero;
-                count = half_mfma16<BF16>(half_from_codes<BF16>(bad[0], bad[1], 1.0f), sees_key[0], count);
-                count = half_mfma16<BF16>(half_from_codes<BF16>(bad[2], bad[3], 1.0f), sees_key[1], count);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (count[j] > 0.0f) o[i][j] = __uint_as_float(0x7fc00000u);
-            }
-        }
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
             o[i] = half_mfma16<BF16>(half_from_codes<BF16>(vf[i].x, vf[i].y, value_scale), p[0], o[i]);
             o[i] = half_mfma16<BF16>(half_from_codes<BF16>(vf[i].z, vf[i].w, value_scale), p[1], o[i]);
         }
+        if (some_nan) {
+            // NaN values were left out of the product: they are the end of the sums of the rows that see them
+            const int keys = limit - j0;
+            const uint64_t sees = keys >= 64 ? ~0ull : (keys <= 0 ? 0ull : (1ull << keys) - 1);
+            __builtin_amdgcn_wave_barrier();                                  // (one wave's LDS operations take effect in order)
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (*reinterpret_cast<const uint64_t*>(nan_keys[wave][16 * i + 4 * g + j]) & sees) o[i][j] = __uint_as_float(0x7fc00000u);
+            __builtin_amdgcn_wave_barrier();
+        }
+    };
+    constexpr int kStride = kStep * kWaves;
+    int j0 = begin + kStep * wave;
+    Step x;
+    auto start = [&]() {
+        int key_page, value_page;
+        pages(j0, key_page, value_page);
+        request(x, j0, key_page, value_page);
+    };
+    if (j0 < end) start();
+    // the queries, behind the first codes; rows that the tile does not have as zeros
+    {
+        const int row = tid / (D / 8), d = 8 * (tid % (D / 8)), at = kRows * tile + row;
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (row < kRows && at < rows) q = *reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(s) * a.steps + at / group) * a.q_stride + (kvh * group + at % group) * D + d);
+        if constexpr (BF16) {
+            // queries so large that products with codes could pass the largest float, where the scaled score need not: a power of two off, on again behind
+            float v[8], top = 0.0f;
+            half_eight<true>(q, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+            if (__syncthreads_or(top >= 0x1p60f)) {
+                late = 0x1p64f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= 0x1p-64f;
+                q = half_pack<true>(v);
+            }
+        }
+        if (row < kRows) *reinterpret_cast<uint4*>(&queries[row][d]) = q;
+    }
+    __syncthreads();
+    while (j0 < end) {
+        work(x, j0);
+        j0 += kStride;
+        if (j0 < end) start();
     }
     {
         float x, y;
@@ -249,55 +255,62 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_kernel(const DecodeA
     }
 }
 
-// A wave per query row: its runs together, in their order.
+// A workgroup per query row: its runs together, an order that the number of runs fixes.  All of up to 64 runs are requested at once.
 template <bool BF16, int D>
 __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const DecodeArgs a) {
-    constexpr int kPer = D / 64;
-    const int lane = threadIdx.x & 63, group = a.heads / a.kv_heads, rows = a.steps * group;
-    const int64_t index = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
-    if (index >= static_cast<int64_t>(a.seqs) * a.kv_heads * rows) return;
-    const int row = static_cast<int>(index % rows), kvh = static_cast<int>(index / rows % a.kv_heads), s = static_cast<int>(index / rows / a.kv_heads);
-    const int runs = max(1, paged_runs(paged_length(a.lengths[s], a.width, a.page_shift), a.kv_heads));
-    const float2* stats = a.stats + index * a.runs_bound;
-    const float* sums = a.sums + index * a.runs_bound * D + kPer * lane;
-    float top = -FLT_MAX;
-    for (int i = lane; i < runs; i += 64) top = fmaxf(top, stats[i].x);
-    top = group_max<64>(top);
-    float den = 0.0f, total[kPer] = {};
-    for (int base = 0; base < runs; base += 64) {
-        const float2 mine = base + lane < runs ? stats[base + lane] : make_float2(-FLT_MAX, 0.0f);
-        const float factor = __builtin_amdgcn_exp2f(mine.x - top);
-        const float weight = mine.y * factor;
-        const int here = min(64, runs - base);
-        for (int i0 = 0; i0 < here; i0 += 8) {
-            float v[8][kPer];
+    constexpr int kLanes = D / 4, kSlots = kThreads / kLanes, kBatch = 8;     // threads that share a run; runs side by side; of each of them at a time
+    __shared__ float factors[256];
+    __shared__ __align__(16) float sums[kSlots][D];
+    __shared__ float red[2 * kWaves];
+    const int tid = threadIdx.x, group = a.heads / a.kv_heads, rows = a.steps * group;
+    const int index = blockIdx.x, row = index % rows, kvh = index / rows % a.kv_heads, s = index / rows / a.kv_heads;
+    const int runs = max(1, paged_runs(paged_length(a.lengths[s], a.width, a.page_shift), a.kv_heads));     // (256 at most)
+    const float2* stats = a.stats + static_cast<size_t>(index) * a.runs_bound;
+    const int slot = tid / kLanes, d = 4 * (tid % kLanes);
+    const float* part = a.sums + static_cast<size_t>(index) * a.runs_bound * D + d;
+    v4f first[kBatch];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < kBatch; ++i) first[i] = *reinterpret_cast<const v4f*>(part + static_cast<size_t>(min(slot + kSlots * i, runs - 1)) * D);
+    const float2 mine = tid < runs ? stats[tid] : make_float2(-FLT_MAX, 0.0f);
+    float top = group_max<64>(mine.x);
+    if ((tid & 63) == 0) red[tid >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float factor = __builtin_amdgcn_exp2f(mine.x - top);
+    factors[tid] = factor;
+    float den = group_sum<64>(mine.y * factor);
+    if ((tid & 63) == 0) red[kWaves + (tid >> 6)] = den;
+    __syncthreads();
+    den = (red[kWaves] + red[kWaves + 1]) + (red[kWaves + 2] + red[kWaves + 3]);
+    v4f total = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int base = slot; base < runs; base += kSlots * kBatch) {
+        if (base != slot)
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) v[i][j] = sums[static_cast<size_t>(base + min(i0 + i, here - 1)) * D + j];
+            for (int i = 0; i < kBatch; ++i) first[i] = *reinterpret_cast<const v4f*>(part + static_cast<size_t>(min(base + kSlots * i, runs - 1)) * D);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (i0 + i >= here) break;
-                const float f = __shfl(factor, i0 + i), w = __shfl(weight, i0 + i);
-                den += w;
+        for (int i = 0; i < kBatch; ++i) {
+            const float f = base + kSlots * i < runs ? factors[base + kSlots * i] : 0.0f;
+            if (base + kSlots * i < runs)
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) total[j] = __builtin_fmaf(v[i][j], f, total[j]);
-            }
+                for (int j = 0; j < 4; ++j) total[j] = __builtin_fmaf(first[i][j], f, total[j]);
         }
     }
+    *reinterpret_cast<v4f*>(&sums[slot][d]) = total;
+    __syncthreads();
+    if (tid >= D / 2) return;
+    float x = 0.0f, y = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) { x += sums[i][2 * tid]; y += sums[i][2 * tid + 1]; }
     const float inv = den == 0.0f ? 0.0f : 2.0f / den;
-    uint16_t* out = a.out + ((static_cast<size_t>(s) * a.steps + row / group) * a.heads + kvh * group + row % group) * D + kPer * lane;
-    if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(out) = half_pair<BF16>(total[0] * inv, total[1] * inv);
-    else *out = static_cast<uint16_t>(half_pair<BF16>(total[0] * inv, 0.0f));
+    *reinterpret_cast<uint32_t*>(a.out + ((static_cast<size_t>(s) * a.steps + row / group) * a.heads + kvh * group + row % group) * D + 2 * tid) = half_pair<BF16>(x * inv, y * inv);
 }
 
 template <bool BF16, int D>
 int launch(const DecodeArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_decode_kernel<BF16, D>), dim3(a.runs_bound * a.row_tiles, a.kv_heads, a.seqs), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((paged_decode_kernel<BF16, D>), dim3(a.row_tiles * a.kv_heads, a.runs_bound, a.seqs), dim3(kThreads), 0, stream, a);
     if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
     if (a.sums) {
-        const int64_t rows = static_cast<int64_t>(a.seqs) * a.steps * a.heads;
-        hipLaunchKernelGGL((paged_merge_kernel<BF16, D>), dim3(static_cast<unsigned>((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((paged_merge_kernel<BF16, D>), dim3(a.seqs * a.steps * a.heads), dim3(kThreads), 0, stream, a);
         if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
     }
     return PLLM_OK;
@@ -330,7 +343,7 @@ int pllm_paged_attention_decode(const void* q, int64_t q_stride, int dtype, cons
         return PLLM_ERR_INVALID_ARGUMENT;
     if ((head_dim != 64 && head_dim != 128) || (page_tokens != 16 && page_tokens != 32 && page_tokens != 64 && page_tokens != 128)) return PLLM_ERR_UNSUPPORTED;
     // pages and positions in 32 bits, one grid row per head and sequence
-    if (seqs > 65535 || heads > 1024 || steps * (heads / kv_heads) > 4096 || seqs * steps * heads > 0x3ffffff || pool > 0x7fffffff || table_width > 0x3fffffff / page_tokens) return PLLM_ERR_UNSUPPORTED;
+    if (seqs > 65535 || heads > 1024 || steps * (heads / kv_heads) > 4096 || seqs * steps * heads > 0xffffff || pool > 0x7fffffff || table_width > 0x3fffffff / page_tokens) return PLLM_ERR_UNSUPPORTED;
     const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) |
                            reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace);
     const uintptr_t narrow = reinterpret_cast<uintptr_t>(key_scales) | reinterpret_cast<uintptr_t>(value_scales) | reinterpret_cast<uintptr_t>(block_table) |

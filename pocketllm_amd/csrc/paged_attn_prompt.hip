@@ -9,10 +9,11 @@
 // of 16 value codes (tokens innermost in a page) in turn.  The keys' scale, one per 16 keys, goes into the product that takes scores to exponents; the
 // values' scale (halved, so that fp16 holds every value that rounds up from its largest) into the conversion.
 // 16-byte pieces of a row lie permuted in LDS (key rows by row % 16, value rows by row / 2 % 8), so 16 neighbouring rows read at one piece meet no
-// bank twice.  Tiles of queries are dealt out in slots (paged_cache.h), the longest of a sequence first; rows behind the last sequence get zeros.
+// bank twice.  Rows behind the last sequence get zeros.
 #include "paged_device.h"
 #include "pllm_internal.h"
 
+#include <algorithm>
 #include <cfloat>
 #include <type_traits>
 
@@ -29,9 +30,64 @@ struct PagedPromptArgs {
     const int32_t* table; size_t table_stride;
     const int32_t* lengths; const int32_t* cu_steps;
     uint16_t* out;
+    float* sums; float2* stats;                 // of several runs of a block's keys: [runs][tokens * heads][D], maximum (base 2) and sum of weights; or null
     float scale;                                // base 2
-    int tokens, seqs, heads, kv_heads, page_shift, pool, width, slots;
+    int runs, tokens, seqs, heads, kv_heads, page_shift, pool, width, slots;
 };
+
+// The block of query rows that index `index` of the grid is: sequence s (a.seqs: the rows behind the last one), rows row0 .. row0 + kBlockRows - 1 of it.
+// Those with the most keys come first, so that what is left at the end is short (six prompts and continuations, 64 and 8 heads: TODO us); of more than 63
+// sequences only each one's own blocks are in that order, by slots.
+__device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, int group, int& s, int& row0) {
+    const int lane = threadIdx.x & 63;
+    if (a.seqs < 64) {
+        int rows = 0, first = 0, keys = 0;                                    // of the lane's sequence
+        if (lane <= a.seqs) {
+            const int offset = paged_offset(a.cu_steps, lane, 0, a.tokens);
+            const int n = max((lane == a.seqs ? a.tokens : paged_offset(a.cu_steps, lane + 1, 0, a.tokens)) - offset, 0);
+            keys = lane == a.seqs || n == 0 ? 0 : paged_length(a.lengths[lane], a.width, a.page_shift);
+            rows = n * group;
+            first = keys - n;
+        }
+        // (counts stay far below 2^24)
+        auto seeing = [&](int tiles) { return paged_blocks_seeing(tiles, rows, first, group, kBlockRows); };
+        auto all = [&](int count) { return static_cast<int>(group_sum<64>(static_cast<float>(count))); };
+        if (index >= all(seeing(0))) return false;
+        int low = 0, high = static_cast<int>(group_max<64>(static_cast<float>((keys + kTile - 1) / kTile))) + 1;
+        while (low < high) {                                                  // the most tiles that more than `index` blocks see
+            const int middle = (low + high + 1) / 2;
+            if (all(seeing(middle)) > index) low = middle;
+            else high = middle - 1;
+        }
+        const int mine = seeing(low) - seeing(low + 1), place = index - all(seeing(low + 1));
+        int until = mine;                                                     // blocks of this length of the sequences up to the lane's
+#pragma unroll
+        for (int i = 1; i < 64; i *= 2) {
+            const int before = __shfl_up(until, i);
+            if (lane >= i) until += before;
+        }
+        const uint64_t behind = __ballot(until > place);
+        s = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(behind)) - 1);
+        const int block = (rows + kBlockRows - 1) / kBlockRows - seeing(low) + place - (until - mine);
+        row0 = __builtin_amdgcn_readlane(block, s) * kBlockRows;
+        return true;
+    }
+    const int64_t slot = a.slots - 1 - static_cast<int64_t>(index);
+    int owners = 0;
+    for (int base = 0; base <= a.seqs; base += 64) {
+        const int c = base + lane;
+        const bool begun = c <= a.seqs && paged_first_slot(static_cast<int64_t>(paged_offset(a.cu_steps, c, 0, a.tokens)) * group, c, kBlockRows, 1) <= slot;
+        const int n = __popcll(__ballot(begun));
+        owners += n;
+        if (n < 64) break;
+    }
+    s = __builtin_amdgcn_readfirstlane(max(owners - 1, 0));
+    const int offset = paged_offset(a.cu_steps, s, 0, a.tokens), n = (s == a.seqs ? a.tokens : paged_offset(a.cu_steps, s + 1, 0, a.tokens)) - offset;
+    const int64_t row = (slot - paged_first_slot(static_cast<int64_t>(offset) * group, s, kBlockRows, 1)) * kBlockRows;
+    if (n <= 0 || row < 0 || row >= static_cast<int64_t>(n) * group) return false;
+    row0 = static_cast<int>(row);
+    return true;
+}
 
 template <bool BF16, int D>
 __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPromptArgs a) {
@@ -41,37 +97,25 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     __shared__ __align__(16) float factors[4][8];                             // of tile t at t % 4: per chunk the keys' scale times `scale`, and 0 or -inf
     __shared__ int nan_values[4];                                             // of tile t at t % 4 (masked tiles): some value code is NaN,
     __shared__ float unread[64 + 4 * 8];
-    __shared__ __align__(8) uint16_t nan_keys[2][D][4];                       // which ones: a bit per key and dimension, of tile t at t % 2
+    __shared__ __align__(8) uint16_t nan_keys[2][D][4];                       // which ones: a bit per key and dimension, in the tile's half
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.x, group = a.heads / a.kv_heads;
-    const int64_t slot = a.slots - 1 - static_cast<int64_t>(blockIdx.y);
     // rows of one key/value head: token * group + head in the group; the tokens behind the last sequence are one more, without keys
-    int s = 0;
-    {
-        int owners = 0;
-        for (int base = 0; base <= a.seqs; base += 64) {
-            const int c = base + lane;
-            const bool begun = c <= a.seqs && paged_first_slot(static_cast<int64_t>(paged_offset(a.cu_steps, c, 0, a.tokens)) * group, c, kBlockRows, 1) <= slot;
-            const int n = __popcll(__ballot(begun));
-            owners += n;
-            if (n < 64) break;
-        }
-        s = __builtin_amdgcn_readfirstlane(max(owners - 1, 0));
-    }
+    int s = 0, row0 = 0;
+    if (!find_block(a, blockIdx.y, group, s, row0)) return;
     const bool tail = s == a.seqs;
     const int offset = paged_offset(a.cu_steps, s, 0, a.tokens), n = (tail ? a.tokens : paged_offset(a.cu_steps, s + 1, 0, a.tokens)) - offset;
-    const int64_t row_first = (slot - paged_first_slot(static_cast<int64_t>(offset) * group, s, kBlockRows, 1)) * kBlockRows;
-    const int64_t seq_rows = static_cast<int64_t>(n) * group;
-    if (n <= 0 || row_first < 0 || row_first >= seq_rows) return;
-    const int row0 = static_cast<int>(row_first), rows = static_cast<int>(seq_rows);
+    const int rows = n * group;                                               // (fits: the host's check)
     const int given = tail ? 0 : a.lengths[s], length = paged_length(given, a.width, a.page_shift);
     // keys that a row sees: up to its token's position
     auto visible = [&](int row) {
         const int64_t v = static_cast<int64_t>(given) - n + row / group + 1;
         return tail ? 0 : static_cast<int>(v < 0 ? 0 : (v > length ? length : v));
     };
-    const int tiles = (visible(min(rows, row0 + kBlockRows) - 1) + kTile - 1) / kTile;
+    const int all_tiles = (visible(min(rows, row0 + kBlockRows) - 1) + kTile - 1) / kTile;
+    const int run = (all_tiles + static_cast<int>(gridDim.z) - 1) / static_cast<int>(gridDim.z), t0 = min(static_cast<int>(blockIdx.z) * run, all_tiles);
+    const int end = min(t0 + run, all_tiles), tiles = end - t0;               // this workgroup's tiles: t0 .. end - 1
     const int full = visible(row0) / kTile;                                   // tiles that every row of the workgroup sees whole
     const int w0 = row0 + 32 * wave, my_row = min(w0 + r, rows - 1);
     const int limit = visible(my_row);
@@ -114,7 +158,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
         const uint32_t keep = here ? 0xffffffffu : 0u;
         return make_uint4(raw.x & keep, raw.y & keep, raw.z & keep, raw.w & keep);
     };
-    // `half`: the tile's place in LDS, t % 2
+    // `half`: the tile's place in LDS, the first in the first half
     auto store_keys = [&](int t, int half, bool here, uint4 raw, float key_scale) {
         if (copies_keys) {
             raw = blank(raw, here);                                           // (NaN codes would outlive the minus infinity below)
@@ -191,22 +235,23 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     Place keys_at{0, false}, next_at{0, false};                               // of key_raw's tile, of the one behind
     int entry_next = 0;                                                       // of the one behind that
     float key_scale = 0.0f, value_scale = 0.0f, value_scale_keys = 0.0f;      // of key_raw's tile; of value_raw's; of key_raw's tile again
-    const int last = tiles - 1;
+    const int last = end - 1;
     if (tiles > 0) {
         if (tid < 4) nan_values[tid] = 0;
-        const int e0 = entry(0), e1 = entry(min(1, last)), e2 = entry(min(2, last)), e3 = entry(min(3, last));
-        const Place p0 = checked(0, e0), p1 = checked(min(1, last), e1);
-        keys_at = checked(min(2, last), e2);
-        next_at = checked(min(3, last), e3);
+        const int t1 = min(t0 + 1, last), t2 = min(t0 + 2, last), t3 = min(t0 + 3, last), t4 = min(t0 + 4, last);
+        const int e0 = entry(t0), e1 = entry(t1), e2 = entry(t2), e3 = entry(t3);
+        const Place p0 = checked(t0, e0), p1 = checked(t1, e1);
+        keys_at = checked(t2, e2);
+        next_at = checked(t3, e3);
         values_here = p1.here;
-        const uint4 k0 = load_keys(0, p0), v0 = load_values(0, p0), k1 = load_keys(min(1, last), p1);
+        const uint4 k0 = load_keys(t0, p0), v0 = load_values(t0, p0), k1 = load_keys(t1, p1);
         const float ks0 = a.key_scales[p0.at], vs0 = a.value_scales[p0.at], ks1 = a.key_scales[p1.at];
         value_scale = a.value_scales[p1.at];
         key_scale = a.key_scales[keys_at.at];
         value_scale_keys = a.value_scales[keys_at.at];
-        key_raw = load_keys(min(2, last), keys_at);
-        value_raw = load_values(min(1, last), p1);
-        entry_next = entry(min(4, last));
+        key_raw = load_keys(t2, keys_at);
+        value_raw = load_values(t1, p1);
+        entry_next = entry(t4);
         // bf16 queries so large that products with codes could pass the largest float, where the scaled score need not: a power of two off, on again behind
         if constexpr (BF16) {
             float top = 0.0f;
@@ -230,12 +275,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
                 }
             }
         } else __syncthreads();
-        store_keys(0, 0, p0.here, k0, ks0);
-        store_values(std::false_type{}, 0, 0, p0.here, v0, vs0);
-        store_keys(1, 1, p1.here, k1, ks1);                                   // (one tile only: the same again, in the other half)
+        store_keys(t0, 0, p0.here, k0, ks0);
+        store_values(std::false_type{}, t0, 0, p0.here, v0, vs0);
+        store_keys(t0 + 1, 1, p1.here, k1, ks1);                                  // (one tile only: the same again, in the other half)
         __syncthreads();
         scores(0, sa);
-        load_factors(0, f, b);
+        load_factors(t0, f, b);
         top = row_top(sa, f, b);
     }
 
@@ -347,19 +392,33 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
         }
         __syncthreads();
     };
-    int t = 0;
-    for (; t + 3 <= full; t += 2) {                                           // (both steps copy values of tiles that every row sees whole)
+    int t = t0;
+    for (; t + 3 <= min(full, end); t += 2) {                                 // (both steps copy values of tiles that every row sees whole)
         step(std::false_type{}, t, 0, sa, sb);
         step(std::false_type{}, t + 1, 1, sb, sa);
     }
-    for (; t < tiles; ++t) {
-        step(std::true_type{}, t, t & 1, sa, sb);
+    for (; t < end; ++t) {
+        step(std::true_type{}, t, (t - t0) & 1, sa, sb);
 #pragma unroll
         for (int u = 0; u < 2; ++u) sa[u] = sb[u];
     }
     float lower, upper;
     swapped_pair<32>(l, lower, upper);
-    const float den = lower + upper, inv = den == 0.0f ? 0.0f : 2.0f / den;   // (twice: the values went in halved)
+    const float den = lower + upper;
+    if (a.sums) {
+        // one of several runs of the block's keys: sums and statistics as they are, for the kernel that brings them together
+        if (w0 + r < rows) {
+            const size_t row = (static_cast<size_t>(blockIdx.z) * a.tokens + offset + my_row / group) * a.heads + kvh * group + my_row % group;
+            if (h == 0) a.stats[row] = make_float2(m, den);
+#pragma unroll
+            for (int u = 0; u < kDimTiles; ++u)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<float4*>(a.sums + row * D + 32 * u + 8 * g + 4 * h) = make_float4(o[u][4 * g], o[u][4 * g + 1], o[u][4 * g + 2], o[u][4 * g + 3]);
+        }
+        return;
+    }
+    const float inv = den == 0.0f ? 0.0f : 2.0f / den;                        // (twice: the values went in halved)
     // lane: query r, dimensions 32 u + 8 (v / 4) + 4 h + v % 4; through the wave's own part of LDS to whole rows
     unsigned char* turn = smem + wave * (32 * 2 * D);
 #pragma unroll
@@ -379,24 +438,78 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     }
 }
 
+// A wave per query row: its runs together, in their order.
+template <bool BF16, int D>
+__global__ __launch_bounds__(256) void paged_prompt_merge_kernel(const PagedPromptArgs a) {
+    constexpr int kPer = D / 64;
+    const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads, row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    const float2 mine = lane < a.runs ? a.stats[lane * rows + row] : make_float2(-FLT_MAX, 0.0f);           // (at most 64 runs)
+    const float top = group_max<64>(mine.x), factor = __builtin_amdgcn_exp2f(mine.x - top), den = group_sum<64>(mine.y * factor);
+    float total[kPer] = {};
+    for (int i0 = 0; i0 < a.runs; i0 += 8) {
+        float v[8][kPer];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) v[i][j] = a.sums[(min(i0 + i, a.runs - 1) * rows + row) * D + kPer * lane + j];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i0 + i >= a.runs) break;
+            const float f = __shfl(factor, i0 + i);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) total[j] = __builtin_fmaf(v[i][j], f, total[j]);
+        }
+    }
+    const float inv = den == 0.0f ? 0.0f : 2.0f / den;
+    uint16_t* out = a.out + row * D + kPer * lane;
+    if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(out) = half_pair<BF16>(total[0] * inv, total[1] * inv);
+    else *out = static_cast<uint16_t>(half_pair<BF16>(total[0] * inv, 0.0f));
+}
+
 template <bool BF16, int D>
 int launch(const PagedPromptArgs& a, hipStream_t stream) {
     static SmemGrant granted;
     const size_t smem = 2 * 2 * kTile * D * 2;
     // (with the kernel's own arrays beside it, 128-wide heads pass 64 KB)
     if (!grant_dynamic_smem(reinterpret_cast<const void*>(paged_prompt_kernel<BF16, D>), smem + 4096, granted)) return PLLM_ERR_LAUNCH;
-    hipLaunchKernelGGL((paged_prompt_kernel<BF16, D>), dim3(a.kv_heads, a.slots), dim3(kThreads), smem, stream, a);
-    return hipGetLastError() == hipSuccess ? PLLM_OK : PLLM_ERR_LAUNCH;
+    hipLaunchKernelGGL((paged_prompt_kernel<BF16, D>), dim3(a.kv_heads, a.slots, a.runs), dim3(kThreads), smem, stream, a);
+    if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
+    if (a.sums) {
+        const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
+        hipLaunchKernelGGL((paged_prompt_merge_kernel<BF16, D>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream, a);
+        if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
+    }
+    return PLLM_OK;
+}
+
+// Runs that the keys of every block of query rows are cut in: as many as give every compute unit a workgroup when there are few rows before a
+// long context, none of them shorter than 16 tiles of a sequence that fills the table.
+int prompt_runs(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t positions) {
+    const int64_t blocks = (tokens * (heads / kv_heads) + kBlockRows - 1) / kBlockRows * kv_heads;
+    const int64_t runs = std::min(std::min(compute_units() / blocks, positions / (16 * kTile)), int64_t{64});
+    return static_cast<int>(std::max(runs, int64_t{1}));
 }
 
 }  // namespace
 }  // namespace pllm
 
-extern "C" int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pages, const uint8_t* value_pages,
+extern "C" {
+
+size_t pllm_paged_attention_prompt_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
+    if (tokens <= 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0 || positions <= 0 || tokens > 0x3fffff || heads > 1024 || head_dim > 256) return 0;
+    const int runs = pllm::prompt_runs(tokens, heads, kv_heads, positions);
+    if (runs == 1) return 0;
+    const size_t parts = static_cast<size_t>(runs) * tokens * heads;
+    return pllm::align256(parts * head_dim * sizeof(float)) + pllm::align256(parts * sizeof(float2));
+}
+
+int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pages, const uint8_t* value_pages,
                                            const float* key_scales, const float* value_scales, int64_t pool, int64_t page_tokens,
                                            const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* lengths,
                                            const int32_t* cu_steps, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                                           float scale, void* out, void* stream) {
+                                           float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
     using namespace pllm;
     if (!q || !key_pages || !value_pages || !key_scales || !value_scales || !block_table || !lengths || !cu_steps || !out) return PLLM_ERR_INVALID_ARGUMENT;
     if (dtype != PLLM_F16 && dtype != PLLM_BF16) return PLLM_ERR_INVALID_ARGUMENT;
@@ -408,7 +521,8 @@ extern "C" int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int 
     if (tokens > 0x3fffff || seqs > 0xffff || heads > 1024 || pool > 0x7fffffff || table_width > 0x3fffffff / page_tokens) return PLLM_ERR_UNSUPPORTED;
     const int64_t rows = tokens * (heads / kv_heads), slots = paged_slots(rows, static_cast<int>(seqs) + 1, kBlockRows, 1);
     if (rows > 0x3fffffff || slots > 0xffff) return PLLM_ERR_UNSUPPORTED;
-    const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) | reinterpret_cast<uintptr_t>(out);
+    const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) | reinterpret_cast<uintptr_t>(out) |
+                           reinterpret_cast<uintptr_t>(workspace);
     const uintptr_t narrow = reinterpret_cast<uintptr_t>(key_scales) | reinterpret_cast<uintptr_t>(value_scales) | reinterpret_cast<uintptr_t>(block_table) |
                              reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(cu_steps);
     if ((wide & 15u) || (narrow & 3u) || q_stride % 8) return PLLM_ERR_INVALID_ARGUMENT;
@@ -422,7 +536,15 @@ extern "C" int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int 
     a.page_shift = page_tokens == 16 ? 4 : page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7;
     a.pool = static_cast<int>(pool); a.width = static_cast<int>(table_width);
     a.slots = static_cast<int>(slots);
+    a.runs = prompt_runs(tokens, heads, kv_heads, table_width * page_tokens);
+    if (a.runs > 1) {
+        if (!workspace || workspace_bytes < pllm_paged_attention_prompt_workspace_bytes(tokens, heads, kv_heads, head_dim, table_width * page_tokens)) return PLLM_ERR_WORKSPACE;
+        a.sums = static_cast<float*>(workspace);
+        a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + align256(static_cast<size_t>(a.runs) * tokens * heads * head_dim * sizeof(float)));
+    }
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (head_dim == 128) return dtype == PLLM_BF16 ? launch<true, 128>(a, st) : launch<false, 128>(a, st);
     return dtype == PLLM_BF16 ? launch<true, 64>(a, st) : launch<false, 64>(a, st);
 }
+
+}  // extern "C"

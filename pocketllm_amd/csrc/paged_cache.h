@@ -21,6 +21,8 @@ namespace pllm {
 
 constexpr int kPagedChunk = 16;                 // positions that are certain to share a page
 constexpr int kPagedRunStep = 256;              // keys that a workgroup of the decode kernel takes at a time
+constexpr int kPagedOneRun = 1024;              // sequences of up to so many keys are one run of it
+constexpr int kPagedLeastRun = 512;             // and longer ones are cut in runs of at least so many
 
 PLLM_HD int clamp_int(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
@@ -41,6 +43,15 @@ PLLM_HD int paged_offset(const int32_t* cu_steps, int s, int even_steps, int row
 PLLM_HD int64_t paged_first_slot(int64_t offset, int s, int unit, int spare) { return offset / unit + static_cast<int64_t>(spare) * s; }
 PLLM_HD int64_t paged_slots(int64_t rows, int seqs, int unit, int spare) { return rows / unit + static_cast<int64_t>(spare) * seqs; }
 
+// Blocks of `block` query rows of one sequence that see keys of at least `tiles` tiles of 64: the last ones, since a row sees no fewer keys than those
+// before it.  `rows` = new tokens * group, the first of which see `first` + 1 keys.
+PLLM_HD int paged_blocks_seeing(int tiles, int rows, int first, int group, int block) {
+    const int blocks = (rows + block - 1) / block;
+    const int64_t need = (64 * (static_cast<int64_t>(tiles) - 1) - first) * group;           // the first row that does
+    if (tiles <= 0 || need <= 0) return blocks;
+    return need > rows - 1 ? 0 : blocks - static_cast<int>(need / block);
+}
+
 // page number of a position, or -1 where the table has none that lies in the pool
 PLLM_HD int paged_page(const int32_t* table_row, int position, int width, int page_shift, int pool) {
     const int at = position >> page_shift;
@@ -50,12 +61,13 @@ PLLM_HD int paged_page(const int32_t* table_row, int position, int width, int pa
 }
 
 // Keys of one run of the decode kernel.  By the sequence's own length and the number of heads alone, so that a sequence's sums have the
-// same order in every batch: runs of 256 keys as long as one sequence has no more of them than fill the machine.
+// same order in every batch: runs of at least kPagedLeastRun keys, as long as one sequence has no more of them than fill the machine.
 PLLM_HD int paged_most_runs(int kv_heads) { return clamp_int(512 / kv_heads, 8, 256); }
 PLLM_HD int paged_run_keys(int length, int kv_heads) {
     const int most = paged_most_runs(kv_heads), steps = (length + kPagedRunStep - 1) / kPagedRunStep;
     const int per = (steps + most - 1) / most;
-    return (per < 1 ? 1 : per) * kPagedRunStep;
+    if (length <= kPagedOneRun) return kPagedOneRun;
+    return (per * kPagedRunStep < kPagedLeastRun ? kPagedLeastRun : per * kPagedRunStep);
 }
 PLLM_HD int paged_runs(int length, int kv_heads) {
     const int keys = paged_run_keys(length, kv_heads);
@@ -63,9 +75,9 @@ PLLM_HD int paged_runs(int length, int kv_heads) {
 }
 // runs that a sequence of up to `length` positions can have
 PLLM_HD int paged_runs_bound(int64_t length, int kv_heads) {
-    const int64_t steps = (length + kPagedRunStep - 1) / kPagedRunStep;
+    const int64_t runs = length <= kPagedOneRun ? 1 : (length + kPagedLeastRun - 1) / kPagedLeastRun;
     const int most = paged_most_runs(kv_heads);
-    return steps < 1 ? 1 : (steps < most ? static_cast<int>(steps) : most);
+    return runs < 1 ? 1 : (runs < most ? static_cast<int>(runs) : most);
 }
 
 }  // namespace pllm

@@ -769,7 +769,9 @@ def paged_attention_prompt_forward(q: torch.Tensor, key_pages: torch.Tensor, val
                                    block_table: torch.Tensor, lengths: torch.Tensor, cu_steps: torch.Tensor, *, scale: float | None = None) -> torch.Tensor:
     """paged_attention_decode_forward for many new tokens per sequence (prompts, with or without a past, any mix of lengths): q
     [tokens, heads * head_dim], the tokens of sequence s in rows cu_steps[s] .. cu_steps[s + 1] - 1 (int32 [seqs + 1], from 0 on).  Rows behind the last sequence
-    are zeros.  Sequences of one or a few new tokens behind a long past are the decode form's work."""
+    are zeros.  Few rows before a wide table have its keys cut in runs that meet in a second launch: how many goes by
+    tokens, heads and the table's width, so the last bits of a sequence's outputs may differ between calls of other sizes.  Sequences of one or a few new
+    tokens behind a long past are the decode form's work."""
     what = "paged_attention_prompt"
     _check(q.dim() == 2, f"{what}: q must be [tokens, heads * head_dim]")
     pool, kv_heads, page, dim = _paged_cache(what, q, key_pages, value_pages, key_scales, value_scales, block_table, lengths)
@@ -780,11 +782,14 @@ def paged_attention_prompt_forward(q: torch.Tensor, key_pages: torch.Tensor, val
         return torch.zeros(tokens, width, dtype=q.dtype, device=q.device)
     out = torch.empty(tokens, width, dtype=q.dtype, device=q.device)
     rows = _rows16(q)
+    lib = _lib()
+    need = lib.pllm_paged_attention_prompt_workspace_bytes(tokens, width // dim, kv_heads, dim, block_table.size(1) * page)
     with _on_device(q.device):
-        st = _lib().pllm_paged_attention_prompt(rows.data_ptr(), rows.stride(0), _DTYPE_CODE[q.dtype], key_pages.data_ptr(), value_pages.data_ptr(),
+        ws = _workspace(need, q.device) if need else None
+        st = lib.pllm_paged_attention_prompt(rows.data_ptr(), rows.stride(0), _DTYPE_CODE[q.dtype], key_pages.data_ptr(), value_pages.data_ptr(),
                                                 key_scales.data_ptr(), value_scales.data_ptr(), pool, page, block_table.data_ptr(), _table_stride(block_table),
                                                 block_table.size(1), lengths.data_ptr(), cu_steps.data_ptr(), tokens, seqs, width // dim, kv_heads, dim,
-                                                float(dim ** -0.5 if scale is None else scale), out.data_ptr(), _stream(q.device))
+                                                float(dim ** -0.5 if scale is None else scale), out.data_ptr(), None if ws is None else ws.data_ptr(), need, _stream(q.device))
     _ffi.check(st, "paged_attention_prompt_forward")
     return out
 

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from pocketllm_amd import hip_kernel as K
+from pocketllm_amd import _ffi, hip_kernel as K
 from paged_cases import DEV, Cache, close, queries
 
 pytestmark = pytest.mark.gpu
@@ -155,7 +155,7 @@ def test_scale_strides_and_narrow_tables():
 
 
 def test_a_sequence_does_not_depend_on_its_batch():
-    lengths = [1, 900, 5000, 64, 2049, 17]
+    lengths = [1, 900, 5000, 64, 2049, 1024]
     cache = Cache(lengths, 2, 128, 64, seed=12)
     q = queries(6, 16, 128, BF).to(DEV)
     kp, vp, ks, vs, table, held = cache.device()
@@ -165,13 +165,42 @@ def test_a_sequence_does_not_depend_on_its_batch():
         alone = K.paged_attention_decode_forward(q[s:s + 1], kp, vp, ks, vs, table[s:s + 1], held[s:s + 1])
         narrow = K.paged_attention_decode_forward(q[s:s + 1], kp, vp, ks, vs, table[s:s + 1, :-(-lengths[s] // 64)], held[s:s + 1])
         assert torch.equal(alone[0], together[s]) and torch.equal(narrow[0], together[s])
-    steps = [1, 200, 333, 64, 49, 17]
+
+
+def test_a_prompt_does_not_depend_on_what_the_others_hold():
+    """The same call with other queries and another cache in the other sequences: equal bits."""
+    lengths, steps = [1, 900, 5000, 64, 2049, 17], [1, 200, 333, 64, 49, 17]
+    cache = Cache(lengths, 2, 128, 64, seed=12)
     cu = torch.tensor([0] + list(np.cumsum(steps)), dtype=torch.int32, device=DEV)
     q = queries(sum(steps), 16, 128, BF).to(DEV)
+    kp, vp, ks, vs, table, held = cache.device()
     together = K.paged_attention_prompt_forward(q, kp, vp, ks, vs, table, held, cu)
+    assert torch.equal(together, K.paged_attention_prompt_forward(q, kp, vp, ks, vs, table, held, cu))
     for s in range(6):
-        one = torch.tensor([0, steps[s]], dtype=torch.int32, device=DEV)
-        assert torch.equal(K.paged_attention_prompt_forward(q[cu[s]:cu[s + 1]].contiguous(), kp, vp, ks, vs, table[s:s + 1], held[s:s + 1], one), together[cu[s]:cu[s + 1]])
+        other_q, other_k, other_held = torch.randn_like(q), torch.full_like(kp.view(torch.uint8), 0x30), torch.ones_like(held)
+        other_q[cu[s]:cu[s + 1]] = q[cu[s]:cu[s + 1]]
+        pages = table[s, :-(-lengths[s] // 64)].long()
+        other_k[pages] = kp.view(torch.uint8)[pages]
+        other_held[s] = held[s]
+        got = K.paged_attention_prompt_forward(other_q, other_k, vp.view(torch.uint8), ks, vs, table, other_held, cu)
+        assert torch.equal(got[cu[s]:cu[s + 1]], together[cu[s]:cu[s + 1]])
+
+
+# few rows before a long context: the keys in runs, some of them empty for a short sequence beside a long one
+@pytest.mark.parametrize("steps,pasts,heads,kv_heads,dim,page,dtype", [
+    ([3], [3100], 6, 1, 128, 64, BF), ([40, 2, 0, 1], [2000, 0, 0, 4095], 2, 1, 64, 16, HF), ([17, 70], [5000, 10], 8, 2, 128, 128, HF), ([1], [9000], 16, 2, 64, 32, BF)])
+def test_prompt_in_runs_against_float64(steps, pasts, heads, kv_heads, dim, page, dtype):
+    cache = Cache([n + p if n else 0 for n, p in zip(steps, pasts)], kv_heads, dim, page, seed=sum(steps) + heads)
+    cu = np.concatenate([[0], np.cumsum(steps)])
+    q = queries(cu[-1] + 5, heads, dim, dtype, seed=2)
+    lib = _ffi.load_library()
+    assert lib.pllm_paged_attention_prompt_workspace_bytes(cu[-1] + 5, heads, kv_heads, dim, cache.width * page) > 0, "the case has one run"
+    if steps[0] == 17:
+        cache.table[0, 5] = -1
+    got = K.paged_attention_prompt_forward(q.to(DEV), *cache.device(), torch.tensor(cu, dtype=torch.int32, device=DEV))
+    want, note = cache.attention(q[:cu[-1]].view(-1, heads, dim).double().numpy(), cu)
+    close(got[:cu[-1]], want, note, dtype)
+    assert (got[cu[-1]:] == 0).all()
 
 
 def test_many_sequences():

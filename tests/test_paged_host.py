@@ -81,7 +81,22 @@ def test_runs_cover_a_sequence_and_stay_below_their_bound(index):
             assert runs <= index.idx_runs_bound(length, kv_heads)
             assert index.idx_runs_bound(length, kv_heads) >= bound                # a longer table has room for the runs of every shorter sequence
             bound = index.idx_runs_bound(length, kv_heads)
-        assert index.idx_run_keys(0, kv_heads) == 256 and index.idx_runs(0, kv_heads) == 0 and index.idx_runs_bound(0, kv_heads) == 1
+        assert index.idx_runs(0, kv_heads) == 0 and [index.idx_runs_bound(n, kv_heads) for n in (0, 1, 1024)] == [1, 1, 1]
+        assert index.idx_runs(1024, kv_heads) == 1 and index.idx_runs(1025, kv_heads) == 3
+
+
+def test_blocks_that_see_so_many_tiles(index):
+    """The closed form by which the prompt kernel orders its blocks against a count."""
+    rng = random.Random(1)
+    for _ in range(300):
+        group, block, n = rng.choice([1, 3, 6, 8]), rng.choice([128, 256]), rng.choice([0, 1, rng.randint(1, 300)])
+        keys = n + rng.choice([0, -n, rng.randint(-n, 0), rng.randint(0, 1000)])
+        rows = n * group
+        blocks = [min(rows, block * (b + 1)) - 1 for b in range(-(-rows // block))]      # their last rows
+        sees = [max(0, keys - n + r // group + 1) for r in blocks]
+        for tiles in range(0, 25):
+            want = sum(tiles == 0 or -(-v // 64) >= tiles for v in sees)
+            assert index.idx_blocks_seeing(tiles, rows, keys - n, group, block) == want, (tiles, rows, keys, n, group, block)
 
 
 def test_e4m3_of_the_oracle_is_torchs():
@@ -164,7 +179,7 @@ def test_c_entries_refuse_before_anything_is_launched():
         return lib.pllm_paged_attention_decode(*a.values(), None)
 
     def prompt(**kw):
-        a = {**base, **dict(cu=at, tokens=5, seqs=2, heads=4, kv=2, dim=64, scale=0.1, out=at), **kw}
+        a = {**base, **dict(cu=at, tokens=5, seqs=2, heads=4, kv=2, dim=64, scale=0.1, out=at, ws=None, need=0), **kw}
         return lib.pllm_paged_attention_prompt(*a.values(), None)
 
     def append(**kw):
@@ -183,8 +198,12 @@ def test_c_entries_refuse_before_anything_is_launched():
     assert decode(steps=0) == invalid and decode(steps=5000) == unsupported and prompt(cu=None) == invalid and prompt(tokens=0) == invalid and prompt(tokens=2**23) == unsupported
     assert decode(width=300, table_stride=300) == workspace
     need = lib.pllm_paged_attention_decode_workspace_bytes(2, 1, 4, 2, 64, 4800)
-    assert need >= 2 * 4 * 19 * 66 * 4 and decode(width=300, table_stride=300, ws=at, need=need - 1) == workspace
-    assert lib.pllm_paged_attention_decode_workspace_bytes(2, 1, 4, 2, 64, 256) == 0 and lib.pllm_paged_attention_decode_workspace_bytes(-1, 1, 4, 2, 64, 256) == 0
+    assert need >= 2 * 4 * 10 * 66 * 4 and decode(width=300, table_stride=300, ws=at, need=need - 1) == workspace
+    assert lib.pllm_paged_attention_decode_workspace_bytes(2, 1, 4, 2, 64, 1024) == 0 and lib.pllm_paged_attention_decode_workspace_bytes(-1, 1, 4, 2, 64, 256) == 0
+    assert prompt(width=200, table_stride=200) == workspace
+    need = lib.pllm_paged_attention_prompt_workspace_bytes(5, 4, 2, 64, 3200)
+    assert need >= 3 * 5 * 4 * 66 * 4 and prompt(width=200, table_stride=200, ws=at, need=need - 1) == workspace
+    assert lib.pllm_paged_attention_prompt_workspace_bytes(5, 4, 2, 64, 1024) == 0 and lib.pllm_paged_attention_prompt_workspace_bytes(100000, 4, 2, 64, 10**6) == 0
     for kw in (dict(k=None), dict(v=None), dict(q=None), dict(q_out=None), dict(dtype=0), dict(rows=0), dict(seqs=0), dict(kv=0), dict(heads=0), dict(pool=0), dict(width=0),
                dict(table_stride=1), dict(cu=None), dict(k_stride=127), dict(v_stride=120), dict(q_stride=200), dict(rope=-16), dict(rope=80), dict(cos=None), dict(sin=None),
                dict(positions=47), dict(k=at + 8), dict(cos=at + 4), dict(k_stride=132), dict(lengths=at + 1)):
