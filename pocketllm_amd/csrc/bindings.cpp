@@ -20,6 +20,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <cmath>
 #include <vector>
 
 #include "../../include/pllm_hip.h"
@@ -35,6 +36,7 @@ const Tensor* tensor(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVaria
 bool dense(const Tensor* t) { return t && t->layout() == at::kStrided && t->has_storage() && t->is_contiguous(); }
 bool plain(const Tensor* t) { return dense(t) && t->is_cuda(); }
 bool plain(const Tensor* t, at::ScalarType st) { return plain(t) && t->scalar_type() == st; }
+bool on16(const Tensor* t) { return reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0; }
 bool here(const Tensor* t) { return t->get_device() == c10::hip::current_device(); }
 
 int code_of(at::ScalarType st) { return st == at::kFloat ? PLLM_F32 : (st == at::kHalf ? PLLM_F16 : (st == at::kBFloat16 ? PLLM_BF16 : -1)); }
@@ -350,6 +352,156 @@ PyObject* moe_single_token(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// (name, x, residual or None, weight, eps, quant_eps, round_scale_pow2, in_place) -> (codes, scales, total)
+PyObject* add_norm_fp8(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    float eps, quant_eps;
+    if (nargs != 8) Py_RETURN_NONE;
+    const Tensor *x = tensor(a[1]), *residual = a[2] == Py_None ? nullptr : tensor(a[2]), *weight = tensor(a[3]);
+    if (!plain(x) || !here(x) || x->dim() < 1 || !plain(weight, at::kFloat) || !float_arg(a[4], eps) || !float_arg(a[5], quant_eps) || !PyBool_Check(a[6]) || !PyBool_Check(a[7]))
+        Py_RETURN_NONE;
+    const at::ScalarType st = x->scalar_type();
+    const int64_t dim = x->size(-1);
+    if (code_of(st) < 0 || dim <= 0 || dim % 128 != 0 || dim > 32768 || x->numel() == 0 || weight->dim() != 1 || weight->size(0) != dim || !(quant_eps > 0.0f) ||
+        weight->get_device() != x->get_device())
+        Py_RETURN_NONE;
+    if (a[2] != Py_None && (!plain(residual, st) || residual->sizes() != x->sizes() || residual->get_device() != x->get_device())) Py_RETURN_NONE;
+    const bool in_place = a[7] == Py_True;
+    if ((in_place && !residual) || !on16(x) || !on16(weight) || (residual && !on16(residual))) Py_RETURN_NONE;
+    c10::SmallVector<int64_t, 5> blocks(x->sizes().begin(), x->sizes().end());
+    blocks.back() = dim / 128;
+    Tensor codes = at::empty(x->sizes(), x->options().dtype(at::kFloat8_e4m3fn)), scales = at::empty(blocks, x->options().dtype(at::kFloat));
+    Tensor total = !residual ? *x : (in_place ? *residual : at::empty(x->sizes(), x->options()));
+    const int status = unlocked(pllm_fused_add_rms_norm_fp8, x->const_data_ptr(), residual ? residual->const_data_ptr() : nullptr, code_of(st), weight->const_data_ptr<float>(),
+                                residual ? total.data_ptr() : nullptr, static_cast<uint8_t*>(codes.data_ptr()), scales.data_ptr<float>(), x->numel() / dim, dim, eps, quant_eps,
+                                a[6] == Py_True, stream_of(*x));
+    if (status != PLLM_OK) return failed(a[0], status);
+    PyObject* r = PyTuple_New(3);
+    if (!r) return nullptr;
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(codes)));
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(scales)));
+    PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(std::move(total)));
+    return r;
+    END_HANDLE_TH_ERRORS
+}
+
+// The six tensors of a paged cache: a[0] .. a[5] = key pages, value pages, key scales, value scales, block table, lengths.
+struct Paged {
+    const Tensor *keys = nullptr, *values = nullptr, *key_scales = nullptr, *value_scales = nullptr, *table = nullptr, *lengths = nullptr;
+    int64_t pool = 0, kv_heads = 0, page = 0, dim = 0, seqs = 0, width = 0, table_stride = 0;
+    const uint8_t* key_codes() const { return static_cast<const uint8_t*>(keys->const_data_ptr()); }
+    const uint8_t* value_codes() const { return static_cast<const uint8_t*>(values->const_data_ptr()); }
+};
+bool paged_args(PyObject* const* a, const Tensor* like, Paged& p) {
+    p.keys = tensor(a[0]); p.values = tensor(a[1]); p.key_scales = tensor(a[2]); p.value_scales = tensor(a[3]); p.table = tensor(a[4]); p.lengths = tensor(a[5]);
+    if (!plain(p.keys) || !plain(p.values) || (p.keys->scalar_type() != at::kFloat8_e4m3fn && p.keys->scalar_type() != at::kByte) ||
+        p.values->scalar_type() != p.keys->scalar_type() || !plain(p.key_scales, at::kFloat) || !plain(p.value_scales, at::kFloat) || !plain(p.lengths, at::kInt))
+        return false;
+    if (!p.table || p.table->layout() != at::kStrided || !p.table->has_storage() || !p.table->is_cuda() || p.table->scalar_type() != at::kInt || p.table->dim() != 2) return false;
+    if (p.keys->dim() != 4 || p.values->dim() != 4) return false;
+    p.pool = p.keys->size(0); p.kv_heads = p.keys->size(1); p.page = p.keys->size(2); p.dim = p.keys->size(3);
+    p.seqs = p.table->size(0); p.width = p.table->size(1);
+    if (p.values->size(0) != p.pool || p.values->size(1) != p.kv_heads || p.values->size(2) != p.dim || p.values->size(3) != p.page) return false;
+    if ((p.page != 16 && p.page != 32 && p.page != 64 && p.page != 128) || (p.dim != 64 && p.dim != 128) || p.pool <= 0 || p.kv_heads <= 0 || p.seqs <= 0 || p.width <= 0) return false;
+    if (p.key_scales->dim() != 2 || p.key_scales->size(0) != p.pool || p.key_scales->size(1) != p.kv_heads || p.value_scales->sizes() != p.key_scales->sizes()) return false;
+    if (p.lengths->dim() != 1 || p.lengths->size(0) != p.seqs || p.table->stride(1) != 1 || (p.seqs > 1 && p.table->stride(0) < p.width)) return false;
+    p.table_stride = p.seqs > 1 ? p.table->stride(0) : p.width;
+    if (!on16(p.keys) || !on16(p.values)) return false;
+    for (const Tensor* t : {p.keys, p.values, p.key_scales, p.value_scales, p.table, p.lengths})
+        if (t->get_device() != like->get_device()) return false;
+    return true;
+}
+// rows [tokens, width] that the kernels read as they lie: values side by side, every row on 16 bytes
+bool rows16(const Tensor* t) {
+    return t && t->layout() == at::kStrided && t->has_storage() && t->is_cuda() && t->dim() == 2 && t->stride(1) == 1 && t->stride(0) % 8 == 0 && t->stride(0) >= t->size(1) && on16(t);
+}
+bool half_type(const Tensor* t) { return t->scalar_type() == at::kHalf || t->scalar_type() == at::kBFloat16; }
+
+// (name, q or None, k_new, v_new, the cache's six, cu_steps or None, cos_table, sin_table, rope_dim) -> the turned queries; with rope_dim 0 or without
+// queries True
+PyObject* paged_kv_append(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int64_t rope;
+    if (nargs != 14 || !int_arg(a[13], rope)) Py_RETURN_NONE;
+    const Tensor *q = a[1] == Py_None ? nullptr : tensor(a[1]), *k = tensor(a[2]), *v = tensor(a[3]);
+    Paged p;
+    if (!rows16(k) || !rows16(v) || !half_type(k) || !here(k) || v->scalar_type() != k->scalar_type() || v->get_device() != k->get_device() || !paged_args(a + 4, k, p)) Py_RETURN_NONE;
+    const int64_t tokens = k->size(0);
+    if (tokens <= 0 || k->size(1) != p.kv_heads * p.dim || v->sizes() != k->sizes() || rope < 0 || rope > p.dim || rope % 16 != 0) Py_RETURN_NONE;
+    if (a[1] != Py_None && (!rows16(q) || q->scalar_type() != k->scalar_type() || q->get_device() != k->get_device() || q->size(0) != tokens || q->size(1) % p.dim || q->size(1) == 0))
+        Py_RETURN_NONE;
+    const int32_t* cu = nullptr;
+    if (a[10] != Py_None) {
+        const Tensor* t = tensor(a[10]);
+        if (!plain(t, at::kInt) || t->dim() != 1 || t->size(0) != p.seqs + 1 || t->get_device() != k->get_device()) Py_RETURN_NONE;
+        cu = t->const_data_ptr<int32_t>();
+    } else if (tokens % p.seqs) Py_RETURN_NONE;
+    const Tensor *cos = nullptr, *sin = nullptr;
+    if (rope) {
+        cos = tensor(a[11]);
+        sin = tensor(a[12]);
+        for (const Tensor* t : {cos, sin})
+            if (!plain(t, at::kFloat) || t->dim() != 2 || t->size(1) != p.dim || t->size(0) < p.width * p.page || t->get_device() != k->get_device() || !on16(t)) Py_RETURN_NONE;
+    }
+    const bool turns = q && rope;
+    Tensor out;
+    if (turns) out = at::empty(q->sizes(), q->options());
+    const int st = unlocked(pllm_paged_kv_append, turns ? q->const_data_ptr() : nullptr, turns ? q->stride(0) : 0, k->const_data_ptr(), k->stride(0), v->const_data_ptr(), v->stride(0),
+                            code_of(k->scalar_type()), turns ? out.data_ptr() : nullptr, static_cast<uint8_t*>(p.keys->data_ptr()), static_cast<uint8_t*>(p.values->data_ptr()),
+                            p.key_scales->data_ptr<float>(), p.value_scales->data_ptr<float>(), p.pool, p.page, p.table->const_data_ptr<int32_t>(), p.table_stride, p.width,
+                            p.lengths->const_data_ptr<int32_t>(), cu, cos ? cos->const_data_ptr<float>() : nullptr, sin ? sin->const_data_ptr<float>() : nullptr,
+                            cos ? std::min(cos->size(0), sin->size(0)) : 0, rope, tokens, p.seqs, turns ? q->size(1) / p.dim : 0, p.kv_heads, p.dim, stream_of(*k));
+    if (st != PLLM_OK) return failed(a[0], st);
+    if (!turns) Py_RETURN_TRUE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// (name, q, the cache's six, scale or None) -> out
+PyObject* paged_attention_decode(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 9) Py_RETURN_NONE;
+    const Tensor* q = tensor(a[1]);
+    Paged p;
+    if (!plain(q) || !here(q) || !half_type(q) || (q->dim() != 2 && q->dim() != 3) || q->numel() == 0 || !on16(q) || !paged_args(a + 2, q, p)) Py_RETURN_NONE;
+    const int64_t seqs = q->size(0), steps = q->dim() == 3 ? q->size(1) : 1, width = q->size(-1);
+    if (seqs != p.seqs || width % p.dim || (width / p.dim) % p.kv_heads) Py_RETURN_NONE;
+    float scale = 1.0f / std::sqrt(static_cast<float>(p.dim));
+    if (a[8] != Py_None && (!float_arg(a[8], scale) || !(scale >= 0.0f && std::isfinite(scale)))) Py_RETURN_NONE;
+    const int64_t heads = width / p.dim;
+    Tensor out = at::empty(q->sizes(), q->options()), ws;
+    const size_t bytes = pllm_paged_attention_decode_workspace_bytes(seqs, steps, heads, p.kv_heads, p.dim, p.width * p.page);
+    if (bytes) ws = workspace(*q, bytes);
+    const int st = unlocked(pllm_paged_attention_decode, q->const_data_ptr(), width, code_of(q->scalar_type()), p.key_codes(), p.value_codes(), p.key_scales->const_data_ptr<float>(),
+                            p.value_scales->const_data_ptr<float>(), p.pool, p.page, p.table->const_data_ptr<int32_t>(), p.table_stride, p.width,
+                            p.lengths->const_data_ptr<int32_t>(), seqs, steps, heads, p.kv_heads, p.dim, scale, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes, stream_of(*q));
+    return st == PLLM_OK ? THPVariable_Wrap(std::move(out)) : failed(a[0], st);
+    END_HANDLE_TH_ERRORS
+}
+
+// (name, q, the cache's six, cu_steps, scale or None) -> out
+PyObject* paged_attention_prompt(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 10) Py_RETURN_NONE;
+    const Tensor *q = tensor(a[1]), *cu = tensor(a[8]);
+    Paged p;
+    if (!rows16(q) || !here(q) || !half_type(q) || q->numel() == 0 || !paged_args(a + 2, q, p)) Py_RETURN_NONE;
+    if (!plain(cu, at::kInt) || cu->dim() != 1 || cu->size(0) != p.seqs + 1 || cu->get_device() != q->get_device()) Py_RETURN_NONE;
+    const int64_t tokens = q->size(0), width = q->size(1), heads = width / p.dim;
+    if (width % p.dim || heads % p.kv_heads) Py_RETURN_NONE;
+    float scale = 1.0f / std::sqrt(static_cast<float>(p.dim));
+    if (a[9] != Py_None && (!float_arg(a[9], scale) || !(scale >= 0.0f && std::isfinite(scale)))) Py_RETURN_NONE;
+    Tensor out = at::empty(q->sizes(), q->options()), ws;
+    const size_t bytes = pllm_paged_attention_prompt_workspace_bytes(tokens, heads, p.kv_heads, p.dim, p.width * p.page);
+    if (bytes) ws = workspace(*q, bytes);
+    const int st = unlocked(pllm_paged_attention_prompt, q->const_data_ptr(), q->stride(0), code_of(q->scalar_type()), p.key_codes(), p.value_codes(),
+                            p.key_scales->const_data_ptr<float>(), p.value_scales->const_data_ptr<float>(), p.pool, p.page, p.table->const_data_ptr<int32_t>(), p.table_stride,
+                            p.width, p.lengths->const_data_ptr<int32_t>(), cu->const_data_ptr<int32_t>(), tokens, p.seqs, heads, p.kv_heads, p.dim, scale, out.data_ptr(),
+                            bytes ? ws.data_ptr() : nullptr, bytes, stream_of(*q));
+    return st == PLLM_OK ? THPVariable_Wrap(std::move(out)) : failed(a[0], st);
+    END_HANDLE_TH_ERRORS
+}
+
 // (tensor) -> whether the functions above may read its memory as it lies (the device aside)
 PyObject* dense_tensor(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
@@ -361,6 +513,7 @@ PyMethodDef methods[] = {
 #define PLLM_FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
     PLLM_FN(quant_gemm), PLLM_FN(quant_gemm_accumulate), PLLM_FN(quant_gemm_multi), PLLM_FN(q8_0_gemm), PLLM_FN(fp8_block_gemm),
     PLLM_FN(attention_decode), PLLM_FN(route_rmsnorm), PLLM_FN(moe_single_token), PLLM_FN(dense_tensor),
+    PLLM_FN(add_norm_fp8), PLLM_FN(paged_kv_append), PLLM_FN(paged_attention_decode), PLLM_FN(paged_attention_prompt),
 #undef PLLM_FN
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_bindings", "Native host path of the per-token operators.", -1, methods, nullptr, nullptr, nullptr, nullptr};

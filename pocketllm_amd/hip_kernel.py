@@ -616,6 +616,9 @@ def fused_add_rms_norm_fp8_forward(x: torch.Tensor, residual: torch.Tensor | Non
     fp8_act_quant_forward of fused_rms_norm_forward(total, weight, eps) with the normalized values kept in float32 in between.  x and residual
     [..., dim] of one type, dim a multiple of 128 (up to 32768); without a residual total is x.  in_place: total is written into residual.
     Returns (codes float8_e4m3fn [..., dim], scales float32 [..., dim / 128], total).  A block of 128 with an infinity or a NaN has NaN codes."""
+    made = _bindings.add_norm_fp8("fused_add_rms_norm_fp8_forward", x, residual, weight, float(eps), float(quant_eps), bool(round_scale_pow2), bool(in_place))
+    if made is not None:
+        return made
     _check(x.dim() >= 1, "add_rms_norm_fp8: x must have shape [..., dim]")
     dim = x.size(-1)
     _check_x(x)
@@ -697,6 +700,10 @@ def paged_kv_append_forward(q: torch.Tensor | None, k_new: torch.Tensor, v_new: 
     The scale of a page and head is the least power of two with amax / scale <= 448; when it has to grow, the page's older codes are scaled
     down with it.  Rows without a position in the table store nothing, their queries leave as zeros.  No two sequences may write into one page."""
     what = "paged_kv_append"
+    made = _bindings.paged_kv_append("paged_kv_append_forward", q, k_new, v_new, key_pages, value_pages, key_scales, value_scales, block_table, lengths, cu_steps,
+                                     cos_table, sin_table, rope_dim)
+    if made is not None:
+        return q if made is True else made
     pool, kv_heads, page, dim = _paged_cache(what, k_new, key_pages, value_pages, key_scales, value_scales, block_table, lengths)
     _check(k_new.dim() == 2 and k_new.size(1) == kv_heads * dim and v_new.shape == k_new.shape, f"{what}: k_new and v_new must be [tokens, kv_heads * head_dim]")
     _check(v_new.dtype == k_new.dtype and v_new.device == k_new.device, f"{what}: k_new and v_new must have one dtype and device")
@@ -742,10 +749,14 @@ def paged_attention_decode_forward(q: torch.Tensor, key_pages: torch.Tensor, val
     scale: head_dim ** -0.5 by default.  Returns q's shape and dtype; tokens that see no key get zeros.  The table's width bounds the work that is
     dealt out: pass a narrower view, block_table[:, :n], where no sequence is longer."""
     what = "paged_attention_decode"
+    out = _bindings.paged_attention_decode("paged_attention_decode_forward", q, key_pages, value_pages, key_scales, value_scales, block_table, lengths, scale)
+    if out is not None:
+        return out
     _check(q.dim() in (2, 3), f"{what}: q must be [seqs, steps, heads * head_dim] or [seqs, heads * head_dim]")
     pool, kv_heads, page, dim = _paged_cache(what, q, key_pages, value_pages, key_scales, value_scales, block_table, lengths)
     seqs, steps, width = q.size(0), q.size(1) if q.dim() == 3 else 1, q.size(-1)
     _check(seqs == block_table.size(0), f"{what}: q and block_table must have the same sequences")
+    _check(scale is None or 0.0 <= float(scale) < float("inf"), f"{what}: scale must be finite and not negative")
     _check(width % dim == 0 and width > 0 and (width // dim) % kv_heads == 0, f"{what}: heads must be a multiple of the cache's key/value heads")
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if out.numel() == 0:
@@ -773,10 +784,14 @@ def paged_attention_prompt_forward(q: torch.Tensor, key_pages: torch.Tensor, val
     tokens, heads and the table's width, so the last bits of a sequence's outputs may differ between calls of other sizes.  Sequences of one or a few new
     tokens behind a long past are the decode form's work."""
     what = "paged_attention_prompt"
+    out = _bindings.paged_attention_prompt("paged_attention_prompt_forward", q, key_pages, value_pages, key_scales, value_scales, block_table, lengths, cu_steps, scale)
+    if out is not None:
+        return out
     _check(q.dim() == 2, f"{what}: q must be [tokens, heads * head_dim]")
     pool, kv_heads, page, dim = _paged_cache(what, q, key_pages, value_pages, key_scales, value_scales, block_table, lengths)
     tokens, width, seqs = q.size(0), q.size(1), block_table.size(0)
     _paged_offsets(what, cu_steps, seqs, q.device)
+    _check(scale is None or 0.0 <= float(scale) < float("inf"), f"{what}: scale must be finite and not negative")
     _check(width % dim == 0 and width > 0 and (width // dim) % kv_heads == 0, f"{what}: heads must be a multiple of the cache's key/value heads")
     if tokens == 0 or seqs == 0:
         return torch.zeros(tokens, width, dtype=q.dtype, device=q.device)
