@@ -6,7 +6,9 @@
 // Values that are not finite become NaN codes and do not count for the scale.
 //
 // A workgroup owns a page's keys, or its values, of one head: its scale needs no atomics and no second pass.  Values turn in LDS, since a page
-// holds them with the tokens innermost.  The queries are rows behind these workgroups in the same grid, one workgroup to a token.
+// holds them with the tokens innermost.  The queries are rows behind these workgroups in the same grid.
+// Bound: bytes for prompts (4096 tokens of 48 and 8 heads of 128: 128 MB in 23 us, 5.5 TB/s; with pages of 16 tokens 25), the chain of a workgroup's loads
+// (offset, length, row and page, scale: 4 us) and the number of workgroups (two for every page and head) for decode steps.
 #include "paged_device.h"
 #include "pllm_internal.h"
 
@@ -15,8 +17,7 @@
 namespace pllm {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMostPage = 128;
+constexpr int kHeadPasses = 4;                  // heads that a thread of a query's workgroup turns, one after the other
 
 struct AppendArgs {
     const uint16_t* q; const uint16_t* k; const uint16_t* v;
@@ -27,7 +28,8 @@ struct AppendArgs {
     const int32_t* table; size_t table_stride;
     const int32_t* lengths; const int32_t* cu_steps;
     const float* cos_table; const float* sin_table;             // [>= width * page][D]
-    int rows, seqs, even_steps, heads, kv_heads, page_shift, pool, width, rope_half, page_blocks;
+    int rows, seqs, even_steps, even_pages, heads,            // even: every sequence has that many new tokens, which touch that many pages at most
+        kv_heads, pool, width, rope_half, page_blocks, head_blocks;
 };
 
 struct Phases { float4 c[2], s[2]; };
@@ -63,14 +65,15 @@ __device__ __forceinline__ uint32_t scaled_codes(uint32_t w, float ratio) {
     return four_codes(lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio);
 }
 
-template <bool BF16, int D>
-__device__ __forceinline__ void turn_queries(const AppendArgs& a, int row) {
-    constexpr int kChunks = D / 8, kHeadsPerPass = kThreads / kChunks;
-    const int s = paged_sequence(a.cu_steps, a.even_steps, a.rows, a.seqs + 1, 1, 0, row);
+template <bool BF16, int D, int THREADS>
+__device__ __forceinline__ void turn_queries(const AppendArgs& a, int block, int page_shift) {
+    constexpr int kChunks = D / 8, kHeadsPerPass = THREADS / kChunks;
+    const int row = block / a.head_blocks, head0 = block % a.head_blocks * (kHeadPasses * kHeadsPerPass) + threadIdx.x / kChunks;
+    const int s = a.cu_steps ? paged_sequence(a.cu_steps, a.rows, a.seqs + 1, 1, 0, row) : row / a.even_steps;
     const int chunk = threadIdx.x % kChunks, d0 = 8 * chunk, half = a.rope_half;
     int64_t at = -1;
     if (s < a.seqs) at = static_cast<int64_t>(a.lengths[s]) - paged_offset(a.cu_steps, s + 1, a.even_steps, a.rows) + row;
-    const bool placed = at >= 0 && at < (static_cast<int64_t>(a.width) << a.page_shift);
+    const bool placed = at >= 0 && at < (static_cast<int64_t>(a.width) << page_shift);
     const int position = static_cast<int>(at);
     const bool turns = placed && d0 < 2 * half;
     Phases p;
@@ -78,7 +81,10 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, int row) {
     const int partner = d0 < half ? d0 + half : d0 - half;
     const uint16_t* src = a.q + static_cast<size_t>(row) * a.q_stride;
     uint16_t* dst = a.q_out + static_cast<size_t>(row) * a.heads * D;
-    for (int h = threadIdx.x / kChunks; h < a.heads; h += kHeadsPerPass) {
+#pragma unroll
+    for (int i = 0; i < kHeadPasses; ++i) {
+        const int h = head0 + kHeadsPerPass * i;
+        if (h >= a.heads) break;
         uint4 out = make_uint4(0, 0, 0, 0);                                   // rows that have no place in a sequence
         if (placed) {
             out = *reinterpret_cast<const uint4*>(src + h * D + d0);
@@ -95,59 +101,69 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, int row) {
     }
 }
 
-template <bool BF16, int D>
-__global__ __launch_bounds__(kThreads) void paged_append_kernel(const AppendArgs a) {
-    constexpr int kChunks = D / 8, kRows = kThreads / kChunks, kPasses = kMostPage / kRows;
-    __shared__ float red[kThreads / 64];
-    __shared__ __align__(16) uint8_t turned[kMostPage * D];
+// FEW: every sequence has the same few new tokens, no more than one pass over 64 threads takes: a workgroup of one wave (one token of each of 64 sequences
+// 6.3 -> 5.3 us, of 256 14.7 -> 9.6; 48 and 8 heads of 128)
+template <bool BF16, int D, int PAGE, bool FEW>
+__global__ __launch_bounds__(FEW ? 64 : 256) void paged_append_kernel(const AppendArgs a) {
+    constexpr int kThreads = FEW ? 64 : 256;
+    constexpr int kChunks = D / 8, kRows = kThreads / kChunks, kPasses = FEW ? 1 : (PAGE + kRows - 1) / kRows;
+    constexpr int kShift = PAGE == 16 ? 4 : PAGE == 32 ? 5 : PAGE == 64 ? 6 : 7;
+    __shared__ float red[4];
+    __shared__ __align__(16) uint8_t turned[(FEW ? kRows : PAGE) * D];
     const int block = blockIdx.x, tid = threadIdx.x;
-    if (block >= a.page_blocks) { turn_queries<BF16, D>(a, block - a.page_blocks); return; }
+    if (block >= a.page_blocks) { turn_queries<BF16, D, kThreads>(a, block - a.page_blocks, kShift); return; }
     const bool values = block & 1;
     const int head = (block >> 1) % a.kv_heads, slot = (block >> 1) / a.kv_heads;
-    const int page_tokens = 1 << a.page_shift;
-    const int s = paged_sequence(a.cu_steps, a.even_steps, a.rows, a.seqs, page_tokens, 2, slot);
+    const int s = a.cu_steps ? paged_sequence(a.cu_steps, a.rows, a.seqs, PAGE, 2, slot) : slot / a.even_pages;
     const int offset = paged_offset(a.cu_steps, s, a.even_steps, a.rows), n = paged_offset(a.cu_steps, s + 1, a.even_steps, a.rows) - offset;
     const int length = max(a.lengths[s], 0);
     const int first = length - n, begin = max(first, 0);                      // (a length below its new tokens: the earliest have no place)
-    const int64_t mine = (begin >> a.page_shift) + (slot - paged_first_slot(offset, s, page_tokens, 2));
+    const int64_t mine = (begin >> kShift) + (a.cu_steps ? slot - paged_first_slot(offset, s, PAGE, 2) : slot % a.even_pages);
     if (n <= 0 || mine < 0 || mine >= a.width) return;
-    const int page0 = static_cast<int>(mine) << a.page_shift;                 // (width << page_shift fits an int: the host's check)
-    const int lo = max(begin, page0), hi = min(length, page0 + page_tokens), count = hi - lo;
+    const int page0 = static_cast<int>(mine) << kShift;                       // (width << kShift fits an int: the host's check)
+    const int lo = max(begin, page0), hi = min(length, page0 + PAGE), count = hi - lo;
     if (count <= 0) return;
-    const int page = paged_page(a.table + static_cast<size_t>(s) * a.table_stride, page0, a.width, a.page_shift, a.pool);
+
+    // the new rows, eight neighbouring values of one token to a thread at a time; requested before the page that they go to is known
+    const int chunk = tid % kChunks, d0 = 8 * chunk, half = a.rope_half;
+    const bool turns = !values && d0 < 2 * half;
+    const int partner = turns ? (d0 < half ? d0 + half : d0 - half) : d0;
+    const uint16_t* src = (values ? a.v : a.k) + head * D;
+    const size_t stride = values ? a.v_stride : a.k_stride;
+    uint4 own[kPasses], other[kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+        const int token = min(tid / kChunks + kRows * i, count - 1);          // (threads behind the last token load it again)
+        const uint16_t* row = src + static_cast<size_t>(offset + (lo + token - first)) * stride;
+        own[i] = *reinterpret_cast<const uint4*>(row + d0);
+        if (turns) other[i] = *reinterpret_cast<const uint4*>(row + partner);
+    }
+    const int page = paged_page(a.table + static_cast<size_t>(s) * a.table_stride, page0, a.width, kShift, a.pool);
     if (page < 0) return;
     const size_t at = static_cast<size_t>(page) * a.kv_heads + head;
-    uint8_t* codes = (values ? a.value_pages : a.key_pages) + at * page_tokens * D;
+    uint8_t* codes = (values ? a.value_pages : a.key_pages) + at * PAGE * D;
     float* scale_at = (values ? a.value_scales : a.key_scales) + at;
     const int held = lo - page0;                                              // tokens that the page keeps
     const float old = held > 0 ? *scale_at : 0.0f;
-
-    // the new rows, eight neighbouring values of one token to a thread at a time
-    const int chunk = tid % kChunks, d0 = 8 * chunk, half = a.rope_half;
-    const bool turns = !values && d0 < 2 * half;
-    const int partner = d0 < half ? d0 + half : d0 - half;
-    const uint16_t* src = (values ? a.v : a.k) + head * D;
-    const size_t stride = values ? a.v_stride : a.k_stride;
     float v[kPasses][8], amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-        const int t = tid / kChunks + kRows * i;
         if (kRows * i >= count) break;
-        const int token = min(t, count - 1);                                  // (threads behind the last token load it again)
-        const uint16_t* row = src + static_cast<size_t>(offset + (lo + token - first)) * stride;
-        half_eight<BF16>(*reinterpret_cast<const uint4*>(row + d0), v[i]);
+        half_eight<BF16>(own[i], v[i]);
         if (turns) {
-            float other[8];
-            half_eight<BF16>(*reinterpret_cast<const uint4*>(row + partner), other);
-            turn(v[i], other, load_phases(a, lo + token, D, d0));
+            float across[8];
+            half_eight<BF16>(other[i], across);
+            turn(v[i], across, load_phases(a, lo + min(tid / kChunks + kRows * i, count - 1), D, d0));
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) amax = fabsf(v[i][j]) <= FLT_MAX ? fmaxf(amax, fabsf(v[i][j])) : amax;
     }
     amax = group_max<64>(amax);
-    if ((tid & 63) == 0) red[tid >> 6] = amax;
-    __syncthreads();
-    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if constexpr (!FEW) {
+        if ((tid & 63) == 0) red[tid >> 6] = amax;
+        __syncthreads();
+        amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    }
     const float need = page_scale(amax), scale = fmaxf(old, need), inv = 1.0f / scale;
     if (tid == 0) *scale_at = scale;
     if (held > 0 && scale > old) {                                            // what the page holds, on the larger scale
@@ -155,7 +171,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(const AppendArgs
         const int pieces = values ? D * ((held + 15) / 16) : held * (D / 16);
         for (int p = tid; p < pieces; p += kThreads) {
             const int across = (held + 15) / 16;
-            uint4* piece = reinterpret_cast<uint4*>(values ? codes + (p / across) * page_tokens + 16 * (p % across) : codes + 16 * p);
+            uint4* piece = reinterpret_cast<uint4*>(values ? codes + (p / across) * PAGE + 16 * (p % across) : codes + 16 * p);
             const int keep = values ? held - 16 * (p % across) : 16;
             const uint4 w = *piece;
             const uint32_t m[4] = {first_bytes(keep), first_bytes(keep - 4), first_bytes(keep - 8), first_bytes(keep - 12)};
@@ -178,7 +194,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(const AppendArgs
     const int c0 = held / 16, pieces = D * ((held + count + 15) / 16 - c0);
     for (int p = tid; p < pieces; p += kThreads) {
         const int d = p % D, t0 = 16 * (c0 + p / D);                          // slots t0 .. t0 + 15 of dimension d
-        uint8_t* dst = codes + static_cast<size_t>(d) * page_tokens + t0;
+        uint8_t* dst = codes + static_cast<size_t>(d) * PAGE + t0;
         const int from = max(held, t0), to = min(held + count, t0 + 16);
         if (to - from == 16) {
             uint32_t w[4];
@@ -192,6 +208,16 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(const AppendArgs
             for (int t = from; t < to; ++t) dst[t - t0] = turned[(t - held) * D + d];
         }
     }
+}
+
+// (a kernel for every page size: small pages need few registers and little LDS, and their workgroups hide one another's waits)
+template <bool BF16, int D, bool FEW>
+void launch(const AppendArgs& a, int64_t page_tokens, dim3 grid, hipStream_t stream) {
+    const dim3 threads(FEW ? 64 : 256);
+    if (page_tokens == 16) hipLaunchKernelGGL((paged_append_kernel<BF16, D, 16, FEW>), grid, threads, 0, stream, a);
+    else if (page_tokens == 32) hipLaunchKernelGGL((paged_append_kernel<BF16, D, 32, FEW>), grid, threads, 0, stream, a);
+    else if (page_tokens == 64) hipLaunchKernelGGL((paged_append_kernel<BF16, D, 64, FEW>), grid, threads, 0, stream, a);
+    else hipLaunchKernelGGL((paged_append_kernel<BF16, D, 128, FEW>), grid, threads, 0, stream, a);
 }
 
 }  // namespace
@@ -214,8 +240,11 @@ extern "C" int pllm_paged_kv_append(const void* q, int64_t q_stride, const void*
         return PLLM_ERR_UNSUPPORTED;
     // pages and positions in 32 bits, and a launch that counts its threads in 32 bits
     if (rows > 0x3fffff || seqs > 0xfffff || kv_heads > 1024 || heads > 1024 || pool > 0x7fffffff || table_width > 0x3fffffff / page_tokens) return PLLM_ERR_UNSUPPORTED;
-    const int64_t slots = paged_slots(rows, static_cast<int>(seqs), static_cast<int>(page_tokens), 2), page_blocks = 2 * slots * kv_heads;
-    if (page_blocks + rows > 0xffffff) return PLLM_ERR_UNSUPPORTED;
+    const int64_t even_pages = paged_pages_touched(rows / seqs, page_tokens);
+    const int64_t slots = cu_steps ? paged_slots(rows, static_cast<int>(seqs), static_cast<int>(page_tokens), 2) : seqs * even_pages, page_blocks = 2 * slots * kv_heads;
+    const bool few = !cu_steps && rows / seqs <= 64 * 8 / head_dim;           // a decode step
+    const int64_t together = kHeadPasses * (few ? 64 : 256) * 8 / head_dim, head_blocks = q ? (heads + together - 1) / together : 0;
+    if (page_blocks + rows * head_blocks > 0xffffff) return PLLM_ERR_UNSUPPORTED;
     const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new) | reinterpret_cast<uintptr_t>(q_out) |
                            reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) | reinterpret_cast<uintptr_t>(cos_table) |
                            reinterpret_cast<uintptr_t>(sin_table);
@@ -229,20 +258,16 @@ extern "C" int pllm_paged_kv_append(const void* q, int64_t q_stride, const void*
     a.key_pages = key_pages; a.value_pages = value_pages; a.key_scales = key_scales; a.value_scales = value_scales;
     a.table = block_table; a.table_stride = static_cast<size_t>(table_stride); a.lengths = lengths; a.cu_steps = cu_steps;
     a.cos_table = cos_table; a.sin_table = sin_table;
-    a.rows = static_cast<int>(rows); a.seqs = static_cast<int>(seqs); a.even_steps = static_cast<int>(rows / seqs);
+    a.rows = static_cast<int>(rows); a.seqs = static_cast<int>(seqs); a.even_steps = static_cast<int>(rows / seqs); a.even_pages = static_cast<int>(even_pages);
     a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
-    a.page_shift = page_tokens == 16 ? 4 : page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7;
     a.pool = static_cast<int>(pool); a.width = static_cast<int>(table_width); a.rope_half = static_cast<int>(rope_dim / 2);
     a.page_blocks = static_cast<int>(page_blocks);
-    const dim3 grid(static_cast<unsigned>(page_blocks + (q ? rows : 0)));
+    a.head_blocks = static_cast<int>(head_blocks);
+    const dim3 grid(static_cast<unsigned>(page_blocks + rows * head_blocks));
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool bf16 = dtype == PLLM_BF16;
-    if (head_dim == 128) {
-        if (bf16) hipLaunchKernelGGL((paged_append_kernel<true, 128>), grid, dim3(kThreads), 0, st, a);
-        else hipLaunchKernelGGL((paged_append_kernel<false, 128>), grid, dim3(kThreads), 0, st, a);
-    } else {
-        if (bf16) hipLaunchKernelGGL((paged_append_kernel<true, 64>), grid, dim3(kThreads), 0, st, a);
-        else hipLaunchKernelGGL((paged_append_kernel<false, 64>), grid, dim3(kThreads), 0, st, a);
-    }
+#define PLLM_APPEND(BF16, D) few ? launch<BF16, D, true>(a, page_tokens, grid, st) : launch<BF16, D, false>(a, page_tokens, grid, st)
+    if (head_dim == 128) dtype == PLLM_BF16 ? (PLLM_APPEND(true, 128)) : (PLLM_APPEND(false, 128));
+    else dtype == PLLM_BF16 ? (PLLM_APPEND(true, 64)) : (PLLM_APPEND(false, 64));
+#undef PLLM_APPEND
     return hipGetLastError() == hipSuccess ? PLLM_OK : PLLM_ERR_LAUNCH;
 }

@@ -43,6 +43,9 @@ PLLM_HD int paged_offset(const int32_t* cu_steps, int s, int even_steps, int row
 PLLM_HD int64_t paged_first_slot(int64_t offset, int s, int unit, int spare) { return offset / unit + static_cast<int64_t>(spare) * s; }
 PLLM_HD int64_t paged_slots(int64_t rows, int seqs, int unit, int spare) { return rows / unit + static_cast<int64_t>(spare) * seqs; }
 
+// pages that `steps` neighbouring positions touch at most
+PLLM_HD int64_t paged_pages_touched(int64_t steps, int64_t page) { return steps <= 0 ? 1 : (steps + page - 2) / page + 1; }
+
 // Blocks of `block` query rows of one sequence that see keys of at least `tiles` tiles of 64: the last ones, since a row sees no fewer keys than those
 // before it.  `rows` = new tokens * group, the first of which see `first` + 1 keys.
 PLLM_HD int paged_blocks_seeing(int tiles, int rows, int first, int group, int block) {

@@ -86,12 +86,12 @@ __device__ __forceinline__ uint32_t without_nan(uint32_t w) {
 __device__ __forceinline__ uint32_t first_bytes(int count) { return count >= 4 ? 0xffffffffu : (count <= 0 ? 0u : (1u << (8 * count)) - 1u); }
 
 // The sequence that owns a slot of work: the last of the first `count` whose first slot is not behind it.  All lanes look together.
-__device__ __forceinline__ int paged_sequence(const int32_t* cu_steps, int even_steps, int rows, int count, int unit, int spare, int64_t slot) {
+__device__ __forceinline__ int paged_sequence(const int32_t* cu_steps, int rows, int count, int unit, int spare, int64_t slot) {
     const int lane = threadIdx.x & 63;
     int owners = 0;
     for (int base = 0; base < count; base += 64) {
         const int s = base + lane;
-        const bool begun = s < count && paged_first_slot(paged_offset(cu_steps, s, even_steps, rows), s, unit, spare) <= slot;
+        const bool begun = s < count && paged_first_slot(paged_offset(cu_steps, s, 0, rows), s, unit, spare) <= slot;
         const int n = __popcll(__ballot(begun));
         owners += n;
         if (n < 64) break;

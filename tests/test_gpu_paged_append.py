@@ -105,6 +105,13 @@ def test_even_steps_without_offsets():
     _run([3] * 70, [int(p) for p in np.random.default_rng(0).integers(0, 90, 70)], 4, 2, 128, 32, 64, BF, seed=3, even=True)
 
 
+@pytest.mark.parametrize("steps,heads,kv_heads,dim,page", [(1, 48, 8, 128, 64), (4, 5, 1, 128, 16), (5, 17, 1, 128, 128), (8, 33, 1, 64, 32), (9, 2, 2, 64, 16), (1, 130, 2, 64, 128)])
+def test_even_steps_of_one_wave_and_more(steps, heads, kv_heads, dim, page):
+    """Four tokens of 128-wide heads, eight of 64-wide ones are one wave's; heads beyond one workgroup's share."""
+    pasts = [0, 1, page - 1, page, 3 * page - 2, 2 * page - steps if steps < 2 * page else 0]
+    _run([steps] * 6, pasts, heads, kv_heads, dim, page, 32, BF if steps % 2 else HF, seed=steps, even=True, spread=2.0)
+
+
 def test_rows_behind_the_last_sequence_store_nothing():
     _, _, out = _run([4, 6], [0, 29], 2, 1, 128, 16, 32, BF, extra=9)
     assert (out[10:] == 0).all()

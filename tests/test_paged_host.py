@@ -85,6 +85,13 @@ def test_runs_cover_a_sequence_and_stay_below_their_bound(index):
         assert index.idx_runs(1024, kv_heads) == 1 and index.idx_runs(1025, kv_heads) == 3
 
 
+def test_pages_that_a_number_of_tokens_touches(index):
+    index.idx_pages_touched.restype = ctypes.c_int64
+    for page in (16, 32, 64, 128):
+        for steps in list(range(1, 300)) + [4096, 2**31]:
+            assert index.idx_pages_touched(ctypes.c_int64(steps), ctypes.c_int64(page)) == max((at + steps - 1) // page + 1 for at in range(page))
+
+
 def test_blocks_that_see_so_many_tiles(index):
     """The closed form by which the prompt kernel orders its blocks against a count."""
     rng = random.Random(1)
