@@ -36,10 +36,17 @@ struct PagedPromptArgs {
 };
 
 // The block of query rows that index `index` of the grid is: sequence s (a.seqs: the rows behind the last one), rows row0 .. row0 + kBlockRows - 1 of it.
-// Those with the most keys come first, so that what is left at the end is short (six prompts and continuations, 64 and 8 heads: TODO us); of more than 63
-// sequences only each one's own blocks are in that order, by slots.
+// Those with the most keys come first, so that what is left at the end is short (48 and 8 heads: 30 continuations of up to 200 tokens behind up to 4000
+// 267 -> 215 us, 12 of up to 300 behind up to 16000 809 -> 693; where a sequence's own order is as good already, four prompts of up to 2000 tokens, 117 -> 123); of
+// more than 63 sequences only each one's own blocks are in that order, by slots.
 __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, int group, int& s, int& row0) {
     const int lane = threadIdx.x & 63;
+    if (a.seqs == 1) {                                                        // (1024 tokens of 48 and 8 heads: 42.0 -> 40.5 us)
+        const int n = paged_offset(a.cu_steps, 1, 0, a.tokens), blocks = (n * group + kBlockRows - 1) / kBlockRows;
+        s = index < blocks ? 0 : 1;
+        row0 = (index < blocks ? blocks - 1 - index : index - blocks) * kBlockRows;
+        return row0 < (s ? a.tokens - n : n) * group;
+    }
     if (a.seqs < 64) {
         int rows = 0, first = 0, keys = 0;                                    // of the lane's sequence
         if (lane <= a.seqs) {
@@ -89,7 +96,7 @@ __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, 
     return true;
 }
 
-template <bool BF16, int D>
+template <bool BF16, int D, bool RUNS>
 __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPromptArgs a) {
     constexpr int kKeyBytes = kTile * D * 2, kTileBytes = 2 * kKeyBytes;      // keys [64][D], values [D][64]
     constexpr int kDimTiles = D / 32, kSteps = D / 16;
@@ -114,8 +121,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
         return tail ? 0 : static_cast<int>(v < 0 ? 0 : (v > length ? length : v));
     };
     const int all_tiles = (visible(min(rows, row0 + kBlockRows) - 1) + kTile - 1) / kTile;
-    const int run = (all_tiles + static_cast<int>(gridDim.z) - 1) / static_cast<int>(gridDim.z), t0 = min(static_cast<int>(blockIdx.z) * run, all_tiles);
-    const int end = min(t0 + run, all_tiles), tiles = end - t0;               // this workgroup's tiles: t0 .. end - 1
+    // this workgroup's tiles: t0 .. end - 1
+    const int run = RUNS ? (all_tiles + static_cast<int>(gridDim.z) - 1) / static_cast<int>(gridDim.z) : all_tiles, t0 = RUNS ? min(static_cast<int>(blockIdx.z) * run, all_tiles) : 0;
+    const int end = RUNS ? min(t0 + run, all_tiles) : all_tiles, tiles = end - t0;
     const int full = visible(row0) / kTile;                                   // tiles that every row of the workgroup sees whole
     const int w0 = row0 + 32 * wave, my_row = min(w0 + r, rows - 1);
     const int limit = visible(my_row);
@@ -405,7 +413,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     float lower, upper;
     swapped_pair<32>(l, lower, upper);
     const float den = lower + upper;
-    if (a.sums) {
+    if constexpr (RUNS) {
         // one of several runs of the block's keys: sums and statistics as they are, for the kernel that brings them together
         if (w0 + r < rows) {
             const size_t row = (static_cast<size_t>(blockIdx.z) * a.tokens + offset + my_row / group) * a.heads + kvh * group + my_row % group;
@@ -470,11 +478,12 @@ __global__ __launch_bounds__(256) void paged_prompt_merge_kernel(const PagedProm
 
 template <bool BF16, int D>
 int launch(const PagedPromptArgs& a, hipStream_t stream) {
-    static SmemGrant granted;
+    static SmemGrant granted[2];
     const size_t smem = 2 * 2 * kTile * D * 2;
     // (with the kernel's own arrays beside it, 128-wide heads pass 64 KB)
-    if (!grant_dynamic_smem(reinterpret_cast<const void*>(paged_prompt_kernel<BF16, D>), smem + 4096, granted)) return PLLM_ERR_LAUNCH;
-    hipLaunchKernelGGL((paged_prompt_kernel<BF16, D>), dim3(a.kv_heads, a.slots, a.runs), dim3(kThreads), smem, stream, a);
+    const auto kernel = a.sums ? paged_prompt_kernel<BF16, D, true> : paged_prompt_kernel<BF16, D, false>;
+    if (!grant_dynamic_smem(reinterpret_cast<const void*>(kernel), smem + 4096, granted[a.sums != nullptr])) return PLLM_ERR_LAUNCH;
+    hipLaunchKernelGGL(kernel, dim3(a.kv_heads, a.slots, a.runs), dim3(kThreads), smem, stream, a);
     if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
     if (a.sums) {
         const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
