@@ -505,10 +505,11 @@ int pllm_paged_attention_decode(const void* q, int64_t q_stride, int dtype, cons
 
 /*
  * The same for many new tokens per sequence, ragged by cu_steps (required): prompts, with or without a past; no counterpart in the reference (its prompt
- * attention: src/models/minimax_m2/architecture.py:158-266).  q [tokens, heads * head_dim]; out contiguous; rows behind the last sequence are zeros.  Few rows
- * before a long table have its keys cut in runs: how many goes by tokens, heads and table, not by what they hold.
+ * attention: src/models/minimax_m2/architecture.py:158-266).  q [tokens, heads * head_dim]; out contiguous; rows behind the last sequence are zeros.  Keys of few
+ * rows before a long table are cut in runs, and sequences of very few rows go through the decode kernel: by the numbers of tokens, sequences and heads and
+ * the table, not by what they hold.  workspace as its function says, 16-byte aligned.
  */
-size_t pllm_paged_attention_prompt_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions);
+size_t pllm_paged_attention_prompt_workspace_bytes(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions);
 int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pages, const uint8_t* value_pages, const float* key_scales,
                                 const float* value_scales, int64_t pool, int64_t page_tokens, const int32_t* block_table, int64_t table_stride,
                                 int64_t table_width, const int32_t* lengths, const int32_t* cu_steps, int64_t tokens, int64_t seqs, int64_t heads,

@@ -84,7 +84,7 @@ SIGNATURES = {
     "pllm_paged_attention_decode_workspace_bytes": (_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "pllm_paged_attention_decode": (_int, [_c_void_p, _i64, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p,
                                            _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _c_void_p, _c_void_p, _size_t, _c_void_p]),
-    "pllm_paged_attention_prompt_workspace_bytes": (_size_t, [_i64, _i64, _i64, _i64, _i64]),
+    "pllm_paged_attention_prompt_workspace_bytes": (_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "pllm_paged_attention_prompt": (_int, [_c_void_p, _i64, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p,
                                            _c_void_p, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _c_void_p, _c_void_p, _size_t, _c_void_p]),
 }

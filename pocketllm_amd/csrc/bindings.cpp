@@ -492,7 +492,7 @@ PyObject* paged_attention_prompt(PyObject*, PyObject* const* a, Py_ssize_t nargs
     float scale = 1.0f / std::sqrt(static_cast<float>(p.dim));
     if (a[9] != Py_None && (!float_arg(a[9], scale) || !(scale >= 0.0f && std::isfinite(scale)))) Py_RETURN_NONE;
     Tensor out = at::empty(q->sizes(), q->options()), ws;
-    const size_t bytes = pllm_paged_attention_prompt_workspace_bytes(tokens, heads, p.kv_heads, p.dim, p.width * p.page);
+    const size_t bytes = pllm_paged_attention_prompt_workspace_bytes(tokens, p.seqs, heads, p.kv_heads, p.dim, p.width * p.page);
     if (bytes) ws = workspace(*q, bytes);
     const int st = unlocked(pllm_paged_attention_prompt, q->const_data_ptr(), q->stride(0), code_of(q->scalar_type()), p.key_codes(), p.value_codes(),
                             p.key_scales->const_data_ptr<float>(), p.value_scales->const_data_ptr<float>(), p.pool, p.page, p.table->const_data_ptr<int32_t>(), p.table_stride,

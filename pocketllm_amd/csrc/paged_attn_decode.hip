@@ -2,81 +2,83 @@
 //     out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - m),  k_j, v_j = code * scale of the page and head, j up to the query's position.
 // Two launches: runs of keys with a running maximum each, then the runs of a row together (one launch where no sequence can have two runs).
 //
-// A workgroup has a run of one sequence's keys for one key/value head and up to 16 query rows (the heads that share it, times the new tokens).  Its
+// A workgroup has a run of one sequence's keys for one key/value head and 16 or 32 query rows (the heads that share it, times the new tokens).  Its
 // four waves take 64 keys at a time each, with statistics of their own, and meet in LDS once, at the end.  A wave forms S^T = K Q^T
 // (v_mfma_f32_16x16x32: matrix rows are keys, columns queries), whose accumulator layout, rounded to 16 bits, is what O^T = V^T P^T wants as its
 // second operand if row 4 g + i of score tile t is key 16 g + 4 t + i: then a lane of group g has the 16 neighbouring keys 16 g .. + 15, and its
 // values are 16 neighbouring bytes of a value page.  16 neighbouring keys share a page, so a lane needs one page number for its keys' rows, one for
 // its values and two scales, whatever the page size.  Codes become 16-bit values in registers: E4M3 is exact in both types; the keys' scale goes on the
 // scores, the values' scale (halved, so that fp16 holds every value that rounds up from its largest) into the conversion, both exact.
-// Bound: bytes, 2 * length * D codes per head, once for each 16 rows.
+// Bound: bytes, 2 * length * D codes per head, once for each 16 or 32 rows, and the latency of a wave's next 64 keys, whose codes are only requested when
+// the last ones are done with: three workgroups of a compute unit cover it in part.  64 sequences of 1 to 8192 positions, 567 MB: 136 us, 4.2 TB/s, where a
+// kernel that only reads reaches 6.
+#include "paged_attention.h"
 #include "paged_device.h"
-#include "pllm_internal.h"
 
+#include <algorithm>
 #include <cfloat>
 
 namespace pllm {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kRows = 16;                       // query rows of a workgroup
 constexpr int kStep = 64;                       // keys that a wave takes at a time
 
-struct DecodeArgs {
-    const uint16_t* q; size_t q_stride;         // elements between tokens
-    const uint8_t* key_pages; const uint8_t* value_pages;
-    const float* key_scales; const float* value_scales;
-    const int32_t* table; size_t table_stride;
-    const int32_t* lengths;
-    float* sums;                                // [rows][runs_bound][D], null: outputs are written at once
-    float2* stats;                              // [rows][runs_bound]: maximum (base 2), sum of weights
-    uint16_t* out;
-    float scale;                                // base 2
-    int seqs, steps, heads, kv_heads, page_shift, pool, width, runs_bound, row_tiles;
-};
-
-// row of a workgroup's tile -> new token and head; rows of one key/value head: token * group + head in the group
-template <bool BF16, int D>
-__global__ __launch_bounds__(kThreads, 3) void paged_decode_kernel(const DecodeArgs a) {
+// SETS of 16 query rows; rows of one key/value head: token * group + head in the group
+template <bool BF16, int D, int SETS>
+__global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kernel(const PagedDecodeArgs a, int least_rows, int most_rows) {
     constexpr int kPieces = D / 64;             // 16-byte pieces of a key row per lane
     constexpr int kTiles = D / 16;              // output tiles
     constexpr int kPitch = D + 4;
-    __shared__ __align__(16) float sums[kWaves][kRows * kPitch];
-    __shared__ float2 stats[kWaves][kRows];
+    constexpr int kRows = 16 * SETS;
+    __shared__ __align__(16) float sums[kWaves][16 * kPitch];
+    __shared__ float2 stats[kWaves][16];
     __shared__ __align__(16) uint16_t queries[kRows][D + 8];                  // (in registers they cost the third workgroup of a compute unit)
     __shared__ __align__(8) uint16_t nan_keys[kWaves][D][4];                  // keys of a wave's step whose value is NaN, a bit each, per dimension
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     // Neighbouring workgroups run on different XCDs: heads first, and the runs of every sequence from another one on, or the XCDs of the first runs, which
     // every sequence has, would do the most (64 sequences of 1 to 8192 positions, run numbers first / heads first 198 / 147 us).
-    const int tile = blockIdx.x % a.row_tiles, kvh = blockIdx.x / a.row_tiles, s = blockIdx.z, run = (blockIdx.y + blockIdx.z) % a.runs_bound;
-    const int group = a.heads / a.kv_heads, rows = a.steps * group;
+    const int kvh = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, s = blockIdx.z, run = (blockIdx.y + blockIdx.z) % a.runs_bound;
+    const int group = a.heads / a.kv_heads;
+    const int offset = a.cu_steps ? paged_offset(a.cu_steps, s, 0, a.tokens) : s * a.steps;
+    const int n = a.cu_steps ? paged_offset(a.cu_steps, s + 1, 0, a.tokens) - offset : a.steps;
+    const int64_t all_rows = static_cast<int64_t>(n) * group;
+    if (all_rows < least_rows || all_rows > most_rows || kRows * tile >= all_rows) return;
+    const int rows = static_cast<int>(all_rows);
     const int given = a.lengths[s], length = paged_length(given, a.width, a.page_shift);
     const int run_keys = paged_run_keys(length, a.kv_heads), begin = run * run_keys, end = min(begin + run_keys, length);
     if (run > 0 && begin >= length) return;
     const int32_t* table = a.table + static_cast<size_t>(s) * a.table_stride;
 
-    // the column's query row and how many keys it sees
-    const int r = kRows * tile + col, token = r / group;
-    const bool row_real = r < rows;
-    const int64_t sees = static_cast<int64_t>(given) - a.steps + token + 1;
-    const int limit = row_real ? static_cast<int>(sees < 0 ? 0 : (sees > length ? length : sees)) : 0x7fffffff;
-    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    v4f o[kTiles];
+    // the columns' query rows and how many keys they see
+    int limit[SETS];
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) o[i] = zero;
-    float m = -FLT_MAX, l = 0.0f, late = 1.0f;  // of the column; l over the lane's own keys
+    for (int c = 0; c < SETS; ++c) {
+        const int r = kRows * tile + 16 * c + col;
+        const int64_t sees = static_cast<int64_t>(given) - n + r / group + 1;
+        limit[c] = r < rows ? static_cast<int>(sees < 0 ? 0 : (sees > length ? length : sees)) : 0x7fffffff;
+    }
+    const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    v4f o[SETS][kTiles];
+    float m[SETS], l[SETS], late = 1.0f;        // of the column; l over the lane's own keys
+#pragma unroll
+    for (int c = 0; c < SETS; ++c) {
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) o[c][i] = zero;
+        m[c] = -FLT_MAX;
+        l[c] = 0.0f;
+    }
     const size_t head_bytes = static_cast<size_t>(D) << a.page_shift, page_mask = (size_t{1} << a.page_shift) - 1;
     // page numbers of the lane's key rows (chunk col / 4 of the step) and of its values and scales (chunk g)
     auto pages = [&](int j0, int& key_page, int& value_page) {
         key_page = paged_page(table, min(j0 + 16 * (col >> 2), length - 1), a.width, a.page_shift, a.pool);
         value_page = j0 + 16 * g < length ? paged_page(table, j0 + 16 * g, a.width, a.page_shift, a.pool) : -1;
     };
-    // What is on its way: the codes and scales of a step while the one before is worked on, its page numbers a step before that.
     struct Step { uint4 keys[4][kPieces], values[kTiles]; float key_scale, value_scale; bool here; };
     auto request = [&](Step& x, int j0, int key_page, int value_page) {
         const size_t key_at = (static_cast<size_t>(max(key_page, 0)) * a.kv_heads + kvh) * head_bytes + ((j0 + 16 * (col >> 2)) & page_mask) * D;
-        const size_t value_at = (static_cast<size_t>(max(value_page, 0)) * a.kv_heads + kvh) * head_bytes + ((j0 + 16 * g) & page_mask);
+        const size_t value_at = (static_cast<size_t>(max(value_page, 0)) * a.kv_heads + kvh) * head_bytes + ((j0 + 16 * g) & page_mask) + (static_cast<uint32_t>(col) << a.page_shift);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -86,51 +88,62 @@ __global__ __launch_bounds__(kThreads, 3) void paged_decode_kernel(const DecodeA
         x.value_scale = a.value_scales[scale_at];
         x.here = value_page >= 0;
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) x.values[i] = *reinterpret_cast<const uint4*>(a.value_pages + value_at + (static_cast<size_t>(16 * i + col) << a.page_shift));
+        for (int i = 0; i < kTiles; ++i) x.values[i] = *reinterpret_cast<const uint4*>(a.value_pages + value_at + (static_cast<size_t>(16 * i) << a.page_shift));
     };
     auto work = [&](Step& x, int j0) {
         auto& kf = x.keys;
         auto& vf = x.values;
         const float key_factor = x.key_scale * a.scale, value_scale = x.here ? 0.5f * x.value_scale : 1.0f;
-        uint4 qf[2 * kPieces];
+        v4f sc[SETS][4];
 #pragma unroll
-        for (int i = 0; i < 2 * kPieces; ++i) qf[i] = *reinterpret_cast<const uint4*>(&queries[col][64 * (i >> 1) + 16 * g + 8 * (i & 1)]);
-        v4f sc[4];
+        for (int c = 0; c < SETS; ++c)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            sc[t] = zero;
+            for (int t = 0; t < 4; ++t) sc[c][t] = zero;
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                sc[t] = half_mfma16<BF16>(half_from_codes<BF16>(kf[t][i].x, kf[t][i].y, 1.0f), qf[2 * i], sc[t]);
-                sc[t] = half_mfma16<BF16>(half_from_codes<BF16>(kf[t][i].z, kf[t][i].w, 1.0f), qf[2 * i + 1], sc[t]);
+        for (int i = 0; i < kPieces; ++i) {
+            uint4 qf[SETS][2];
+#pragma unroll
+            for (int c = 0; c < SETS; ++c)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) qf[c][u] = *reinterpret_cast<const uint4*>(&queries[16 * c + col][64 * i + 16 * g + 8 * u]);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const uint4 lo = half_from_codes<BF16>(kf[t][i].x, kf[t][i].y, 1.0f), hi = half_from_codes<BF16>(kf[t][i].z, kf[t][i].w, 1.0f);
+#pragma unroll
+                for (int c = 0; c < SETS; ++c) sc[c][t] = half_mfma16<BF16>(hi, qf[c][1], half_mfma16<BF16>(lo, qf[c][0], sc[c][t]));
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[t][i] *= key_factor;
         }
-        if constexpr (BF16) {
-            if (late != 1.0f)
+        const float factor = BF16 ? fminf(key_factor * late, FLT_MAX) : key_factor;
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[t][i] *= late;
-        }
-        const int first = j0 + 16 * g, seen = x.here ? limit - first : 0;          // the lane's keys that its column sees
-        bool unseen_nan = false, some_nan = false;
-        if (!__all(seen >= 16)) {
-            const int stored = x.here ? length - first : 0;
+        for (int c = 0; c < SETS; ++c)
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sc[t][i] = 4 * t + i < seen ? sc[t][i] : -INFINITY;
+                for (int i = 0; i < 4; ++i) sc[c][t][i] *= factor;
+        const int first = j0 + 16 * g;
+        bool whole = true, some_nan = false;                                  // every column sees all of the lane's keys
+#pragma unroll
+        for (int c = 0; c < SETS; ++c) whole &= x.here && limit[c] - first >= 16;
+        if (!__all(whole)) {
+#pragma unroll
+            for (int c = 0; c < SETS; ++c) {
+                const int seen = x.here ? limit[c] - first : 0;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[c][t][i] = 4 * t + i < seen ? sc[c][t][i] : -INFINITY;
+            }
             // what lies behind the last key may be anything, NaN codes too, and zero times NaN is NaN
+            const int stored = x.here ? length - first : 0;
             const uint32_t keep[4] = {first_bytes(stored), first_bytes(stored - 4), first_bytes(stored - 8), first_bytes(stored - 12)};
+            bool nan = false;
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
                 vf[i].x &= keep[0]; vf[i].y &= keep[1]; vf[i].z &= keep[2]; vf[i].w &= keep[3];
-                unseen_nan |= any_nan_code(vf[i].x) | any_nan_code(vf[i].y) | any_nan_code(vf[i].z) | any_nan_code(vf[i].w);
+                nan |= any_nan_code(vf[i].x) | any_nan_code(vf[i].y) | any_nan_code(vf[i].z) | any_nan_code(vf[i].w);
             }
-            some_nan = __any(unseen_nan);
-            if (some_nan)                                                     // of keys that not every row sees: none into the product, where zero times NaN is NaN
+            some_nan = __any(nan);
+            if (some_nan)                                                     // of keys that not every row sees: none into the product
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i) {
                     nan_keys[wave][16 * i + col][g] =
@@ -138,46 +151,53 @@ __global__ __launch_bounds__(kThreads, 3) void paged_decode_kernel(const DecodeA
                     vf[i].x = without_nan(vf[i].x); vf[i].y = without_nan(vf[i].y); vf[i].z = without_nan(vf[i].z); vf[i].w = without_nan(vf[i].w);
                 }
         }
-        float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+        uint4 p[SETS][2];
 #pragma unroll
-        for (int t = 1; t < 4; ++t) top = fmaxf(top, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])));
-        float lower, upper;
-        swapped_pair<16>(top, lower, upper);
-        swapped_pair<32>(fmaxf(lower, upper), lower, upper);
-        const float m_new = fmaxf(m, fmaxf(lower, upper));
-        if (__any(m_new > m)) {
-            const float back = __builtin_amdgcn_exp2f(m - m_new);
-            l *= back;
+        for (int c = 0; c < SETS; ++c) {
+            float top = fmaxf(fmaxf(sc[c][0][0], sc[c][0][1]), fmaxf(sc[c][0][2], sc[c][0][3]));
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i)
+            for (int t = 1; t < 4; ++t) top = fmaxf(top, fmaxf(fmaxf(sc[c][t][0], sc[c][t][1]), fmaxf(sc[c][t][2], sc[c][t][3])));
+            float lower, upper;
+            swapped_pair<16>(top, lower, upper);
+            swapped_pair<32>(fmaxf(lower, upper), lower, upper);
+            const float m_new = fmaxf(m[c], fmaxf(lower, upper));
+            if (__any(m_new > m[c])) {
+                const float back = __builtin_amdgcn_exp2f(m[c] - m_new);
+                l[c] *= back;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[i][j] *= back;
-            m = m_new;
-        }
-        uint4 p[2];
+                for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            float e[8];
+                    for (int j = 0; j < 4; ++j) o[c][i][j] *= back;
+                m[c] = m_new;
+            }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(sc[2 * u + (j >> 2)][j & 3] - m);
-            l += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-            p[u] = half_pack<BF16>(e);
+            for (int u = 0; u < 2; ++u) {
+                float e[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(sc[c][2 * u + (j >> 2)][j & 3] - m[c]);
+                l[c] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+                p[c][u] = half_pack<BF16>(e);
+            }
         }
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
-            o[i] = half_mfma16<BF16>(half_from_codes<BF16>(vf[i].x, vf[i].y, value_scale), p[0], o[i]);
-            o[i] = half_mfma16<BF16>(half_from_codes<BF16>(vf[i].z, vf[i].w, value_scale), p[1], o[i]);
+            const uint4 lo = half_from_codes<BF16>(vf[i].x, vf[i].y, value_scale), hi = half_from_codes<BF16>(vf[i].z, vf[i].w, value_scale);
+#pragma unroll
+            for (int c = 0; c < SETS; ++c) o[c][i] = half_mfma16<BF16>(hi, p[c][1], half_mfma16<BF16>(lo, p[c][0], o[c][i]));
         }
         if (some_nan) {
             // NaN values were left out of the product: they are the end of the sums of the rows that see them
-            const int keys = limit - j0;
-            const uint64_t sees = keys >= 64 ? ~0ull : (keys <= 0 ? 0ull : (1ull << keys) - 1);
             __builtin_amdgcn_wave_barrier();                                  // (one wave's LDS operations take effect in order)
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i)
+            for (int c = 0; c < SETS; ++c) {
+                const int keys = limit[c] - j0;
+                const uint64_t sees = keys >= 64 ? ~0ull : (keys <= 0 ? 0ull : (1ull << keys) - 1);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (*reinterpret_cast<const uint64_t*>(nan_keys[wave][16 * i + 4 * g + j]) & sees) o[i][j] = __uint_as_float(0x7fc00000u);
+                for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (*reinterpret_cast<const uint64_t*>(nan_keys[wave][16 * i + 4 * g + j]) & sees) o[c][i][j] = __uint_as_float(0x7fc00000u);
+            }
             __builtin_amdgcn_wave_barrier();
         }
     };
@@ -192,23 +212,39 @@ __global__ __launch_bounds__(kThreads, 3) void paged_decode_kernel(const DecodeA
     if (j0 < end) start();
     // the queries, behind the first codes; rows that the tile does not have as zeros
     {
-        const int row = tid / (D / 8), d = 8 * (tid % (D / 8)), at = kRows * tile + row;
-        uint4 q = make_uint4(0, 0, 0, 0);
-        if (row < kRows && at < rows) q = *reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(s) * a.steps + at / group) * a.q_stride + (kvh * group + at % group) * D + d);
-        if constexpr (BF16) {
-            // queries so large that products with codes could pass the largest float, where the scaled score need not: a power of two off, on again behind
-            float v[8], top = 0.0f;
-            half_eight<true>(q, v);
+        constexpr int kChunks = D / 8, kAtOnce = kThreads / kChunks, kPasses = (kRows + kAtOnce - 1) / kAtOnce;
+        uint4 q[kPasses];
+        float top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
-            if (__syncthreads_or(top >= 0x1p60f)) {
-                late = 0x1p64f;
+        for (int i = 0; i < kPasses; ++i) {
+            const int row = tid / kChunks + kAtOnce * i, at = kRows * tile + row;
+            q[i] = make_uint4(0, 0, 0, 0);
+            if (row < kRows && at < rows)
+                q[i] = *reinterpret_cast<const uint4*>(a.q + (static_cast<size_t>(offset) + at / group) * a.q_stride + (kvh * group + at % group) * D + 8 * (tid % kChunks));
+            if constexpr (BF16) {
+                float v[8];
+                half_eight<true>(q[i], v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= 0x1p-64f;
-                q = half_pack<true>(v);
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(v[j]));
             }
         }
-        if (row < kRows) *reinterpret_cast<uint4*>(&queries[row][d]) = q;
+        // bf16 queries so large that products with codes could pass the largest float, where the scaled score need not: a power of two off, on again behind
+        if (BF16 && __syncthreads_or(top >= 0x1p60f)) {
+            late = 0x1p64f;
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) {
+                float v[8];
+                half_eight<true>(q[i], v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] *= 0x1p-64f;
+                q[i] = half_pack<true>(v);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const int row = tid / kChunks + kAtOnce * i;
+            if (row < kRows) *reinterpret_cast<uint4*>(&queries[row][8 * (tid % kChunks)]) = q[i];
+        }
     }
     __syncthreads();
     while (j0 < end) {
@@ -216,107 +252,146 @@ __global__ __launch_bounds__(kThreads, 3) void paged_decode_kernel(const DecodeA
         j0 += kStride;
         if (j0 < end) start();
     }
-    {
-        float x, y;
-        swapped_pair<16>(l, x, y);
-        swapped_pair<32>(x + y, x, y);
-        if (g == 0) stats[wave][col] = make_float2(m, x + y);
+    // the waves together, in their order, one set of rows after the other
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) *reinterpret_cast<v4f*>(&sums[wave][col * kPitch + 16 * i + 4 * g]) = o[i];
-    }
-    __syncthreads();
-    // the waves together, in their order
+    for (int c = 0; c < SETS; ++c) {
+        float lower, upper;
+        swapped_pair<16>(l[c], lower, upper);
+        swapped_pair<32>(lower + upper, lower, upper);
+        if (c > 0) __syncthreads();
+        if (g == 0) stats[wave][col] = make_float2(m[c], lower + upper);
 #pragma unroll
-    for (int i = 0; i < kRows * D / 4 / kThreads; ++i) {
-        const int e = tid + kThreads * i, c = e / (D / 4), d = 4 * (e % (D / 4)), row = kRows * tile + c;
-        if (row >= rows) continue;
-        float top = stats[0][c].x;
+        for (int i = 0; i < kTiles; ++i) *reinterpret_cast<v4f*>(&sums[wave][col * kPitch + 16 * i + 4 * g]) = o[c][i];
+        __syncthreads();
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, stats[w][c].x);
-        float den = 0.0f;
-        v4f total = zero;
+        for (int i = 0; i < 16 * D / 4 / kThreads; ++i) {
+            const int e = tid + kThreads * i, k = e / (D / 4), d = 4 * (e % (D / 4)), row = kRows * tile + 16 * c + k;
+            if (row >= rows) continue;
+            float top = stats[0][k].x;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f(stats[w][c].x - top);
-            den = __builtin_fmaf(stats[w][c].y, f, den);
-            const v4f part = *reinterpret_cast<const v4f*>(&sums[w][c * kPitch + d]);
+            for (int w = 1; w < kWaves; ++w) top = fmaxf(top, stats[w][k].x);
+            float den = 0.0f;
+            v4f total = zero;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) total[j] = __builtin_fmaf(part[j], f, total[j]);
-        }
-        if (a.sums) {
-            const size_t at = ((static_cast<size_t>(s) * a.kv_heads + kvh) * rows + row) * a.runs_bound + run;
-            *reinterpret_cast<v4f*>(a.sums + at * D + d) = total;
-            if (d == 0) a.stats[at] = make_float2(top, den);
-        } else {
-            const float inv = den == 0.0f ? 0.0f : 2.0f / den;                 // (twice: the values went in halved)
-            const size_t at = ((static_cast<size_t>(s) * a.steps + row / group) * a.heads + kvh * group + row % group) * D + d;
-            *reinterpret_cast<uint2*>(a.out + at) = make_uint2(half_pair<BF16>(total[0] * inv, total[1] * inv), half_pair<BF16>(total[2] * inv, total[3] * inv));
+            for (int w = 0; w < kWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f(stats[w][k].x - top);
+                den = __builtin_fmaf(stats[w][k].y, f, den);
+                const v4f part = *reinterpret_cast<const v4f*>(&sums[w][k * kPitch + d]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) total[j] = __builtin_fmaf(part[j], f, total[j]);
+            }
+            if (a.sums) {
+                const size_t at = ((static_cast<size_t>(s) * a.kv_heads + kvh) * a.part_rows + row) * a.runs_bound + run;
+                *reinterpret_cast<v4f*>(a.sums + at * D + d) = total;
+                if (d == 0) a.stats[at] = make_float2(top, den);
+            } else {
+                const float inv = den == 0.0f ? 0.0f : 2.0f / den;            // (twice: the values went in halved)
+                const size_t at = ((static_cast<size_t>(offset) + row / group) * a.heads + kvh * group + row % group) * D + d;
+                *reinterpret_cast<uint2*>(a.out + at) = make_uint2(half_pair<BF16>(total[0] * inv, total[1] * inv), half_pair<BF16>(total[2] * inv, total[3] * inv));
+            }
         }
     }
 }
 
-// A workgroup per query row: its runs together, an order that the number of runs fixes.  All of up to 64 runs are requested at once.
+// A workgroup per query row (where sequences have different numbers of rows, per 16th row): its runs together, an order that the number of runs fixes.
+// All of up to 64 runs are requested at once.
 template <bool BF16, int D>
-__global__ __launch_bounds__(kThreads) void paged_merge_kernel(const DecodeArgs a) {
+__global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedDecodeArgs a) {
     constexpr int kLanes = D / 4, kSlots = kThreads / kLanes, kBatch = 8;     // threads that share a run; runs side by side; of each of them at a time
     __shared__ float factors[256];
     __shared__ __align__(16) float sums[kSlots][D];
     __shared__ float red[2 * kWaves];
-    const int tid = threadIdx.x, group = a.heads / a.kv_heads, rows = a.steps * group;
-    const int index = blockIdx.x, row = index % rows, kvh = index / rows % a.kv_heads, s = index / rows / a.kv_heads;
+    const int tid = threadIdx.x, group = a.heads / a.kv_heads;
+    const int index0 = blockIdx.x * a.part_rows, kvh = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads;
+    const int offset = a.cu_steps ? paged_offset(a.cu_steps, s, 0, a.tokens) : s * a.steps;
+    const int64_t rows = static_cast<int64_t>(a.cu_steps ? paged_offset(a.cu_steps, s + 1, 0, a.tokens) - offset : a.steps) * group;
+    if (rows > a.part_rows) return;
     const int runs = max(1, paged_runs(paged_length(a.lengths[s], a.width, a.page_shift), a.kv_heads));     // (256 at most)
-    const float2* stats = a.stats + static_cast<size_t>(index) * a.runs_bound;
     const int slot = tid / kLanes, d = 4 * (tid % kLanes);
-    const float* part = a.sums + static_cast<size_t>(index) * a.runs_bound * D + d;
-    v4f first[kBatch];
+    for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+        const size_t index = static_cast<size_t>(index0) + row;
+        const float2* stats = a.stats + index * a.runs_bound;
+        const float* part = a.sums + index * a.runs_bound * D + d;
+        v4f first[kBatch];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) first[i] = *reinterpret_cast<const v4f*>(part + static_cast<size_t>(min(slot + kSlots * i, runs - 1)) * D);
-    const float2 mine = tid < runs ? stats[tid] : make_float2(-FLT_MAX, 0.0f);
-    float top = group_max<64>(mine.x);
-    if ((tid & 63) == 0) red[tid >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float factor = __builtin_amdgcn_exp2f(mine.x - top);
-    factors[tid] = factor;
-    float den = group_sum<64>(mine.y * factor);
-    if ((tid & 63) == 0) red[kWaves + (tid >> 6)] = den;
-    __syncthreads();
-    den = (red[kWaves] + red[kWaves + 1]) + (red[kWaves + 2] + red[kWaves + 3]);
-    v4f total = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int base = slot; base < runs; base += kSlots * kBatch) {
-        if (base != slot)
+        for (int i = 0; i < kBatch; ++i) first[i] = *reinterpret_cast<const v4f*>(part + static_cast<size_t>(min(slot + kSlots * i, runs - 1)) * D);
+        const float2 mine = tid < runs ? stats[tid] : make_float2(-FLT_MAX, 0.0f);
+        float top = group_max<64>(mine.x);
+        if ((tid & 63) == 0) red[tid >> 6] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const float factor = __builtin_amdgcn_exp2f(mine.x - top);
+        factors[tid] = factor;
+        float den = group_sum<64>(mine.y * factor);
+        if ((tid & 63) == 0) red[kWaves + (tid >> 6)] = den;
+        __syncthreads();
+        den = (red[kWaves] + red[kWaves + 1]) + (red[kWaves + 2] + red[kWaves + 3]);
+        v4f total = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int base = slot; base < runs; base += kSlots * kBatch) {
+            if (base != slot)
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) first[i] = *reinterpret_cast<const v4f*>(part + static_cast<size_t>(min(base + kSlots * i, runs - 1)) * D);
+                for (int i = 0; i < kBatch; ++i) first[i] = *reinterpret_cast<const v4f*>(part + static_cast<size_t>(min(base + kSlots * i, runs - 1)) * D);
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const float f = base + kSlots * i < runs ? factors[base + kSlots * i] : 0.0f;
-            if (base + kSlots * i < runs)
+            for (int i = 0; i < kBatch; ++i) {
+                const float f = base + kSlots * i < runs ? factors[base + kSlots * i] : 0.0f;
+                if (base + kSlots * i < runs)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) total[j] = __builtin_fmaf(first[i][j], f, total[j]);
+                    for (int j = 0; j < 4; ++j) total[j] = __builtin_fmaf(first[i][j], f, total[j]);
+            }
         }
-    }
-    *reinterpret_cast<v4f*>(&sums[slot][d]) = total;
-    __syncthreads();
-    if (tid >= D / 2) return;
-    float x = 0.0f, y = 0.0f;
+        *reinterpret_cast<v4f*>(&sums[slot][d]) = total;
+        __syncthreads();
+        if (tid < D / 2) {
+            float x = 0.0f, y = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kSlots; ++i) { x += sums[i][2 * tid]; y += sums[i][2 * tid + 1]; }
-    const float inv = den == 0.0f ? 0.0f : 2.0f / den;
-    *reinterpret_cast<uint32_t*>(a.out + ((static_cast<size_t>(s) * a.steps + row / group) * a.heads + kvh * group + row % group) * D + 2 * tid) = half_pair<BF16>(x * inv, y * inv);
+            for (int i = 0; i < kSlots; ++i) { x += sums[i][2 * tid]; y += sums[i][2 * tid + 1]; }
+            const float inv = den == 0.0f ? 0.0f : 2.0f / den;
+            *reinterpret_cast<uint32_t*>(a.out + ((static_cast<size_t>(offset) + row / group) * a.heads + kvh * group + row % group) * D + 2 * tid) = half_pair<BF16>(x * inv, y * inv);
+        }
+        if (row + gridDim.y < rows) __syncthreads();
+    }
 }
 
 template <bool BF16, int D>
-int launch(const DecodeArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_decode_kernel<BF16, D>), dim3(a.row_tiles * a.kv_heads, a.runs_bound, a.seqs), dim3(kThreads), 0, stream, a);
+int launch(const PagedDecodeArgs& a, hipStream_t stream) {
+    // Two sets of rows share what is read: eight sequences behind 20718 positions, four new tokens of eight heads each, 116 -> 96 us.  They cost a compute
+    // unit's third workgroup, so sequences that have one set get the other launch: 64 of one token of six heads behind up to 8000 positions, in a call
+    // that may hold more, 253 -> 201 us.
+    const int most = a.cu_steps ? std::min(a.part_rows, 16) : a.part_rows;
+    if (most <= 16) hipLaunchKernelGGL((paged_decode_kernel<BF16, D, 1>), dim3(a.kv_heads, a.runs_bound, a.seqs), dim3(kThreads), 0, stream, a, 1, most);
+    if (a.part_rows > 16)
+        hipLaunchKernelGGL((paged_decode_kernel<BF16, D, 2>), dim3((a.part_rows + 31) / 32 * a.kv_heads, a.runs_bound, a.seqs), dim3(kThreads), 0, stream, a, most < a.part_rows ? 17 : 1,
+                           a.part_rows);
     if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
     if (a.sums) {
-        hipLaunchKernelGGL((paged_merge_kernel<BF16, D>), dim3(a.seqs * a.steps * a.heads), dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((paged_merge_kernel<BF16, D>), dim3(a.seqs * a.kv_heads, a.cu_steps ? std::min(a.part_rows, 16) : a.part_rows), dim3(kThreads), 0, stream, a);
         if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
     }
     return PLLM_OK;
 }
 
 }  // namespace
+
+size_t paged_decode_parts_bytes(int64_t seqs, int64_t part_rows, int64_t kv_heads, int64_t head_dim, int64_t positions) {
+    const size_t runs = static_cast<size_t>(paged_runs_bound(positions, static_cast<int>(kv_heads)));
+    if (runs == 1) return 0;
+    const size_t parts = static_cast<size_t>(seqs) * part_rows * kv_heads * runs;
+    return align256(parts * head_dim * sizeof(float)) + align256(parts * sizeof(float2));
+}
+
+int paged_decode_launch(PagedDecodeArgs& a, void* workspace, bool bf16, int head_dim, hipStream_t stream) {
+    a.runs_bound = paged_runs_bound(static_cast<int64_t>(a.width) << a.page_shift, a.kv_heads);
+    a.sums = nullptr;
+    a.stats = nullptr;
+    if (a.runs_bound > 1) {
+        a.sums = static_cast<float*>(workspace);
+        a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) +
+                                            align256(static_cast<size_t>(a.seqs) * a.part_rows * a.kv_heads * a.runs_bound * head_dim * sizeof(float)));
+    }
+    if (head_dim == 128) return bf16 ? launch<true, 128>(a, stream) : launch<false, 128>(a, stream);
+    return bf16 ? launch<true, 64>(a, stream) : launch<false, 64>(a, stream);
+}
+
 }  // namespace pllm
 
 extern "C" {
@@ -325,10 +400,7 @@ size_t pllm_paged_attention_decode_workspace_bytes(int64_t seqs, int64_t steps, 
     if (seqs <= 0 || steps <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || positions <= 0 || seqs > 65535 || steps > 4096 || heads > 1024 || kv_heads > heads ||
         head_dim > 256)
         return 0;
-    const size_t runs = static_cast<size_t>(pllm::paged_runs_bound(positions, static_cast<int>(kv_heads)));
-    if (runs == 1) return 0;
-    const size_t parts = static_cast<size_t>(seqs) * steps * heads * runs;
-    return pllm::align256(parts * head_dim * sizeof(float)) + pllm::align256(parts * sizeof(float2));
+    return pllm::paged_decode_parts_bytes(seqs, steps * (heads / kv_heads), kv_heads, head_dim, positions);
 }
 
 int pllm_paged_attention_decode(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pages, const uint8_t* value_pages, const float* key_scales,
@@ -352,7 +424,7 @@ int pllm_paged_attention_decode(const void* q, int64_t q_stride, int dtype, cons
     const int64_t positions = table_width * page_tokens;
     const size_t need = pllm_paged_attention_decode_workspace_bytes(seqs, steps, heads, kv_heads, head_dim, positions);
     if (need > 0 && (!workspace || workspace_bytes < need)) return PLLM_ERR_WORKSPACE;
-    DecodeArgs a{};
+    PagedDecodeArgs a{};
     a.q = static_cast<const uint16_t*>(q); a.q_stride = static_cast<size_t>(q_stride);
     a.key_pages = key_pages; a.value_pages = value_pages; a.key_scales = key_scales; a.value_scales = value_scales;
     a.table = block_table; a.table_stride = static_cast<size_t>(table_stride); a.lengths = lengths;
@@ -361,15 +433,8 @@ int pllm_paged_attention_decode(const void* q, int64_t q_stride, int dtype, cons
     a.seqs = static_cast<int>(seqs); a.steps = static_cast<int>(steps); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
     a.page_shift = page_tokens == 16 ? 4 : page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7;
     a.pool = static_cast<int>(pool); a.width = static_cast<int>(table_width);
-    a.runs_bound = paged_runs_bound(positions, a.kv_heads);
-    a.row_tiles = (a.steps * (a.heads / a.kv_heads) + kRows - 1) / kRows;
-    if (need > 0) {
-        a.sums = static_cast<float*>(workspace);
-        a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + align256(static_cast<size_t>(seqs) * steps * heads * a.runs_bound * head_dim * sizeof(float)));
-    }
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (head_dim == 128) return dtype == PLLM_BF16 ? launch<true, 128>(a, st) : launch<false, 128>(a, st);
-    return dtype == PLLM_BF16 ? launch<true, 64>(a, st) : launch<false, 64>(a, st);
+    a.part_rows = static_cast<int>(steps * (heads / kv_heads));
+    return paged_decode_launch(a, workspace, dtype == PLLM_BF16, static_cast<int>(head_dim), static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

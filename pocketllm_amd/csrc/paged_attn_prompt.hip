@@ -1,7 +1,7 @@
 // Causal attention of many new tokens per sequence (prompts, their continuations, any mix of lengths) over a paged E4M3 cache that holds their keys
 // and values already: out = softmax(scale q K^T) V, every query up to its own position.
 //
-// A workgroup of four waves takes 128 query rows of one key/value head, a wave 32 of them; rows are tokens times the heads that share the
+// A workgroup of eight waves takes 256 query rows of one key/value head, a wave 32 of them; rows are tokens times the heads that share the
 // key/value head, so short prompts fill tiles too and keys are fetched once for the whole group.  64 keys at a time: their codes are requested one
 // tile ahead into registers, become 16-bit values there (exact) and go to LDS, double-buffered; every wave reads them from there as operands.  The
 // wave forms S^T = K Q^T (v_mfma_f32_32x32x16: matrix rows are keys, columns queries), so a lane holds half of one query's scores and what it leaves is,
@@ -10,8 +10,12 @@
 // values' scale (halved, so that fp16 holds every value that rounds up from its largest) into the conversion.
 // 16-byte pieces of a row lie permuted in LDS (key rows by row % 16, value rows by row / 2 % 8), so 16 neighbouring rows read at one piece meet no
 // bank twice.  Rows behind the last sequence get zeros.
+//
+// Bound: 4 D operations per row and key.  8192 tokens of 48 and 8 heads, 825 G operations: 800 us, 1030 T/s, where a large matrix product of the library
+// reaches 1155; what is between is the softmax's vector instructions (44 % of the cycles, the matrix unit 42 %: the two waves of a SIMD overlap them in
+// part) and the barrier of each tile.
+#include "paged_attention.h"
 #include "paged_device.h"
-#include "pllm_internal.h"
 
 #include <algorithm>
 #include <cfloat>
@@ -32,17 +36,28 @@ struct PagedPromptArgs {
     uint16_t* out;
     float* sums; float2* stats;                 // of several runs of a block's keys: [runs][tokens * heads][D], maximum (base 2) and sum of weights; or null
     float scale;                                // base 2
+    int few_rows;                               // sequences of so many query rows or fewer are another kernel's
     int runs, tokens, seqs, heads, kv_heads, page_shift, pool, width, slots;
 };
+
+// sum of the lanes up to this one
+__device__ __forceinline__ int lanes_until(int x) {
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+        const int before = __shfl_up(x, i);
+        if ((threadIdx.x & 63) >= i) x += before;
+    }
+    return x;
+}
 
 // The block of query rows that index `index` of the grid is: sequence s (a.seqs: the rows behind the last one), rows row0 .. row0 + kBlockRows - 1 of it.
 // Those with the most keys come first, so that what is left at the end is short (48 and 8 heads: 30 continuations of up to 200 tokens behind up to 4000
 // 267 -> 215 us, 12 of up to 300 behind up to 16000 809 -> 693; where a sequence's own order is as good already, four prompts of up to 2000 tokens, 117 -> 123); of
-// more than 63 sequences only each one's own blocks are in that order, by slots.
+// more than 63 sequences only each one's own blocks are in that order.
 __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, int group, int& s, int& row0) {
     const int lane = threadIdx.x & 63;
     if (a.seqs == 1) {                                                        // (1024 tokens of 48 and 8 heads: 42.0 -> 40.5 us)
-        const int n = paged_offset(a.cu_steps, 1, 0, a.tokens), blocks = (n * group + kBlockRows - 1) / kBlockRows;
+        const int n = paged_offset(a.cu_steps, 1, 0, a.tokens), blocks = n * group > a.few_rows ? (n * group + kBlockRows - 1) / kBlockRows : 0;
         s = index < blocks ? 0 : 1;
         row0 = (index < blocks ? blocks - 1 - index : index - blocks) * kBlockRows;
         return row0 < (s ? a.tokens - n : n) * group;
@@ -53,7 +68,7 @@ __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, 
             const int offset = paged_offset(a.cu_steps, lane, 0, a.tokens);
             const int n = max((lane == a.seqs ? a.tokens : paged_offset(a.cu_steps, lane + 1, 0, a.tokens)) - offset, 0);
             keys = lane == a.seqs || n == 0 ? 0 : paged_length(a.lengths[lane], a.width, a.page_shift);
-            rows = n * group;
+            rows = lane < a.seqs && n * group <= a.few_rows ? 0 : n * group;
             first = keys - n;
         }
         // (counts stay far below 2^24)
@@ -67,33 +82,29 @@ __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, 
             else high = middle - 1;
         }
         const int mine = seeing(low) - seeing(low + 1), place = index - all(seeing(low + 1));
-        int until = mine;                                                     // blocks of this length of the sequences up to the lane's
-#pragma unroll
-        for (int i = 1; i < 64; i *= 2) {
-            const int before = __shfl_up(until, i);
-            if (lane >= i) until += before;
-        }
+        const int until = lanes_until(mine);                                  // blocks of this length of the sequences up to the lane's
         const uint64_t behind = __ballot(until > place);
         s = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(behind)) - 1);
         const int block = (rows + kBlockRows - 1) / kBlockRows - seeing(low) + place - (until - mine);
         row0 = __builtin_amdgcn_readlane(block, s) * kBlockRows;
         return true;
     }
-    const int64_t slot = a.slots - 1 - static_cast<int64_t>(index);
-    int owners = 0;
+    int place = index;
     for (int base = 0; base <= a.seqs; base += 64) {
         const int c = base + lane;
-        const bool begun = c <= a.seqs && paged_first_slot(static_cast<int64_t>(paged_offset(a.cu_steps, c, 0, a.tokens)) * group, c, kBlockRows, 1) <= slot;
-        const int n = __popcll(__ballot(begun));
-        owners += n;
-        if (n < 64) break;
+        int rows = 0;
+        if (c <= a.seqs) rows = max((c == a.seqs ? a.tokens : paged_offset(a.cu_steps, c + 1, 0, a.tokens)) - paged_offset(a.cu_steps, c, 0, a.tokens), 0) * group;
+        const int blocks = c < a.seqs && rows <= a.few_rows ? 0 : (rows + kBlockRows - 1) / kBlockRows, until = lanes_until(blocks);
+        const uint64_t behind = __ballot(until > place);
+        if (behind) {
+            const int owner = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(behind)) - 1);
+            s = base + owner;
+            row0 = __builtin_amdgcn_readlane(until - 1 - place, owner) * kBlockRows;
+            return true;
+        }
+        place -= __builtin_amdgcn_readlane(until, 63);
     }
-    s = __builtin_amdgcn_readfirstlane(max(owners - 1, 0));
-    const int offset = paged_offset(a.cu_steps, s, 0, a.tokens), n = (s == a.seqs ? a.tokens : paged_offset(a.cu_steps, s + 1, 0, a.tokens)) - offset;
-    const int64_t row = (slot - paged_first_slot(static_cast<int64_t>(offset) * group, s, kBlockRows, 1)) * kBlockRows;
-    if (n <= 0 || row < 0 || row >= static_cast<int64_t>(n) * group) return false;
-    row0 = static_cast<int>(row);
-    return true;
+    return false;
 }
 
 template <bool BF16, int D, bool RUNS>
@@ -453,6 +464,10 @@ __global__ __launch_bounds__(256) void paged_prompt_merge_kernel(const PagedProm
     const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads, row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= rows) return;
+    if (a.few_rows > 0) {                                                     // rows without runs are the other kernel's
+        const int s = paged_sequence(a.cu_steps, a.tokens, a.seqs + 1, 1, 0, row / a.heads);
+        if (s < a.seqs && (paged_offset(a.cu_steps, s + 1, 0, a.tokens) - paged_offset(a.cu_steps, s, 0, a.tokens)) * (a.heads / a.kv_heads) <= a.few_rows) return;
+    }
     const float2 mine = lane < a.runs ? a.stats[lane * rows + row] : make_float2(-FLT_MAX, 0.0f);           // (at most 64 runs)
     const float top = group_max<64>(mine.x), factor = __builtin_amdgcn_exp2f(mine.x - top), den = group_sum<64>(mine.y * factor);
     float total[kPer] = {};
@@ -494,11 +509,36 @@ int launch(const PagedPromptArgs& a, hipStream_t stream) {
 }
 
 // Runs that the keys of every block of query rows are cut in: as many as give every compute unit a workgroup when there are few rows before a
-// long context, none of them shorter than 16 tiles of a sequence that fills the table.
+// long context, none of them shorter than 8 tiles of a sequence that fills the table.
 int prompt_runs(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t positions) {
     const int64_t blocks = (tokens * (heads / kv_heads) + kBlockRows - 1) / kBlockRows * kv_heads;
-    const int64_t runs = std::min(std::min(compute_units() / blocks, positions / (16 * kTile)), int64_t{64});
+    const int64_t runs = std::min(std::min(compute_units() / blocks, positions / (8 * kTile)), int64_t{64});
     return static_cast<int>(std::max(runs, int64_t{1}));
+}
+
+// Query rows up to which a sequence goes to the kernel of the decode steps, whose tiles have 16 or 32 rows where these have 256, and which cuts every
+// sequence's keys by its own length (48 and 8 heads: 64 single tokens behind up to 8000 positions 434 -> 150 us, 142 times one or two behind up to 3000
+// 377 -> 173; 64 and 8 heads, 8 times 8 tokens behind up to 8000 86 -> 54).  Its launches cost a few microseconds where no sequence is so short (30
+// continuations of up to 200 tokens behind up to 4000 209 -> 215 us, six prompts 319 -> 323): 16 rows or one token's, unless most
+// sequences must be short.  Only where tables are wider than one run of it; of one sequence by the rows of the call, so that one kernel's launches are enough; not
+// where what the rows would keep between two launches passes a gigabyte.
+int few_rows(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
+    const int64_t group = heads / kv_heads, all = tokens * group;
+    if (positions <= kPagedOneRun || (seqs == 1 && all > kPagedFewRows)) return 0;
+    int64_t rows = std::min<int64_t>(all <= 2 * kPagedFewRows * seqs ? kPagedFewRows : std::min<int64_t>(std::max<int64_t>(group, 16), kPagedFewRows), all);
+    while (rows > 0 && paged_decode_parts_bytes(seqs, rows, kv_heads, head_dim, positions) > (size_t{1} << 30)) rows /= 2;
+    return static_cast<int>(rows);
+}
+
+struct Parts { int runs, few; size_t run_bytes, few_bytes; };
+Parts parts_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
+    Parts p{};
+    p.few = few_rows(tokens, seqs, heads, kv_heads, head_dim, positions);
+    p.few_bytes = p.few > 0 ? paged_decode_parts_bytes(seqs, p.few, kv_heads, head_dim, positions) : 0;
+    p.runs = tokens * (heads / kv_heads) <= p.few ? 1 : prompt_runs(tokens, heads, kv_heads, positions);
+    const size_t parts = static_cast<size_t>(p.runs) * tokens * heads;
+    p.run_bytes = p.runs > 1 ? align256(parts * head_dim * sizeof(float)) + align256(parts * sizeof(float2)) : 0;
+    return p;
 }
 
 }  // namespace
@@ -506,12 +546,11 @@ int prompt_runs(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t positio
 
 extern "C" {
 
-size_t pllm_paged_attention_prompt_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
-    if (tokens <= 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0 || positions <= 0 || tokens > 0x3fffff || heads > 1024 || head_dim > 256) return 0;
-    const int runs = pllm::prompt_runs(tokens, heads, kv_heads, positions);
-    if (runs == 1) return 0;
-    const size_t parts = static_cast<size_t>(runs) * tokens * heads;
-    return pllm::align256(parts * head_dim * sizeof(float)) + pllm::align256(parts * sizeof(float2));
+size_t pllm_paged_attention_prompt_workspace_bytes(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
+    if (tokens <= 0 || seqs <= 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0 || positions <= 0 || tokens > 0x3fffff || seqs > 0xffff || heads > 1024 || head_dim > 256)
+        return 0;
+    const pllm::Parts p = pllm::parts_of(tokens, seqs, heads, kv_heads, head_dim, positions);
+    return p.run_bytes + p.few_bytes;
 }
 
 int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pages, const uint8_t* value_pages,
@@ -528,7 +567,9 @@ int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int dtype, cons
     if ((head_dim != 64 && head_dim != 128) || (page_tokens != 16 && page_tokens != 32 && page_tokens != 64 && page_tokens != 128)) return PLLM_ERR_UNSUPPORTED;
     // pages, positions and rows in 32 bits
     if (tokens > 0x3fffff || seqs > 0xffff || heads > 1024 || pool > 0x7fffffff || table_width > 0x3fffffff / page_tokens) return PLLM_ERR_UNSUPPORTED;
-    const int64_t rows = tokens * (heads / kv_heads), slots = paged_slots(rows, static_cast<int>(seqs) + 1, kBlockRows, 1);
+    const Parts parts = parts_of(tokens, seqs, heads, kv_heads, head_dim, table_width * page_tokens);
+    // blocks of all sequences: whole ones, and a last one of every sequence that can have any and of the rows behind the last
+    const int64_t rows = tokens * (heads / kv_heads), slots = rows / kBlockRows + std::min(seqs, rows / (parts.few + 1)) + 1;
     if (rows > 0x3fffffff || slots > 0xffff) return PLLM_ERR_UNSUPPORTED;
     const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) | reinterpret_cast<uintptr_t>(out) |
                            reinterpret_cast<uintptr_t>(workspace);
@@ -545,15 +586,23 @@ int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int dtype, cons
     a.page_shift = page_tokens == 16 ? 4 : page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7;
     a.pool = static_cast<int>(pool); a.width = static_cast<int>(table_width);
     a.slots = static_cast<int>(slots);
-    a.runs = prompt_runs(tokens, heads, kv_heads, table_width * page_tokens);
+    if (parts.run_bytes + parts.few_bytes > 0 && (!workspace || workspace_bytes < parts.run_bytes + parts.few_bytes)) return PLLM_ERR_WORKSPACE;
+    a.runs = parts.runs;
+    a.few_rows = parts.few;
     if (a.runs > 1) {
-        if (!workspace || workspace_bytes < pllm_paged_attention_prompt_workspace_bytes(tokens, heads, kv_heads, head_dim, table_width * page_tokens)) return PLLM_ERR_WORKSPACE;
         a.sums = static_cast<float*>(workspace);
         a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + align256(static_cast<size_t>(a.runs) * tokens * heads * head_dim * sizeof(float)));
     }
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (head_dim == 128) return dtype == PLLM_BF16 ? launch<true, 128>(a, st) : launch<false, 128>(a, st);
-    return dtype == PLLM_BF16 ? launch<true, 64>(a, st) : launch<false, 64>(a, st);
+    const bool bf16 = dtype == PLLM_BF16;
+    const int status = head_dim == 128 ? (bf16 ? launch<true, 128>(a, st) : launch<false, 128>(a, st)) : (bf16 ? launch<true, 64>(a, st) : launch<false, 64>(a, st));
+    if (status != PLLM_OK || a.few_rows == 0) return status;
+    PagedDecodeArgs d{};
+    d.q = a.q; d.q_stride = a.q_stride; d.key_pages = key_pages; d.value_pages = value_pages; d.key_scales = key_scales; d.value_scales = value_scales;
+    d.table = a.table; d.table_stride = a.table_stride; d.lengths = lengths; d.cu_steps = cu_steps; d.out = a.out; d.scale = a.scale;
+    d.seqs = a.seqs; d.tokens = a.tokens; d.heads = a.heads; d.kv_heads = a.kv_heads; d.page_shift = a.page_shift; d.pool = a.pool; d.width = a.width;
+    d.part_rows = a.few_rows;
+    return paged_decode_launch(d, static_cast<unsigned char*>(workspace) + parts.run_bytes, bf16, static_cast<int>(head_dim), st);
 }
 
 }  // extern "C"

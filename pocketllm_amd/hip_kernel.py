@@ -780,9 +780,9 @@ def paged_attention_prompt_forward(q: torch.Tensor, key_pages: torch.Tensor, val
                                    block_table: torch.Tensor, lengths: torch.Tensor, cu_steps: torch.Tensor, *, scale: float | None = None) -> torch.Tensor:
     """paged_attention_decode_forward for many new tokens per sequence (prompts, with or without a past, any mix of lengths): q
     [tokens, heads * head_dim], the tokens of sequence s in rows cu_steps[s] .. cu_steps[s + 1] - 1 (int32 [seqs + 1], from 0 on).  Rows behind the last sequence
-    are zeros.  Few rows before a wide table have its keys cut in runs that meet in a second launch: how many goes by
-    tokens, heads and the table's width, so the last bits of a sequence's outputs may differ between calls of other sizes.  Sequences of one or a few new
-    tokens behind a long past are the decode form's work."""
+    are zeros.  The keys of few rows before a wide table are cut in runs that meet in a second launch, and sequences of very few rows (decode steps in a
+    batch with prompts) go through the decode form's kernel: by the numbers of tokens, sequences and heads and the table's width, never by what they hold, so
+    the last bits of a sequence's outputs may differ between calls of other sizes."""
     what = "paged_attention_prompt"
     out = _bindings.paged_attention_prompt("paged_attention_prompt_forward", q, key_pages, value_pages, key_scales, value_scales, block_table, lengths, cu_steps, scale)
     if out is not None:
@@ -798,7 +798,7 @@ def paged_attention_prompt_forward(q: torch.Tensor, key_pages: torch.Tensor, val
     out = torch.empty(tokens, width, dtype=q.dtype, device=q.device)
     rows = _rows16(q)
     lib = _lib()
-    need = lib.pllm_paged_attention_prompt_workspace_bytes(tokens, width // dim, kv_heads, dim, block_table.size(1) * page)
+    need = lib.pllm_paged_attention_prompt_workspace_bytes(tokens, seqs, width // dim, kv_heads, dim, block_table.size(1) * page)
     with _on_device(q.device):
         ws = _workspace(need, q.device) if need else None
         st = lib.pllm_paged_attention_prompt(rows.data_ptr(), rows.stride(0), _DTYPE_CODE[q.dtype], key_pages.data_ptr(), value_pages.data_ptr(),

@@ -211,9 +211,12 @@ def test_c_entries_refuse_before_anything_is_launched():
     assert need >= 2 * 4 * 10 * 66 * 4 and decode(width=300, table_stride=300, ws=at, need=need - 1) == workspace
     assert lib.pllm_paged_attention_decode_workspace_bytes(2, 1, 4, 2, 64, 1024) == 0 and lib.pllm_paged_attention_decode_workspace_bytes(-1, 1, 4, 2, 64, 256) == 0
     assert prompt(width=200, table_stride=200) == workspace
-    need = lib.pllm_paged_attention_prompt_workspace_bytes(5, 4, 2, 64, 3200)
-    assert need >= 3 * 5 * 4 * 66 * 4 and prompt(width=200, table_stride=200, ws=at, need=need - 1) == workspace
-    assert lib.pllm_paged_attention_prompt_workspace_bytes(5, 4, 2, 64, 1024) == 0 and lib.pllm_paged_attention_prompt_workspace_bytes(100000, 4, 2, 64, 10**6) == 0
+    need = lib.pllm_paged_attention_prompt_workspace_bytes(5, 2, 4, 2, 64, 3200)
+    assert need >= 2 * 10 * 2 * 7 * 66 * 4 and prompt(width=200, table_stride=200, ws=at, need=need - 1) == workspace
+    assert lib.pllm_paged_attention_prompt_workspace_bytes(5, 2, 4, 2, 64, 511) == 0 and lib.pllm_paged_attention_prompt_workspace_bytes(100000, 1, 4, 2, 64, 10**6) == 0
+    # what sequences of few rows keep between two launches stays below a gigabyte, whatever the batch
+    for seqs, kv, positions in ((1, 8, 10**6), (64, 8, 131072), (2000, 8, 131072), (65535, 1, 10**6), (300, 64, 40000)):
+        assert lib.pllm_paged_attention_prompt_workspace_bytes(100000, seqs, 2 * kv, kv, 128, positions) <= 2**30 + 512
     for kw in (dict(k=None), dict(v=None), dict(q=None), dict(q_out=None), dict(dtype=0), dict(rows=0), dict(seqs=0), dict(kv=0), dict(heads=0), dict(pool=0), dict(width=0),
                dict(table_stride=1), dict(cu=None), dict(k_stride=127), dict(v_stride=120), dict(q_stride=200), dict(rope=-16), dict(rope=80), dict(cos=None), dict(sin=None),
                dict(positions=47), dict(k=at + 8), dict(cos=at + 4), dict(k_stride=132), dict(lengths=at + 1)):
