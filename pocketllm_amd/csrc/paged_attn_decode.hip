@@ -9,14 +9,17 @@
 // values are 16 neighbouring bytes of a value page.  16 neighbouring keys share a page, so a lane needs one page number for its keys' rows, one for
 // its values and two scales, whatever the page size.  Codes become 16-bit values in registers: E4M3 is exact in both types; the keys' scale goes on the
 // scores, the values' scale (halved, so that fp16 holds every value that rounds up from its largest) into the conversion, both exact.
-// Bound: bytes, 2 * length * D codes per head, once for each 16 or 32 rows, and the latency of a wave's next 64 keys, whose codes are only requested when
-// the last ones are done with: three workgroups of a compute unit cover it in part.  64 sequences of 1 to 8192 positions, 567 MB: 136 us, 4.2 TB/s, where a
-// kernel that only reads reaches 6.
+// The next 64 keys' codes are requested as soon as the registers of the last ones are free, the keys' before the softmax and the values' behind their
+// product, and page numbers a step ahead of them (64 sequences 139 -> 122 us, one of 100001 positions 49 -> 44; all at the end of the step before).
+// Bound: bytes, 2 * length * D codes per head, once for each 16 or 32 rows.  64 sequences of 1 to 8192 positions, 567 MB: 121 us, 4.7 TB/s, where a kernel
+// that only reads reaches 6: runs of 512 keys, which one sequence needs to fill the machine, begin and end too often (of 1024: 119 us, but 2048 positions
+// of one sequence 13.2 for 10.4).
 #include "paged_attention.h"
 #include "paged_device.h"
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 namespace pllm {
 namespace {
@@ -30,7 +33,7 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
     constexpr int kPieces = D / 64;             // 16-byte pieces of a key row per lane
     constexpr int kTiles = D / 16;              // output tiles
     constexpr int kPitch = D + 4;
-    constexpr int kRows = 16 * SETS;
+    constexpr int kRows = 16 * SETS, kStride = kStep * kWaves;
     __shared__ __align__(16) float sums[kWaves][16 * kPitch];
     __shared__ float2 stats[kWaves][16];
     __shared__ __align__(16) uint16_t queries[kRows][D + 8];                  // (in registers they cost the third workgroup of a compute unit)
@@ -70,15 +73,18 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
         l[c] = 0.0f;
     }
     const size_t head_bytes = static_cast<size_t>(D) << a.page_shift, page_mask = (size_t{1} << a.page_shift) - 1;
-    // page numbers of the lane's key rows (chunk col / 4 of the step) and of its values and scales (chunk g)
+    // page numbers of the lane's key rows (chunk col / 4 of the step) and of its values and scales (chunk g), as the table has them: checked where they are
+    // used, a step later, so that nothing waits for them here
     auto pages = [&](int j0, int& key_page, int& value_page) {
-        key_page = paged_page(table, min(j0 + 16 * (col >> 2), length - 1), a.width, a.page_shift, a.pool);
-        value_page = j0 + 16 * g < length ? paged_page(table, j0 + 16 * g, a.width, a.page_shift, a.pool) : -1;
+        key_page = table[min(j0 + 16 * (col >> 2), length - 1) >> a.page_shift];
+        value_page = table[min(j0 + 16 * g, length - 1) >> a.page_shift];
     };
+    auto checked = [&](int page) { return page >= 0 && page < a.pool ? page : -1; };
     struct Step { uint4 keys[4][kPieces], values[kTiles]; float key_scale, value_scale; bool here; };
-    auto request = [&](Step& x, int j0, int key_page, int value_page) {
+    auto request_keys = [&](Step& x, int j0, int key_page, int value_page) {
+        key_page = checked(key_page);
+        value_page = j0 + 16 * g < length ? checked(value_page) : -1;
         const size_t key_at = (static_cast<size_t>(max(key_page, 0)) * a.kv_heads + kvh) * head_bytes + ((j0 + 16 * (col >> 2)) & page_mask) * D;
-        const size_t value_at = (static_cast<size_t>(max(value_page, 0)) * a.kv_heads + kvh) * head_bytes + ((j0 + 16 * g) & page_mask) + (static_cast<uint32_t>(col) << a.page_shift);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -87,10 +93,16 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
         x.key_scale = a.key_scales[scale_at];
         x.value_scale = a.value_scales[scale_at];
         x.here = value_page >= 0;
+    };
+    auto request_values = [&](Step& x, int j0, int value_page) {
+        const size_t value_at = (static_cast<size_t>(max(checked(value_page), 0)) * a.kv_heads + kvh) * head_bytes + ((j0 + 16 * g) & page_mask) + (static_cast<uint32_t>(col) << a.page_shift);
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) x.values[i] = *reinterpret_cast<const uint4*>(a.value_pages + value_at + (static_cast<size_t>(16 * i) << a.page_shift));
     };
-    auto work = [&](Step& x, int j0) {
+    int key_page = 0, value_page = 0;           // of the next step to request
+    // a step; with MORE the next one's keys are requested as soon as this one's are used, its values likewise
+    auto work = [&](auto more, Step& x, int j0) {
+        constexpr bool MORE = decltype(more)::value;
         auto& kf = x.keys;
         auto& vf = x.values;
         const float key_factor = x.key_scale * a.scale, value_scale = x.here ? 0.5f * x.value_scale : 1.0f;
@@ -151,6 +163,11 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
                     vf[i].x = without_nan(vf[i].x); vf[i].y = without_nan(vf[i].y); vf[i].z = without_nan(vf[i].z); vf[i].w = without_nan(vf[i].w);
                 }
         }
+        const int next_page = value_page;
+        if constexpr (MORE) {
+            request_keys(x, j0 + kStride, key_page, value_page);
+            pages(j0 + 2 * kStride, key_page, value_page);                    // (before the values: loads arrive in order)
+        }
         uint4 p[SETS][2];
 #pragma unroll
         for (int c = 0; c < SETS; ++c) {
@@ -185,6 +202,7 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
 #pragma unroll
             for (int c = 0; c < SETS; ++c) o[c][i] = half_mfma16<BF16>(hi, p[c][1], half_mfma16<BF16>(lo, p[c][0], o[c][i]));
         }
+        if constexpr (MORE) request_values(x, j0 + kStride, next_page);
         if (some_nan) {
             // NaN values were left out of the product: they are the end of the sums of the rows that see them
             __builtin_amdgcn_wave_barrier();                                  // (one wave's LDS operations take effect in order)
@@ -201,15 +219,15 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
             __builtin_amdgcn_wave_barrier();
         }
     };
-    constexpr int kStride = kStep * kWaves;
     int j0 = begin + kStep * wave;
     Step x;
-    auto start = [&]() {
-        int key_page, value_page;
+    if (j0 < end) {
         pages(j0, key_page, value_page);
-        request(x, j0, key_page, value_page);
-    };
-    if (j0 < end) start();
+        const int page = value_page;
+        request_keys(x, j0, key_page, page);
+        pages(j0 + kStride, key_page, value_page);
+        request_values(x, j0, page);
+    }
     // the queries, behind the first codes; rows that the tile does not have as zeros
     {
         constexpr int kChunks = D / 8, kAtOnce = kThreads / kChunks, kPasses = (kRows + kAtOnce - 1) / kAtOnce;
@@ -247,11 +265,8 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
         }
     }
     __syncthreads();
-    while (j0 < end) {
-        work(x, j0);
-        j0 += kStride;
-        if (j0 < end) start();
-    }
+    for (; j0 + kStride < end; j0 += kStride) work(std::true_type{}, x, j0);
+    if (j0 < end) work(std::false_type{}, x, j0);
     // the waves together, in their order, one set of rows after the other
 #pragma unroll
     for (int c = 0; c < SETS; ++c) {
