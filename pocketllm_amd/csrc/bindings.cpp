@@ -467,7 +467,7 @@ PyObject* paged_attention_decode(PyObject*, PyObject* const* a, Py_ssize_t nargs
     const int64_t seqs = q->size(0), steps = q->dim() == 3 ? q->size(1) : 1, width = q->size(-1);
     if (seqs != p.seqs || width % p.dim || (width / p.dim) % p.kv_heads) Py_RETURN_NONE;
     float scale = 1.0f / std::sqrt(static_cast<float>(p.dim));
-    if (a[8] != Py_None && (!float_arg(a[8], scale) || !(scale >= 0.0f && std::isfinite(scale)))) Py_RETURN_NONE;
+    if (a[8] != Py_None && (!float_arg(a[8], scale) || !(scale >= 0.0f && scale <= 0x1p127f))) Py_RETURN_NONE;
     const int64_t heads = width / p.dim;
     Tensor out = at::empty(q->sizes(), q->options()), ws;
     const size_t bytes = pllm_paged_attention_decode_workspace_bytes(seqs, steps, heads, p.kv_heads, p.dim, p.width * p.page);
@@ -490,7 +490,7 @@ PyObject* paged_attention_prompt(PyObject*, PyObject* const* a, Py_ssize_t nargs
     const int64_t tokens = q->size(0), width = q->size(1), heads = width / p.dim;
     if (width % p.dim || heads % p.kv_heads) Py_RETURN_NONE;
     float scale = 1.0f / std::sqrt(static_cast<float>(p.dim));
-    if (a[9] != Py_None && (!float_arg(a[9], scale) || !(scale >= 0.0f && std::isfinite(scale)))) Py_RETURN_NONE;
+    if (a[9] != Py_None && (!float_arg(a[9], scale) || !(scale >= 0.0f && scale <= 0x1p127f))) Py_RETURN_NONE;
     Tensor out = at::empty(q->sizes(), q->options()), ws;
     const size_t bytes = pllm_paged_attention_prompt_workspace_bytes(tokens, p.seqs, heads, p.kv_heads, p.dim, p.width * p.page);
     if (bytes) ws = workspace(*q, bytes);

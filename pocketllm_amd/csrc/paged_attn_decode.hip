@@ -426,7 +426,7 @@ int pllm_paged_attention_decode(const void* q, int64_t q_stride, int dtype, cons
     if (!q || !key_pages || !value_pages || !key_scales || !value_scales || !block_table || !lengths || !out) return PLLM_ERR_INVALID_ARGUMENT;
     if (dtype != PLLM_F16 && dtype != PLLM_BF16) return PLLM_ERR_INVALID_ARGUMENT;
     if (seqs <= 0 || steps <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || pool <= 0 || table_width <= 0 || table_stride < table_width ||
-        q_stride < heads * head_dim || !(scale >= 0.0f && scale <= FLT_MAX))
+        q_stride < heads * head_dim || !(scale >= 0.0f && scale <= 0x1p127f))
         return PLLM_ERR_INVALID_ARGUMENT;
     if ((head_dim != 64 && head_dim != 128) || (page_tokens != 16 && page_tokens != 32 && page_tokens != 64 && page_tokens != 128)) return PLLM_ERR_UNSUPPORTED;
     // pages and positions in 32 bits, one grid row per head and sequence

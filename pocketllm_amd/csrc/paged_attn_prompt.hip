@@ -524,10 +524,10 @@ int prompt_runs(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t positio
 // where what the rows would keep between two launches passes a gigabyte.
 int few_rows(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
     const int64_t group = heads / kv_heads, all = tokens * group;
-    if (positions <= kPagedOneRun || (seqs == 1 && all > kPagedFewRows)) return 0;
+    if (positions <= kPagedOneRun || group > kPagedFewRows || (seqs == 1 && all > kPagedFewRows)) return 0;
     int64_t rows = std::min<int64_t>(all <= 2 * kPagedFewRows * seqs ? kPagedFewRows : std::min<int64_t>(std::max<int64_t>(group, 16), kPagedFewRows), all);
     while (rows > 0 && paged_decode_parts_bytes(seqs, rows, kv_heads, head_dim, positions) > (size_t{1} << 30)) rows /= 2;
-    return static_cast<int>(rows);
+    return rows < group ? 0 : static_cast<int>(rows);
 }
 
 struct Parts { int runs, few; size_t run_bytes, few_bytes; };
@@ -562,7 +562,7 @@ int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int dtype, cons
     if (!q || !key_pages || !value_pages || !key_scales || !value_scales || !block_table || !lengths || !cu_steps || !out) return PLLM_ERR_INVALID_ARGUMENT;
     if (dtype != PLLM_F16 && dtype != PLLM_BF16) return PLLM_ERR_INVALID_ARGUMENT;
     if (tokens <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || pool <= 0 || table_width <= 0 || table_stride < table_width ||
-        q_stride < heads * head_dim || !(scale >= 0.0f && scale <= FLT_MAX))
+        q_stride < heads * head_dim || !(scale >= 0.0f && scale <= 0x1p127f))
         return PLLM_ERR_INVALID_ARGUMENT;
     if ((head_dim != 64 && head_dim != 128) || (page_tokens != 16 && page_tokens != 32 && page_tokens != 64 && page_tokens != 128)) return PLLM_ERR_UNSUPPORTED;
     // pages, positions and rows in 32 bits

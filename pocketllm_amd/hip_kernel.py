@@ -698,7 +698,8 @@ def paged_kv_append_forward(q: torch.Tensor | None, k_new: torch.Tensor, v_new: 
     [pool, kv_heads], block_table int32 [seqs, pages]: written in place.  cos_table / sin_table float32 [positions, head_dim] as RotaryTable keeps them, rows for
     every position that the table can name; rope_dim a multiple of 16.
     The scale of a page and head is the least power of two with amax / scale <= 448; when it has to grow, the page's older codes are scaled
-    down with it.  Rows without a position in the table store nothing, their queries leave as zeros.  No two sequences may write into one page."""
+    down with it.  Rows without a position in the table store nothing, their queries leave as zeros.  What a call writes has one
+    page of its own for each part of a sequence: no page stands twice among the entries that new tokens go to (pages that are only read may be shared)."""
     what = "paged_kv_append"
     made = _bindings.paged_kv_append("paged_kv_append_forward", q, k_new, v_new, key_pages, value_pages, key_scales, value_scales, block_table, lengths, cu_steps,
                                      cos_table, sin_table, rope_dim)
@@ -756,7 +757,7 @@ def paged_attention_decode_forward(q: torch.Tensor, key_pages: torch.Tensor, val
     pool, kv_heads, page, dim = _paged_cache(what, q, key_pages, value_pages, key_scales, value_scales, block_table, lengths)
     seqs, steps, width = q.size(0), q.size(1) if q.dim() == 3 else 1, q.size(-1)
     _check(seqs == block_table.size(0), f"{what}: q and block_table must have the same sequences")
-    _check(scale is None or 0.0 <= float(scale) < float("inf"), f"{what}: scale must be finite and not negative")
+    _check(scale is None or 0.0 <= float(scale) <= 2.0 ** 127, f"{what}: scale must be from 0 to 2 ** 127")
     _check(width % dim == 0 and width > 0 and (width // dim) % kv_heads == 0, f"{what}: heads must be a multiple of the cache's key/value heads")
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if out.numel() == 0:
@@ -791,7 +792,7 @@ def paged_attention_prompt_forward(q: torch.Tensor, key_pages: torch.Tensor, val
     pool, kv_heads, page, dim = _paged_cache(what, q, key_pages, value_pages, key_scales, value_scales, block_table, lengths)
     tokens, width, seqs = q.size(0), q.size(1), block_table.size(0)
     _paged_offsets(what, cu_steps, seqs, q.device)
-    _check(scale is None or 0.0 <= float(scale) < float("inf"), f"{what}: scale must be finite and not negative")
+    _check(scale is None or 0.0 <= float(scale) <= 2.0 ** 127, f"{what}: scale must be from 0 to 2 ** 127")
     _check(width % dim == 0 and width > 0 and (width // dim) % kv_heads == 0, f"{what}: heads must be a multiple of the cache's key/value heads")
     if tokens == 0 or seqs == 0:
         return torch.zeros(tokens, width, dtype=q.dtype, device=q.device)

@@ -189,7 +189,7 @@ def test_a_prompt_does_not_depend_on_what_the_others_hold():
 # few rows before a long context: the keys in runs, some of them empty for a short sequence beside a long one
 @pytest.mark.parametrize("steps,pasts,heads,kv_heads,dim,page,dtype", [
     ([3], [3100], 6, 1, 128, 64, BF), ([1, 300, 10, 11, 1, 0, 2], [1500, 700, 1024, 3, 0, 0, 5000], 6, 1, 128, 32, BF), ([1] * 70 + [90], list(range(1000, 1070)) + [30], 2, 2, 64, 64, HF),
-    ([64, 65, 8], [1100, 1100, 4000], 1, 1, 128, 16, HF), ([33], [1200], 2, 1, 128, 64, BF), ([32], [1200], 2, 1, 128, 64, BF), ([40, 2, 0, 1], [2000, 0, 0, 4095], 2, 1, 64, 16, HF), ([17, 70], [5000, 10], 8, 2, 128, 128, HF), ([1], [9000], 16, 2, 64, 32, BF)])
+    ([64, 65, 8], [1100, 1100, 4000], 1, 1, 128, 16, HF), ([33], [1200], 2, 1, 128, 64, BF), ([1, 2, 40], [1500, 2000, 100], 32, 1, 64, 32, BF), ([1, 3], [3000, 100], 128, 1, 64, 64, HF), ([32], [1200], 2, 1, 128, 64, BF), ([40, 2, 0, 1], [2000, 0, 0, 4095], 2, 1, 64, 16, HF), ([17, 70], [5000, 10], 8, 2, 128, 128, HF), ([1], [9000], 16, 2, 64, 32, BF)])
 def test_prompt_in_runs_against_float64(steps, pasts, heads, kv_heads, dim, page, dtype):
     cache = Cache([n + p if n else 0 for n, p in zip(steps, pasts)], kv_heads, dim, page, seed=sum(steps) + heads)
     cu = np.concatenate([[0], np.cumsum(steps)])

@@ -148,7 +148,7 @@ def test_caches_are_refused(bad, words):
 
 @pytest.mark.parametrize("page,dim", [(8, 64), (24, 64), (256, 64), (16, 80), (16, 256)])
 def test_page_and_head_sizes_are_refused(page, dim):
-    for scale in (-1.0, float("nan"), float("inf")):
+    for scale in (-1.0, float("nan"), float("inf"), 3e38):
         with pytest.raises(RuntimeError, match="scale must be" if page == 16 and dim == 64 else "pages of 16"):
             K.paged_attention_decode_forward(torch.zeros(2, 4 * dim, dtype=torch.float16), **_cache(page=page, dim=dim), scale=scale)
     with pytest.raises(RuntimeError, match="pages of 16"):
@@ -201,7 +201,7 @@ def test_c_entries_refuse_before_anything_is_launched():
     for call in (decode, prompt):
         for kw in (dict(q=None), dict(kp=None), dict(vp=None), dict(ks=None), dict(vs=None), dict(table=None), dict(lengths=None), dict(out=None), dict(dtype=0), dict(dtype=3),
                    dict(seqs=0), dict(heads=0), dict(kv=0), dict(heads=3), dict(pool=0), dict(width=0), dict(table_stride=2), dict(q_stride=255), dict(q=at + 2), dict(q_stride=257),
-                   dict(kp=at + 8), dict(table=at + 2), dict(scale=-0.1), dict(scale=float("nan")), dict(scale=float("inf"))):
+                   dict(kp=at + 8), dict(table=at + 2), dict(scale=-0.1), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=3e38)):
             assert call(**kw) == invalid, kw
         for kw in (dict(page=8), dict(page=256), dict(dim=96, q_stride=512), dict(pool=2**31), dict(width=2**28, table_stride=2**28), dict(seqs=10**6), dict(heads=2048, q_stride=2**20)):
             assert call(**kw) == unsupported, kw
