@@ -11,6 +11,8 @@
 // 16-byte pieces of a row lie permuted in LDS (key rows by row % 16, value rows by row / 2 % 8), so 16 neighbouring rows read at one piece meet no
 // bank twice.  Rows behind the last sequence get zeros.
 //
+// SPLIT, for calls of few blocks: 128 rows, waves 4 to 7 have those of 0 to 3 and the other 32 keys of every tile, and what they leave meets in LDS at the end.
+//
 // Bound: 4 D operations per row and key.  8192 tokens of 48 and 8 heads, 825 G operations: 800 us, 1030 T/s, where a large matrix product of the library
 // reaches 1155; what is between is the softmax's vector instructions (44 % of the cycles, the matrix unit 42 %: the two waves of a SIMD overlap them in
 // part) and the barrier of each tile.
@@ -54,12 +56,13 @@ __device__ __forceinline__ int lanes_until(int x) {
 // Those with the most keys come first, so that what is left at the end is short (48 and 8 heads: 30 continuations of up to 200 tokens behind up to 4000
 // 267 -> 215 us, 12 of up to 300 behind up to 16000 809 -> 693; where a sequence's own order is as good already, four prompts of up to 2000 tokens, 117 -> 123); of
 // more than 63 sequences only each one's own blocks are in that order.
+template <int ROWS>
 __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, int group, int& s, int& row0) {
     const int lane = threadIdx.x & 63;
     if (a.seqs == 1) {                                                        // (1024 tokens of 48 and 8 heads: 42.0 -> 40.5 us)
-        const int n = paged_offset(a.cu_steps, 1, 0, a.tokens), blocks = n * group > a.few_rows ? (n * group + kBlockRows - 1) / kBlockRows : 0;
+        const int n = paged_offset(a.cu_steps, 1, 0, a.tokens), blocks = n * group > a.few_rows ? (n * group + ROWS - 1) / ROWS : 0;
         s = index < blocks ? 0 : 1;
-        row0 = (index < blocks ? blocks - 1 - index : index - blocks) * kBlockRows;
+        row0 = (index < blocks ? blocks - 1 - index : index - blocks) * ROWS;
         return row0 < (s ? a.tokens - n : n) * group;
     }
     if (a.seqs < 64) {
@@ -72,7 +75,7 @@ __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, 
             first = keys - n;
         }
         // (counts stay far below 2^24)
-        auto seeing = [&](int tiles) { return paged_blocks_seeing(tiles, rows, first, group, kBlockRows); };
+        auto seeing = [&](int tiles) { return paged_blocks_seeing(tiles, rows, first, group, ROWS); };
         auto all = [&](int count) { return static_cast<int>(group_sum<64>(static_cast<float>(count))); };
         if (index >= all(seeing(0))) return false;
         int low = 0, high = static_cast<int>(group_max<64>(static_cast<float>((keys + kTile - 1) / kTile))) + 1;
@@ -85,8 +88,8 @@ __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, 
         const int until = lanes_until(mine);                                  // blocks of this length of the sequences up to the lane's
         const uint64_t behind = __ballot(until > place);
         s = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(behind)) - 1);
-        const int block = (rows + kBlockRows - 1) / kBlockRows - seeing(low) + place - (until - mine);
-        row0 = __builtin_amdgcn_readlane(block, s) * kBlockRows;
+        const int block = (rows + ROWS - 1) / ROWS - seeing(low) + place - (until - mine);
+        row0 = __builtin_amdgcn_readlane(block, s) * ROWS;
         return true;
     }
     int place = index;
@@ -94,12 +97,12 @@ __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, 
         const int c = base + lane;
         int rows = 0;
         if (c <= a.seqs) rows = max((c == a.seqs ? a.tokens : paged_offset(a.cu_steps, c + 1, 0, a.tokens)) - paged_offset(a.cu_steps, c, 0, a.tokens), 0) * group;
-        const int blocks = c < a.seqs && rows <= a.few_rows ? 0 : (rows + kBlockRows - 1) / kBlockRows, until = lanes_until(blocks);
+        const int blocks = c < a.seqs && rows <= a.few_rows ? 0 : (rows + ROWS - 1) / ROWS, until = lanes_until(blocks);
         const uint64_t behind = __ballot(until > place);
         if (behind) {
             const int owner = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(behind)) - 1);
             s = base + owner;
-            row0 = __builtin_amdgcn_readlane(until - 1 - place, owner) * kBlockRows;
+            row0 = __builtin_amdgcn_readlane(until - 1 - place, owner) * ROWS;
             return true;
         }
         place -= __builtin_amdgcn_readlane(until, 63);
@@ -107,21 +110,24 @@ __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, 
     return false;
 }
 
-template <bool BF16, int D, bool RUNS>
+template <bool BF16, int D, bool RUNS, bool SPLIT>
 __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPromptArgs a) {
     constexpr int kKeyBytes = kTile * D * 2, kTileBytes = 2 * kKeyBytes;      // keys [64][D], values [D][64]
     constexpr int kDimTiles = D / 32, kSteps = D / 16;
+    constexpr int kRows = SPLIT ? kBlockRows / 2 : kBlockRows, kSets = SPLIT ? 1 : 2;         // of a workgroup; 32 keys of a tile that a wave takes
     extern __shared__ __align__(1024) unsigned char smem[];                   // [2][kTileBytes]
     __shared__ __align__(16) float factors[4][8];                             // of tile t at t % 4: per chunk the keys' scale times `scale`, and 0 or -inf
     __shared__ int nan_values[4];                                             // of tile t at t % 4 (masked tiles): some value code is NaN,
     __shared__ float unread[64 + 4 * 8];
+    __shared__ float2 halves[SPLIT ? kBlockRows / 2 : 1];
     __shared__ __align__(8) uint16_t nan_keys[2][D][4];                       // which ones: a bit per key and dimension, in the tile's half
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int place = SPLIT ? wave & 3 : wave, second = SPLIT ? wave >> 2 : 0;                // the wave's rows, the half of a tile's keys
     const int kvh = blockIdx.x, group = a.heads / a.kv_heads;
     // rows of one key/value head: token * group + head in the group; the tokens behind the last sequence are one more, without keys
     int s = 0, row0 = 0;
-    if (!find_block(a, blockIdx.y, group, s, row0)) return;
+    if (!find_block<kRows>(a, blockIdx.z, group, s, row0)) return;
     const bool tail = s == a.seqs;
     const int offset = paged_offset(a.cu_steps, s, 0, a.tokens), n = (tail ? a.tokens : paged_offset(a.cu_steps, s + 1, 0, a.tokens)) - offset;
     const int rows = n * group;                                               // (fits: the host's check)
@@ -131,12 +137,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
         const int64_t v = static_cast<int64_t>(given) - n + row / group + 1;
         return tail ? 0 : static_cast<int>(v < 0 ? 0 : (v > length ? length : v));
     };
-    const int all_tiles = (visible(min(rows, row0 + kBlockRows) - 1) + kTile - 1) / kTile;
+    const int all_tiles = (visible(min(rows, row0 + kRows) - 1) + kTile - 1) / kTile;
     // this workgroup's tiles: t0 .. end - 1
-    const int run = RUNS ? (all_tiles + static_cast<int>(gridDim.z) - 1) / static_cast<int>(gridDim.z) : all_tiles, t0 = RUNS ? min(static_cast<int>(blockIdx.z) * run, all_tiles) : 0;
+    const int run = RUNS ? (all_tiles + static_cast<int>(gridDim.y) - 1) / static_cast<int>(gridDim.y) : all_tiles, t0 = RUNS ? min(static_cast<int>(blockIdx.y) * run, all_tiles) : 0;
     const int end = RUNS ? min(t0 + run, all_tiles) : all_tiles, tiles = end - t0;
     const int full = visible(row0) / kTile;                                   // tiles that every row of the workgroup sees whole
-    const int w0 = row0 + 32 * wave, my_row = min(w0 + r, rows - 1);
+    const int w0 = row0 + 32 * place, my_row = min(w0 + r, rows - 1);
     const int limit = visible(my_row);
     const int wave_end = w0 < rows ? visible(min(rows, w0 + 32) - 1) : 0;     // keys that one of the wave's rows sees
     const int32_t* table = a.table + static_cast<size_t>(tail ? 0 : s) * a.table_stride;
@@ -163,7 +169,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     auto entry = [&](int t) { return table[min(first_key(t) >> a.page_shift, a.width - 1)]; };            // the wave's page of tile t, unchecked
     auto checked = [&](int t, int page) {
         page = __builtin_amdgcn_readfirstlane(page);
-                const bool here = page >= 0 && page < a.pool && first_key(t) < length;     // (no branch: the step is one block)
+        const bool here = page >= 0 && page < a.pool && first_key(t) < length;     // (no branch: the step is one block)
         return Place{static_cast<size_t>(here ? page : 0) * a.kv_heads + kvh, here};
     };
     auto load_keys = [&](int t, const Place& p) { return *reinterpret_cast<const uint4*>(a.key_pages + p.at * head_bytes + (first_key(t) & page_mask) * D + key_lane); };
@@ -210,27 +216,27 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     };
 
     const v16f zero = {};
-    v16f o[kDimTiles], sa[2], sb[2];
+    v16f o[kDimTiles], sa[kSets], sb[kSets];
 #pragma unroll
     for (int i = 0; i < kDimTiles; ++i) o[i] = zero;
     float m = -FLT_MAX, l = 0.0f;                                             // of the lane's query; l over its half of the keys
     // S^T of the tile in one half of LDS
-    auto scores = [&](int half, v16f (&sc)[2]) {
-        const unsigned char* kt = smem + half * kTileBytes;
+    auto scores = [&](int half, v16f (&sc)[kSets]) {
+        const unsigned char* kt = smem + half * kTileBytes + 32 * second * (2 * D);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < kSets; ++u) {
                 const uint4 kf = *reinterpret_cast<const uint4*>(kt + (32 * u + r) * (2 * D) + (((2 * i + h) ^ (r & (D / 8 - 1))) << 4));
                 sc[u] = half_mfma32<BF16>(kf, qf[i], i == 0 ? zero : sc[u]);
             }
     };
 
     // the largest score of the lane's row, in the exponent's units
-    auto row_top = [&](const v16f (&sc)[2], const float (&f)[4], const float (&b)[4]) {
+    auto row_top = [&](const v16f (&sc)[kSets], const float (&f)[2 * kSets], const float (&b)[2 * kSets]) {
         float most = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2 * kSets; ++c) {
             // (a maximum that hands NaN on takes three operands in one instruction and needs no quieting of them; a NaN score is its row's end either way)
             float x = sc[c >> 1][8 * (c & 1)];
 #pragma unroll
@@ -241,12 +247,18 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
         swapped_pair<32>(most, lower, upper);
         return __builtin_elementwise_maximum(lower, upper);
     };
-    auto load_factors = [&](int t, float (&f)[4], float (&b)[4]) {
-        const float4 f4 = *reinterpret_cast<const float4*>(factors[t & 3]), b4 = *reinterpret_cast<const float4*>(factors[t & 3] + 4);
-        f[0] = f4.x; f[1] = f4.y; f[2] = f4.z; f[3] = f4.w;
-        b[0] = b4.x; b[1] = b4.y; b[2] = b4.z; b[3] = b4.w;
+    auto load_factors = [&](int t, float (&f)[2 * kSets], float (&b)[2 * kSets]) {
+        if constexpr (SPLIT) {
+            const float2 f2 = *reinterpret_cast<const float2*>(factors[t & 3] + 2 * second), b2 = *reinterpret_cast<const float2*>(factors[t & 3] + 4 + 2 * second);
+            f[0] = f2.x; f[1] = f2.y;
+            b[0] = b2.x; b[1] = b2.y;
+        } else {
+            const float4 f4 = *reinterpret_cast<const float4*>(factors[t & 3]), b4 = *reinterpret_cast<const float4*>(factors[t & 3] + 4);
+            f[0] = f4.x; f[1] = f4.y; f[2] = f4.z; f[3] = f4.w;
+            b[0] = b4.x; b[1] = b4.y; b[2] = b4.z; b[3] = b4.w;
+        }
     };
-    float f[4] = {}, b[4] = {}, top = -INFINITY;                              // of the tile whose scores are there
+    float f[2 * kSets] = {}, b[2 * kSets] = {}, top = -INFINITY;                              // of the tile whose scores are there
 
     // what is on its way: codes of keys two tiles ahead of the products, of values one, page numbers and scales ahead of them
     uint4 key_raw, value_raw;
@@ -304,7 +316,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     }
 
     // One tile: its softmax weights beside the next tile's scores, its value product beside the copies of the tiles behind.
-    auto step = [&](auto masked, int t, int half, v16f (&cur)[2], v16f (&next)[2]) {
+    auto step = [&](auto masked, int t, int half, v16f (&cur)[kSets], v16f (&next)[kSets]) {
         constexpr bool MASKED = decltype(masked)::value;
         // the copies: keys two tiles ahead take the place of this tile's, values of the next tile that of the one before (behind the last tile: its
         // codes again, which nobody reads)
@@ -322,12 +334,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
             next_at = checked(min(t + 4, last), entry_next);
             entry_next = entry(min(t + 5, last));
         };
-        const int seen = limit - kTile * t - 4 * h;
+        const int seen = limit - kTile * t - 32 * second - 4 * h;
         auto hidden = [&](int u, int v) { return MASKED && 32 * u + 8 * (v >> 2) + (v & 3) >= seen; };
         if constexpr (MASKED) {
             top = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < kSets; ++u)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
                     const float x = __builtin_fmaf(cur[u][v], f[2 * u + (v >> 3)], b[2 * u + (v >> 3)]);
@@ -351,17 +363,17 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
         // row, but past the exponent's range from 2^31 on.  Scores that far out are multiplied and rounded first.
         if (__any(fabsf(m) > 0x1p20f)) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < kSets; ++u)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) cur[u][v] = __builtin_fmaf(cur[u][v], f[2 * u + (v >> 3)], b[2 * u + (v >> 3)]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) { f[c] = 1.0f; b[c] = 0.0f; }
+            for (int c = 0; c < 2 * kSets; ++c) { f[c] = 1.0f; b[c] = 0.0f; }
         }
         copies();
         scores(half ^ 1, next);
-        uint4 p[4];
+        uint4 p[2 * kSets];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2 * kSets; ++c) {
             float e[8];
             const float behind = b[c] - m;
 #pragma unroll
@@ -375,10 +387,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
         }
         load_factors(t + 1, f, b);
         const unsigned char* vt = smem + half * kTileBytes + kKeyBytes;
-        auto value_piece = [&](int u, int c) { return *reinterpret_cast<const uint4*>(vt + (32 * u + r) * (2 * kTile) + (((2 * c + h) ^ ((r >> 1) & 7)) << 4)); };
-        if (!MASKED || kTile * t < wave_end) {
+        auto value_piece = [&](int u, int c) { return *reinterpret_cast<const uint4*>(vt + (32 * u + r) * (2 * kTile) + (((4 * second + 2 * c + h) ^ ((r >> 1) & 7)) << 4)); };
+        if (!MASKED || kTile * t + 32 * second < wave_end) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 2 * kSets; ++c)
 #pragma unroll
                 for (int u = 0; u < kDimTiles; ++u) o[u] = half_mfma32<BF16>(value_piece(u, c), p[c], o[u]);
         }
@@ -387,13 +399,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
             // the order that this stretch is issued in: operands a few instructions ahead, a share of the exponentials behind every matrix instruction
             __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
-            for (int i = 0; i < 2 * kSteps; ++i) {
+            for (int i = 0; i < kSets * kSteps; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
             }
 #pragma unroll
-            for (int i = 0; i < 4 * kDimTiles; ++i) {
+            for (int i = 0; i < 2 * kSets * kDimTiles; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
@@ -419,15 +431,41 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     for (; t < end; ++t) {
         step(std::true_type{}, t, (t - t0) & 1, sa, sb);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) sa[u] = sb[u];
+        for (int u = 0; u < kSets; ++u) sa[u] = sb[u];
     }
     float lower, upper;
     swapped_pair<32>(l, lower, upper);
-    const float den = lower + upper;
+    float den = lower + upper;
+    if constexpr (SPLIT) {
+        // the two halves of the keys together, lane by lane
+        float4* other = reinterpret_cast<float4*>(smem + place * (32 * D * 4)) + lane;
+        if (second) {
+            if (h == 0) halves[32 * place + r] = make_float2(m, den);
+#pragma unroll
+            for (int u = 0; u < kDimTiles; ++u)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) other[64 * (4 * u + g)] = make_float4(o[u][4 * g], o[u][4 * g + 1], o[u][4 * g + 2], o[u][4 * g + 3]);
+        }
+        __syncthreads();
+        if (second) return;
+        const float2 theirs = halves[32 * place + r];
+        const float most = fmaxf(m, theirs.x), mine_by = __builtin_amdgcn_exp2f(m - most), theirs_by = __builtin_amdgcn_exp2f(theirs.x - most);
+        den = __builtin_fmaf(den, mine_by, theirs.y * theirs_by);
+        m = most;
+#pragma unroll
+        for (int u = 0; u < kDimTiles; ++u)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 x = other[64 * (4 * u + g)];
+                const float with[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[u][4 * g + i] = __builtin_fmaf(o[u][4 * g + i], mine_by, with[i] * theirs_by);
+            }
+    }
     if constexpr (RUNS) {
         // one of several runs of the block's keys: sums and statistics as they are, for the kernel that brings them together
         if (w0 + r < rows) {
-            const size_t row = (static_cast<size_t>(blockIdx.z) * a.tokens + offset + my_row / group) * a.heads + kvh * group + my_row % group;
+            const size_t row = (static_cast<size_t>(blockIdx.y) * a.tokens + offset + my_row / group) * a.heads + kvh * group + my_row % group;
             if (h == 0) a.stats[row] = make_float2(m, den);
 #pragma unroll
             for (int u = 0; u < kDimTiles; ++u)
@@ -439,7 +477,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     }
     const float inv = den == 0.0f ? 0.0f : 2.0f / den;                        // (twice: the values went in halved)
     // lane: query r, dimensions 32 u + 8 (v / 4) + 4 h + v % 4; through the wave's own part of LDS to whole rows
-    unsigned char* turn = smem + wave * (32 * 2 * D);
+    unsigned char* turn = smem + place * (32 * D * (SPLIT ? 4 : 2));
 #pragma unroll
     for (int u = 0; u < kDimTiles; ++u)
 #pragma unroll
@@ -460,7 +498,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
 // A wave per query row: its runs together, in their order.
 template <bool BF16, int D>
 __global__ __launch_bounds__(256) void paged_prompt_merge_kernel(const PagedPromptArgs a) {
-    constexpr int kPer = D / 64;
+    constexpr int kPer = D / 64, kBatch = 8;
     const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads, row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= rows) return;
@@ -471,14 +509,14 @@ __global__ __launch_bounds__(256) void paged_prompt_merge_kernel(const PagedProm
     const float2 mine = lane < a.runs ? a.stats[lane * rows + row] : make_float2(-FLT_MAX, 0.0f);           // (at most 64 runs)
     const float top = group_max<64>(mine.x), factor = __builtin_amdgcn_exp2f(mine.x - top), den = group_sum<64>(mine.y * factor);
     float total[kPer] = {};
-    for (int i0 = 0; i0 < a.runs; i0 += 8) {
-        float v[8][kPer];
+    for (int i0 = 0; i0 < a.runs; i0 += kBatch) {
+        float v[kBatch][kPer];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < kBatch; ++i)
 #pragma unroll
             for (int j = 0; j < kPer; ++j) v[i][j] = a.sums[(min(i0 + i, a.runs - 1) * rows + row) * D + kPer * lane + j];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kBatch; ++i) {
             if (i0 + i >= a.runs) break;
             const float f = __shfl(factor, i0 + i);
 #pragma unroll
@@ -492,13 +530,17 @@ __global__ __launch_bounds__(256) void paged_prompt_merge_kernel(const PagedProm
 }
 
 template <bool BF16, int D>
-int launch(const PagedPromptArgs& a, hipStream_t stream) {
-    static SmemGrant granted[2];
+int launch(const PagedPromptArgs& a, bool split, hipStream_t stream) {
+    static SmemGrant granted[4];
     const size_t smem = 2 * 2 * kTile * D * 2;
+    const bool runs = a.sums != nullptr;
+    const auto kernel = runs ? (split ? paged_prompt_kernel<BF16, D, true, true> : paged_prompt_kernel<BF16, D, true, false>)
+                             : (split ? paged_prompt_kernel<BF16, D, false, true> : paged_prompt_kernel<BF16, D, false, false>);
     // (with the kernel's own arrays beside it, 128-wide heads pass 64 KB)
-    const auto kernel = a.sums ? paged_prompt_kernel<BF16, D, true> : paged_prompt_kernel<BF16, D, false>;
-    if (!grant_dynamic_smem(reinterpret_cast<const void*>(kernel), smem + 4096, granted[a.sums != nullptr])) return PLLM_ERR_LAUNCH;
-    hipLaunchKernelGGL(kernel, dim3(a.kv_heads, a.slots, a.runs), dim3(kThreads), smem, stream, a);
+    if (!grant_dynamic_smem(reinterpret_cast<const void*>(kernel), smem + 8192, granted[2 * runs + split])) return PLLM_ERR_LAUNCH;
+    // Runs before blocks: indexes without a block come last.  Workgroups go to the shader engines in turn, those that end at once too, and an engine that got more
+    // of the others than it has compute units works a second round (128 tokens behind 30000 positions in blocks of half the rows 213 -> 117 us).
+    hipLaunchKernelGGL(kernel, dim3(a.kv_heads, a.runs, a.slots), dim3(kThreads), smem, stream, a);
     if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
     if (a.sums) {
         const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
@@ -508,11 +550,15 @@ int launch(const PagedPromptArgs& a, hipStream_t stream) {
     return PLLM_OK;
 }
 
-// Runs that the keys of every block of query rows are cut in: as many as give every compute unit a workgroup when there are few rows before a
-// long context, none of them shorter than 8 tiles of a sequence that fills the table.
-int prompt_runs(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t positions) {
-    const int64_t blocks = (tokens * (heads / kv_heads) + kBlockRows - 1) / kBlockRows * kv_heads;
-    const int64_t runs = std::min(std::min(compute_units() / blocks, positions / (8 * kTile)), int64_t{64});
+// Blocks of so many query rows that the sequences of a call can have: whole ones, and a last one of every sequence with more than `few` rows.
+int64_t blocks_of(int64_t rows, int64_t seqs, int64_t few, int block_rows) {
+    return seqs == 1 ? (rows + block_rows - 1) / block_rows : rows / block_rows + std::min(seqs, rows / (few + 1));
+}
+
+// Runs that the keys of so many blocks and heads are cut in: as many as give every compute unit a workgroup when there are few rows before a long context (one
+// workgroup more than that costs a second round), none of them shorter than 4 tiles of a sequence that fills the table.
+int prompt_runs(int64_t blocks, int64_t positions) {
+    const int64_t runs = std::min(std::min(compute_units() / std::max(blocks, int64_t{1}), positions / (4 * kTile)), int64_t{64});
     return static_cast<int>(std::max(runs, int64_t{1}));
 }
 
@@ -530,12 +576,22 @@ int few_rows(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
     return rows < group ? 0 : static_cast<int>(rows);
 }
 
-struct Parts { int runs, few; size_t run_bytes, few_bytes; };
+struct Parts { int runs, few; bool split; size_t run_bytes, few_bytes; };
 Parts parts_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
     Parts p{};
+    const int64_t rows = tokens * (heads / kv_heads);
     p.few = few_rows(tokens, seqs, heads, kv_heads, head_dim, positions);
     p.few_bytes = p.few > 0 ? paged_decode_parts_bytes(seqs, p.few, kv_heads, head_dim, positions) : 0;
-    p.runs = tokens * (heads / kv_heads) <= p.few ? 1 : prompt_runs(tokens, heads, kv_heads, positions);
+    // Half the rows per workgroup while the workgroups are not more than the compute units, and of one prompt without a past, whose last rows see so much more
+    // than the mean, up to twice as many (48 and 8 heads, 200 tokens 19.3 -> 14.0 us, 700 31.0 -> 24.5, 1024 42.2 -> 36.2, 1365 52 -> 46, but 1700 60 -> 71; 8 of
+    // up to 300 of 32 and 8 heads 23.3 -> 26.9): every tile's codes become 16-bit values for half as many rows.  In runs too (8 and 8 heads, 128 tokens behind
+    // 16000 positions 59 -> 34, 300 behind 2000 38 -> 26), but not where whole blocks' runs fill the machine and are long (48 and 8 heads, 128 behind 30000 109 / 117).
+    const bool alone = seqs == 1 && positions <= 2 * tokens;
+    const int64_t whole = blocks_of(rows, seqs, p.few, kBlockRows) * kv_heads, half = blocks_of(rows, seqs, p.few, kBlockRows / 2) * kv_heads;
+    const int whole_runs = prompt_runs(whole, positions);
+    p.split = half <= (alone ? 2 : 1) * compute_units() && (whole_runs == 1 || positions < 32 * kTile * whole_runs);
+    p.runs = rows <= p.few ? 1 : (p.split ? prompt_runs(half, positions) : whole_runs);
+    if (alone && p.runs == 2) p.runs = 1;                                     // (the second launch: 1024 tokens of 16 and 8 heads 32.0 -> 26.4)
     const size_t parts = static_cast<size_t>(p.runs) * tokens * heads;
     p.run_bytes = p.runs > 1 ? align256(parts * head_dim * sizeof(float)) + align256(parts * sizeof(float2)) : 0;
     return p;
@@ -568,8 +624,8 @@ int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int dtype, cons
     // pages, positions and rows in 32 bits
     if (tokens > 0x3fffff || seqs > 0xffff || heads > 1024 || pool > 0x7fffffff || table_width > 0x3fffffff / page_tokens) return PLLM_ERR_UNSUPPORTED;
     const Parts parts = parts_of(tokens, seqs, heads, kv_heads, head_dim, table_width * page_tokens);
-    // blocks of all sequences: whole ones, and a last one of every sequence that can have any and of the rows behind the last
-    const int64_t rows = tokens * (heads / kv_heads), slots = rows / kBlockRows + std::min(seqs, rows / (parts.few + 1)) + 1;
+    // (the rows behind the last sequence: what is left of the whole blocks, and one more)
+    const int64_t rows = tokens * (heads / kv_heads), slots = blocks_of(rows, seqs, parts.few, parts.split ? kBlockRows / 2 : kBlockRows) + 1;
     if (rows > 0x3fffffff || slots > 0xffff) return PLLM_ERR_UNSUPPORTED;
     const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) | reinterpret_cast<uintptr_t>(out) |
                            reinterpret_cast<uintptr_t>(workspace);
@@ -595,7 +651,7 @@ int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int dtype, cons
     }
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool bf16 = dtype == PLLM_BF16;
-    const int status = head_dim == 128 ? (bf16 ? launch<true, 128>(a, st) : launch<false, 128>(a, st)) : (bf16 ? launch<true, 64>(a, st) : launch<false, 64>(a, st));
+    const int status = head_dim == 128 ? (bf16 ? launch<true, 128>(a, parts.split, st) : launch<false, 128>(a, parts.split, st)) : (bf16 ? launch<true, 64>(a, parts.split, st) : launch<false, 64>(a, parts.split, st));
     if (status != PLLM_OK || a.few_rows == 0) return status;
     PagedDecodeArgs d{};
     d.q = a.q; d.q_stride = a.q_stride; d.key_pages = key_pages; d.value_pages = value_pages; d.key_scales = key_scales; d.value_scales = value_scales;

@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import paged_oracle as P
 from pocketllm_amd import _ffi, hip_kernel as K
 from paged_cases import DEV, Cache, close, queries
 
@@ -202,6 +203,27 @@ def test_prompt_in_runs_against_float64(steps, pasts, heads, kv_heads, dim, page
     want, note = cache.attention(q[:cu[-1]].view(-1, heads, dim).double().numpy(), cu)
     close(got[:cu[-1]], want, note, dtype)
     assert (got[cu[-1]:] == 0).all()
+
+
+# Calls of many rows and heads, of which a few heads are checked: one prompt whose workgroups are up to twice the compute units, the same behind a past, two long
+# runs of the keys, ragged ones, more sequences than a wave has lanes with several blocks in some.
+@pytest.mark.parametrize("steps,pasts,kv_heads,group,dim,page,dtype", [
+    ([700], [0], 64, 1, 64, 64, BF), ([600], [700], 64, 1, 128, 32, HF), ([300], [4200], 64, 1, 64, 128, BF), ([290, 1, 310], [100, 900, 700], 64, 1, 128, 32, BF),
+    ([3] * 69 + [700, 0, 300], [10] * 69 + [0, 0, 200], 16, 2, 64, 16, HF)])
+def test_calls_of_many_rows(steps, pasts, kv_heads, group, dim, page, dtype):
+    """NaN values: of the first sequence's sixth key in one dimension, of the last one's last key (one query sees it) in another."""
+    lengths = [n + p if n else 0 for n, p in zip(steps, pasts)]
+    cache = Cache(lengths, kv_heads, dim, page, seed=sum(steps))
+    cache.value_codes[cache.table[0, 0], :, 7, 5] = 0x7f
+    cache.value_codes[cache.table[-1, (lengths[-1] - 1) // page], :, 30, (lengths[-1] - 1) % page] = 0xff
+    cu = np.concatenate([[0], np.cumsum(steps)])
+    q = queries(cu[-1], kv_heads * group, dim, dtype, seed=3)
+    got = K.paged_attention_prompt_forward(q.to(DEV), *cache.device(), torch.tensor(cu, dtype=torch.int32, device=DEV)).view(-1, kv_heads, group, dim)
+    for head in (0, kv_heads - 1):
+        want, note = P.attention(q.view(-1, kv_heads, group, dim)[:, head].double().numpy(), *(a[:, head:head + 1] for a in (
+            cache.key_codes, cache.value_codes, cache.key_scales, cache.value_scales)), cache.table, cache.lengths, cu, dim ** -0.5)
+        assert np.isnan(want).sum() == group * (min(steps[0], lengths[0] - 5) + 1)
+        close(got[:, head], want, note, dtype)
 
 
 def test_many_sequences():
