@@ -3,10 +3,12 @@
 //     t = round(x + residual);  n = t * rsqrt(mean(t^2) + eps) * weight;  per 128 values s = max(amax |n|, quant_eps) / 448 (a power of two
 //     when asked for), code = E4M3(n / s)
 // The sum leaves rounded to the stream's type, and what is normalized is that rounded value, so the operator says what the three separate ones
-// say; the normalized values stay in float32 until they become codes (the separate operators round them to 16 bits in between).
-// Bound: bytes for prompts (8192 rows of 5120 bf16 values: 295 MB in 53 us, 5.6 TB/s, what a large copy reaches), the start of a launch and one round
-// trip to memory for few rows (3.8 us).
-#include "pllm_device.h"
+// say; the normalized values become codes as they are (the separate operators round them to 16 bits in between).  Without power-of-two scales the root
+// falls out of the codes, E4M3(448 t w / max |t w|).  Products, quotient and root are in 64 bits (32 by 8 to 24 bits: exact) and cut on the way to a code so that
+// it is the one that the values themselves round to: in 32 bits one in a million is its neighbour, 6 % away.
+// Bound: bytes for prompts (8192 rows of 5120 bf16 values: 295 MB in 55 us, 5.4 TB/s, what a large copy reaches; in 32 bits the same), the start of a launch and
+// one round trip to memory for few rows (4.1 us; in 32 bits 3.8).
+#include "paged_device.h"
 #include "pllm_internal.h"
 
 #include <cfloat>
@@ -18,7 +20,7 @@ struct NormArgs {
     const void* x; const void* residual; const float* weight;
     void* total; uint8_t* codes; float* scales;
     int rows, dim, pow2;
-    float eps, quant_eps;
+    double inv_dim, eps, quant_eps;
 };
 
 template <int DT> struct Eight { uint4 a[DT == PLLM_F32 ? 2 : 1]; };
@@ -38,14 +40,6 @@ template <int DT> __device__ __forceinline__ float eight_value(const Eight<DT>& 
         return DT == PLLM_BF16 ? __uint_as_float(h << 16) : f16_bits_to_float(h);
     }
 }
-template <int DT> __device__ __forceinline__ uint32_t type_bits(float v) {
-    if constexpr (DT == PLLM_BF16) return from_float<bf16_t>(v).bits;
-    else {
-        union { _Float16 h; uint16_t u; } c;
-        c.h = static_cast<_Float16>(v);
-        return c.u;
-    }
-}
 // eight sums rounded to the type, as they are stored
 template <int DT> __device__ __forceinline__ Eight<DT> pack_eight(const float v[8]) {
     Eight<DT> e;
@@ -56,17 +50,30 @@ template <int DT> __device__ __forceinline__ Eight<DT> pack_eight(const float v[
     } else {
         uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = type_bits<DT>(v[2 * i]) | (type_bits<DT>(v[2 * i + 1]) << 16);
+        for (int i = 0; i < 4; ++i) w[i] = half_pair<DT == PLLM_BF16>(v[2 * i], v[2 * i + 1]);
         e.a[0] = make_uint4(w[0], w[1], w[2], w[3]);
     }
     return e;
+}
+
+template <int OFF> __device__ __forceinline__ double wide_peer(double v) {
+    const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v));
+    const uint32_t lo = __float_as_uint(butterfly_peer<OFF>(__uint_as_float(static_cast<uint32_t>(b)))), hi = __float_as_uint(butterfly_peer<OFF>(__uint_as_float(static_cast<uint32_t>(b >> 32))));
+    return __longlong_as_double(static_cast<long long>((static_cast<uint64_t>(hi) << 32) | lo));
+}
+// 1 / v, off by a few 2^-53, for v far from the ends of the range
+__device__ __forceinline__ double reciprocal(double v) {
+    double r = __builtin_amdgcn_rcp(v);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) r = __builtin_fma(__builtin_fma(-v, r, 1.0), r, r);
+    return r;
 }
 
 // WAVES waves share a row (one: four rows to a workgroup), PIECES pieces of eight values per lane; the whole row stays in registers.  Sixteen
 // neighbouring lanes hold the 128 values of one scale.
 template <int DT, int WAVES, int PIECES>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void add_norm_fp8_kernel(const NormArgs a) {
-    __shared__ float red[WAVES == 1 ? 4 : WAVES];
+    __shared__ double red[WAVES == 1 ? 4 : WAVES];
     const int tid = WAVES == 1 ? static_cast<int>(threadIdx.x & 63) : static_cast<int>(threadIdx.x);
     const int row = WAVES == 1 ? static_cast<int>(blockIdx.x * 4 + (threadIdx.x >> 6)) : static_cast<int>(blockIdx.x);
     if (WAVES == 1 && row >= a.rows) return;                                  // (no barrier below where a wave has a row of its own)
@@ -84,7 +91,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void add_norm_fp8_ke
         if (a.residual) rv[j] = load_eight<DT>(a.residual, base + at);
         g[j] = load_eight<PLLM_F32>(a.weight, at);
     }
-    float v[PIECES][8], ss = 0.0f;
+    double ss = 0.0;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
         if (a.residual) {
@@ -100,47 +107,57 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void add_norm_fp8_ke
         }
         float part = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v[j][i] = eight_value(xv[j], i);
-            part = __builtin_fmaf(v[j][i], v[j][i], part);
-        }
-        ss += inside[j] ? part : 0.0f;
+        for (int i = 0; i < 8; ++i) part = __builtin_fmaf(eight_value(xv[j], i), eight_value(xv[j], i), part);
+        ss += inside[j] ? static_cast<double>(part) : 0.0;
     }
-    ss = group_sum<64>(ss);
+    ss += wide_peer<1>(ss);
+    ss += wide_peer<2>(ss);
+    ss += wide_peer<4>(ss);
+    ss += wide_peer<8>(ss);
+    ss += wide_peer<16>(ss);
+    ss += wide_peer<32>(ss);
     if constexpr (WAVES > 1) {
         if ((tid & 63) == 0) red[tid >> 6] = ss;
         __syncthreads();
-        ss = 0.0f;
+        ss = 0.0;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) ss += red[w];
     }
-    const float rstd = rsqrtf(ss / static_cast<float>(a.dim) + a.eps);
+    const double rstd = rsqrt(__builtin_fma(ss, a.inv_dim, a.eps));
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
         // t * weight; the root is one factor of the whole row and goes with the block's scale: one product per value behind one division per block
-        uint32_t top = 0;                                                     // magnitudes as integers: in the order of their values, NaN above all
+        double v[8], top = 0.0, none = 0.0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            v[j][i] *= eight_value(g[j], i);
-            top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
+            v[i] = static_cast<double>(eight_value(xv[j], i)) * static_cast<double>(eight_value(g[j], i));
+            top = fmax(top, fabs(v[i]));
+            none = __builtin_fma(v[i], 0.0, none);                            // NaN from infinities and NaN, which a maximum may drop
         }
-        top = max(top, __float_as_uint(butterfly_peer<1>(__uint_as_float(top))));
-        top = max(top, __float_as_uint(butterfly_peer<2>(__uint_as_float(top))));
-        top = max(top, __float_as_uint(butterfly_peer<4>(__uint_as_float(top))));
-        top = max(top, __float_as_uint(butterfly_peer<8>(__uint_as_float(top))));
-        const float amax = __uint_as_float(top) * rstd;
-        float s = fmaxf(amax, a.quant_eps) / 448.0f;
+        top = none == 0.0 ? top : HUGE_VAL;
+        top = fmax(top, wide_peer<1>(top));
+        top = fmax(top, wide_peer<2>(top));
+        top = fmax(top, wide_peer<4>(top));
+        top = fmax(top, wide_peer<8>(top));
+        const double amax = top * rstd, most = fmax(amax, a.quant_eps);
+        const bool usual = amax >= a.quant_eps;
+        float s;
+        double factor;
         if (a.pow2) {
             int e;
-            const float m = frexpf(fmaxf(s, 1.17549435e-38f), &e);            // s = m * 2^e, m in [0.5, 1)
-            s = ldexpf(1.0f, m == 0.5f ? e - 1 : e);
+            const double m = frexp(most, &e);                                 // 448 = 0.875 * 2^9
+            e = max(m <= 0.875 ? e - 9 : e - 8, -126);
+            s = static_cast<float>(ldexp(1.0, e));
+            factor = ldexp(rstd, -e);
+        } else {
+            s = static_cast<float>(most * (1.0 / 448.0));
+            factor = (usual ? 448.0 : 448.0 * rstd) * reciprocal(usual ? top : a.quant_eps);
         }
         uint32_t lo, hi;
-        if (amax <= FLT_MAX) {
-            const float factor = rstd / s;
+        if (amax <= FLT_MAX && s <= FLT_MAX) {
             float c[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) c[i] = fminf(fmaxf(v[j][i] * factor, -448.0f), 448.0f);
+            for (int i = 0; i < 8; ++i) c[i] = odd_float(v[i] * factor);      // (448 and the product's own rounding at most)
             int l = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false), h = __builtin_amdgcn_cvt_pk_fp8_f32(c[4], c[5], 0, false);
             lo = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], l, true));
             hi = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c[6], c[7], h, true));
@@ -163,14 +180,11 @@ void launch(const NormArgs& a, hipStream_t stream) {
 
 template <int DT>
 void launch_rows(const NormArgs& a, hipStream_t stream) {
-    // A row in one piece per lane where every row finds a compute unit of its own (5120 bf16 values, us with one piece of ten waves / three pieces of four:
-    // 1 row 3.8 / 4.2, 64 4.1 / 4.5, 256 4.8 / 5.0, 512 6.8 / 6.6, 8192 73 / 53), else pieces of four waves, which wait for one another less
-    // (eight waves: 55).
-    const bool few = a.rows <= compute_units();
+    // Four waves to a row up to 8192 values, in as many pieces as that takes: a row in one piece of more waves is as fast where every row finds a compute unit of
+    // its own (64 rows, us with eight or sixteen waves / four: 4096 bf16 values 3.8 / 3.9, 5120 4.5 / 4.4, 8192 4.8 / 5.0) and waits longer for itself where
+    // not (8192 rows of 5120 78 / 55).
     if (a.dim <= 512) launch<DT, 1, 1>(a, stream);
     else if (a.dim <= 2048) launch<DT, 4, 1>(a, stream);
-    else if (few && a.dim <= 4096) launch<DT, 8, 1>(a, stream);
-    else if (few && a.dim <= 8192) launch<DT, 16, 1>(a, stream);
     else if (a.dim <= 4096) launch<DT, 4, 2>(a, stream);
     else if (a.dim <= 6144) launch<DT, 4, 3>(a, stream);
     else if (a.dim <= 8192) launch<DT, 4, 4>(a, stream);
@@ -194,7 +208,7 @@ extern "C" int pllm_fused_add_rms_norm_fp8(const void* x, const void* residual, 
                            reinterpret_cast<uintptr_t>(total);
     if ((wide & 15u) || (reinterpret_cast<uintptr_t>(codes) & 7u) || (reinterpret_cast<uintptr_t>(scales) & 3u)) return PLLM_ERR_INVALID_ARGUMENT;
     if (rows > 0x3fffff || dim > kWidestRow) return PLLM_ERR_UNSUPPORTED;     // (a launch counts its threads in 32 bits)
-    const NormArgs a{x, residual, weight, total, codes, scales, static_cast<int>(rows), static_cast<int>(dim), round_scale_pow2 != 0, eps, quant_eps};
+    const NormArgs a{x, residual, weight, total, codes, scales, static_cast<int>(rows), static_cast<int>(dim), round_scale_pow2 != 0, 1.0 / static_cast<double>(dim), eps, quant_eps};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == PLLM_F32) launch_rows<PLLM_F32>(a, st);
     else if (dtype == PLLM_F16) launch_rows<PLLM_F16>(a, st);

@@ -1,5 +1,5 @@
 // New keys and values into a paged E4M3 cache, the rotary phases on the way, and the new queries turned beside them: one launch.
-//     k' = k cos_p + swap(k) sin_p (float32, the halves of the rotary part swapped), p = lengths[s] - n_s + i for token i of sequence s
+//     k' = k cos_p + swap(k) sin_p (the halves of the rotary part swapped; for keys in 64 bits), p = lengths[s] - n_s + i for token i of sequence s
 //     scale of a page and head: the least power of two with amax / scale <= 448 over what the page holds;  code = E4M3(k' / scale)
 // A page that a call continues keeps its scale unless the new tokens need a larger one; then its older codes are scaled down by the ratio, a power
 // of two: exact, but for codes that get below E4M3's normal values, which are rounded again.  A page that a call begins forgets what it held.
@@ -7,7 +7,7 @@
 //
 // A workgroup owns a page's keys, or its values, of one head: its scale needs no atomics and no second pass.  Values turn in LDS, since a page
 // holds them with the tokens innermost.  The queries are rows behind these workgroups in the same grid.
-// Bound: bytes for prompts (4096 tokens of 48 and 8 heads of 128: 128 MB in 23 us, 5.5 TB/s; with pages of 16 tokens 25), the chain of a workgroup's loads
+// Bound: bytes for prompts (4096 tokens of 48 and 8 heads of 128: 128 MB in 25 us, 5.1 TB/s; in 32 bits 24), the chain of a workgroup's loads
 // (offset, length, row and page, scale: 4 us) and the number of workgroups (two for every page and head) for decode steps.
 #include "paged_device.h"
 #include "pllm_internal.h"
@@ -47,6 +47,12 @@ __device__ __forceinline__ Phases load_phases(const AppendArgs& a, int position,
 __device__ __forceinline__ void turn(float own[8], const float other[8], const Phases& p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) own[i] = __builtin_fmaf(other[i], of4(p.s, i), own[i] * of4(p.c, i));
+}
+// the same for what becomes codes: products and sum in 64 bits, cut so that the codes are those of the sum itself (in 32 bits one in about a million is not)
+__device__ __forceinline__ void turn_for_codes(float own[8], const float other[8], const Phases& p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        own[i] = odd_float(__builtin_fma(static_cast<double>(other[i]), static_cast<double>(of4(p.s, i)), static_cast<double>(own[i]) * static_cast<double>(of4(p.c, i))));
 }
 // the least power of two that brings amax to 448 = 1.75 * 2^8 or below, at least 2^-120
 __device__ __forceinline__ float page_scale(float amax) {
@@ -153,7 +159,7 @@ __global__ __launch_bounds__(FEW ? 64 : 256) void paged_append_kernel(const Appe
         if (turns) {
             float across[8];
             half_eight<BF16>(other[i], across);
-            turn(v[i], across, load_phases(a, lo + min(tid / kChunks + kRows * i, count - 1), D, d0));
+            turn_for_codes(v[i], across, load_phases(a, lo + min(tid / kChunks + kRows * i, count - 1), D, d0));
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) amax = fabsf(v[i][j]) <= FLT_MAX ? fmaxf(amax, fabsf(v[i][j])) : amax;

@@ -60,6 +60,15 @@ template <bool BF16> __device__ __forceinline__ v16f half_mfma32(const uint4& a,
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
+// v, cut to its sign, exponent and 19 bits and with the last of 20 set if anything was cut off (round to odd): what is rounded to fewer bits from here comes out
+// as if rounded from v itself
+__device__ __forceinline__ float odd_float(double v) {
+    const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v));
+    uint32_t odd;
+    asm("v_min_u32 %0, 1, %1" : "=v"(odd) : "v"(static_cast<uint32_t>(b)));  // (one instruction where a comparison and a choice are two)
+    return static_cast<float>(__longlong_as_double(static_cast<long long>(static_cast<uint64_t>(static_cast<uint32_t>(b >> 32) | odd) << 32)));
+}
+
 // sum + both 16-bit values of a pair
 template <bool BF16> __device__ __forceinline__ float half_pair_sum(uint32_t pair, float sum) {
     if constexpr (BF16) {

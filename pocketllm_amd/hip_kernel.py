@@ -613,7 +613,7 @@ def _aligned16(t: torch.Tensor) -> torch.Tensor:
 def fused_add_rms_norm_fp8_forward(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float, *, quant_eps: float = 1e-4,
                                    round_scale_pow2: bool = False, in_place: bool = False):
     """The step from one projection to the next FP8 one (fp8_gemm_forward) in one launch: total = x + residual rounded to their type,
-    fp8_act_quant_forward of fused_rms_norm_forward(total, weight, eps) with the normalized values kept in float32 in between.  x and residual
+    fp8_act_quant_forward of fused_rms_norm_forward(total, weight, eps) with the normalized values not rounded in between.  x and residual
     [..., dim] of one type, dim a multiple of 128 (up to 32768); without a residual total is x.  in_place: total is written into residual.
     Returns (codes float8_e4m3fn [..., dim], scales float32 [..., dim / 128], total).  A block of 128 with an infinity or a NaN has NaN codes."""
     made = _bindings.add_norm_fp8("fused_add_rms_norm_fp8_forward", x, residual, weight, float(eps), float(quant_eps), bool(round_scale_pow2), bool(in_place))
