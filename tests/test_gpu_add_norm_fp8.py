@@ -1,8 +1,8 @@
 """Residual + RMS normalisation + E4M3 codes in one launch against a float64 form.
 
 Errors counted: the sum of x and residual is rounded once, as torch rounds it (equal bits).  Normalized values: a product of three factors whose
-relative error is that of the sum of squares (at most 32 values one after the other, 22 levels above them, halved by the root), the reciprocal root
-(two units of float32) and two products: below (27 + 2 + 2) * 2^-23 < 2^-18.  Scales inherit it and a division.  Codes round a value that
+relative error is that of the sum of squares (eight values one after the other in float32, halved by the root): below 8 * 2^-24, held to 2^-18.  Scales inherit
+it and one rounding.  Codes round a value that
 is off by 2^-17 at most, so each lies between the codes of the two ends."""
 import numpy as np
 import pytest
@@ -46,6 +46,17 @@ def test_against_float64(rows, dim, pow2, dtype):
     assert codes.dtype == torch.float8_e4m3fn and scales.shape == (rows, dim // 128)
     assert torch.equal(total.cpu(), (x.float() + r.float()).to(dtype))
     _check_codes(codes, scales, total, w, pow2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_codes_are_those_of_the_exact_values(dtype):
+    """Without power-of-two scales the root falls out of a code: 448 t w / max |t w|, a product of 48 bits, a quotient and a product in 64: below 2^-45 off."""
+    x, r, w = _inputs(300, 4096, dtype, seed=6)
+    codes, _, total = K.fused_add_rms_norm_fp8_forward(x.to(DEV), r.to(DEV), w.to(DEV), EPS, quant_eps=QUANT_EPS)
+    n, s = P.add_norm(total.cpu().float().numpy(), w.numpy(), EPS, QUANT_EPS, False)
+    v = n / np.repeat(s, 128, axis=1)
+    got, lo, hi = codes.cpu().float().numpy().astype(np.float64), P.e4m3_round(v - np.abs(v) * 2.0 ** -45), P.e4m3_round(v + np.abs(v) * 2.0 ** -45)
+    assert ((got >= lo) & (got <= hi)).all()
 
 
 def test_in_place_no_residual_and_shapes():

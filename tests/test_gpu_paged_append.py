@@ -1,7 +1,7 @@
 """Appending to the paged E4M3 cache against a float64 form.
 
-Values: no arithmetic before the quantization and power-of-two scales, so codes and scales are equal.  Keys and queries turned in float32: x cos + y sin
-with one rounding of the product and one of the fused sum, so off by at most 2^-23 (|x cos| + |y sin|); a key's code lies between those of the two
+Values: no arithmetic before the quantization and power-of-two scales, so codes and scales are equal.  Queries turned in float32: x cos + y sin
+with one rounding of the product and one of the fused sum, so off by at most 2^-23 (|x cos| + |y sin|); keys in 64 bits, held to the same; a key's code lies between those of the two
 ends, a page's scale between theirs, and a query is within half a step of its type of a value between them."""
 import numpy as np
 import pytest
@@ -99,6 +99,28 @@ CASES = [
 @pytest.mark.parametrize("steps,pasts,heads,kv_heads,dim,page,rope,dtype", CASES)
 def test_against_float64(steps, pasts, heads, kv_heads, dim, page, rope, dtype):
     _run(steps, pasts, heads, kv_heads, dim, page, rope, dtype, seed=sum(steps))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_keys_codes_are_those_of_the_exact_values(dtype):
+    """Turned keys are two exact products and one sum in 64 bits: off by 2^-52 of the products at most."""
+    steps, dim, page, kv_heads, rope = [700, 500], 128, 64, 4, 128
+    cache, args, _ = _run(steps, [0, 0], 4, kv_heads, dim, page, rope, dtype, seed=8)
+    cos, sin = P.rotary_rows(cache.width * page, dim, rope)
+    pos = np.concatenate([np.arange(n) for n in steps])
+    k = _rows(sum(steps), kv_heads * dim, dtype, 9).float().numpy().astype(np.float64).reshape(-1, kv_heads, dim)
+    turned, off = P.turn(k, cos[pos], sin[pos], rope), 2.0 ** -52 * P.turn(np.abs(k), np.abs(cos[pos]), np.abs(sin[pos]), rope)
+    got, scales, at = P.e4m3_decode(args[0].view(torch.uint8).cpu().numpy()), args[2].cpu().numpy().astype(np.float64), 0
+    for s, n in enumerate(steps):
+        for p in range(-(-n // page)):
+            which, rows = cache.table[s, p], slice(at + p * page, at + min(n, (p + 1) * page))
+            v, e = turned[rows].transpose(1, 0, 2), off[rows].transpose(1, 0, 2)
+            scale = P.page_scale(np.abs(v).max((1, 2)))
+            assert np.array_equal(scales[which], scale)
+            lo, hi = P.e4m3_round((v - e) / scale[:, None, None]), P.e4m3_round((v + e) / scale[:, None, None])
+            mine = got[which][:, :v.shape[1]]
+            assert ((mine >= lo) & (mine <= hi)).all()
+        at += n
 
 
 def test_even_steps_without_offsets():
