@@ -205,10 +205,10 @@ def test_prompt_in_runs_against_float64(steps, pasts, heads, kv_heads, dim, page
     assert (got[cu[-1]:] == 0).all()
 
 
-# Calls of many rows and heads, of which a few heads are checked: one prompt whose workgroups are up to twice the compute units, the same behind a past, two long
+# Calls of many rows and heads, of which a few heads are checked (and one of few rows, in runs): one prompt whose workgroups are up to twice the compute units, the same behind a past, two long
 # runs of the keys, ragged ones, more sequences than a wave has lanes with several blocks in some.
 @pytest.mark.parametrize("steps,pasts,kv_heads,group,dim,page,dtype", [
-    ([700], [0], 64, 1, 64, 64, BF), ([600], [700], 64, 1, 128, 32, HF), ([300], [4200], 64, 1, 64, 128, BF), ([290, 1, 310], [100, 900, 700], 64, 1, 128, 32, BF),
+    ([20, 30], [600, 900], 2, 3, 128, 64, BF), ([700], [0], 64, 1, 64, 64, BF), ([600], [700], 64, 1, 128, 32, HF), ([300], [4200], 64, 1, 64, 128, BF), ([290, 1, 310], [100, 900, 700], 64, 1, 128, 32, BF),
     ([3] * 69 + [700, 0, 300], [10] * 69 + [0, 0, 200], 16, 2, 64, 16, HF)])
 def test_calls_of_many_rows(steps, pasts, kv_heads, group, dim, page, dtype):
     """NaN values: of the first sequence's sixth key in one dimension, of the last one's last key (one query sees it) in another."""
