@@ -316,14 +316,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     }
 
     // One tile: its softmax weights beside the next tile's scores, its value product beside the copies of the tiles behind.
-    auto step = [&](auto masked, int t, int half, v16f (&cur)[kSets], v16f (&next)[kSets]) {
-        constexpr bool MASKED = decltype(masked)::value;
+    // MASKED: some row does not see all of it; PLAIN: every row sees all of the next.
+    auto step = [&](auto masked, auto plain, int t, int half, v16f (&cur)[kSets], v16f (&next)[kSets]) {
+        constexpr bool MASKED = decltype(masked)::value, PLAIN = decltype(plain)::value;
         // the copies: keys two tiles ahead take the place of this tile's, values of the next tile that of the one before (behind the last tile: its
         // codes again, which nobody reads)
         auto copies = [&]() {
-            if (MASKED && tid == 0) nan_values[(t + 2) & 3] = 0;              // read two steps ago, written in the next
+            if (!PLAIN && tid == 0) nan_values[(t + 2) & 3] = 0;              // read two steps ago, written in the next
             store_keys(t + 2, half, keys_at.here, key_raw, key_scale);
-            store_values(std::integral_constant<bool, !MASKED>{}, t + 1, half ^ 1, values_here, value_raw, value_scale);
+            store_values(plain, t + 1, half ^ 1, values_here, value_raw, value_scale);
             value_raw = load_values(min(t + 2, last), keys_at);
             key_raw = load_keys(min(t + 3, last), next_at);
             key_scale = a.key_scales[next_at.at];
@@ -424,14 +425,23 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
         __syncthreads();
     };
     int t = t0;
+    const std::true_type yes;
+    const std::false_type no;
     for (; t + 3 <= min(full, end); t += 2) {                                 // (both steps copy values of tiles that every row sees whole)
-        step(std::false_type{}, t, 0, sa, sb);
-        step(std::false_type{}, t + 1, 1, sb, sa);
+        step(no, yes, t, 0, sa, sb);
+        step(no, yes, t + 1, 1, sb, sa);
     }
-    for (; t < end; ++t) {
-        step(std::true_type{}, t, (t - t0) & 1, sa, sb);
+    auto swap = [&]() {
 #pragma unroll
         for (int u = 0; u < kSets; ++u) sa[u] = sb[u];
+    };
+    for (; t < min(full, end); ++t) {                                         // (four prompts of up to 2000 tokens, 32 and 8 heads of 64: 64.4 -> 61.5 us)
+        step(no, no, t, (t - t0) & 1, sa, sb);
+        swap();
+    }
+    for (; t < end; ++t) {
+        step(yes, no, t, (t - t0) & 1, sa, sb);
+        swap();
     }
     float lower, upper;
     swapped_pair<32>(l, lower, upper);
