@@ -320,3 +320,35 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_prompts_in_runs_captured_and_on_two_streams_at_once():
+    """Workspaces between two launches: captured graphs replayed in turn on other lengths and offsets, and eager calls on two streams, against calls alone."""
+    cache = Cache([2500, 800, 1900], 2, 128, 64, seed=18)
+    args = cache.device()
+    held = args[5]
+    qs = [queries(120, 12, 128, BF, seed=i).to(DEV) for i in range(2)]
+    cu = torch.tensor([0, 70, 71, 110], dtype=torch.int32, device=DEV)
+    assert _ffi.load_library().pllm_paged_attention_prompt_workspace_bytes(120, 3, 12, 2, 128, cache.width * 64) > 0
+    want = [K.paged_attention_prompt_forward(q, *args, cu) for q in qs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(K.paged_attention_prompt_forward(qs[i], *args, cu))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph):
+            outs.append(K.paged_attention_prompt_forward(qs[i], *args, cu))
+    for lengths, offsets in (([2500, 800, 1900], [0, 70, 71, 110]), ([70, 1, 40], [0, 70, 71, 110]), ([1000, 0, 1800], [0, 5, 5, 120]), ([2400, 790, 1000], [0, 1, 100, 101])):
+        held.copy_(torch.tensor(lengths, dtype=torch.int32, device=DEV))
+        cu.copy_(torch.tensor(offsets, dtype=torch.int32, device=DEV))
+        for graph in graphs:
+            graph.replay()
+        for i in range(2):
+            assert torch.equal(outs[i], K.paged_attention_prompt_forward(qs[i], *args, cu)) and bool((outs[i][offsets[-1]:] == 0).all())
+        torch.cuda.synchronize()
