@@ -92,6 +92,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void add_norm_fp8_ke
         g[j] = load_eight<PLLM_F32>(a.weight, at);
     }
     double ss = 0.0;
+    bool held = true;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
         if (a.residual) {
@@ -108,7 +109,22 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void add_norm_fp8_ke
         float part = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) part = __builtin_fmaf(eight_value(xv[j], i), eight_value(xv[j], i), part);
+        held &= part >= 0x1p-80f && part <= FLT_MAX;
         ss += inside[j] ? static_cast<double>(part) : 0.0;
+    }
+    if (!__all(held)) {                                                       // squares that float32 does not hold, or not to its precision; zeros too
+        ss = 0.0;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            Eight<DT> again = xv[j];                                          // (nothing of this is to be shared with what follows: 20 registers)
+#pragma unroll
+            for (int i = 0; i < (DT == PLLM_F32 ? 2 : 1); ++i) asm("" : "+v"(again.a[i].x), "+v"(again.a[i].y), "+v"(again.a[i].z), "+v"(again.a[i].w));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const double v = eight_value(again, i);
+                ss += inside[j] ? v * v : 0.0;
+            }
+        }
     }
     ss += wide_peer<1>(ss);
     ss += wide_peer<2>(ss);

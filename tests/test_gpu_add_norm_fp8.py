@@ -59,6 +59,23 @@ def test_codes_are_those_of_the_exact_values(dtype):
     assert ((got >= lo) & (got <= hi)).all()
 
 
+@pytest.mark.parametrize("size", [2.0 ** 90, 2.0 ** -90])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_values_whose_squares_float32_does_not_hold(dtype, size):
+    x, r, w = _inputs(5, 2048, dtype, seed=12)
+    x, r = x * size, r * size
+    x[3], r[3] = 0, 0
+    codes, scales, total = K.fused_add_rms_norm_fp8_forward(x.to(DEV), r.to(DEV), w.to(DEV), 0.0 if size < 1 else EPS, quant_eps=QUANT_EPS)
+    live = [0, 1, 2, 4]
+    n, s = P.add_norm(total.cpu().float().numpy()[live] / size, w.numpy(), 0.0, QUANT_EPS, False)
+    assert (np.abs(scales.cpu().numpy()[live] - s) <= 2.0 ** -17 * s).all()
+    v = n / np.repeat(s, 128, axis=1)
+    got, lo, hi = codes.cpu().float().numpy().astype(np.float64)[live], P.e4m3_round(v - np.abs(v) * 2.0 ** -45), P.e4m3_round(v + np.abs(v) * 2.0 ** -45)
+    assert ((got >= lo) & (got <= hi)).all()
+    if size > 1:
+        assert (codes[3].float() == 0).all()
+
+
 def test_in_place_no_residual_and_shapes():
     x, r, w = _inputs(6, 1024, torch.bfloat16)
     xd, rd, wd = x.to(DEV), r.to(DEV), w.to(DEV)
