@@ -11,9 +11,9 @@
 // scores, the values' scale (halved, so that fp16 holds every value that rounds up from its largest) into the conversion, both exact.
 // The next 64 keys' codes are requested as soon as the registers of the last ones are free, the keys' before the softmax and the values' behind their
 // product, and page numbers a step ahead of them (64 sequences 139 -> 122 us, one of 100001 positions 49 -> 44; all at the end of the step before).
-// Bound: bytes, 2 * length * D codes per head, once for each 16 or 32 rows.  64 sequences of 1 to 8192 positions, 567 MB: 121 us, 4.7 TB/s, where a kernel
-// that only reads reaches 6: runs of 512 keys, which one sequence needs to fill the machine, begin and end too often (of 1024: 119 us, but 2048 positions
-// of one sequence 13.2 for 10.4).
+// Bound: bytes, 2 * length * D codes per head, once for each 16 or 32 rows.  64 sequences of 1 to 8192 positions, 567 MB: 118 us, 4.8 TB/s, where a kernel
+// that only reads reaches 6: runs of 512 keys, which one sequence needs to fill the machine, begin and end too often (of 1024: 3 % less,
+// but 2048 positions of one sequence 13.2 for 10.4).
 #include "paged_attention.h"
 #include "paged_device.h"
 
@@ -367,6 +367,48 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedDecode
     }
 }
 
+// The same for up to kFewRuns runs, a wave per query row: no waits for other waves (142 sequences of one or two tokens behind up to 3000 positions, in a call
+// that may hold more, 152 -> 133 us, seven of four tokens behind up to 6000 20.7 -> 18.7, 64 of one behind up to 8191 122.7 -> 117.9; twice as many runs in
+// registers 23 and 133).
+constexpr int kFewRuns = 16;
+template <bool BF16, int D>
+__global__ __launch_bounds__(kThreads) void paged_merge_few_kernel(const PagedDecodeArgs a) {
+    constexpr int kPer = D / 64;
+    const int lane = threadIdx.x & 63, group = a.heads / a.kv_heads, kvh = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads;
+    const int offset = a.cu_steps ? paged_offset(a.cu_steps, s, 0, a.tokens) : s * a.steps;
+    const int64_t rows = static_cast<int64_t>(a.cu_steps ? paged_offset(a.cu_steps, s + 1, 0, a.tokens) - offset : a.steps) * group;
+    if (rows > a.part_rows) return;
+    const int runs = max(1, paged_runs(paged_length(a.lengths[s], a.width, a.page_shift), a.kv_heads));
+    for (int row = kWaves * blockIdx.y + (threadIdx.x >> 6); row < rows; row += kWaves * gridDim.y) {
+        const size_t index = (static_cast<size_t>(blockIdx.x) * a.part_rows + row) * a.runs_bound;
+        const float2 mine = lane < runs ? a.stats[index + lane] : make_float2(-FLT_MAX, 0.0f);
+        float v[kFewRuns][kPer];
+#pragma unroll
+        for (int i0 = 0; i0 < kFewRuns; i0 += 4) {
+            if (i0 >= runs) break;                                            // (requests for a run again cost as much as for another)
+#pragma unroll
+            for (int i = i0; i < i0 + 4; ++i) {
+                const float* part = a.sums + (index + min(i, runs - 1)) * D + kPer * lane;
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) v[i][j] = part[j];
+            }
+        }
+        const float top = group_max<64>(mine.x), factor = __builtin_amdgcn_exp2f(mine.x - top), den = group_sum<64>(mine.y * factor);
+        float total[kPer] = {};
+#pragma unroll
+        for (int i = 0; i < kFewRuns; ++i) {
+            if (i >= runs) break;
+            const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(factor), i));
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) total[j] = __builtin_fmaf(v[i][j], f, total[j]);
+        }
+        const float inv = den == 0.0f ? 0.0f : 2.0f / den;
+        uint16_t* out = a.out + ((static_cast<size_t>(offset) + row / group) * a.heads + kvh * group + row % group) * D + kPer * lane;
+        if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(out) = half_pair<BF16>(total[0] * inv, total[1] * inv);
+        else *out = static_cast<uint16_t>(half_pair<BF16>(total[0] * inv, 0.0f));
+    }
+}
+
 template <bool BF16, int D>
 int launch(const PagedDecodeArgs& a, hipStream_t stream) {
     // Two sets of rows share what is read: eight sequences behind 20718 positions, four new tokens of eight heads each, 116 -> 96 us.  They cost a compute
@@ -379,7 +421,9 @@ int launch(const PagedDecodeArgs& a, hipStream_t stream) {
                            a.part_rows);
     if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
     if (a.sums) {
-        hipLaunchKernelGGL((paged_merge_kernel<BF16, D>), dim3(a.seqs * a.kv_heads, a.cu_steps ? std::min(a.part_rows, 16) : a.part_rows), dim3(kThreads), 0, stream, a);
+        const int rows = a.cu_steps ? std::min(a.part_rows, 16) : a.part_rows;
+        if (a.runs_bound <= kFewRuns) hipLaunchKernelGGL((paged_merge_few_kernel<BF16, D>), dim3(a.seqs * a.kv_heads, (rows + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, a);
+        else hipLaunchKernelGGL((paged_merge_kernel<BF16, D>), dim3(a.seqs * a.kv_heads, rows), dim3(kThreads), 0, stream, a);
         if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
     }
     return PLLM_OK;
