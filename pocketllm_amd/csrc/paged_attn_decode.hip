@@ -10,7 +10,7 @@
 // its values and two scales, whatever the page size.  Codes become 16-bit values in registers: E4M3 is exact in both types; the keys' scale goes on the
 // scores, the values' scale (halved, so that fp16 holds every value that rounds up from its largest) into the conversion, both exact.
 // The next 64 keys' codes are requested as soon as the registers of the last ones are free, the keys' before the softmax and the values' behind their
-// product, and page numbers a step ahead of them (64 sequences 139 -> 122 us, one of 100001 positions 49 -> 44; all at the end of the step before).
+// product, and page numbers a step ahead of them (with all of it requested at the end of a step 64 sequences took 139 us for 122, one of 100001 positions 49 for 44).
 // Bound: bytes, 2 * length * D codes per head, once for each 16 or 32 rows.  64 sequences of 1 to 8192 positions, 567 MB: 118 us, 4.8 TB/s, where a kernel
 // that only reads reaches 6: runs of 512 keys, which one sequence needs to fill the machine, begin and end too often (of 1024: 3 % less,
 // but 2048 positions of one sequence 13.2 for 10.4).
