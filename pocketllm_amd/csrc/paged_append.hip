@@ -29,7 +29,8 @@ struct AppendArgs {
     const int32_t* lengths; const int32_t* cu_steps;
     const float* cos_table; const float* sin_table;             // [>= width * page][D]
     int rows, seqs, even_steps, even_pages, heads,            // even: every sequence has that many new tokens, which touch that many pages at most
-        kv_heads, pool, width, rope_half, page_blocks, head_blocks;
+        kv_heads, pool, width, rope_half, page_blocks, head_blocks,
+        row_heads;                                              // few heads: a workgroup turns so many rows of them at a time
 };
 
 struct Phases { float4 c[2], s[2]; };
@@ -107,13 +108,56 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, int block, int
     }
 }
 
+// The same where all heads of a row, or of several, are one pass of the workgroup: kHeadPasses times as many rows (27170 tokens of 4 heads of 128, with 2 heads' keys
+// and values in pages of 64: 34.9 -> 23.8 us; a workgroup per row costs a nanosecond of the launch each).
+template <bool BF16, int D, int THREADS>
+__device__ __forceinline__ void turn_rows(const AppendArgs& a, int block, int page_shift) {
+    constexpr int kChunks = D / 8;
+    const int slot = threadIdx.x / kChunks, chunk = threadIdx.x % kChunks, d0 = 8 * chunk, half = a.rope_half, h = slot % a.heads;
+    const int partner = d0 < half ? d0 + half : d0 - half;
+#pragma unroll
+    for (int i = 0; i < kHeadPasses; ++i) {
+        const int row = (block * kHeadPasses + i) * a.row_heads + slot / a.heads;
+        const bool mine = slot < a.row_heads * a.heads && row < a.rows;
+        int s = mine ? row / max(a.even_steps, 1) : a.seqs;
+        if (a.cu_steps) {
+            s = a.seqs;
+            for (uint64_t left = __ballot(mine); left;) {                     // (a wave has eight rows at most)
+                const int one = __builtin_amdgcn_readlane(row, __ffsll(static_cast<unsigned long long>(left)) - 1);
+                const int found = paged_sequence(a.cu_steps, a.rows, a.seqs + 1, 1, 0, one);
+                const bool same = mine && row == one;
+                if (same) s = found;
+                left &= ~__ballot(same);
+            }
+        }
+        int64_t at = -1;
+        if (s < a.seqs) at = static_cast<int64_t>(a.lengths[s]) - paged_offset(a.cu_steps, s + 1, a.even_steps, a.rows) + row;
+        if (!mine) continue;
+        uint4 out = make_uint4(0, 0, 0, 0);                                   // rows that have no place in a sequence
+        if (at >= 0 && at < (static_cast<int64_t>(a.width) << page_shift)) {
+            const uint16_t* src = a.q + static_cast<size_t>(row) * a.q_stride + h * D;
+            out = *reinterpret_cast<const uint4*>(src + d0);
+            if (d0 < 2 * half) {
+                const uint4 across = *reinterpret_cast<const uint4*>(src + partner);
+                float own[8], other[8];
+                half_eight<BF16>(out, own);
+                half_eight<BF16>(across, other);
+                turn(own, other, load_phases(a, static_cast<int>(at), D, d0));
+                out = half_pack<BF16>(own);
+            }
+        }
+        *reinterpret_cast<uint4*>(a.q_out + (static_cast<size_t>(row) * a.heads + h) * D + d0) = out;
+    }
+}
+
 // Waves per SIMD that the rows of a page leave registers for (a thread's pass: eight for what is loaded, eight for what becomes codes).  Without the bound the 64-bit
 // products take half as many again (38 prompts of 715 tokens, 4 and 2 heads of 128, pages of 64: 40.6 us, with it 35.2, in 32 bits 34.6).
 constexpr int append_waves(int dim, int page) { return page * dim <= 4096 ? 8 : page * dim <= 8192 ? 6 : 4; }
 
+// ROWS: the queries go by turn_rows (in a kernel of its own: a choice in this one cost the others 2 - 7 %).
 // FEW: every sequence has the same few new tokens, no more than one pass over 64 threads takes: a workgroup of one wave (one token of each of 64 sequences
 // 6.3 -> 5.3 us, of 256 14.7 -> 9.6; 48 and 8 heads of 128)
-template <bool BF16, int D, int PAGE, bool FEW>
+template <bool BF16, int D, int PAGE, bool FEW, bool ROWS>
 __global__ __launch_bounds__(FEW ? 64 : 256, FEW ? 1 : append_waves(D, PAGE)) void paged_append_kernel(const AppendArgs a) {
     constexpr int kThreads = FEW ? 64 : 256;
     constexpr int kChunks = D / 8, kRows = kThreads / kChunks, kPasses = FEW ? 1 : (PAGE + kRows - 1) / kRows;
@@ -121,7 +165,11 @@ __global__ __launch_bounds__(FEW ? 64 : 256, FEW ? 1 : append_waves(D, PAGE)) vo
     __shared__ float red[4];
     __shared__ __align__(16) uint8_t turned[(FEW ? kRows : PAGE) * D];
     const int block = blockIdx.x, tid = threadIdx.x;
-    if (block >= a.page_blocks) { turn_queries<BF16, D, kThreads>(a, block - a.page_blocks, kShift); return; }
+    if (block >= a.page_blocks) {
+        if constexpr (ROWS) turn_rows<BF16, D, kThreads>(a, block - a.page_blocks, kShift);
+        else turn_queries<BF16, D, kThreads>(a, block - a.page_blocks, kShift);
+        return;
+    }
     const bool values = block & 1;
     const int head = (block >> 1) % a.kv_heads, slot = (block >> 1) / a.kv_heads;
     const int s = a.cu_steps ? paged_sequence(a.cu_steps, a.rows, a.seqs, PAGE, 2, slot) : slot / a.even_pages;
@@ -221,13 +269,13 @@ __global__ __launch_bounds__(FEW ? 64 : 256, FEW ? 1 : append_waves(D, PAGE)) vo
 }
 
 // (a kernel for every page size: small pages need few registers and little LDS, and their workgroups hide one another's waits)
-template <bool BF16, int D, bool FEW>
+template <bool BF16, int D, bool FEW, bool ROWS>
 void launch(const AppendArgs& a, int64_t page_tokens, dim3 grid, hipStream_t stream) {
     const dim3 threads(FEW ? 64 : 256);
-    if (page_tokens == 16) hipLaunchKernelGGL((paged_append_kernel<BF16, D, 16, FEW>), grid, threads, 0, stream, a);
-    else if (page_tokens == 32) hipLaunchKernelGGL((paged_append_kernel<BF16, D, 32, FEW>), grid, threads, 0, stream, a);
-    else if (page_tokens == 64) hipLaunchKernelGGL((paged_append_kernel<BF16, D, 64, FEW>), grid, threads, 0, stream, a);
-    else hipLaunchKernelGGL((paged_append_kernel<BF16, D, 128, FEW>), grid, threads, 0, stream, a);
+    if (page_tokens == 16) hipLaunchKernelGGL((paged_append_kernel<BF16, D, 16, FEW, ROWS>), grid, threads, 0, stream, a);
+    else if (page_tokens == 32) hipLaunchKernelGGL((paged_append_kernel<BF16, D, 32, FEW, ROWS>), grid, threads, 0, stream, a);
+    else if (page_tokens == 64) hipLaunchKernelGGL((paged_append_kernel<BF16, D, 64, FEW, ROWS>), grid, threads, 0, stream, a);
+    else hipLaunchKernelGGL((paged_append_kernel<BF16, D, 128, FEW, ROWS>), grid, threads, 0, stream, a);
 }
 
 }  // namespace
@@ -253,8 +301,10 @@ extern "C" int pllm_paged_kv_append(const void* q, int64_t q_stride, const void*
     const int64_t even_pages = paged_pages_touched(rows / seqs, page_tokens);
     const int64_t slots = cu_steps ? paged_slots(rows, static_cast<int>(seqs), static_cast<int>(page_tokens), 2) : seqs * even_pages, page_blocks = 2 * slots * kv_heads;
     const bool few = !cu_steps && rows / seqs <= 64 * 8 / head_dim;           // a decode step
-    const int64_t together = kHeadPasses * (few ? 64 : 256) * 8 / head_dim, head_blocks = q ? (heads + together - 1) / together : 0;
-    if (page_blocks + rows * head_blocks > 0xffffff) return PLLM_ERR_UNSUPPORTED;
+    const int64_t at_once = (few ? 64 : 256) * 8 / head_dim, head_blocks = q ? (heads + kHeadPasses * at_once - 1) / (kHeadPasses * at_once) : 0;
+    const int64_t row_heads = q && !few && heads <= at_once ? at_once / heads : 0;
+    const int64_t query_blocks = row_heads ? (rows + kHeadPasses * row_heads - 1) / (kHeadPasses * row_heads) : rows * head_blocks;
+    if (page_blocks + query_blocks > 0xffffff) return PLLM_ERR_UNSUPPORTED;
     const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new) | reinterpret_cast<uintptr_t>(q_out) |
                            reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) | reinterpret_cast<uintptr_t>(cos_table) |
                            reinterpret_cast<uintptr_t>(sin_table);
@@ -273,9 +323,10 @@ extern "C" int pllm_paged_kv_append(const void* q, int64_t q_stride, const void*
     a.pool = static_cast<int>(pool); a.width = static_cast<int>(table_width); a.rope_half = static_cast<int>(rope_dim / 2);
     a.page_blocks = static_cast<int>(page_blocks);
     a.head_blocks = static_cast<int>(head_blocks);
-    const dim3 grid(static_cast<unsigned>(page_blocks + rows * head_blocks));
+    a.row_heads = static_cast<int>(row_heads);
+    const dim3 grid(static_cast<unsigned>(page_blocks + query_blocks));
     const hipStream_t st = static_cast<hipStream_t>(stream);
-#define PLLM_APPEND(BF16, D) few ? launch<BF16, D, true>(a, page_tokens, grid, st) : launch<BF16, D, false>(a, page_tokens, grid, st)
+#define PLLM_APPEND(BF16, D) few ? launch<BF16, D, true, false>(a, page_tokens, grid, st) : row_heads ? launch<BF16, D, false, true>(a, page_tokens, grid, st) : launch<BF16, D, false, false>(a, page_tokens, grid, st)
     if (head_dim == 128) dtype == PLLM_BF16 ? (PLLM_APPEND(true, 128)) : (PLLM_APPEND(false, 128));
     else dtype == PLLM_BF16 ? (PLLM_APPEND(true, 64)) : (PLLM_APPEND(false, 64));
 #undef PLLM_APPEND
