@@ -115,20 +115,16 @@ __device__ __forceinline__ void turn_rows(const AppendArgs& a, int block, int pa
     constexpr int kChunks = D / 8;
     const int slot = threadIdx.x / kChunks, chunk = threadIdx.x % kChunks, d0 = 8 * chunk, half = a.rope_half, h = slot % a.heads;
     const int partner = d0 < half ? d0 + half : d0 - half;
+    // (the first row's sequence by a search, the others' from there on: 400 sequences of up to 60 tokens 32.2 -> 23.2 us)
+    int from = a.cu_steps ? paged_sequence(a.cu_steps, a.rows, a.seqs + 1, 1, 0, block * kHeadPasses * a.row_heads) : 0;
 #pragma unroll
     for (int i = 0; i < kHeadPasses; ++i) {
         const int row = (block * kHeadPasses + i) * a.row_heads + slot / a.heads;
         const bool mine = slot < a.row_heads * a.heads && row < a.rows;
         int s = mine ? row / max(a.even_steps, 1) : a.seqs;
         if (a.cu_steps) {
-            s = a.seqs;
-            for (uint64_t left = __ballot(mine); left;) {                     // (a wave has eight rows at most)
-                const int one = __builtin_amdgcn_readlane(row, __ffsll(static_cast<unsigned long long>(left)) - 1);
-                const int found = paged_sequence(a.cu_steps, a.rows, a.seqs + 1, 1, 0, one);
-                const bool same = mine && row == one;
-                if (same) s = found;
-                left &= ~__ballot(same);
-            }
+            while (mine && from < a.seqs && paged_offset(a.cu_steps, from + 1, 0, a.rows) <= row) ++from;
+            s = from;
         }
         int64_t at = -1;
         if (s < a.seqs) at = static_cast<int64_t>(a.lengths[s]) - paged_offset(a.cu_steps, s + 1, a.even_steps, a.rows) + row;
