@@ -93,6 +93,7 @@ CASES = [
     ([1], [0], 1, 1, 64, 16, 64, BF), ([1, 1, 1, 1], [0, 15, 16, 63], 6, 1, 128, 16, 64, HF), ([5, 17, 1], [14, 0, 31], 4, 2, 128, 32, 128, BF),
     ([64, 65, 63], [0, 0, 1], 48, 8, 128, 64, 64, BF), ([130, 3, 200], [0, 125, 77], 5, 5, 64, 128, 32, HF), ([33], [100], 16, 2, 128, 128, 96, BF),
     ([100, 50], [7, 60], 2, 2, 128, 16, 16, HF), ([40], [0], 8, 1, 64, 64, 0, BF), ([7, 0, 9], [3, 0, 20], 3, 1, 64, 32, 48, BF),
+    ([i % 4 for i in range(130)], [(7 * i) % 40 if i % 4 else 0 for i in range(130)], 3, 1, 128, 16, 64, BF), ([0, 0, 5] * 30, [0, 0, 9] * 30, 17, 1, 128, 32, 128, HF),
 ]
 
 
