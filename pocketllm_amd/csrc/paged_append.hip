@@ -7,7 +7,7 @@
 //
 // A workgroup owns a page's keys, or its values, of one head: its scale needs no atomics and no second pass.  Values turn in LDS, since a page
 // holds them with the tokens innermost.  The queries are rows behind these workgroups in the same grid.
-// Bound: bytes for prompts (4096 tokens of 48 and 8 heads of 128: 128 MB in 25 us, 5.1 TB/s; in 32 bits 24), the chain of a workgroup's loads
+// Bound: bytes for prompts (4096 tokens of 48 and 8 heads of 128: 128 MB in 24 us, 5.3 TB/s; in 32 bits 23.6), the chain of a workgroup's loads
 // (offset, length, row and page, scale: 4 us) and the number of workgroups (two for every page and head) for decode steps.
 #include "paged_device.h"
 #include "pllm_internal.h"
