@@ -576,12 +576,18 @@ int prompt_runs(int64_t blocks, int64_t positions) {
 // sequence's keys by its own length (48 and 8 heads: 64 single tokens behind up to 8000 positions 434 -> 150 us, 142 times one or two behind up to 3000
 // 377 -> 173; 64 and 8 heads, 8 times 8 tokens behind up to 8000 86 -> 54).  Its launches cost a few microseconds where no sequence is so short (30
 // continuations of up to 200 tokens behind up to 4000 209 -> 215 us, six prompts 319 -> 323): 16 rows or one token's, unless most
-// sequences must be short.  Only where tables are wider than one run of it; of one sequence by the rows of the call, so that one kernel's launches are enough; not
-// where what the rows would keep between two launches passes a gigabyte.
+// sequences must be short.  Of one sequence by the rows of the call, so that one kernel's launches are enough; not where what the rows would keep between
+// two launches passes a gigabyte.  Where tables are no wider than one of its runs, only if most sequences have 16 rows at most and their blocks here would pass half the
+// compute units (64 single tokens behind up to 900 positions 58 -> 18.6 us, behind 100 23.7 -> 9.9, 142 of one or two 115 -> 36; but eight of up to three 17.7 -> 25.8), or
+// all of them together are few (four of one or two 15.7 -> 11.3).
 int few_rows(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
-    const int64_t group = heads / kv_heads, all = tokens * group;
-    if (positions <= kPagedOneRun || group > kPagedFewRows || (seqs == 1 && all > kPagedFewRows)) return 0;
-    int64_t rows = std::min<int64_t>(all <= 2 * kPagedFewRows * seqs ? kPagedFewRows : std::min<int64_t>(std::max<int64_t>(group, 16), kPagedFewRows), all);
+    const int64_t group = heads / kv_heads, all = tokens * group, least = std::max<int64_t>(group, 16);
+    if (group > kPagedFewRows) return 0;
+    int64_t rows;
+    if (positions > kPagedOneRun) rows = seqs == 1 && all > kPagedFewRows ? 0 : (all <= 2 * kPagedFewRows * seqs ? kPagedFewRows : least);
+    else if (seqs == 1) rows = 0;
+    else rows = all <= kPagedFewRows ? all : (all <= least * seqs && 2 * seqs * kv_heads > compute_units() ? least : 0);
+    rows = std::min(rows, all);
     while (rows > 0 && paged_decode_parts_bytes(seqs, rows, kv_heads, head_dim, positions) > (size_t{1} << 30)) rows /= 2;
     return rows < group ? 0 : static_cast<int>(rows);
 }

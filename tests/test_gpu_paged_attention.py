@@ -240,6 +240,19 @@ def test_many_sequences():
     close(_decode(cache, q), *cache.attention(q.view(-1, 3, 64).double().numpy(), _even(150, 1)), HF)
 
 
+@pytest.mark.parametrize("steps,pasts,heads,kv_heads,dim,page,dtype", [
+    ([1, 2, 1, 0, 1], [500, 30, 0, 0, 900], 6, 1, 128, 64, BF), ([1] * 40 + [9, 0, 1], list(range(0, 800, 20)) + [300, 0, 5], 12, 4, 64, 32, HF),
+    ([1, 1, 40] * 12, [100, 0, 70] * 12, 16, 16, 64, 16, BF)])
+def test_short_sequences_before_narrow_tables(steps, pasts, heads, kv_heads, dim, page, dtype):
+    """Few rows in all, mostly short ones of many sequences and heads, rows behind the last."""
+    cache = Cache([n + p if n else 0 for n, p in zip(steps, pasts)], kv_heads, dim, page, seed=sum(steps))
+    cu = np.concatenate([[0], np.cumsum(steps)])
+    q = queries(cu[-1] + 3, heads, dim, dtype, seed=4)
+    got = K.paged_attention_prompt_forward(q.to(DEV), *cache.device(), torch.tensor(cu, dtype=torch.int32, device=DEV))
+    close(got[:cu[-1]], *cache.attention(q[:cu[-1]].view(-1, heads, dim).double().numpy(), cu), dtype)
+    assert (got[cu[-1]:] == 0).all()
+
+
 def test_no_sequences_and_no_tokens():
     cache = Cache([10], 1, 64, 16)
     kp, vp, ks, vs, table, lengths = cache.device()
