@@ -350,9 +350,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
             swapped_pair<32>(top, lower, upper);
             top = __builtin_elementwise_maximum(lower, upper);
         }
-        // The maximum follows when a row's weights would pass 2^8: what it is exactly falls out of the quotient.
-        if (__any(top > m + 8.0f)) {
-            const float m_new = top > m + 8.0f ? top : m, back = __builtin_amdgcn_exp2f(m - m_new);
+        // The maximum follows when a row's weights would pass 2^8: what it is exactly falls out of the quotient.  (By the difference, which neighbours have
+        // exactly: from 2^27 on m + 8 may be the next float, m + 16, and a weight of 2^16 is fp16's infinity.)
+        const bool follows = top - m > 8.0f;
+        if (__any(follows)) {
+            const float m_new = follows ? top : m, back = __builtin_amdgcn_exp2f(m - m_new);
             l *= back;
 #pragma unroll
             for (int i = 0; i < kDimTiles; ++i)
