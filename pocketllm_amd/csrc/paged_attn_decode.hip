@@ -27,6 +27,16 @@ namespace {
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kStep = 64;                       // keys that a wave takes at a time
 
+// Softmax weights are 2^(score - m) and are rounded to 16 bits for the second product (matrix instructions on float32 have a sixteenth of the rate); their sum takes
+// them unrounded: roundings to the nearest lean to no side.  In fp16 a weight below 2^-14 is rounded to a multiple of 2^-24, one below 2^-25 to nothing, so the
+// largest of a wave's is 2^15 there: what is lost of a weight is 2^-40 of it at most (with 1, 1024 keys whose scores are 16.5 below another, to base e, lost an
+// eighth of what they add up to).  The factor is in numerator and denominator alike; scores from 2^20 on, whose steps could make more of 15, are compared with
+// themselves.  bf16 has float32's range.
+template <bool BF16> __device__ __forceinline__ float weights_from(float top) {
+    if constexpr (BF16) return top;
+    else return fabsf(top) < 0x1p20f ? top - 15.0f : top;
+}
+
 // SETS of 16 query rows; rows of one key/value head: token * group + head in the group
 template <bool BF16, int D, int SETS>
 __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kernel(const PagedDecodeArgs a, int least_rows, int most_rows) {
@@ -64,7 +74,7 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
     }
     const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
     v4f o[SETS][kTiles];
-    float m[SETS], l[SETS], late = 1.0f;        // of the column; l over the lane's own keys
+    float m[SETS], l[SETS], late = 1.0f;        // of the column, m as weights_from has it; l over the lane's own keys
 #pragma unroll
     for (int c = 0; c < SETS; ++c) {
 #pragma unroll
@@ -177,7 +187,7 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
             float lower, upper;
             swapped_pair<16>(top, lower, upper);
             swapped_pair<32>(fmaxf(lower, upper), lower, upper);
-            const float m_new = fmaxf(m[c], fmaxf(lower, upper));
+            const float m_new = fmaxf(m[c], weights_from<BF16>(fmaxf(lower, upper)));
             if (__any(m_new > m[c])) {
                 const float back = __builtin_amdgcn_exp2f(m[c] - m_new);
                 l[c] *= back;

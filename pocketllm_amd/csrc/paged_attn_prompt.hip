@@ -29,6 +29,18 @@ namespace {
 constexpr int kWaves = 8, kThreads = 64 * kWaves, kBlockRows = 32 * kWaves;
 constexpr int kTile = 64;                       // keys per step
 
+// Softmax weights are 2^(score - m), m what the row's largest score is compared with.  They are rounded to 16 bits for the second product (matrix instructions on
+// float32 have a sixteenth of the rate), and in fp16 a weight below 2^-14 is rounded to a multiple of 2^-24, one below 2^-25 to nothing.  So m stays 2^11 below
+// the largest score where it is set and follows when a weight would pass 2^15: what is lost of a weight is 2^-36 of the row's largest at most, of a hundred
+// thousand together 2^-19.  (With m at the largest score 32768 keys whose scores are 16.5 below one, to base e, lost an eighth of what they add up to.)  The
+// factor is in numerator and denominator alike.  Scores from 2^20 on, whose steps could make more of 11, are compared with themselves.  bf16 has float32's
+// range: m is the largest score, and follows from 2^8 on.
+template <bool BF16> constexpr float kMostWeight = BF16 ? 8.0f : 15.0f;
+template <bool BF16> __device__ __forceinline__ float weights_from(float top) {
+    if constexpr (BF16) return top;
+    else return fabsf(top) < 0x1p20f ? top - 11.0f : top;
+}
+
 struct PagedPromptArgs {
     const uint16_t* q; size_t q_stride;         // elements between tokens
     const uint8_t* key_pages; const uint8_t* value_pages;
@@ -36,7 +48,7 @@ struct PagedPromptArgs {
     const int32_t* table; size_t table_stride;
     const int32_t* lengths; const int32_t* cu_steps;
     uint16_t* out;
-    float* sums; float2* stats;                 // of several runs of a block's keys: [runs][tokens * heads][D], maximum (base 2) and sum of weights; or null
+    float* sums; float2* stats;                 // of several runs of a block's keys: [runs][tokens * heads][D], m (base 2) and sum of weights; or null
     float scale;                                // base 2
     int few_rows;                               // sequences of so many query rows or fewer are another kernel's
     int runs, tokens, seqs, heads, kv_heads, page_shift, pool, width, slots;
@@ -219,7 +231,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     v16f o[kDimTiles], sa[kSets], sb[kSets];
 #pragma unroll
     for (int i = 0; i < kDimTiles; ++i) o[i] = zero;
-    float m = -FLT_MAX, l = 0.0f;                                             // of the lane's query; l over its half of the keys
+    float m = -FLT_MAX, l = 0.0f;                                             // of the lane's query, as weights_from has it; l over its half of the keys
     // S^T of the tile in one half of LDS
     auto scores = [&](int half, v16f (&sc)[kSets]) {
         const unsigned char* kt = smem + half * kTileBytes + 32 * second * (2 * D);
@@ -350,11 +362,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
             swapped_pair<32>(top, lower, upper);
             top = __builtin_elementwise_maximum(lower, upper);
         }
-        // The maximum follows when a row's weights would pass 2^8: what it is exactly falls out of the quotient.  (By the difference, which neighbours have
-        // exactly: from 2^27 on m + 8 may be the next float, m + 16, and a weight of 2^16 is fp16's infinity.)
-        const bool follows = top - m > 8.0f;
+        // The maximum follows when a row's weights would pass their most: what it is exactly falls out of the quotient.  (By the difference, which neighbours
+        // have exactly: from 2^27 on m + 8 may be the next float, m + 16, and a weight of 2^16 is fp16's infinity.)
+        const bool follows = top - m > kMostWeight<BF16>;
         if (__any(follows)) {
-            const float m_new = follows ? top : m, back = __builtin_amdgcn_exp2f(m - m_new);
+            const float m_new = follows ? weights_from<BF16>(top) : m, back = __builtin_amdgcn_exp2f(m - m_new);
             l *= back;
 #pragma unroll
             for (int i = 0; i < kDimTiles; ++i)
