@@ -135,7 +135,7 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
                 for (int c = 0; c < SETS; ++c) sc[c][t] = half_mfma16<BF16>(hi, qf[c][1], half_mfma16<BF16>(lo, qf[c][0], sc[c][t]));
             }
         }
-        const float factor = BF16 ? fminf(key_factor * late, FLT_MAX) : key_factor;
+        const float factor = fminf(key_factor * late, FLT_MAX);               // (beyond float32 a score of zero would be NaN)
 #pragma unroll
         for (int c = 0; c < SETS; ++c)
 #pragma unroll
