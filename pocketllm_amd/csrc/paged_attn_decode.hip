@@ -318,6 +318,42 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
     }
 }
 
+// The runs of one query row together, by a wave, in their order: no waits for other waves (142 sequences of one or two tokens behind up to 3000 positions, in a call
+// that may hold more, 152 -> 133 us, seven of four tokens behind up to 6000 20.7 -> 18.7, 64 of one behind up to 8191 122.7 -> 117.9; twice as many runs in
+// registers 23 and 133).
+constexpr int kFewRuns = 16;
+template <bool BF16, int D>
+__device__ __forceinline__ void merge_few(const PagedDecodeArgs& a, int index0, int row, int runs, int offset, int kvh, int group) {
+    constexpr int kPer = D / 64;
+    const int lane = threadIdx.x & 63;
+    const size_t index = (static_cast<size_t>(index0) + row) * a.runs_bound;
+    const float2 mine = lane < runs ? a.stats[index + lane] : make_float2(-FLT_MAX, 0.0f);
+    float v[kFewRuns][kPer];
+#pragma unroll
+    for (int i0 = 0; i0 < kFewRuns; i0 += 4) {
+        if (i0 >= runs) break;                                                // (requests for a run again cost as much as for another)
+#pragma unroll
+        for (int i = i0; i < i0 + 4; ++i) {
+            const float* part = a.sums + (index + min(i, runs - 1)) * D + kPer * lane;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) v[i][j] = part[j];
+        }
+    }
+    const float top = group_max<64>(mine.x), factor = __builtin_amdgcn_exp2f(mine.x - top), den = group_sum<64>(mine.y * factor);
+    float total[kPer] = {};
+#pragma unroll
+    for (int i = 0; i < kFewRuns; ++i) {
+        if (i >= runs) break;
+        const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(factor), i));
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) total[j] = __builtin_fmaf(v[i][j], f, total[j]);
+    }
+    const float inv = den == 0.0f ? 0.0f : 2.0f / den;
+    uint16_t* out = a.out + ((static_cast<size_t>(offset) + row / group) * a.heads + kvh * group + row % group) * D + kPer * lane;
+    if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(out) = half_pair<BF16>(total[0] * inv, total[1] * inv);
+    else *out = static_cast<uint16_t>(half_pair<BF16>(total[0] * inv, 0.0f));
+}
+
 // A workgroup per query row (where sequences have different numbers of rows, per 16th row): its runs together, an order that the number of runs fixes.
 // All of up to 64 runs are requested at once.
 template <bool BF16, int D>
@@ -332,6 +368,10 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedDecode
     const int64_t rows = static_cast<int64_t>(a.cu_steps ? paged_offset(a.cu_steps, s + 1, 0, a.tokens) - offset : a.steps) * group;
     if (rows > a.part_rows) return;
     const int runs = max(1, paged_runs(paged_length(a.lengths[s], a.width, a.page_shift), a.kv_heads));     // (256 at most)
+    if (runs <= kFewRuns) {                                                   // (by the sequence, not by the table that has room for more: equal bits)
+        for (int row = blockIdx.y + gridDim.y * (tid >> 6); row < rows; row += kWaves * gridDim.y) merge_few<BF16, D>(a, index0, row, runs, offset, kvh, group);
+        return;
+    }
     const int slot = tid / kLanes, d = 4 * (tid % kLanes);
     for (int row = blockIdx.y; row < rows; row += gridDim.y) {
         const size_t index = static_cast<size_t>(index0) + row;
@@ -377,46 +417,16 @@ __global__ __launch_bounds__(kThreads) void paged_merge_kernel(const PagedDecode
     }
 }
 
-// The same for up to kFewRuns runs, a wave per query row: no waits for other waves (142 sequences of one or two tokens behind up to 3000 positions, in a call
-// that may hold more, 152 -> 133 us, seven of four tokens behind up to 6000 20.7 -> 18.7, 64 of one behind up to 8191 122.7 -> 117.9; twice as many runs in
-// registers 23 and 133).
-constexpr int kFewRuns = 16;
+// For tables that have room for kFewRuns runs at most: a wave per query row.
 template <bool BF16, int D>
 __global__ __launch_bounds__(kThreads) void paged_merge_few_kernel(const PagedDecodeArgs a) {
-    constexpr int kPer = D / 64;
-    const int lane = threadIdx.x & 63, group = a.heads / a.kv_heads, kvh = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads;
+    const int group = a.heads / a.kv_heads, kvh = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads;
     const int offset = a.cu_steps ? paged_offset(a.cu_steps, s, 0, a.tokens) : s * a.steps;
     const int64_t rows = static_cast<int64_t>(a.cu_steps ? paged_offset(a.cu_steps, s + 1, 0, a.tokens) - offset : a.steps) * group;
     if (rows > a.part_rows) return;
     const int runs = max(1, paged_runs(paged_length(a.lengths[s], a.width, a.page_shift), a.kv_heads));
-    for (int row = kWaves * blockIdx.y + (threadIdx.x >> 6); row < rows; row += kWaves * gridDim.y) {
-        const size_t index = (static_cast<size_t>(blockIdx.x) * a.part_rows + row) * a.runs_bound;
-        const float2 mine = lane < runs ? a.stats[index + lane] : make_float2(-FLT_MAX, 0.0f);
-        float v[kFewRuns][kPer];
-#pragma unroll
-        for (int i0 = 0; i0 < kFewRuns; i0 += 4) {
-            if (i0 >= runs) break;                                            // (requests for a run again cost as much as for another)
-#pragma unroll
-            for (int i = i0; i < i0 + 4; ++i) {
-                const float* part = a.sums + (index + min(i, runs - 1)) * D + kPer * lane;
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) v[i][j] = part[j];
-            }
-        }
-        const float top = group_max<64>(mine.x), factor = __builtin_amdgcn_exp2f(mine.x - top), den = group_sum<64>(mine.y * factor);
-        float total[kPer] = {};
-#pragma unroll
-        for (int i = 0; i < kFewRuns; ++i) {
-            if (i >= runs) break;
-            const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(factor), i));
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) total[j] = __builtin_fmaf(v[i][j], f, total[j]);
-        }
-        const float inv = den == 0.0f ? 0.0f : 2.0f / den;
-        uint16_t* out = a.out + ((static_cast<size_t>(offset) + row / group) * a.heads + kvh * group + row % group) * D + kPer * lane;
-        if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(out) = half_pair<BF16>(total[0] * inv, total[1] * inv);
-        else *out = static_cast<uint16_t>(half_pair<BF16>(total[0] * inv, 0.0f));
-    }
+    for (int row = kWaves * blockIdx.y + (threadIdx.x >> 6); row < rows; row += kWaves * gridDim.y)
+        merge_few<BF16, D>(a, blockIdx.x * a.part_rows, row, runs, offset, kvh, group);
 }
 
 template <bool BF16, int D>
