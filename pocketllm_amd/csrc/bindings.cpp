@@ -411,9 +411,10 @@ bool paged_args(PyObject* const* a, const Tensor* like, Paged& p) {
         if (t->get_device() != like->get_device()) return false;
     return true;
 }
-// rows [tokens, width] that the kernels read as they lie: values side by side, every row on 16 bytes
+// rows [tokens, width] that the kernels read as they lie: values side by side, every row on 16 bytes (one row's view may have any stride between rows)
+int64_t row_stride(const Tensor* t) { return t->size(0) > 1 ? t->stride(0) : t->size(1); }
 bool rows16(const Tensor* t) {
-    return t && t->layout() == at::kStrided && t->has_storage() && t->is_cuda() && t->dim() == 2 && t->stride(1) == 1 && t->stride(0) % 8 == 0 && t->stride(0) >= t->size(1) && on16(t);
+    return t && t->layout() == at::kStrided && t->has_storage() && t->is_cuda() && t->dim() == 2 && t->stride(1) == 1 && row_stride(t) % 8 == 0 && row_stride(t) >= t->size(1) && on16(t);
 }
 bool half_type(const Tensor* t) { return t->scalar_type() == at::kHalf || t->scalar_type() == at::kBFloat16; }
 
@@ -446,7 +447,7 @@ PyObject* paged_kv_append(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const bool turns = q && rope;
     Tensor out;
     if (turns) out = at::empty(q->sizes(), q->options());
-    const int st = unlocked(pllm_paged_kv_append, turns ? q->const_data_ptr() : nullptr, turns ? q->stride(0) : 0, k->const_data_ptr(), k->stride(0), v->const_data_ptr(), v->stride(0),
+    const int st = unlocked(pllm_paged_kv_append, turns ? q->const_data_ptr() : nullptr, turns ? row_stride(q) : 0, k->const_data_ptr(), row_stride(k), v->const_data_ptr(), row_stride(v),
                             code_of(k->scalar_type()), turns ? out.data_ptr() : nullptr, static_cast<uint8_t*>(p.keys->data_ptr()), static_cast<uint8_t*>(p.values->data_ptr()),
                             p.key_scales->data_ptr<float>(), p.value_scales->data_ptr<float>(), p.pool, p.page, p.table->const_data_ptr<int32_t>(), p.table_stride, p.width,
                             p.lengths->const_data_ptr<int32_t>(), cu, cos ? cos->const_data_ptr<float>() : nullptr, sin ? sin->const_data_ptr<float>() : nullptr,
@@ -494,7 +495,7 @@ PyObject* paged_attention_prompt(PyObject*, PyObject* const* a, Py_ssize_t nargs
     Tensor out = at::empty(q->sizes(), q->options()), ws;
     const size_t bytes = pllm_paged_attention_prompt_workspace_bytes(tokens, p.seqs, heads, p.kv_heads, p.dim, p.width * p.page);
     if (bytes) ws = workspace(*q, bytes);
-    const int st = unlocked(pllm_paged_attention_prompt, q->const_data_ptr(), q->stride(0), code_of(q->scalar_type()), p.key_codes(), p.value_codes(),
+    const int st = unlocked(pllm_paged_attention_prompt, q->const_data_ptr(), row_stride(q), code_of(q->scalar_type()), p.key_codes(), p.value_codes(),
                             p.key_scales->const_data_ptr<float>(), p.value_scales->const_data_ptr<float>(), p.pool, p.page, p.table->const_data_ptr<int32_t>(), p.table_stride,
                             p.width, p.lengths->const_data_ptr<int32_t>(), cu->const_data_ptr<int32_t>(), tokens, p.seqs, heads, p.kv_heads, p.dim, scale, out.data_ptr(),
                             bytes ? ws.data_ptr() : nullptr, bytes, stream_of(*q));

@@ -650,6 +650,8 @@ def fused_add_rms_norm_fp8_forward(x: torch.Tensor, residual: torch.Tensor | Non
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t [tokens, width] as rows that the kernels can read: values side by side, every row on 16 bytes (slices of a wider projection pass as they are)."""
+    if t.size(0) == 1 and t.stride(1) == 1:
+        t = t[0].unsqueeze(0)                                                  # one row: its view may have any stride between rows, of a transposed column 1
     if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.size(1) and t.data_ptr() % 16 == 0:
         return t
     return _aligned16(t)
