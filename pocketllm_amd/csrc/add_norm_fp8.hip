@@ -3,11 +3,11 @@
 //     t = round(x + residual);  n = t * rsqrt(mean(t^2) + eps) * weight;  per 128 values s = max(amax |n|, quant_eps) / 448 (a power of two
 //     when asked for), code = E4M3(n / s)
 // The sum leaves rounded to the stream's type, and what is normalized is that rounded value, so the operator says what the three separate ones
-// say; the normalized values become codes as they are (the separate operators round them to 16 bits in between).  Without power-of-two scales the root
-// falls out of the codes, E4M3(448 t w / max |t w|).  Products, quotient and root are in 64 bits (32 by 8 to 24 bits: exact) and cut on the way to a code so that
-// it is the one that the values themselves round to: in 32 bits one in a million is its neighbour, 6 % away.
-// Bound: bytes for prompts (8192 rows of 5120 bf16 values: 295 MB in 55 us, 5.4 TB/s, what a large copy reaches; in 32 bits the same), the start of a launch and
-// one round trip to memory for few rows (4.1 us; in 32 bits 3.8).
+// say; the normalized values become codes as they are (the separate operators round them to 16 bits in between).  Squares, their sum, root, products and quotient are
+// in 64 bits, and a value is cut on the way to a code so that the code is the one that the value itself rounds to: in 32 bits one in a million is its neighbour, 6 %
+// away.  (Without power-of-two scales the root falls out of the codes of all blocks above quant_eps, E4M3(448 t w / max |t w|).)
+// Bound: bytes for prompts (8192 rows of 5120 bf16 values: 295 MB in 55 us, 5.4 TB/s; with squares summed in 32 bits 54 - 56), the start of a launch and one round trip to
+// memory for few rows (3.0 us from begin to end, 4.2 from one launch to the next).
 #include "paged_device.h"
 #include "pllm_internal.h"
 
@@ -99,7 +99,6 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void add_norm_fp8_ke
         g[j] = load_eight<PLLM_F32>(a.weight, inside[j] ? e0[j] : 0);
     }
     double ss = 0.0;
-    bool held = true;
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
         if (a.residual) {
@@ -113,25 +112,17 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void add_norm_fp8_ke
                 for (int i = 0; i < (DT == PLLM_F32 ? 2 : 1); ++i) dst[i] = xv[j].a[i];
             }
         }
-        float part = 0.0f;
+        // squares and their sum in 64 bits: exact squares, and no row whose sum float32 would not hold
+        Eight<DT> again = xv[j];                                              // (nothing of this is to be shared with what follows: 20 registers)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) part = __builtin_fmaf(eight_value(xv[j], i), eight_value(xv[j], i), part);
-        held &= !inside[j] || (part >= 0x1p-80f && part <= FLT_MAX);
-        ss += inside[j] ? static_cast<double>(part) : 0.0;
-    }
-    if (!__all(held)) {                                                       // squares that float32 does not hold, or not to its precision; zeros too
-        ss = 0.0;
+        for (int i = 0; i < (DT == PLLM_F32 ? 2 : 1); ++i) asm("" : "+v"(again.a[i].x), "+v"(again.a[i].y), "+v"(again.a[i].z), "+v"(again.a[i].w));
+        double part = 0.0;
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) {
-            Eight<DT> again = xv[j];                                          // (nothing of this is to be shared with what follows: 20 registers)
-#pragma unroll
-            for (int i = 0; i < (DT == PLLM_F32 ? 2 : 1); ++i) asm("" : "+v"(again.a[i].x), "+v"(again.a[i].y), "+v"(again.a[i].z), "+v"(again.a[i].w));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const double v = eight_value(again, i);
-                ss += inside[j] ? v * v : 0.0;
-            }
+        for (int i = 0; i < 8; ++i) {
+            const double v = eight_value(again, i);
+            part = __builtin_fma(v, v, part);
         }
+        ss += inside[j] ? part : 0.0;
     }
     ss += wide_peer<1>(ss);
     ss += wide_peer<2>(ss);
