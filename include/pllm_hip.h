@@ -477,7 +477,8 @@ int pllm_fused_add_rms_norm_fp8(const void* x, const void* residual, int dtype, 
  *                lengths[s] - 1; null: every sequence has rows / seqs of them
  * page_tokens 16, 32, 64 or 128; head_dim 64 or 128; 16-bit types; pages, rows and tables on 16 (scales, tables on 4) bytes.  Table entries outside
  * the pool and positions outside the table have no page: nothing is stored there and no key is seen there.  No two sequences of a call may write
- * into one page; full pages may be shared.
+ * into one page; full pages may be shared.  An fp16 attention call reads values of up to 131008 (what fp16 tokens append is below); a cache that bf16 tokens
+ * filled may hold larger ones, which are infinities to it.
  *
  * Appends: keys turned by the rotary rows of their positions (cos_table, sin_table float32 [table_positions, head_dim], half-split pairs, sin carrying
  * the sign, as one position's rows of pllm_attention_decode; table_positions >= table_width * page_tokens; rope_dim a multiple of 16, 0: none) and

@@ -13,8 +13,8 @@
 //
 // SPLIT, for calls of few blocks: 128 rows, waves 4 to 7 have those of 0 to 3 and the other 32 keys of every tile, and what they leave meets in LDS at the end.
 //
-// Bound: 4 D operations per row and key.  8192 tokens of 48 and 8 heads, 825 G operations: 800 us, 1030 T/s, where a large matrix product of the library
-// reaches 1155; what is between is the softmax's vector instructions (44 % of the cycles, the matrix unit 42 %: the two waves of a SIMD overlap them in
+// Bound: 4 D operations per row and key.  8192 tokens of 48 and 8 heads, 825 G operations: 793 us, 1040 T/s, where a large matrix product of the library
+// reaches 1155; what is between is the softmax's vector instructions (48 % of the cycles, the matrix unit 47 %: the two waves of a SIMD overlap them in
 // part) and the barrier of each tile.
 #include "paged_attention.h"
 #include "paged_device.h"
@@ -587,8 +587,8 @@ int prompt_runs(int64_t blocks, int64_t positions) {
 }
 
 // Query rows up to which a sequence goes to the kernel of the decode steps, whose tiles have 16 or 32 rows where these have 256, and which cuts every
-// sequence's keys by its own length (48 and 8 heads: 64 single tokens behind up to 8000 positions 434 -> 150 us, 142 times one or two behind up to 3000
-// 377 -> 173; 64 and 8 heads, 8 times 8 tokens behind up to 8000 86 -> 54).  Its launches cost a few microseconds where no sequence is so short (30
+// sequence's keys by its own length (48 and 8 heads: 64 single tokens behind up to 8000 positions 434 -> 131 us, 142 times one or two behind up to 3000
+// 377 -> 133; 64 and 8 heads, 8 times 8 tokens behind up to 8000 86 -> 52).  Its launches cost a few microseconds where no sequence is so short (30
 // continuations of up to 200 tokens behind up to 4000 209 -> 215 us, six prompts 319 -> 323): 16 rows or one token's, unless most
 // sequences must be short.  Of one sequence by the rows of the call, so that one kernel's launches are enough; not where what the rows would keep between
 // two launches passes a gigabyte.  Where tables are no wider than one of its runs, only if most sequences have 16 rows at most and their blocks here would pass half the

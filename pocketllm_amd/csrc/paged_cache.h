@@ -38,7 +38,7 @@ PLLM_HD int paged_offset(const int32_t* cu_steps, int s, int even_steps, int row
     return clamp_int(cu_steps ? cu_steps[s] : s * even_steps, 0, rows);
 }
 
-// Work on ragged rows is dealt out in units (pages, tiles of queries) without a plan made beforehand: sequence s has the slots
+// The pages that ragged rows go to are dealt out (units of a page's tokens) without a plan made beforehand: sequence s has the slots
 // from offset_s / unit + spare * s on.  Offsets that grow give every sequence at least n / unit + spare slots of its own.
 PLLM_HD int64_t paged_first_slot(int64_t offset, int s, int unit, int spare) { return offset / unit + static_cast<int64_t>(spare) * s; }
 PLLM_HD int64_t paged_slots(int64_t rows, int seqs, int unit, int spare) { return rows / unit + static_cast<int64_t>(spare) * seqs; }

@@ -750,7 +750,8 @@ def paged_attention_decode_forward(q: torch.Tensor, key_pages: torch.Tensor, val
     """Grouped-query attention of one or a few new tokens per sequence over a paged E4M3 cache that holds them already (paged_kv_append_forward): q
     [seqs, steps, heads * head_dim] (or [seqs, heads * head_dim]), token i of `steps` at position lengths[s] - steps + i, seeing the positions up to its own.
     scale: head_dim ** -0.5 by default.  Returns q's shape and dtype; tokens that see no key get zeros.  The table's width bounds the work that is
-    dealt out: pass a narrower view, block_table[:, :n], where no sequence is longer."""
+    dealt out: pass a narrower view, block_table[:, :n], where no sequence is longer (the same bits).  float16 queries read values of up to 131008, more than
+    float16 tokens append; larger ones, of a cache that bfloat16 tokens filled, are infinities to them."""
     what = "paged_attention_decode"
     out = _bindings.paged_attention_decode("paged_attention_decode_forward", q, key_pages, value_pages, key_scales, value_scales, block_table, lengths, scale)
     if out is not None:
