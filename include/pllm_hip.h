@@ -517,6 +517,77 @@ int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int dtype, cons
                                 int64_t kv_heads, int64_t head_dim, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 
+/*
+ * pllm_paged_kv_append for new tokens that are turned by the rotary rows positions[row] (int32 [rows], clamped to the tables; null: by their places in the cache):
+ * the nodes of a drafted tree lie one behind the other, and siblings have one position (no counterpart in the reference).  With positions the tables may have any number of rows.
+ */
+int pllm_paged_kv_append_at(const void* q, int64_t q_stride, const void* k_new, int64_t k_stride, const void* v_new, int64_t v_stride, int dtype, void* q_out,
+                            uint8_t* key_pages, uint8_t* value_pages, float* key_scales, float* value_scales, int64_t pool, int64_t page_tokens,
+                            const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* lengths, const int32_t* cu_steps,
+                            const float* cos_table, const float* sin_table, int64_t table_positions, const int32_t* positions, int64_t rope_dim, int64_t rows,
+                            int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, void* stream);
+
+/*
+ * Serving by drafted trees over the paged cache; no counterpart in the reference, which decodes one token at a time (src/models/minimax_m2/architecture.py:417-472).
+ *
+ * A tree: the new tokens of a sequence (cu_steps, or rows / seqs each) are its nodes, at most 256; parents [rows] int32 is the node that each hangs from,
+ * counted within the sequence: an earlier one, or -1 (as is anything else) for a node that follows the past.
+ *
+ * Attention of all nodes over the cache that already holds them: every node sees the positions before the tree, its ancestors and itself.  Otherwise as
+ * pllm_paged_attention_prompt; cu_steps may be null.  A sequence with more than 256 new tokens gets zeros.
+ * workspace: pllm_paged_attention_tree_workspace_bytes(..., even: no cu_steps, ..., table_width * page_tokens) bytes, 16-byte aligned.
+ */
+size_t pllm_paged_attention_tree_workspace_bytes(int64_t tokens, int64_t seqs, int even, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions);
+int pllm_paged_attention_tree(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pages, const uint8_t* value_pages, const float* key_scales,
+                              const float* value_scales, int64_t pool, int64_t page_tokens, const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                              const int32_t* lengths, const int32_t* parents, const int32_t* cu_steps, int64_t tokens, int64_t seqs, int64_t heads,
+                              int64_t kv_heads, int64_t head_dim, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The path of each tree that the sampled tokens follow (no counterpart in the reference): from node 0 on the first child whose drafted token (int64 [rows]) is the one sampled (int64 [rows]) at
+ * the node before it.  kept [seqs, most] int32 its nodes, -1 behind them (a path ends at `most`, 1 .. 256, nodes); counts [seqs]; tokens [seqs] int64 what is sampled at its last node;
+ * new_lengths [seqs] = lengths - new tokens + counts.  A sequence without new tokens: count 0, token -1.
+ */
+int pllm_draft_tree_accept(const int32_t* parents, const int64_t* drafted, const int64_t* sampled, const int32_t* lengths, const int32_t* cu_steps, int64_t rows,
+                           int64_t seqs, int64_t most, int32_t* kept, int32_t* counts, int64_t* tokens, int32_t* new_lengths, void* stream);
+
+/*
+ * The keys and values of that path to the places right behind the past, in every layer's cache (no counterpart in the reference): with n new tokens (cu_steps, or `steps`) in lengths[s] positions, token
+ * lengths[s] - n + kept[s][j] becomes token lengths[s] - n + j, j < counts[s] (and until kept stops rising or leaves the tree).
+ *   caches  [layers][4] on the host: key_pages, value_pages, key_scales, value_scales of every layer; read during the call
+ * The scale of a page that tokens move to becomes the largest that its content had; codes are scaled down to it.  Tokens without a page on either side stay away.
+ * No two sequences write into one page.
+ */
+int pllm_paged_cache_compact(void* const* caches, int64_t layers, int64_t pool, int64_t page_tokens, const int32_t* block_table, int64_t table_stride,
+                             int64_t table_width, const int32_t* lengths, const int32_t* kept, int64_t most, const int32_t* counts, const int32_t* cu_steps,
+                             int64_t steps, int64_t seqs, int64_t kv_heads, int64_t head_dim, void* stream);
+
+/*
+ * The sequences of the next step out of the present ones (no counterpart in the reference).  Row r of new_table [rows, table_width] goes on with the first kept[r] tokens of row sources[r] of block_table
+ * [seqs, table_width] (any other source: with none) and has pages for reserve[r] tokens.
+ *   uses    [pool] int32: holders of every page, the entries of block_table among them (a page is free at 0); entries outside the pool (-1) hold nothing
+ * Whole kept pages are shared.  A page that is kept in part stays the row's if no other new row and no holder outside block_table has it (of rows that keep it in part
+ * the first has it), the others get a copy in every layer.  Free pages go lowest first to the rows in their order; missing [rows] int32 says how many pages a
+ * row lacks (their entries are -1).  new_uses [pool]: the holders afterwards; block_table's rows hold nothing any more.  caches as above.
+ */
+size_t pllm_paged_cache_fork_workspace_bytes(int64_t rows, int64_t pool);
+int pllm_paged_cache_fork(void* const* caches, int64_t layers, int64_t pool, int64_t page_tokens, const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                          const int32_t* uses, const int32_t* sources, const int32_t* kept, const int32_t* reserve, int64_t seqs, int64_t rows, int64_t kv_heads,
+                          int64_t head_dim, int32_t* new_table, int32_t* new_uses, int32_t* missing, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * A token per row of logits [rows, vocab] (stride elements apart; float32, fp16 or bf16), from a random number uniform[row] of [0, 1) (clamped to it):
+ *     w_i = exp((x_i - max x) / temperature); in the order x falling, index rising, what is kept is the first min(n_k, n_p, n_m): n_k = top_k (0: all), n_p the least n
+ *     whose first n have top_p of what the first n_k add up to (from 1 on: all), n_m those with w >= min_p (up to 1)
+ *     token = the least i with (sum of w over kept j <= i) > uniform * (sum of w over kept)
+ * Temperature 0: the largest logit, the first of equal ones.  NaN and minus infinity are never a token; -1 where a row has no other.  Parameters per row (float32, top_k
+ * int32), or null and one value for all.  A row's token depends on the row alone.  vocab up to 2^20, rows up to 65535; no counterpart in the reference.
+ */
+size_t pllm_sample_tokens_workspace_bytes(int64_t rows, int64_t vocab, int dtype);
+int pllm_sample_tokens(const void* logits, int64_t stride, int dtype, const float* uniform, const float* temperature, float temperature_all, const int32_t* top_k,
+                       int64_t top_k_all, const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t rows, int64_t vocab, int64_t* tokens,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -87,6 +87,19 @@ SIGNATURES = {
     "pllm_paged_attention_prompt_workspace_bytes": (_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "pllm_paged_attention_prompt": (_int, [_c_void_p, _i64, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p,
                                            _c_void_p, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _c_void_p, _c_void_p, _size_t, _c_void_p]),
+    "pllm_paged_kv_append_at": (_int, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64,
+                                       _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64, _i64, _i64, _c_void_p]),
+    "pllm_paged_attention_tree_workspace_bytes": (_size_t, [_i64, _i64, _int, _i64, _i64, _i64, _i64]),
+    "pllm_paged_attention_tree": (_int, [_c_void_p, _i64, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p,
+                                         _c_void_p, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _c_void_p, _c_void_p, _size_t, _c_void_p]),
+    "pllm_draft_tree_accept": (_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "pllm_paged_cache_compact": (_int, [_c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p]),
+    "pllm_paged_cache_fork_workspace_bytes": (_size_t, [_i64, _i64]),
+    "pllm_paged_cache_fork": (_int, [_c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _c_void_p,
+                                     _c_void_p, _c_void_p, _size_t, _c_void_p]),
+    "pllm_sample_tokens_workspace_bytes": (_size_t, [_i64, _i64, _int]),
+    "pllm_sample_tokens": (_int, [_c_void_p, _i64, _int, _c_void_p, _c_void_p, ctypes.c_float, _c_void_p, _i64, _c_void_p, ctypes.c_float, _c_void_p, ctypes.c_float, _i64, _i64,
+                                  _c_void_p, _c_void_p, _size_t, _c_void_p]),
 }
 
 _LIB = None

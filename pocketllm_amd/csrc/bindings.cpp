@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <vector>
 
 #include "../../include/pllm_hip.h"
@@ -503,6 +504,197 @@ PyObject* paged_attention_prompt(PyObject*, PyObject* const* a, Py_ssize_t nargs
     END_HANDLE_TH_ERRORS
 }
 
+bool ints(const Tensor* t, const Tensor* like, int64_t n) { return plain(t, at::kInt) && t->dim() == 1 && t->size(0) == n && t->get_device() == like->get_device(); }
+// cu_steps or None
+bool offsets_arg(PyObject* o, const Tensor* like, int64_t seqs, const int32_t*& cu) {
+    cu = nullptr;
+    if (o == Py_None) return true;
+    const Tensor* t = tensor(o);
+    if (!ints(t, like, seqs + 1)) return false;
+    cu = t->const_data_ptr<int32_t>();
+    return true;
+}
+
+// (name, q, the cache's six, parents, cu_steps or None, scale or None) -> out
+PyObject* paged_attention_tree(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 11) Py_RETURN_NONE;
+    const Tensor *q = tensor(a[1]), *parents = tensor(a[8]);
+    Paged p;
+    const int32_t* cu;
+    if (!rows16(q) || !here(q) || !half_type(q) || q->numel() == 0 || !paged_args(a + 2, q, p) || !ints(parents, q, q->size(0)) || !offsets_arg(a[9], q, p.seqs, cu)) Py_RETURN_NONE;
+    const int64_t tokens = q->size(0), width = q->size(1), heads = width / p.dim;
+    if (width % p.dim || heads % p.kv_heads || (!cu && (tokens % p.seqs || tokens / p.seqs > 256))) Py_RETURN_NONE;
+    float scale = 1.0f / std::sqrt(static_cast<float>(p.dim));
+    if (a[10] != Py_None && (!float_arg(a[10], scale) || !(scale >= 0.0f && scale <= 0x1p127f))) Py_RETURN_NONE;
+    Tensor out = at::empty(q->sizes(), q->options()), ws;
+    const size_t bytes = pllm_paged_attention_tree_workspace_bytes(tokens, p.seqs, cu == nullptr, heads, p.kv_heads, p.dim, p.width * p.page);
+    if (bytes) ws = workspace(*q, bytes);
+    const int st = unlocked(pllm_paged_attention_tree, q->const_data_ptr(), row_stride(q), code_of(q->scalar_type()), p.key_codes(), p.value_codes(), p.key_scales->const_data_ptr<float>(),
+                            p.value_scales->const_data_ptr<float>(), p.pool, p.page, p.table->const_data_ptr<int32_t>(), p.table_stride, p.width, p.lengths->const_data_ptr<int32_t>(),
+                            parents->const_data_ptr<int32_t>(), cu, tokens, p.seqs, heads, p.kv_heads, p.dim, scale, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
+                            stream_of(*q));
+    return st == PLLM_OK ? THPVariable_Wrap(std::move(out)) : failed(a[0], st);
+    END_HANDLE_TH_ERRORS
+}
+
+// a number for all rows or float32 [rows]
+bool row_floats(PyObject* o, const Tensor* like, const float*& each, float& all) {
+    each = nullptr;
+    all = 0.0f;
+    if (float_arg(o, all)) return true;
+    const Tensor* t = tensor(o);
+    if (!plain(t, at::kFloat) || t->dim() != 1 || t->size(0) != like->size(0) || t->get_device() != like->get_device()) return false;
+    each = t->const_data_ptr<float>();
+    return true;
+}
+
+// (name, logits, uniform, temperature, top_k, top_p, min_p) -> tokens
+PyObject* sample_tokens(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 7) Py_RETURN_NONE;
+    const Tensor *x = tensor(a[1]), *u = tensor(a[2]);
+    if (!x || x->layout() != at::kStrided || !x->has_storage() || !x->is_cuda() || x->dim() != 2 || x->numel() == 0 || !here(x) || code_of(x->scalar_type()) < 0) Py_RETURN_NONE;
+    const int64_t rows = x->size(0), vocab = x->size(1), stride = rows > 1 ? x->stride(0) : vocab;
+    if (vocab > (1 << 20) || rows > 0xffff || (x->stride(1) != 1 && vocab > 1) || stride < vocab) Py_RETURN_NONE;
+    if (!plain(u, at::kFloat) || u->dim() != 1 || u->size(0) != rows || u->get_device() != x->get_device()) Py_RETURN_NONE;
+    const float *t = nullptr, *p = nullptr, *m = nullptr;
+    float t_all, p_all, m_all;
+    if (!row_floats(a[3], x, t, t_all) || !row_floats(a[5], x, p, p_all) || !row_floats(a[6], x, m, m_all)) Py_RETURN_NONE;
+    const int32_t* k = nullptr;
+    int64_t k_all = 0;
+    if (!int_arg(a[4], k_all)) {
+        const Tensor* ks = tensor(a[4]);
+        if (!ints(ks, x, rows)) Py_RETURN_NONE;
+        k = ks->const_data_ptr<int32_t>();
+        k_all = 0;
+    }
+    if (!(t_all >= 0.0f) || !(p_all >= 0.0f) || !(m_all >= 0.0f && m_all <= 1.0f) || k_all < 0) Py_RETURN_NONE;
+    const int code = code_of(x->scalar_type());
+    Tensor tokens = at::empty({rows}, x->options().dtype(at::kLong));
+    const size_t bytes = pllm_sample_tokens_workspace_bytes(rows, vocab, code);
+    Tensor ws = workspace(*x, bytes);
+    const int st = unlocked(pllm_sample_tokens, x->const_data_ptr(), stride, code, u->const_data_ptr<float>(), t, t_all, k, k_all, p, p_all, m, m_all, rows, vocab,
+                            tokens.data_ptr<int64_t>(), ws.data_ptr(), bytes, stream_of(*x));
+    return st == PLLM_OK ? THPVariable_Wrap(std::move(tokens)) : failed(a[0], st);
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* tuple_of(std::initializer_list<Tensor> tensors) {
+    PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
+    if (!out) return nullptr;
+    Py_ssize_t i = 0;
+    for (const Tensor& t : tensors) PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(t));
+    return out;
+}
+
+// (name, parents, drafted, sampled, lengths, cu_steps or None, most or None) -> (kept, counts, tokens, lengths)
+PyObject* draft_tree_accept(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 7) Py_RETURN_NONE;
+    const Tensor *parents = tensor(a[1]), *drafted = tensor(a[2]), *sampled = tensor(a[3]), *lengths = tensor(a[4]);
+    if (!plain(parents, at::kInt) || parents->dim() != 1 || parents->size(0) == 0 || !here(parents) || !plain(lengths, at::kInt) || lengths->dim() != 1 || lengths->size(0) == 0 ||
+        lengths->get_device() != parents->get_device())
+        Py_RETURN_NONE;
+    const int64_t rows = parents->size(0), seqs = lengths->size(0);
+    for (const Tensor* t : {drafted, sampled})
+        if (!plain(t, at::kLong) || t->dim() != 1 || t->size(0) != rows || t->get_device() != parents->get_device()) Py_RETURN_NONE;
+    const int32_t* cu;
+    if (!offsets_arg(a[5], parents, seqs, cu) || (!cu && (rows % seqs || rows / seqs > 256))) Py_RETURN_NONE;
+    int64_t most = cu ? 256 : rows / seqs;
+    if (a[6] != Py_None && (!int_arg(a[6], most) || most < 1 || most > 256)) Py_RETURN_NONE;
+    Tensor kept = at::empty({seqs, most}, lengths->options()), counts = at::empty({seqs}, lengths->options()), news = at::empty({seqs}, lengths->options()),
+           tokens = at::empty({seqs}, drafted->options());
+    const int st = unlocked(pllm_draft_tree_accept, parents->const_data_ptr<int32_t>(), drafted->const_data_ptr<int64_t>(), sampled->const_data_ptr<int64_t>(),
+                            lengths->const_data_ptr<int32_t>(), cu, rows, seqs, most, kept.data_ptr<int32_t>(), counts.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(), news.data_ptr<int32_t>(),
+                            stream_of(*parents));
+    return st == PLLM_OK ? tuple_of({kept, counts, tokens, news}) : failed(a[0], st);
+    END_HANDLE_TH_ERRORS
+}
+
+// The caches of a model's layers: a list of tuples (or lists) of four tensors, all of one shape and on the table's device, which is the current one.
+struct Stack {
+    std::vector<void*> at;
+    Paged p;
+    int64_t layers = 0;
+};
+bool stack_args(PyObject* list, PyObject* table, PyObject* ints_of_seqs, Stack& s) {
+    if ((!PyList_CheckExact(list) && !PyTuple_CheckExact(list)) || PySequence_Fast_GET_SIZE(list) == 0 || PySequence_Fast_GET_SIZE(list) > 1024) return false;
+    const Tensor* of_table = tensor(table);
+    if (!of_table || !of_table->is_cuda() || !here(of_table)) return false;
+    s.layers = PySequence_Fast_GET_SIZE(list);
+    s.at.reserve(4 * s.layers);
+    for (Py_ssize_t i = 0; i < s.layers; ++i) {
+        PyObject* layer = PySequence_Fast_GET_ITEM(list, i);
+        if ((!PyList_CheckExact(layer) && !PyTuple_CheckExact(layer)) || PySequence_Fast_GET_SIZE(layer) != 4) return false;
+        PyObject* six[6];
+        for (int j = 0; j < 4; ++j) six[j] = PySequence_Fast_GET_ITEM(layer, j);
+        six[4] = table;
+        six[5] = ints_of_seqs;
+        Paged p;
+        if (!paged_args(six, of_table, p)) return false;
+        if (i == 0) s.p = p;
+        else if (p.pool != s.p.pool || p.kv_heads != s.p.kv_heads || p.page != s.p.page || p.dim != s.p.dim) return false;
+        for (const Tensor* t : {p.keys, p.values, p.key_scales, p.value_scales}) s.at.push_back(t->data_ptr());
+    }
+    for (int kind = 0; kind < 2; ++kind) {                                    // (the Python path states the error)
+        const uintptr_t bytes = kind ? s.p.key_scales->nbytes() : s.p.keys->nbytes();
+        std::vector<uintptr_t> some;
+        for (int64_t i = 0; i < 4 * s.layers; ++i)
+            if (i % 4 / 2 == kind) some.push_back(reinterpret_cast<uintptr_t>(s.at[i]));
+        std::sort(some.begin(), some.end());
+        for (size_t i = 1; i < some.size(); ++i)
+            if (some[i] - some[i - 1] < bytes) return false;
+    }
+    return true;
+}
+
+// (name, layers, table, lengths, kept, counts, steps or cu_steps) -> True
+PyObject* paged_cache_compact(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    Stack s;
+    if (nargs != 7 || !stack_args(a[1], a[2], a[3], s)) Py_RETURN_NONE;
+    const Tensor *kept = tensor(a[4]), *counts = tensor(a[5]);
+    if (!plain(kept, at::kInt) || kept->dim() != 2 || kept->size(0) != s.p.seqs || kept->size(1) < 1 || kept->size(1) > 256 || kept->get_device() != s.p.table->get_device() ||
+        !ints(counts, s.p.table, s.p.seqs))
+        Py_RETURN_NONE;
+    int64_t steps = 0;
+    const int32_t* cu = nullptr;
+    if (int_arg(a[6], steps)) {
+        if (steps < 1 || steps > 256) Py_RETURN_NONE;
+    } else if (a[6] == Py_None || !offsets_arg(a[6], s.p.table, s.p.seqs, cu)) Py_RETURN_NONE;
+    const int st = unlocked(pllm_paged_cache_compact, s.at.data(), s.layers, s.p.pool, s.p.page, s.p.table->const_data_ptr<int32_t>(), s.p.table_stride, s.p.width,
+                            s.p.lengths->const_data_ptr<int32_t>(), kept->const_data_ptr<int32_t>(), kept->size(1), counts->const_data_ptr<int32_t>(), cu, cu ? 0 : steps, s.p.seqs,
+                            s.p.kv_heads, s.p.dim, stream_of(*s.p.table));
+    if (st != PLLM_OK) return failed(a[0], st);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// (name, layers, table, uses, sources, kept, reserve) -> (table, uses, missing)
+PyObject* paged_cache_fork(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 7) Py_RETURN_NONE;
+    const Tensor *table = tensor(a[2]), *uses = tensor(a[3]), *sources = tensor(a[4]), *kept = tensor(a[5]), *reserve = tensor(a[6]);
+    if (!table || !table->is_cuda() || table->dim() != 2 || table->size(0) <= 0 || !plain(sources, at::kInt) || sources->dim() != 1 || sources->size(0) == 0) Py_RETURN_NONE;
+    Tensor lengths = at::empty({table->size(0)}, sources->options());         // (what the cache's checks ask for)
+    PyObject* wrapped = THPVariable_Wrap(lengths);
+    Stack s;
+    const bool ok = wrapped && stack_args(a[1], a[2], wrapped, s);
+    Py_XDECREF(wrapped);
+    if (!ok) Py_RETURN_NONE;
+    const int64_t rows = sources->size(0);
+    if (!ints(uses, table, s.p.pool) || !ints(sources, table, rows) || !ints(kept, table, rows) || !ints(reserve, table, rows)) Py_RETURN_NONE;
+    Tensor out = at::empty({rows, s.p.width}, sources->options()), new_uses = at::empty({s.p.pool}, sources->options()), missing = at::empty({rows}, sources->options());
+    const size_t bytes = pllm_paged_cache_fork_workspace_bytes(rows, s.p.pool);
+    Tensor ws = workspace(*table, bytes);
+    const int st = unlocked(pllm_paged_cache_fork, s.at.data(), s.layers, s.p.pool, s.p.page, s.p.table->const_data_ptr<int32_t>(), s.p.table_stride, s.p.width,
+                            uses->const_data_ptr<int32_t>(), sources->const_data_ptr<int32_t>(), kept->const_data_ptr<int32_t>(), reserve->const_data_ptr<int32_t>(), s.p.seqs, rows,
+                            s.p.kv_heads, s.p.dim, out.data_ptr<int32_t>(), new_uses.data_ptr<int32_t>(), missing.data_ptr<int32_t>(), ws.data_ptr(), bytes, stream_of(*table));
+    return st == PLLM_OK ? tuple_of({out, new_uses, missing}) : failed(a[0], st);
+    END_HANDLE_TH_ERRORS
+}
+
 // (tensor) -> whether the functions above may read its memory as it lies (the device aside)
 PyObject* dense_tensor(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
@@ -515,6 +707,7 @@ PyMethodDef methods[] = {
     PLLM_FN(quant_gemm), PLLM_FN(quant_gemm_accumulate), PLLM_FN(quant_gemm_multi), PLLM_FN(q8_0_gemm), PLLM_FN(fp8_block_gemm),
     PLLM_FN(attention_decode), PLLM_FN(route_rmsnorm), PLLM_FN(moe_single_token), PLLM_FN(dense_tensor),
     PLLM_FN(add_norm_fp8), PLLM_FN(paged_kv_append), PLLM_FN(paged_attention_decode), PLLM_FN(paged_attention_prompt),
+    PLLM_FN(paged_attention_tree), PLLM_FN(sample_tokens), PLLM_FN(draft_tree_accept), PLLM_FN(paged_cache_compact), PLLM_FN(paged_cache_fork),
 #undef PLLM_FN
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_bindings", "Native host path of the per-token operators.", -1, methods, nullptr, nullptr, nullptr, nullptr};

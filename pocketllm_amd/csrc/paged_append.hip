@@ -27,13 +27,17 @@ struct AppendArgs {
     float* key_scales; float* value_scales;
     const int32_t* table; size_t table_stride;
     const int32_t* lengths; const int32_t* cu_steps;
-    const float* cos_table; const float* sin_table;             // [>= width * page][D]
+    const float* cos_table; const float* sin_table;             // [>= width * page][D], or [positions_end][D] where `positions` says which row
+    const int32_t* positions;                                   // [rows] or null: the place in the cache
+    int positions_end;
     int rows, seqs, even_steps, even_pages, heads,            // even: every sequence has that many new tokens, which touch that many pages at most
         kv_heads, pool, width, rope_half, page_blocks, head_blocks,
         row_heads;                                              // few heads: a workgroup turns so many rows of them at a time
 };
 
 struct Phases { float4 c[2], s[2]; };
+// the row of the phases that a new token is turned by
+__device__ __forceinline__ int turned_by(const AppendArgs& a, int row, int place) { return a.positions ? clamp_int(a.positions[row], 0, a.positions_end - 1) : place; }
 __device__ __forceinline__ float of4(const float4* f, int i) {
     const float4 v = f[i >> 2];
     return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
@@ -63,15 +67,6 @@ __device__ __forceinline__ float page_scale(float amax) {
 __device__ __forceinline__ float codable(float v, float inv) {
     return fabsf(v) <= FLT_MAX ? fminf(fmaxf(v * inv, -448.0f), 448.0f) : __uint_as_float(0x7fc00000u);
 }
-__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d) {
-    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true));
-}
-__device__ __forceinline__ uint32_t scaled_codes(uint32_t w, float ratio) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), true);
-    return four_codes(lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio);
-}
-
 template <bool BF16, int D, int THREADS>
 __device__ __forceinline__ void turn_queries(const AppendArgs& a, int block, int page_shift) {
     constexpr int kChunks = D / 8, kHeadsPerPass = THREADS / kChunks;
@@ -84,7 +79,7 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, int block, int
     const int position = static_cast<int>(at);
     const bool turns = placed && d0 < 2 * half;
     Phases p;
-    if (turns) p = load_phases(a, position, D, d0);
+    if (turns) p = load_phases(a, turned_by(a, row, position), D, d0);
     const int partner = d0 < half ? d0 + half : d0 - half;
     const uint16_t* src = a.q + static_cast<size_t>(row) * a.q_stride;
     uint16_t* dst = a.q_out + static_cast<size_t>(row) * a.heads * D;
@@ -138,7 +133,7 @@ __device__ __forceinline__ void turn_rows(const AppendArgs& a, int block, int pa
                 float own[8], other[8];
                 half_eight<BF16>(out, own);
                 half_eight<BF16>(across, other);
-                turn(own, other, load_phases(a, static_cast<int>(at), D, d0));
+                turn(own, other, load_phases(a, turned_by(a, row, static_cast<int>(at)), D, d0));
                 out = half_pack<BF16>(own);
             }
         }
@@ -207,7 +202,8 @@ __global__ __launch_bounds__(FEW ? 64 : 256, FEW ? 1 : append_waves(D, PAGE)) vo
         if (turns) {
             float across[8];
             half_eight<BF16>(other[i], across);
-            turn_for_codes(v[i], across, load_phases(a, lo + min(tid / kChunks + kRows * i, count - 1), D, d0));
+            const int place = lo + min(tid / kChunks + kRows * i, count - 1);
+            turn_for_codes(v[i], across, load_phases(a, turned_by(a, offset + place - first, place), D, d0));
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) amax = fabsf(v[i][j]) <= FLT_MAX ? fmaxf(amax, fabsf(v[i][j])) : amax;
@@ -277,10 +273,11 @@ void launch(const AppendArgs& a, int64_t page_tokens, dim3 grid, hipStream_t str
 }  // namespace
 }  // namespace pllm
 
-extern "C" int pllm_paged_kv_append(const void* q, int64_t q_stride, const void* k_new, int64_t k_stride, const void* v_new, int64_t v_stride, int dtype,
+extern "C" int pllm_paged_kv_append_at(const void* q, int64_t q_stride, const void* k_new, int64_t k_stride, const void* v_new, int64_t v_stride, int dtype,
                                     void* q_out, uint8_t* key_pages, uint8_t* value_pages, float* key_scales, float* value_scales, int64_t pool,
                                     int64_t page_tokens, const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* lengths,
-                                    const int32_t* cu_steps, const float* cos_table, const float* sin_table, int64_t table_positions, int64_t rope_dim,
+                                    const int32_t* cu_steps, const float* cos_table, const float* sin_table, int64_t table_positions,
+                                    const int32_t* positions, int64_t rope_dim,
                                     int64_t rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, void* stream) {
     using namespace pllm;
     if (!k_new || !v_new || !key_pages || !value_pages || !key_scales || !value_scales || !block_table || !lengths) return PLLM_ERR_INVALID_ARGUMENT;
@@ -288,7 +285,7 @@ extern "C" int pllm_paged_kv_append(const void* q, int64_t q_stride, const void*
     if (rows <= 0 || seqs <= 0 || kv_heads <= 0 || pool <= 0 || table_width <= 0 || table_stride < table_width || (q && heads <= 0)) return PLLM_ERR_INVALID_ARGUMENT;
     if (!cu_steps && rows % seqs != 0) return PLLM_ERR_INVALID_ARGUMENT;
     if (k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim || (q && q_stride < heads * head_dim)) return PLLM_ERR_INVALID_ARGUMENT;
-    if (rope_dim < 0 || rope_dim > head_dim || (rope_dim > 0 && (!cos_table || !sin_table || table_positions < table_width * page_tokens)))
+    if (rope_dim < 0 || rope_dim > head_dim || (rope_dim > 0 && (!cos_table || !sin_table || table_positions <= 0 || (!positions && table_positions < table_width * page_tokens))))
         return PLLM_ERR_INVALID_ARGUMENT;
     if ((head_dim != 64 && head_dim != 128) || rope_dim % 16 != 0 || (page_tokens != 16 && page_tokens != 32 && page_tokens != 64 && page_tokens != 128))
         return PLLM_ERR_UNSUPPORTED;
@@ -305,7 +302,7 @@ extern "C" int pllm_paged_kv_append(const void* q, int64_t q_stride, const void*
                            reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) | reinterpret_cast<uintptr_t>(cos_table) |
                            reinterpret_cast<uintptr_t>(sin_table);
     const uintptr_t narrow = reinterpret_cast<uintptr_t>(key_scales) | reinterpret_cast<uintptr_t>(value_scales) | reinterpret_cast<uintptr_t>(block_table) |
-                             reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(cu_steps);
+                             reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(cu_steps) | reinterpret_cast<uintptr_t>(positions);
     if ((wide & 15u) || (narrow & 3u) || (k_stride % 8) || (v_stride % 8) || (q && q_stride % 8)) return PLLM_ERR_INVALID_ARGUMENT;
     AppendArgs a{};
     a.q = static_cast<const uint16_t*>(q); a.k = static_cast<const uint16_t*>(k_new); a.v = static_cast<const uint16_t*>(v_new);
@@ -313,7 +310,7 @@ extern "C" int pllm_paged_kv_append(const void* q, int64_t q_stride, const void*
     a.q_out = static_cast<uint16_t*>(q_out);
     a.key_pages = key_pages; a.value_pages = value_pages; a.key_scales = key_scales; a.value_scales = value_scales;
     a.table = block_table; a.table_stride = static_cast<size_t>(table_stride); a.lengths = lengths; a.cu_steps = cu_steps;
-    a.cos_table = cos_table; a.sin_table = sin_table;
+    a.cos_table = cos_table; a.sin_table = sin_table; a.positions = positions; a.positions_end = static_cast<int>(table_positions < 0x7fffffff ? table_positions : 0x7fffffff);
     a.rows = static_cast<int>(rows); a.seqs = static_cast<int>(seqs); a.even_steps = static_cast<int>(rows / seqs); a.even_pages = static_cast<int>(even_pages);
     a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
     a.pool = static_cast<int>(pool); a.width = static_cast<int>(table_width); a.rope_half = static_cast<int>(rope_dim / 2);
@@ -327,4 +324,12 @@ extern "C" int pllm_paged_kv_append(const void* q, int64_t q_stride, const void*
     else dtype == PLLM_BF16 ? (PLLM_APPEND(true, 64)) : (PLLM_APPEND(false, 64));
 #undef PLLM_APPEND
     return hipGetLastError() == hipSuccess ? PLLM_OK : PLLM_ERR_LAUNCH;
+}
+
+extern "C" int pllm_paged_kv_append(const void* q, int64_t q_stride, const void* k_new, int64_t k_stride, const void* v_new, int64_t v_stride, int dtype,
+                                    void* q_out, uint8_t* key_pages, uint8_t* value_pages, float* key_scales, float* value_scales, int64_t pool,
+                                    int64_t page_tokens, const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* lengths,
+                                    const int32_t* cu_steps, const float* cos_table, const float* sin_table, int64_t table_positions, int64_t rope_dim,
+                                    int64_t rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, void* stream) {
+    return pllm_paged_kv_append_at(q, q_stride, k_new, k_stride, v_new, v_stride, dtype, q_out, key_pages, value_pages, key_scales, value_scales, pool, page_tokens, block_table, table_stride, table_width, lengths, cu_steps, cos_table, sin_table, table_positions, nullptr, rope_dim, rows, seqs, heads, kv_heads, head_dim, stream);
 }

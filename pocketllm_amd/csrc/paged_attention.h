@@ -11,6 +11,7 @@ struct PagedDecodeArgs {
     const float* key_scales; const float* value_scales;
     const int32_t* table; size_t table_stride;
     const int32_t* lengths; const int32_t* cu_steps;         // cu_steps null: `steps` new tokens each
+    const int32_t* parents;                     // of the new tokens, which are nodes of drafted trees (at most 64 each); null: they follow one another
     float* sums; float2* stats;                 // of the runs of a row: [seqs][kv_heads][part_rows][runs_bound][D], m (base 2) and sum of weights; null: one run
     uint16_t* out;
     float scale;                                // base 2

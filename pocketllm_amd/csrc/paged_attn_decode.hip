@@ -38,7 +38,8 @@ template <bool BF16> __device__ __forceinline__ float weights_from(float top) {
 }
 
 // SETS of 16 query rows; rows of one key/value head: token * group + head in the group
-template <bool BF16, int D, int SETS>
+// TREE: the new tokens are nodes of a tree; the steps that hold some of their keys are masked by the nodes' ancestors
+template <bool BF16, int D, int SETS, bool TREE>
 __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kernel(const PagedDecodeArgs a, int least_rows, int most_rows) {
     constexpr int kPieces = D / 64;             // 16-byte pieces of a key row per lane
     constexpr int kTiles = D / 16;              // output tiles
@@ -48,6 +49,8 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
     __shared__ float2 stats[kWaves][16];
     __shared__ __align__(16) uint16_t queries[kRows][D + 8];                  // (in registers they cost the third workgroup of a compute unit)
     __shared__ __align__(8) uint16_t nan_keys[kWaves][D][4];                  // keys of a wave's step whose value is NaN, a bit each, per dimension
+    __shared__ int parents[TREE ? 64 : 1];
+    __shared__ uint64_t nodes[TREE ? 64 : 1];                                 // what the nodes see of the tree
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     // Neighbouring workgroups run on different XCDs: heads first, and the runs of every sequence from another one on, or the XCDs of the first runs, which
@@ -64,6 +67,11 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
     if (run > 0 && begin >= length) return;
     const int32_t* table = a.table + static_cast<size_t>(s) * a.table_stride;
 
+    const int past = tree_past(given, n);                                     // (TREE)
+    if constexpr (TREE) {
+        if (n > 64) return;
+        if (tid < n) parents[tid] = a.parents[offset + tid];
+    }
     // the columns' query rows and how many keys they see
     int limit[SETS];
 #pragma unroll
@@ -109,6 +117,8 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) x.values[i] = *reinterpret_cast<const uint4*>(a.value_pages + value_at + (static_cast<size_t>(16 * i) << a.page_shift));
     };
+    // (TREE) keys `first` .. + 63 that a column's node sees
+    auto window = [&](int c, int first) { return tree_window(&nodes[min((kRows * tile + 16 * c + col) / group, 63)], 1, past, first, limit[c]); };
     int key_page = 0, value_page = 0;           // of the next step to request
     // a step; with MORE the next one's keys are requested as soon as this one's are used, its values likewise
     auto work = [&](auto more, Step& x, int j0) {
@@ -145,15 +155,16 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
         const int first = j0 + 16 * g;
         bool whole = true, some_nan = false;                                  // every column sees all of the lane's keys
 #pragma unroll
-        for (int c = 0; c < SETS; ++c) whole &= x.here && limit[c] - first >= 16;
+        for (int c = 0; c < SETS; ++c) whole &= x.here && (TREE ? min(past, limit[c]) : limit[c]) - first >= 16;
         if (!__all(whole)) {
 #pragma unroll
             for (int c = 0; c < SETS; ++c) {
                 const int seen = x.here ? limit[c] - first : 0;
+                const uint32_t bits = TREE && x.here ? static_cast<uint32_t>(window(c, first)) : 0;
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[c][t][i] = 4 * t + i < seen ? sc[c][t][i] : -INFINITY;
+                    for (int i = 0; i < 4; ++i) sc[c][t][i] = (TREE ? (bits >> (4 * t + i) & 1) != 0 : 4 * t + i < seen) ? sc[c][t][i] : -INFINITY;
             }
             // what lies behind the last key may be anything, NaN codes too, and zero times NaN is NaN
             const int stored = x.here ? length - first : 0;
@@ -219,7 +230,7 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
 #pragma unroll
             for (int c = 0; c < SETS; ++c) {
                 const int keys = limit[c] - j0;
-                const uint64_t sees = keys >= 64 ? ~0ull : (keys <= 0 ? 0ull : (1ull << keys) - 1);
+                const uint64_t sees = TREE ? window(c, j0) : (keys >= 64 ? ~0ull : (keys <= 0 ? 0ull : (1ull << keys) - 1));
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i)
 #pragma unroll
@@ -272,6 +283,14 @@ __global__ __launch_bounds__(kThreads, SETS == 1 ? 3 : 2) void paged_decode_kern
         for (int i = 0; i < kPasses; ++i) {
             const int row = tid / kChunks + kAtOnce * i;
             if (row < kRows) *reinterpret_cast<uint4*>(&queries[row][8 * (tid % kChunks)]) = q[i];
+        }
+    }
+    if constexpr (TREE) {
+        __syncthreads();
+        if (tid < 64) {
+            uint64_t bits[1] = {0};
+            if (tid < n) tree_ancestors(parents, tid, bits);
+            nodes[tid] = bits[0];
         }
     }
     __syncthreads();
@@ -429,15 +448,15 @@ __global__ __launch_bounds__(kThreads) void paged_merge_few_kernel(const PagedDe
         merge_few<BF16, D>(a, blockIdx.x * a.part_rows, row, runs, offset, kvh, group);
 }
 
-template <bool BF16, int D>
+template <bool BF16, int D, bool TREE>
 int launch(const PagedDecodeArgs& a, hipStream_t stream) {
     // Two sets of rows share what is read: eight sequences behind 20718 positions, four new tokens of eight heads each, 116 -> 96 us.  They cost a compute
     // unit's third workgroup, so sequences that have one set get the other launch: 64 of one token of six heads behind up to 8000 positions, in a call
     // that may hold more, 253 -> 201 us.
     const int most = a.cu_steps ? std::min(a.part_rows, 16) : a.part_rows;
-    if (most <= 16) hipLaunchKernelGGL((paged_decode_kernel<BF16, D, 1>), dim3(a.kv_heads, a.runs_bound, a.seqs), dim3(kThreads), 0, stream, a, 1, most);
+    if (most <= 16) hipLaunchKernelGGL((paged_decode_kernel<BF16, D, 1, TREE>), dim3(a.kv_heads, a.runs_bound, a.seqs), dim3(kThreads), 0, stream, a, 1, most);
     if (a.part_rows > 16)
-        hipLaunchKernelGGL((paged_decode_kernel<BF16, D, 2>), dim3((a.part_rows + 31) / 32 * a.kv_heads, a.runs_bound, a.seqs), dim3(kThreads), 0, stream, a, most < a.part_rows ? 17 : 1,
+        hipLaunchKernelGGL((paged_decode_kernel<BF16, D, 2, TREE>), dim3((a.part_rows + 31) / 32 * a.kv_heads, a.runs_bound, a.seqs), dim3(kThreads), 0, stream, a, most < a.part_rows ? 17 : 1,
                            a.part_rows);
     if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
     if (a.sums) {
@@ -467,8 +486,12 @@ int paged_decode_launch(PagedDecodeArgs& a, void* workspace, bool bf16, int head
         a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) +
                                             align256(static_cast<size_t>(a.seqs) * a.part_rows * a.kv_heads * a.runs_bound * head_dim * sizeof(float)));
     }
-    if (head_dim == 128) return bf16 ? launch<true, 128>(a, stream) : launch<false, 128>(a, stream);
-    return bf16 ? launch<true, 64>(a, stream) : launch<false, 64>(a, stream);
+    if (a.parents) {
+        if (head_dim == 128) return bf16 ? launch<true, 128, true>(a, stream) : launch<false, 128, true>(a, stream);
+        return bf16 ? launch<true, 64, true>(a, stream) : launch<false, 64, true>(a, stream);
+    }
+    if (head_dim == 128) return bf16 ? launch<true, 128, false>(a, stream) : launch<false, 128, false>(a, stream);
+    return bf16 ? launch<true, 64, false>(a, stream) : launch<false, 64, false>(a, stream);
 }
 
 }  // namespace pllm

@@ -47,10 +47,12 @@ struct PagedPromptArgs {
     const float* key_scales; const float* value_scales;
     const int32_t* table; size_t table_stride;
     const int32_t* lengths; const int32_t* cu_steps;
+    const int32_t* parents;                     // drafted trees: of the new tokens, which are their nodes
     uint16_t* out;
     float* sums; float2* stats;                 // of several runs of a block's keys: [runs][tokens * heads][D], m (base 2) and sum of weights; or null
     float scale;                                // base 2
     int few_rows;                               // sequences of so many query rows or fewer are another kernel's
+    int even;                                   // (trees) without cu_steps: new tokens of every sequence
     int runs, tokens, seqs, heads, kv_heads, page_shift, pool, width, slots;
 };
 
@@ -64,15 +66,18 @@ __device__ __forceinline__ int lanes_until(int x) {
     return x;
 }
 
+// row offsets of the sequences' new tokens
+template <bool TREE> __device__ __forceinline__ int offset_of(const PagedPromptArgs& a, int s) { return paged_offset(a.cu_steps, s, TREE ? a.even : 0, a.tokens); }
+
 // The block of query rows that index `index` of the grid is: sequence s (a.seqs: the rows behind the last one), rows row0 .. row0 + kBlockRows - 1 of it.
 // Those with the most keys come first, so that what is left at the end is short (48 and 8 heads: 30 continuations of up to 200 tokens behind up to 4000
 // 267 -> 215 us, 12 of up to 300 behind up to 16000 809 -> 693; where a sequence's own order is as good already, four prompts of up to 2000 tokens, 117 -> 123); of
 // more than 63 sequences only each one's own blocks are in that order.
-template <int ROWS>
+template <int ROWS, bool TREE>
 __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, int group, int& s, int& row0) {
     const int lane = threadIdx.x & 63;
     if (a.seqs == 1) {                                                        // (1024 tokens of 48 and 8 heads: 42.0 -> 40.5 us)
-        const int n = paged_offset(a.cu_steps, 1, 0, a.tokens), blocks = n * group > a.few_rows ? (n * group + ROWS - 1) / ROWS : 0;
+        const int n = offset_of<TREE>(a, 1), blocks = n * group > a.few_rows ? (n * group + ROWS - 1) / ROWS : 0;
         s = index < blocks ? 0 : 1;
         row0 = (index < blocks ? blocks - 1 - index : index - blocks) * ROWS;
         return row0 < (s ? a.tokens - n : n) * group;
@@ -80,8 +85,8 @@ __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, 
     if (a.seqs < 64) {
         int rows = 0, first = 0, keys = 0;                                    // of the lane's sequence
         if (lane <= a.seqs) {
-            const int offset = paged_offset(a.cu_steps, lane, 0, a.tokens);
-            const int n = max((lane == a.seqs ? a.tokens : paged_offset(a.cu_steps, lane + 1, 0, a.tokens)) - offset, 0);
+            const int offset = offset_of<TREE>(a, lane);
+            const int n = max((lane == a.seqs ? a.tokens : offset_of<TREE>(a, lane + 1)) - offset, 0);
             keys = lane == a.seqs || n == 0 ? 0 : paged_length(a.lengths[lane], a.width, a.page_shift);
             rows = lane < a.seqs && n * group <= a.few_rows ? 0 : n * group;
             first = keys - n;
@@ -108,7 +113,7 @@ __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, 
     for (int base = 0; base <= a.seqs; base += 64) {
         const int c = base + lane;
         int rows = 0;
-        if (c <= a.seqs) rows = max((c == a.seqs ? a.tokens : paged_offset(a.cu_steps, c + 1, 0, a.tokens)) - paged_offset(a.cu_steps, c, 0, a.tokens), 0) * group;
+        if (c <= a.seqs) rows = max((c == a.seqs ? a.tokens : offset_of<TREE>(a, c + 1)) - offset_of<TREE>(a, c), 0) * group;
         const int blocks = c < a.seqs && rows <= a.few_rows ? 0 : (rows + ROWS - 1) / ROWS, until = lanes_until(blocks);
         const uint64_t behind = __ballot(until > place);
         if (behind) {
@@ -122,7 +127,8 @@ __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, 
     return false;
 }
 
-template <bool BF16, int D, bool RUNS, bool SPLIT>
+// TREE: the new tokens are nodes of a tree; the tiles that hold some of their keys are masked by the nodes' ancestors
+template <bool BF16, int D, bool RUNS, bool SPLIT, bool TREE>
 __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPromptArgs a) {
     constexpr int kKeyBytes = kTile * D * 2, kTileBytes = 2 * kKeyBytes;      // keys [64][D], values [D][64]
     constexpr int kDimTiles = D / 32, kSteps = D / 16;
@@ -133,32 +139,50 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     __shared__ float unread[64 + 4 * 8];
     __shared__ float2 halves[SPLIT ? kBlockRows / 2 : 1];
     __shared__ __align__(8) uint16_t nan_keys[2][D][4];                       // which ones: a bit per key and dimension, in the tile's half
+    __shared__ int parents[TREE ? kTreeNodes : 1];
+    __shared__ uint64_t nodes[TREE ? kRows : 1][kTreeWords];                  // what the nodes of the workgroup's rows see of the tree, from the first row's on
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int place = SPLIT ? wave & 3 : wave, second = SPLIT ? wave >> 2 : 0;                // the wave's rows, the half of a tile's keys
     const int kvh = blockIdx.x, group = a.heads / a.kv_heads;
     // rows of one key/value head: token * group + head in the group; the tokens behind the last sequence are one more, without keys
     int s = 0, row0 = 0;
-    if (!find_block<kRows>(a, blockIdx.z, group, s, row0)) return;
+    if (!find_block<kRows, TREE>(a, blockIdx.z, group, s, row0)) return;
     const bool tail = s == a.seqs;
-    const int offset = paged_offset(a.cu_steps, s, 0, a.tokens), n = (tail ? a.tokens : paged_offset(a.cu_steps, s + 1, 0, a.tokens)) - offset;
+    const int offset = offset_of<TREE>(a, s), n = (tail ? a.tokens : offset_of<TREE>(a, s + 1)) - offset;
     const int rows = n * group;                                               // (fits: the host's check)
     const int given = tail ? 0 : a.lengths[s], length = paged_length(given, a.width, a.page_shift);
     // keys that a row sees: up to its token's position
     auto visible = [&](int row) {
         const int64_t v = static_cast<int64_t>(given) - n + row / group + 1;
-        return tail ? 0 : static_cast<int>(v < 0 ? 0 : (v > length ? length : v));
+        return tail || (TREE && n > kTreeNodes) ? 0 : static_cast<int>(v < 0 ? 0 : (v > length ? length : v));
     };
+    const int past = tree_past(given, n);                                     // (TREE)
     const int all_tiles = (visible(min(rows, row0 + kRows) - 1) + kTile - 1) / kTile;
     // this workgroup's tiles: t0 .. end - 1
     const int run = RUNS ? (all_tiles + static_cast<int>(gridDim.y) - 1) / static_cast<int>(gridDim.y) : all_tiles, t0 = RUNS ? min(static_cast<int>(blockIdx.y) * run, all_tiles) : 0;
     const int end = RUNS ? min(t0 + run, all_tiles) : all_tiles, tiles = end - t0;
-    const int full = visible(row0) / kTile;                                   // tiles that every row of the workgroup sees whole
+    const int full = (TREE ? clamp_int(past, 0, visible(row0)) : visible(row0)) / kTile;     // tiles that every row of the workgroup sees whole
     const int w0 = row0 + 32 * place, my_row = min(w0 + r, rows - 1);
     const int limit = visible(my_row);
     const int wave_end = w0 < rows ? visible(min(rows, w0 + 32) - 1) : 0;     // keys that one of the wave's rows sees
     const int32_t* table = a.table + static_cast<size_t>(tail ? 0 : s) * a.table_stride;
 
+    if constexpr (TREE) {
+        // (a chain of steps up the tree per node; the first keys are requested behind it)
+        if (kTile * end > past && tiles > 0) {
+            if (tid < min(n, kTreeNodes)) parents[tid] = a.parents[offset + tid];
+            __syncthreads();
+            const int node = row0 / group + tid;
+            uint64_t bits[kTreeWords] = {};
+            if (node < n) tree_ancestors(parents, node, bits);
+            if (tid < kRows)
+#pragma unroll
+                for (int w = 0; w < kTreeWords; ++w) nodes[tid][w] = bits[w];
+        }
+    }
+    // (TREE) keys 64 t .. + 63 that the lane's node sees
+    auto window = [&](int t) { return tree_window(nodes[my_row / group - row0 / group], kTreeWords, past, kTile * t, limit); };
     uint4 qf[kSteps];
     float late = 1.0f;
     {
@@ -348,7 +372,16 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
             entry_next = entry(min(t + 5, last));
         };
         const int seen = limit - kTile * t - 32 * second - 4 * h;
-        auto hidden = [&](int u, int v) { return MASKED && 32 * u + 8 * (v >> 2) + (v & 3) >= seen; };
+        uint32_t bits[2] = {};                                                // (TREE) of the lane's keys from its first on
+        if constexpr (MASKED && TREE) {
+            const uint64_t from = window(t) >> (32 * second + 4 * h);
+            bits[0] = static_cast<uint32_t>(from);
+            bits[1] = static_cast<uint32_t>(from >> 32);
+        }
+        auto hidden = [&](int u, int v) {
+            if constexpr (TREE) return MASKED && (bits[u] >> (8 * (v >> 2) + (v & 3)) & 1) == 0;
+            else return MASKED && 32 * u + 8 * (v >> 2) + (v & 3) >= seen;
+        };
         if constexpr (MASKED) {
             top = -INFINITY;
 #pragma unroll
@@ -429,7 +462,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
         if (MASKED && nan_values[t & 3]) {
             // NaN values were left out of the product: they are the end of the sums of the rows that see them
             const int keys = limit - kTile * t;
-            const uint64_t sees = keys >= 64 ? ~0ull : (keys <= 0 ? 0ull : (1ull << keys) - 1);
+            const uint64_t sees = TREE ? window(t) : keys >= 64 ? ~0ull : (keys <= 0 ? 0ull : (1ull << keys) - 1);
 #pragma unroll
             for (int u = 0; u < kDimTiles; ++u)
 #pragma unroll
@@ -527,7 +560,7 @@ __global__ __launch_bounds__(256) void paged_prompt_merge_kernel(const PagedProm
     const int lane = threadIdx.x & 63;
     if (row >= rows) return;
     if (a.few_rows > 0) {                                                     // rows without runs are the other kernel's
-        const int s = paged_sequence(a.cu_steps, a.tokens, a.seqs + 1, 1, 0, row / a.heads);
+        const int s = paged_sequence(a.cu_steps, a.tokens, a.seqs + 1, 1, 0, row / a.heads);                // (few_rows: the call has cu_steps)
         if (s < a.seqs && (paged_offset(a.cu_steps, s + 1, 0, a.tokens) - paged_offset(a.cu_steps, s, 0, a.tokens)) * (a.heads / a.kv_heads) <= a.few_rows) return;
     }
     const float2 mine = lane < a.runs ? a.stats[lane * rows + row] : make_float2(-FLT_MAX, 0.0f);           // (at most 64 runs)
@@ -553,15 +586,17 @@ __global__ __launch_bounds__(256) void paged_prompt_merge_kernel(const PagedProm
     else *out = static_cast<uint16_t>(half_pair<BF16>(total[0] * inv, 0.0f));
 }
 
-template <bool BF16, int D>
+constexpr int kTreeFewRows = 64;
+
+template <bool BF16, int D, bool TREE>
 int launch(const PagedPromptArgs& a, bool split, hipStream_t stream) {
     static SmemGrant granted[4];
     const size_t smem = 2 * 2 * kTile * D * 2;
     const bool runs = a.sums != nullptr;
-    const auto kernel = runs ? (split ? paged_prompt_kernel<BF16, D, true, true> : paged_prompt_kernel<BF16, D, true, false>)
-                             : (split ? paged_prompt_kernel<BF16, D, false, true> : paged_prompt_kernel<BF16, D, false, false>);
+    const auto kernel = runs ? (split ? paged_prompt_kernel<BF16, D, true, true, TREE> : paged_prompt_kernel<BF16, D, true, false, TREE>)
+                             : (split ? paged_prompt_kernel<BF16, D, false, true, TREE> : paged_prompt_kernel<BF16, D, false, false, TREE>);
     // (with the kernel's own arrays beside it, 128-wide heads pass 64 KB)
-    if (!grant_dynamic_smem(reinterpret_cast<const void*>(kernel), smem + 8192, granted[2 * runs + split])) return PLLM_ERR_LAUNCH;
+    if (!grant_dynamic_smem(reinterpret_cast<const void*>(kernel), smem + (TREE ? 18432 : 8192), granted[2 * runs + split])) return PLLM_ERR_LAUNCH;
     // Runs before blocks: indexes without a block come last.  Workgroups go to the shader engines in turn, those that end at once too, and an engine that got more
     // of the others than it has compute units works a second round (128 tokens behind 30000 positions in blocks of half the rows 213 -> 117 us).
     hipLaunchKernelGGL(kernel, dim3(a.kv_heads, a.runs, a.slots), dim3(kThreads), smem, stream, a);
@@ -607,10 +642,10 @@ int few_rows(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
 }
 
 struct Parts { int runs, few; bool split; size_t run_bytes, few_bytes; };
-Parts parts_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
+Parts parts_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions, int few) {
     Parts p{};
     const int64_t rows = tokens * (heads / kv_heads);
-    p.few = few_rows(tokens, seqs, heads, kv_heads, head_dim, positions);
+    p.few = few;
     p.few_bytes = p.few > 0 ? paged_decode_parts_bytes(seqs, p.few, kv_heads, head_dim, positions) : 0;
     // Half the rows per workgroup while the workgroups are not more than the compute units, and of one prompt without a past, whose last rows see so much more
     // than the mean, up to twice as many (48 and 8 heads, 200 tokens 19.3 -> 14.0 us, 700 31.0 -> 24.5, 1024 42.2 -> 36.2, 1365 52 -> 46, but 1700 60 -> 71; 8 of
@@ -627,15 +662,92 @@ Parts parts_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, in
     return p;
 }
 
+
+// Trees of the same number of nodes: whether the decode kernel takes them.
+bool few_nodes(int64_t nodes, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
+    const int64_t rows = nodes * (heads / kv_heads);
+    return nodes <= 64 && rows <= kTreeFewRows && paged_decode_parts_bytes(seqs, rows, kv_heads, head_dim, positions) <= (size_t{1} << 30);
+}
+Parts tree_parts(int64_t tokens, int64_t seqs, bool even, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
+    if (!even) return parts_of(tokens, seqs, heads, kv_heads, head_dim, positions, few_rows(tokens, seqs, heads, kv_heads, head_dim, positions));
+    Parts p{};
+    if (!few_nodes(tokens / seqs, seqs, heads, kv_heads, head_dim, positions)) return parts_of(tokens, seqs, heads, kv_heads, head_dim, positions, 0);
+    p.few = static_cast<int>(tokens / seqs * (heads / kv_heads));
+    p.few_bytes = paged_decode_parts_bytes(seqs, p.few, kv_heads, head_dim, positions);
+    return p;
+}
+
+bool sizes_ok(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
+    return tokens > 0 && seqs > 0 && kv_heads > 0 && heads >= kv_heads && head_dim > 0 && positions > 0 && tokens <= 0x3fffff && seqs <= 0xffff && heads <= 1024 && head_dim <= 256;
+}
+
+// Both entries.  `tree`: with parents, and cu_steps may be null.
+int attention(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pages, const uint8_t* value_pages, const float* key_scales, const float* value_scales, int64_t pool,
+              int64_t page_tokens, const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* lengths, const int32_t* parents, const int32_t* cu_steps, bool tree,
+              int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, void* out, void* workspace, size_t workspace_bytes, hipStream_t st) {
+    if (!q || !key_pages || !value_pages || !key_scales || !value_scales || !block_table || !lengths || !out || (tree ? !parents : !cu_steps)) return PLLM_ERR_INVALID_ARGUMENT;
+    if (dtype != PLLM_F16 && dtype != PLLM_BF16) return PLLM_ERR_INVALID_ARGUMENT;
+    if (tokens <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || pool <= 0 || table_width <= 0 || table_stride < table_width ||
+        q_stride < heads * head_dim || !(scale >= 0.0f && scale <= 0x1p127f) || (!cu_steps && tokens % seqs != 0))
+        return PLLM_ERR_INVALID_ARGUMENT;
+    if ((head_dim != 64 && head_dim != 128) || (page_tokens != 16 && page_tokens != 32 && page_tokens != 64 && page_tokens != 128)) return PLLM_ERR_UNSUPPORTED;
+    // pages, positions and rows in 32 bits
+    if (tokens > 0x3fffff || seqs > 0xffff || heads > 1024 || pool > 0x7fffffff || table_width > 0x3fffffff / page_tokens || (!cu_steps && tokens / seqs > kTreeNodes)) return PLLM_ERR_UNSUPPORTED;
+    const int64_t positions = table_width * page_tokens;
+    const Parts parts = tree ? tree_parts(tokens, seqs, cu_steps == nullptr, heads, kv_heads, head_dim, positions)
+                             : parts_of(tokens, seqs, heads, kv_heads, head_dim, positions, few_rows(tokens, seqs, heads, kv_heads, head_dim, positions));
+    // (the rows behind the last sequence: what is left of the whole blocks, and one more)
+    const int64_t rows = tokens * (heads / kv_heads), slots = blocks_of(rows, seqs, parts.few, parts.split ? kBlockRows / 2 : kBlockRows) + 1;
+    if (rows > 0x3fffffff || slots > 0xffff) return PLLM_ERR_UNSUPPORTED;
+    const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) | reinterpret_cast<uintptr_t>(out) |
+                           reinterpret_cast<uintptr_t>(workspace);
+    const uintptr_t narrow = reinterpret_cast<uintptr_t>(key_scales) | reinterpret_cast<uintptr_t>(value_scales) | reinterpret_cast<uintptr_t>(block_table) |
+                             reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(cu_steps) | reinterpret_cast<uintptr_t>(parents);
+    if ((wide & 15u) || (narrow & 3u) || q_stride % 8) return PLLM_ERR_INVALID_ARGUMENT;
+    if (parts.run_bytes + parts.few_bytes > 0 && (!workspace || workspace_bytes < parts.run_bytes + parts.few_bytes)) return PLLM_ERR_WORKSPACE;
+    const bool bf16 = dtype == PLLM_BF16;
+    PagedPromptArgs a{};
+    a.q = static_cast<const uint16_t*>(q); a.q_stride = static_cast<size_t>(q_stride);
+    a.key_pages = key_pages; a.value_pages = value_pages; a.key_scales = key_scales; a.value_scales = value_scales;
+    a.table = block_table; a.table_stride = static_cast<size_t>(table_stride); a.lengths = lengths; a.cu_steps = cu_steps; a.parents = parents;
+    a.out = static_cast<uint16_t*>(out);
+    a.scale = scale * 1.4426950408889634f;
+    a.tokens = static_cast<int>(tokens); a.seqs = static_cast<int>(seqs); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
+    a.page_shift = page_tokens == 16 ? 4 : page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7;
+    a.pool = static_cast<int>(pool); a.width = static_cast<int>(table_width);
+    a.slots = static_cast<int>(slots);
+    a.runs = parts.runs;
+    a.few_rows = parts.few;
+    a.even = cu_steps ? 0 : static_cast<int>(tokens / seqs);
+    if (a.runs > 1) {
+        a.sums = static_cast<float*>(workspace);
+        a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + align256(static_cast<size_t>(a.runs) * tokens * heads * head_dim * sizeof(float)));
+    }
+    if (cu_steps || a.few_rows == 0) {                                        // (otherwise every row is the decode kernel's)
+        int status;
+        if (tree) status = head_dim == 128 ? (bf16 ? launch<true, 128, true>(a, parts.split, st) : launch<false, 128, true>(a, parts.split, st))
+                                           : (bf16 ? launch<true, 64, true>(a, parts.split, st) : launch<false, 64, true>(a, parts.split, st));
+        else status = head_dim == 128 ? (bf16 ? launch<true, 128, false>(a, parts.split, st) : launch<false, 128, false>(a, parts.split, st))
+                                      : (bf16 ? launch<true, 64, false>(a, parts.split, st) : launch<false, 64, false>(a, parts.split, st));
+        if (status != PLLM_OK || a.few_rows == 0) return status;
+    }
+    PagedDecodeArgs d{};
+    d.q = a.q; d.q_stride = a.q_stride; d.key_pages = key_pages; d.value_pages = value_pages; d.key_scales = key_scales; d.value_scales = value_scales;
+    d.table = a.table; d.table_stride = a.table_stride; d.lengths = lengths; d.cu_steps = cu_steps; d.parents = parents; d.out = a.out; d.scale = a.scale;
+    d.seqs = a.seqs; d.steps = a.even; d.tokens = a.tokens; d.heads = a.heads; d.kv_heads = a.kv_heads; d.page_shift = a.page_shift; d.pool = a.pool; d.width = a.width;
+    d.part_rows = a.few_rows;
+    return paged_decode_launch(d, static_cast<unsigned char*>(workspace) + parts.run_bytes, bf16, static_cast<int>(head_dim), st);
+}
+
 }  // namespace
 }  // namespace pllm
 
 extern "C" {
 
 size_t pllm_paged_attention_prompt_workspace_bytes(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
-    if (tokens <= 0 || seqs <= 0 || kv_heads <= 0 || heads < kv_heads || head_dim <= 0 || positions <= 0 || tokens > 0x3fffff || seqs > 0xffff || heads > 1024 || head_dim > 256)
-        return 0;
-    const pllm::Parts p = pllm::parts_of(tokens, seqs, heads, kv_heads, head_dim, positions);
+    using namespace pllm;
+    if (!sizes_ok(tokens, seqs, heads, kv_heads, head_dim, positions)) return 0;
+    const Parts p = parts_of(tokens, seqs, heads, kv_heads, head_dim, positions, few_rows(tokens, seqs, heads, kv_heads, head_dim, positions));
     return p.run_bytes + p.few_bytes;
 }
 
@@ -644,51 +756,23 @@ int pllm_paged_attention_prompt(const void* q, int64_t q_stride, int dtype, cons
                                            const int32_t* block_table, int64_t table_stride, int64_t table_width, const int32_t* lengths,
                                            const int32_t* cu_steps, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                            float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+    return pllm::attention(q, q_stride, dtype, key_pages, value_pages, key_scales, value_scales, pool, page_tokens, block_table, table_stride, table_width, lengths, nullptr, cu_steps, false,
+                           tokens, seqs, heads, kv_heads, head_dim, scale, out, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+size_t pllm_paged_attention_tree_workspace_bytes(int64_t tokens, int64_t seqs, int even, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
     using namespace pllm;
-    if (!q || !key_pages || !value_pages || !key_scales || !value_scales || !block_table || !lengths || !cu_steps || !out) return PLLM_ERR_INVALID_ARGUMENT;
-    if (dtype != PLLM_F16 && dtype != PLLM_BF16) return PLLM_ERR_INVALID_ARGUMENT;
-    if (tokens <= 0 || seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || pool <= 0 || table_width <= 0 || table_stride < table_width ||
-        q_stride < heads * head_dim || !(scale >= 0.0f && scale <= 0x1p127f))
-        return PLLM_ERR_INVALID_ARGUMENT;
-    if ((head_dim != 64 && head_dim != 128) || (page_tokens != 16 && page_tokens != 32 && page_tokens != 64 && page_tokens != 128)) return PLLM_ERR_UNSUPPORTED;
-    // pages, positions and rows in 32 bits
-    if (tokens > 0x3fffff || seqs > 0xffff || heads > 1024 || pool > 0x7fffffff || table_width > 0x3fffffff / page_tokens) return PLLM_ERR_UNSUPPORTED;
-    const Parts parts = parts_of(tokens, seqs, heads, kv_heads, head_dim, table_width * page_tokens);
-    // (the rows behind the last sequence: what is left of the whole blocks, and one more)
-    const int64_t rows = tokens * (heads / kv_heads), slots = blocks_of(rows, seqs, parts.few, parts.split ? kBlockRows / 2 : kBlockRows) + 1;
-    if (rows > 0x3fffffff || slots > 0xffff) return PLLM_ERR_UNSUPPORTED;
-    const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) | reinterpret_cast<uintptr_t>(out) |
-                           reinterpret_cast<uintptr_t>(workspace);
-    const uintptr_t narrow = reinterpret_cast<uintptr_t>(key_scales) | reinterpret_cast<uintptr_t>(value_scales) | reinterpret_cast<uintptr_t>(block_table) |
-                             reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(cu_steps);
-    if ((wide & 15u) || (narrow & 3u) || q_stride % 8) return PLLM_ERR_INVALID_ARGUMENT;
-    PagedPromptArgs a{};
-    a.q = static_cast<const uint16_t*>(q); a.q_stride = static_cast<size_t>(q_stride);
-    a.key_pages = key_pages; a.value_pages = value_pages; a.key_scales = key_scales; a.value_scales = value_scales;
-    a.table = block_table; a.table_stride = static_cast<size_t>(table_stride); a.lengths = lengths; a.cu_steps = cu_steps;
-    a.out = static_cast<uint16_t*>(out);
-    a.scale = scale * 1.4426950408889634f;
-    a.tokens = static_cast<int>(tokens); a.seqs = static_cast<int>(seqs); a.heads = static_cast<int>(heads); a.kv_heads = static_cast<int>(kv_heads);
-    a.page_shift = page_tokens == 16 ? 4 : page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7;
-    a.pool = static_cast<int>(pool); a.width = static_cast<int>(table_width);
-    a.slots = static_cast<int>(slots);
-    if (parts.run_bytes + parts.few_bytes > 0 && (!workspace || workspace_bytes < parts.run_bytes + parts.few_bytes)) return PLLM_ERR_WORKSPACE;
-    a.runs = parts.runs;
-    a.few_rows = parts.few;
-    if (a.runs > 1) {
-        a.sums = static_cast<float*>(workspace);
-        a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + align256(static_cast<size_t>(a.runs) * tokens * heads * head_dim * sizeof(float)));
-    }
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool bf16 = dtype == PLLM_BF16;
-    const int status = head_dim == 128 ? (bf16 ? launch<true, 128>(a, parts.split, st) : launch<false, 128>(a, parts.split, st)) : (bf16 ? launch<true, 64>(a, parts.split, st) : launch<false, 64>(a, parts.split, st));
-    if (status != PLLM_OK || a.few_rows == 0) return status;
-    PagedDecodeArgs d{};
-    d.q = a.q; d.q_stride = a.q_stride; d.key_pages = key_pages; d.value_pages = value_pages; d.key_scales = key_scales; d.value_scales = value_scales;
-    d.table = a.table; d.table_stride = a.table_stride; d.lengths = lengths; d.cu_steps = cu_steps; d.out = a.out; d.scale = a.scale;
-    d.seqs = a.seqs; d.tokens = a.tokens; d.heads = a.heads; d.kv_heads = a.kv_heads; d.page_shift = a.page_shift; d.pool = a.pool; d.width = a.width;
-    d.part_rows = a.few_rows;
-    return paged_decode_launch(d, static_cast<unsigned char*>(workspace) + parts.run_bytes, bf16, static_cast<int>(head_dim), st);
+    if (!sizes_ok(tokens, seqs, heads, kv_heads, head_dim, positions)) return 0;
+    const Parts p = tree_parts(tokens, seqs, even != 0, heads, kv_heads, head_dim, positions);
+    return p.run_bytes + p.few_bytes;
+}
+
+int pllm_paged_attention_tree(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pages, const uint8_t* value_pages, const float* key_scales,
+                              const float* value_scales, int64_t pool, int64_t page_tokens, const int32_t* block_table, int64_t table_stride, int64_t table_width,
+                              const int32_t* lengths, const int32_t* parents, const int32_t* cu_steps, int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads,
+                              int64_t head_dim, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+    return pllm::attention(q, q_stride, dtype, key_pages, value_pages, key_scales, value_scales, pool, page_tokens, block_table, table_stride, table_width, lengths, parents, cu_steps, true,
+                           tokens, seqs, heads, kv_heads, head_dim, scale, out, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

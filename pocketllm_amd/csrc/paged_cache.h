@@ -63,6 +63,41 @@ PLLM_HD int paged_page(const int32_t* table_row, int position, int width, int pa
     return page >= 0 && page < pool ? page : -1;
 }
 
+// Drafted trees.  The new tokens of a sequence are nodes, parents[i] the node that i hangs from: an earlier one, or -1 (anything that is not an earlier node) where
+// it follows the past.  A node sees the past, its ancestors and itself.
+constexpr int kTreeNodes = 256;                 // nodes that a tree can have; of one with more no node sees anything
+constexpr int kTreeWords = kTreeNodes / 64;
+
+// position of a tree's first node, of a sequence of `length` positions whose last `n` are the tree's: below zero where the first nodes have none
+PLLM_HD int tree_past(int length, int n) {
+    const int64_t past = static_cast<int64_t>(length) - n;
+    return past < -2 * kTreeNodes ? -2 * kTreeNodes : static_cast<int>(past);
+}
+
+// ancestors of node `i` and itself, a bit each; ends whatever parents hold, since every step goes to an earlier node
+template <int WORDS, typename Parents> PLLM_HD void tree_ancestors(const Parents& parents, int i, uint64_t (&bits)[WORDS]) {
+    for (int w = 0; w < WORDS; ++w) bits[w] = 0;
+    while (i >= 0 && i < 64 * WORDS) {
+        for (int w = 0; w < WORDS; ++w) bits[w] |= i >> 6 == w ? uint64_t{1} << (i & 63) : 0;
+        const int up = parents[i];
+        i = up < i ? up : -1;
+    }
+}
+
+// Keys `first` .. + 63 that a node sees, a bit each, of a sequence whose tree begins at position `past`: those of the past, the ancestors' and its own; none from
+// position `limit` on.  Words behind the node's are zero.
+PLLM_HD uint64_t tree_window(const uint64_t* bits, int words, int64_t past, int64_t first, int64_t limit) {
+    if (first >= limit) return 0;
+    const uint64_t there = limit - first >= 64 ? ~uint64_t{0} : (uint64_t{1} << (limit - first)) - 1;
+    const int64_t base = first - past;                                        // node of the window's first key
+    if (base <= -64) return there;
+    if (base >= 64 * static_cast<int64_t>(words)) return 0;
+    if (base < 0) return ((bits[0] << -base) | ((uint64_t{1} << -base) - 1)) & there;
+    const int word = static_cast<int>(base >> 6), shift = static_cast<int>(base & 63);
+    const uint64_t low = bits[word] >> shift, high = shift > 0 && word + 1 < words ? bits[word + 1] << (64 - shift) : 0;
+    return (low | high) & there;
+}
+
 // Keys of one run of the decode kernel.  By the sequence's own length and the number of heads alone, so that a sequence's sums have the
 // same order in every batch: runs of at least kPagedLeastRun keys, as long as one sequence has no more of them than fill the machine.
 PLLM_HD int paged_most_runs(int kv_heads) { return clamp_int(512 / kv_heads, 8, 256); }

@@ -80,6 +80,16 @@ template <bool BF16> __device__ __forceinline__ float half_pair_sum(uint32_t pai
     }
 }
 
+// four values as E4M3 codes (to the nearest, ties to even; within 448 or NaN); four codes as those of their values times a ratio of at most one
+__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true));
+}
+__device__ __forceinline__ uint32_t scaled_codes(uint32_t w, float ratio) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), true);
+    return four_codes(lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio);
+}
+
 // whether one of four E4M3 codes is NaN (0x7f or 0xff)
 __device__ __forceinline__ bool any_nan_code(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
 // which of them are: bit i for byte i; the codes with zeros in their place

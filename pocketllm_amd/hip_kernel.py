@@ -690,7 +690,7 @@ def _table_stride(block_table: torch.Tensor) -> int:
 def paged_kv_append_forward(q: torch.Tensor | None, k_new: torch.Tensor, v_new: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
                             key_scales: torch.Tensor, value_scales: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, *,
                             cu_steps: torch.Tensor | None = None, cos_table: torch.Tensor | None = None, sin_table: torch.Tensor | None = None,
-                            rope_dim: int = 0) -> torch.Tensor | None:
+                            rope_dim: int = 0, positions: torch.Tensor | None = None) -> torch.Tensor | None:
     """New keys and values of a batch of sequences into a paged E4M3 cache, rotary phases on the way; the queries beside them turned too and
     returned (rope_dim 0: q itself; no q: None).
 
@@ -698,13 +698,14 @@ def paged_kv_append_forward(q: torch.Tensor | None, k_new: torch.Tensor, v_new: 
     sequence s are rows cu_steps[s] .. cu_steps[s + 1] - 1 (int32, from 0 on; None: tokens / seqs each), the last of them at position lengths[s] - 1.
     key_pages [pool, kv_heads, page, head_dim], value_pages [pool, kv_heads, head_dim, page] float8_e4m3fn, key_scales / value_scales float32
     [pool, kv_heads], block_table int32 [seqs, pages]: written in place.  cos_table / sin_table float32 [positions, head_dim] as RotaryTable keeps them, rows for
-    every position that the table can name; rope_dim a multiple of 16.
+    every position that the table can name; rope_dim a multiple of 16.  positions int32 [tokens]: the rows of cos_table / sin_table that the tokens are turned by
+    (clamped to them; the tables may then have any number of rows), where that is not their place in the cache: the nodes of a drafted tree have the past plus their depth.
     The scale of a page and head is the least power of two with amax / scale <= 448; when it has to grow, the page's older codes are scaled
     down with it.  Rows without a position in the table store nothing, their queries leave as zeros.  What a call writes has one
     page of its own for each part of a sequence: no page stands twice among the entries that new tokens go to (pages that are only read may be shared)."""
     what = "paged_kv_append"
     made = _bindings.paged_kv_append("paged_kv_append_forward", q, k_new, v_new, key_pages, value_pages, key_scales, value_scales, block_table, lengths, cu_steps,
-                                     cos_table, sin_table, rope_dim)
+                                     cos_table, sin_table, rope_dim) if positions is None else None
     if made is not None:
         return q if made is True else made
     pool, kv_heads, page, dim = _paged_cache(what, k_new, key_pages, value_pages, key_scales, value_scales, block_table, lengths)
@@ -716,7 +717,7 @@ def paged_kv_append_forward(q: torch.Tensor | None, k_new: torch.Tensor, v_new: 
         for r in (cos_table, sin_table):
             _check(r is not None and r.dim() == 2 and r.size(1) == dim and r.dtype == torch.float32 and r.is_contiguous() and r.device == k_new.device,
                    f"{what}: cos_table / sin_table must be contiguous fp32 [positions, head_dim]")
-            _check(r.size(0) >= width * page, f"{what}: cos_table / sin_table must cover the {width * page} positions of the table")
+            _check(r.size(0) >= (width * page if positions is None else 1), f"{what}: cos_table / sin_table must cover the {width * page} positions of the table")
             _check(r.data_ptr() % 16 == 0, f"{what}: cos_table / sin_table must be on 16 bytes")
     heads = 0
     if q is not None:
@@ -727,6 +728,9 @@ def paged_kv_append_forward(q: torch.Tensor | None, k_new: torch.Tensor, v_new: 
         _paged_offsets(what, cu_steps, seqs, k_new.device)
     else:
         _check(tokens == 0 or (seqs > 0 and tokens % seqs == 0), f"{what}: without cu_steps every sequence has the same number of tokens")
+    if positions is not None:
+        _check(positions.dtype == torch.int32 and tuple(positions.shape) == (tokens,) and positions.is_contiguous() and positions.device == k_new.device,
+               f"{what}: positions must be int32 [tokens]")
     if tokens == 0 or seqs == 0:
         return q if q is None or not rope_dim else torch.zeros_like(q, memory_format=torch.contiguous_format)
     k_new, v_new = _rows16(k_new), _rows16(v_new)
@@ -735,12 +739,13 @@ def paged_kv_append_forward(q: torch.Tensor | None, k_new: torch.Tensor, v_new: 
         q = _rows16(q)
         turned = torch.empty(tokens, heads * dim, dtype=q.dtype, device=q.device)
     with _on_device(k_new.device):
-        st = _lib().pllm_paged_kv_append(
+        st = _lib().pllm_paged_kv_append_at(
             None if turned is None else q.data_ptr(), 0 if turned is None else q.stride(0), k_new.data_ptr(), k_new.stride(0), v_new.data_ptr(), v_new.stride(0),
             _DTYPE_CODE[k_new.dtype], None if turned is None else turned.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(),
             value_scales.data_ptr(), pool, page, block_table.data_ptr(), _table_stride(block_table), width, lengths.data_ptr(),
             None if cu_steps is None else cu_steps.data_ptr(), cos_table.data_ptr() if rope_dim else None, sin_table.data_ptr() if rope_dim else None,
-            cos_table.size(0) if rope_dim else 0, rope_dim, tokens, seqs, heads, kv_heads, dim, _stream(k_new.device))
+            min(cos_table.size(0), sin_table.size(0)) if rope_dim else 0, None if positions is None else positions.data_ptr(), rope_dim, tokens, seqs, heads, kv_heads, dim,
+            _stream(k_new.device))
     _ffi.check(st, "paged_kv_append_forward")
     return turned if rope_dim else q
 
@@ -811,6 +816,225 @@ def paged_attention_prompt_forward(q: torch.Tensor, key_pages: torch.Tensor, val
                                                 float(dim ** -0.5 if scale is None else scale), out.data_ptr(), None if ws is None else ws.data_ptr(), need, _stream(q.device))
     _ffi.check(st, "paged_attention_prompt_forward")
     return out
+
+
+# ---- serving by drafted trees ------------------------------------------------------------------------
+#
+# A step: paged_kv_append_forward (positions: the past plus the nodes' depths), paged_attention_tree_forward, the model's logits, sample_tokens_forward at every node,
+# draft_tree_accept_forward, paged_cache_compact_forward, and paged_cache_fork_forward where sequences branch, end, begin or need pages.
+
+TREE_NODES = 256                 # include/pllm_hip.h: nodes that a tree can have
+
+
+def _even_or_offsets(what: str, cu_steps: torch.Tensor | None, tokens: int, seqs: int, device: torch.device) -> None:
+    """Checks of the split of `tokens` rows over the sequences."""
+    if cu_steps is not None:
+        _paged_offsets(what, cu_steps, seqs, device)
+    else:
+        _check(tokens == 0 or (seqs > 0 and tokens % seqs == 0), f"{what}: without cu_steps every sequence has the same number of tokens")
+        _check(seqs == 0 or tokens // seqs <= TREE_NODES, f"{what}: a tree has at most {TREE_NODES} nodes")
+
+
+def _int32(what: str, name: str, t: torch.Tensor, shape: tuple, device: torch.device) -> None:
+    _check(t.dtype == torch.int32 and tuple(t.shape) == shape and t.is_contiguous() and t.device == device, f"{what}: {name} must be int32 {list(shape)}")
+
+
+def paged_attention_tree_forward(q: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor,
+                                 block_table: torch.Tensor, lengths: torch.Tensor, parents: torch.Tensor, *, cu_steps: torch.Tensor | None = None,
+                                 scale: float | None = None) -> torch.Tensor:
+    """paged_attention_prompt_forward for new tokens that are the nodes of a drafted tree per sequence: each sees the positions before the tree, its ancestors and
+    itself.  q [tokens, heads * head_dim], the nodes of sequence s in rows cu_steps[s] .. cu_steps[s + 1] - 1 (None: tokens / seqs each) and in the last positions
+    of the cache in the same order; parents int32 [tokens]: the node that each hangs from, counted within its sequence, an earlier one, or -1 (as is anything else)
+    for one that follows the past.  At most 256 nodes per sequence (with cu_steps, rows of a sequence with more are zeros).  Rows behind the last
+    sequence are zeros."""
+    what = "paged_attention_tree"
+    out = _bindings.paged_attention_tree("paged_attention_tree_forward", q, key_pages, value_pages, key_scales, value_scales, block_table, lengths, parents, cu_steps, scale)
+    if out is not None:
+        return out
+    _check(q.dim() == 2, f"{what}: q must be [tokens, heads * head_dim]")
+    pool, kv_heads, page, dim = _paged_cache(what, q, key_pages, value_pages, key_scales, value_scales, block_table, lengths)
+    tokens, width, seqs = q.size(0), q.size(1), block_table.size(0)
+    _even_or_offsets(what, cu_steps, tokens, seqs, q.device)
+    _int32(what, "parents", parents, (tokens,), q.device)
+    _check(scale is None or 0.0 <= float(scale) <= 2.0 ** 127, f"{what}: scale must be from 0 to 2 ** 127")
+    _check(width % dim == 0 and width > 0 and (width // dim) % kv_heads == 0, f"{what}: heads must be a multiple of the cache's key/value heads")
+    if tokens == 0 or seqs == 0:
+        return torch.zeros(tokens, width, dtype=q.dtype, device=q.device)
+    out = torch.empty(tokens, width, dtype=q.dtype, device=q.device)
+    rows = _rows16(q)
+    lib = _lib()
+    need = lib.pllm_paged_attention_tree_workspace_bytes(tokens, seqs, int(cu_steps is None), width // dim, kv_heads, dim, block_table.size(1) * page)
+    with _on_device(q.device):
+        ws = _workspace(need, q.device) if need else None
+        st = lib.pllm_paged_attention_tree(rows.data_ptr(), rows.stride(0), _DTYPE_CODE[q.dtype], key_pages.data_ptr(), value_pages.data_ptr(), key_scales.data_ptr(),
+                                           value_scales.data_ptr(), pool, page, block_table.data_ptr(), _table_stride(block_table), block_table.size(1), lengths.data_ptr(),
+                                           parents.data_ptr(), None if cu_steps is None else cu_steps.data_ptr(), tokens, seqs, width // dim, kv_heads, dim,
+                                           float(dim ** -0.5 if scale is None else scale), out.data_ptr(), None if ws is None else ws.data_ptr(), need, _stream(q.device))
+    _ffi.check(st, "paged_attention_tree_forward")
+    return out
+
+
+def sample_tokens_forward(logits: torch.Tensor, uniform: torch.Tensor, *, temperature: float | torch.Tensor = 1.0, top_k: int | torch.Tensor = 0,
+                          top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0) -> torch.Tensor:
+    """A token per row of logits [rows, vocab] (float32, float16 or bfloat16; rows may be slices of a wider matrix), int64 [rows], from the random numbers
+    uniform float32 [rows] of [0, 1) (clamped to it).  Each parameter is a number for all rows or a tensor [rows] (float32, top_k int32).
+
+    With w_i = exp((x_i - max x) / temperature) and the tokens in the order of falling logits, equal ones by rising index, what is kept is the first min(n_k, n_p, n_m):
+    n_k = top_k (0: all), n_p the least n whose first n have top_p of what the first n_k add up to (from 1 on: all), n_m those with w >= min_p (up to 1).  The token is the
+    least i with (sum of w over kept j <= i) > uniform * (sum of w over kept).  temperature 0: the largest logit, the first of equal ones.  NaN and minus
+    infinity are never a token; a row of nothing else gives -1.  A row's token depends on the row alone, and sums are exact: no order of additions changes it."""
+    what = "sample_tokens"
+    made = _bindings.sample_tokens("sample_tokens_forward", logits, uniform, temperature, top_k, top_p, min_p)
+    if made is not None:
+        return made
+    _check(logits.dim() == 2, f"{what}: logits must be [rows, vocab]")
+    _check(logits.dtype in _DTYPE_CODE, f"{what}: logits must be float16, bfloat16, or float32")
+    rows, vocab = logits.shape
+    _check(0 < vocab <= 2 ** 20, f"{what}: a vocabulary of 1 to 2 ** 20 tokens")
+    _check(rows <= 65535, f"{what}: at most 65535 rows")
+    _check(uniform.dtype == torch.float32 and tuple(uniform.shape) == (rows,) and uniform.is_contiguous(), f"{what}: uniform must be float32 [rows]")
+    given = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    for name, v in given.items():
+        if isinstance(v, torch.Tensor):
+            dtype = torch.int32 if name == "top_k" else torch.float32
+            _check(v.dtype == dtype and tuple(v.shape) == (rows,) and v.is_contiguous(), f"{what}: {name} must be a number or {str(dtype)[6:]} [rows]")
+        else:
+            _check(float(v) >= 0, f"{what}: {name} must not be negative")
+    _check(isinstance(min_p, torch.Tensor) or float(min_p) <= 1, f"{what}: min_p must be from 0 to 1")
+    _check(isinstance(top_k, torch.Tensor) or int(top_k) == top_k, f"{what}: top_k must be a whole number")
+    tensors = [logits, uniform] + [v for v in given.values() if isinstance(v, torch.Tensor)]
+    _check(all(t.is_cuda and t.device == logits.device for t in tensors), f"{what}: tensors must be on one CUDA device")
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    if rows == 0:
+        return tokens
+    if logits.stride(1) != 1 and vocab > 1 or (rows > 1 and logits.stride(0) < vocab):
+        logits = logits.contiguous()
+    lib, code = _lib(), _DTYPE_CODE[logits.dtype]
+    need = lib.pllm_sample_tokens_workspace_bytes(rows, vocab, code)
+    each = lambda v: (v.data_ptr(), 0) if isinstance(v, torch.Tensor) else (None, v)
+    with _on_device(logits.device):
+        ws = _workspace(need, logits.device)
+        t, k, p, m = each(temperature), each(top_k), each(top_p), each(min_p)
+        st = lib.pllm_sample_tokens(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, code, uniform.data_ptr(), t[0], float(t[1]), k[0], min(int(k[1]), 2 ** 31 - 1),
+                                    p[0], float(p[1]), m[0], float(m[1]), rows, vocab, tokens.data_ptr(), ws.data_ptr(), need, _stream(logits.device))
+    _ffi.check(st, "sample_tokens_forward")
+    return tokens
+
+
+def draft_tree_accept_forward(parents: torch.Tensor, drafted: torch.Tensor, sampled: torch.Tensor, lengths: torch.Tensor, *, cu_steps: torch.Tensor | None = None,
+                              most: int | None = None):
+    """The path of each sequence's drafted tree that the sampled tokens follow: from node 0 (the sequence's last token) on the first child whose drafted token is the
+    one sampled at the node before it.  parents int32 [tokens] as paged_attention_tree_forward takes them, drafted int64 [tokens] the nodes' tokens, sampled int64
+    [tokens] what the model gives behind each of them, lengths int32 [seqs] with the tree's nodes; cu_steps int32 [seqs + 1] (None: tokens / seqs each).
+    Returns (kept int32 [seqs, most] the path's nodes and -1 behind them, counts int32 [seqs], tokens int64 [seqs] what is sampled at its last node, lengths int32 [seqs] with
+    the path alone).  most, 1 to 256: nodes at which a path ends (default: those of a tree; with cu_steps 256).  A sequence without nodes: 0 and token -1; nodes from the
+    257th on are not looked at."""
+    what = "draft_tree_accept"
+    made = _bindings.draft_tree_accept("draft_tree_accept_forward", parents, drafted, sampled, lengths, cu_steps, most)
+    if made is not None:
+        return made
+    _check(parents.dim() == 1 and lengths.dim() == 1, f"{what}: parents must be int32 [tokens], lengths int32 [seqs]")
+    tokens, seqs, device = parents.size(0), lengths.size(0), parents.device
+    _int32(what, "parents", parents, (tokens,), device)
+    _int32(what, "lengths", lengths, (seqs,), device)
+    _even_or_offsets(what, cu_steps, tokens, seqs, device)
+    for name, t in (("drafted", drafted), ("sampled", sampled)):
+        _check(t.dtype == torch.int64 and tuple(t.shape) == (tokens,) and t.is_contiguous() and t.device == device, f"{what}: {name} must be int64 [tokens]")
+    if most is None:
+        most = max(min(TREE_NODES, tokens // max(seqs, 1) if cu_steps is None else TREE_NODES), 1)
+    _check(1 <= int(most) <= TREE_NODES, f"{what}: most must be from 1 to {TREE_NODES}")
+    _check(parents.is_cuda, f"{what}: tensors must be on one CUDA device")
+    kept = torch.empty(seqs, int(most), dtype=torch.int32, device=device)
+    counts, new_lengths = torch.empty_like(lengths), torch.empty_like(lengths)
+    token = torch.empty(seqs, dtype=torch.int64, device=device)
+    if tokens == 0 or seqs == 0:
+        return kept.fill_(-1), counts.zero_(), token.fill_(-1), new_lengths.copy_(lengths)
+    with _on_device(device):
+        st = _lib().pllm_draft_tree_accept(parents.data_ptr(), drafted.data_ptr(), sampled.data_ptr(), lengths.data_ptr(), None if cu_steps is None else cu_steps.data_ptr(), tokens,
+                                           seqs, int(most), kept.data_ptr(), counts.data_ptr(), token.data_ptr(), new_lengths.data_ptr(), _stream(device))
+    _ffi.check(st, "draft_tree_accept_forward")
+    return kept, counts, token, new_lengths
+
+
+def _paged_layers(what: str, layers, block_table: torch.Tensor):
+    """Checks of the caches of a model's layers, which share a table; returns (addresses, pool, kv_heads, page_tokens, head_dim)."""
+    _check(len(layers) > 0 and all(len(layer) == 4 for layer in layers), f"{what}: layers must be a list of (key_pages, value_pages, key_scales, value_scales)")
+    lengths = torch.empty(block_table.size(0) if block_table.dim() == 2 else 0, dtype=torch.int32, device=block_table.device)
+    like = torch.empty(0, dtype=torch.float16, device=block_table.device)
+    sizes = [_paged_cache(what, like, *layer, block_table, lengths) for layer in layers]
+    _check(len(set(sizes)) == 1 and len(layers) <= 1024, f"{what}: the layers' caches must have one shape, at most 1024 of them")
+    at = [t.data_ptr() for layer in layers for t in layer]
+    for kind in (0, 2):
+        bytes_ = layers[0][kind].numel() * layers[0][kind].element_size()
+        some = sorted(at[i] for i in range(len(at)) if i % 4 // 2 == kind // 2)
+        _check(all(b - a >= bytes_ for a, b in zip(some, some[1:])), f"{what}: the layers' caches must not share memory")
+    return (ctypes.c_void_p * len(at))(*at), *sizes[0]
+
+
+def paged_cache_compact_forward(layers, block_table: torch.Tensor, lengths: torch.Tensor, kept: torch.Tensor, counts: torch.Tensor, steps: int | torch.Tensor) -> None:
+    """The keys and values of the accepted path of each sequence's drafted tree to the places right behind the past, in every layer's cache, in place: with n new tokens in
+    lengths[s] positions (steps: n, or cu_steps int32 [seqs + 1]) token lengths[s] - n + kept[s, j] becomes token lengths[s] - n + j for j < counts[s].
+    layers: a list of (key_pages, value_pages, key_scales, value_scales), one launch for up to 64 of them; block_table int32 [seqs, pages]; lengths
+    as they were before acceptance; kept int32 [seqs, most], counts int32 [seqs] as draft_tree_accept_forward gives them (a row that stops rising or leaves the tree ends there).
+    The scale of a page that tokens move to becomes the largest that its content had, and codes are scaled down to it.  As in paged_kv_append_forward what
+    a call writes has pages of its own.  What lies behind a path stays as it is, or as it was moved over."""
+    what = "paged_cache_compact"
+    if _bindings.paged_cache_compact("paged_cache_compact_forward", layers, block_table, lengths, kept, counts, steps) is not None:
+        return
+    caches, pool, kv_heads, page, dim = _paged_layers(what, layers, block_table)
+    seqs, device = block_table.size(0), block_table.device
+    _int32(what, "lengths", lengths, (seqs,), device)
+    _int32(what, "counts", counts, (seqs,), device)
+    _check(kept.dim() == 2 and 1 <= kept.size(1) <= TREE_NODES, f"{what}: kept must be int32 [seqs, most], most from 1 to {TREE_NODES}")
+    _int32(what, "kept", kept, (seqs, kept.size(1)), device)
+    if isinstance(steps, torch.Tensor):
+        _paged_offsets(what, steps, seqs, device)
+    else:
+        _check(1 <= int(steps) <= TREE_NODES, f"{what}: a tree has 1 to {TREE_NODES} nodes")
+    if seqs == 0:
+        return
+    with _on_device(device):
+        st = _lib().pllm_paged_cache_compact(caches, len(layers), pool, page, block_table.data_ptr(), _table_stride(block_table), block_table.size(1), lengths.data_ptr(), kept.data_ptr(),
+                                             kept.size(1), counts.data_ptr(), steps.data_ptr() if isinstance(steps, torch.Tensor) else None,
+                                             0 if isinstance(steps, torch.Tensor) else int(steps), seqs, kv_heads, dim, _stream(device))
+    _ffi.check(st, "paged_cache_compact_forward")
+
+
+def paged_cache_fork_forward(layers, block_table: torch.Tensor, page_uses: torch.Tensor, sources: torch.Tensor, kept: torch.Tensor, reserve: torch.Tensor):
+    """The sequences of the next step out of the present ones: row r goes on with the first kept[r] tokens of row sources[r] of block_table (any source outside it: with
+    none, a new sequence) and has pages for reserve[r] tokens; all int32 [rows].  A row that no other goes on with ends, and its pages are free.
+
+    block_table int32 [seqs, pages], -1 where a row has no page; page_uses int32 [pool]: how many holders every page has, the table's entries among them, free at 0.
+    Whole kept pages are shared.  A page that is kept in part, which the row will write to, stays the row's where no other new row and no holder outside the table has it (of
+    rows that keep it in part the first has it); the others get a copy in every layer (layers as in paged_cache_compact_forward).  Free pages go to the rows in
+    their order, lowest numbers first.
+    Returns (block_table [rows, pages], page_uses [pool], missing int32 [rows]: pages that a row did not get, -1 in its table); the old table holds nothing any more."""
+    what = "paged_cache_fork"
+    made = _bindings.paged_cache_fork("paged_cache_fork_forward", layers, block_table, page_uses, sources, kept, reserve)
+    if made is not None:
+        return made
+    caches, pool, kv_heads, page, dim = _paged_layers(what, layers, block_table)
+    seqs, width, device = block_table.size(0), block_table.size(1), block_table.device
+    _check(sources.dim() == 1, f"{what}: sources must be int32 [rows]")
+    rows = sources.size(0)
+    for name, t in (("sources", sources), ("kept", kept), ("reserve", reserve)):
+        _int32(what, name, t, (rows,), device)
+    _int32(what, "page_uses", page_uses, (pool,), device)
+    _check(seqs > 0, f"{what}: block_table has no rows")
+    table = torch.empty(rows, width, dtype=torch.int32, device=device)
+    uses, missing = torch.empty_like(page_uses), torch.empty_like(sources)
+    if rows == 0:                                                              # everything ends
+        entries = block_table[(block_table >= 0) & (block_table < pool)].long()
+        uses.copy_(page_uses).index_add_(0, entries, torch.full_like(entries, -1, dtype=torch.int32))
+        return table, uses.clamp_min_(0), missing
+    lib = _lib()
+    need = lib.pllm_paged_cache_fork_workspace_bytes(rows, pool)
+    with _on_device(device):
+        ws = _workspace(need, device)
+        st = lib.pllm_paged_cache_fork(caches, len(layers), pool, page, block_table.data_ptr(), _table_stride(block_table), width, page_uses.data_ptr(), sources.data_ptr(), kept.data_ptr(),
+                                       reserve.data_ptr(), seqs, rows, kv_heads, dim, table.data_ptr(), uses.data_ptr(), missing.data_ptr(), ws.data_ptr(), need, _stream(device))
+    _ffi.check(st, "paged_cache_fork_forward")
+    return table, uses, missing
 
 
 def gguf_quant_gemm_pair_forward(x, blocks0, row_elems0, type_id0, blocks1, row_elems1, type_id1, signed_grid, *,
