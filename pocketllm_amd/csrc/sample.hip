@@ -6,12 +6,14 @@
 // p, min_p and u are compared with is exact in 128 bits.  A weight is off by 2^-44 at most, so a row of 200064 logits gets the token of exact weights but for about one
 // u in 10^9 (float32 weights and sums: one in a hundred).  Weights below 2^-44 are none.
 //
-// Nothing is sorted but a few hundred values.  A row is cut in slices, a workgroup each:
-//   1. the slices' largest and least values
-//   2. a histogram over the distance from the largest, linear from it to the least value or to where weights end: count and sum of weights per bin
-//   3. every workgroup finds in it the bins that the cuts of top-k and top-p lie in; sums of what is kept for certain per slice; the values of the cuts' bins to a list
-//   4. a workgroup per row orders that list, finds the cuts, the slice and in it the token
-// Bound: bytes (the row once from memory, then from the caches), the 64-bit exponential (about 20 instructions a value) and the chain of four launches.
+// Nothing is sorted but a few hundred values:
+//   1. the row's largest and least values
+//   2. a histogram over the distance from the largest, linear from it to the least value or to where weights end: values per bin and, without a small top-k, weights
+//   3. in it the bins that the cuts of top-k and top-p lie in; the values of these bins to a list, of those above them only the sum of weights.  With a top-k of up
+//      to kFew everything above the cut goes to the list, and no other value's weight is ever formed
+//   4. the list in order, the cuts in it, the stretch of the row that the token lies in, the token
+// Many rows: a workgroup each, one launch.  Few rows: four launches, the first three over slices of the rows.
+// Bound: bytes (the row once from memory, then from the caches) and the 64-bit exponential, about 20 instructions a value, where there is no small top-k.
 #include "pllm_device.h"
 #include "pllm_internal.h"
 
@@ -21,10 +23,13 @@
 namespace pllm {
 namespace {
 
-constexpr int kBins = 2048, kListed = 4096;     // bins of a histogram; values of the cuts' bins that are ordered in LDS (equal logits may be more: by bisection)
+constexpr int kBins = 1024, kListed = 2048;     // bins of a histogram; values of the cuts' bins that a list in LDS holds (equal logits may be more)
+constexpr int kTied = 512;                      // values of one part of a bin that are ordered
+constexpr int kDirect = 128;                    // listed values up to which each is compared with all
+constexpr int kFew = kListed / 2;               // top-k up to which everything that is kept goes to the list
 constexpr int kUnit = 43;                       // binary digits of a weight
-constexpr int kThreads = 256, kLastThreads = 1024;
-constexpr uint64_t kOne = uint64_t{1} << kUnit;
+constexpr int kThreads = 256, kRowThreads = 512, kLastThreads = 512;
+constexpr int kStretch = 512, kMostStretches = (1 << 20) / 4 / kStretch + 1;               // chunks whose kept weights are summed up together; of a row
 
 struct SampleArgs {
     const void* logits; size_t stride;          // elements between rows
@@ -33,10 +38,11 @@ struct SampleArgs {
     float temperature_all; int top_k_all; float top_p_all, min_p_all;
     int64_t* tokens;
     uint64_t* best; uint32_t* least;            // [rows][slices]: order key of the largest value, then the complement of its index; order key of the least
-    uint64_t* masses;                           // [rows][slices] of what is kept for certain
+    uint64_t* masses;                           // [rows][stretches] of what is kept for certain
     uint64_t* mass; uint32_t* count;            // [rows][kBins]
     uint64_t* listed; uint32_t* listed_count;   // [rows][kListed], [rows]: order key and complement of the index
-    int rows, vocab, slices, slice_chunks;      // chunks of 16 bytes of a slice
+    int rows, vocab, slices, slice_chunks,      // chunks of 16 bytes of a slice, whole stretches
+        stretches;
 };
 
 // Logits in the order of their values as unsigned numbers; NaN and minus infinity are 0x007fffff, the least of any.
@@ -53,7 +59,6 @@ template <typename T> struct Chunk;             // 16 bytes of logits
 template <> struct Chunk<float> {
     static constexpr int kValues = 4;
     static __device__ __forceinline__ float at(const uint4& u, int i) { return __uint_as_float(i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w); }
-    static __device__ __forceinline__ float one(const void* p, size_t i) { return static_cast<const float*>(p)[i]; }
 };
 struct F16 {};
 struct B16 {};
@@ -63,7 +68,6 @@ template <> struct Chunk<F16> {
         const uint32_t w = i < 2 ? u.x : i < 4 ? u.y : i < 6 ? u.z : u.w;
         return f16_bits_to_float(i & 1 ? w >> 16 : w & 0xffffu);
     }
-    static __device__ __forceinline__ float one(const void* p, size_t i) { return f16_bits_to_float(static_cast<const uint16_t*>(p)[i]); }
 };
 template <> struct Chunk<B16> {
     static constexpr int kValues = 8;
@@ -71,7 +75,6 @@ template <> struct Chunk<B16> {
         const uint32_t w = i < 2 ? u.x : i < 4 ? u.y : i < 6 ? u.z : u.w;
         return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
     }
-    static __device__ __forceinline__ float one(const void* p, size_t i) { return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i]) << 16); }
 };
 
 // A row as chunks of 16 aligned bytes: value `i` of chunk `c` is logit c * kValues + i - skew.
@@ -85,39 +88,67 @@ template <typename T> struct Row {
         vocab = a.vocab;
     }
     __device__ __forceinline__ int chunks() const { return (vocab + skew + kValues - 1) / kValues; }
-    // the chunk's order keys and the index of its first; places outside the row hold kNone
-    __device__ __forceinline__ int keys(int c, uint32_t (&key)[kValues]) const {
-        const int first = c * kValues - skew;
-        if (first >= 0 && first + kValues <= vocab) {
-            const uint4 u = *reinterpret_cast<const uint4*>(base + static_cast<int64_t>(first) * kBytes);
+    __device__ __forceinline__ int first_of(int c) const { return c * kValues - skew; }
+    // the chunk as it lies; places outside the row, and chunks from `end` on, hold NaN
+    __device__ __forceinline__ uint4 load(int c, int end) const {
+        const int first = first_of(c);
+        if (c < end && first >= 0 && first + kValues <= vocab) return *reinterpret_cast<const uint4*>(base + static_cast<int64_t>(first) * kBytes);
+        uint32_t w[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        if (c < end) {
 #pragma unroll
-            for (int i = 0; i < kValues; ++i) key[i] = order_key(Chunk<T>::at(u, i));
-        } else {
-#pragma unroll
-            for (int i = 0; i < kValues; ++i) key[i] = first + i >= 0 && first + i < vocab ? order_key(Chunk<T>::one(base, first + i)) : kNone;
+            for (int i = 0; i < kValues; ++i) {
+                if (first + i < 0 || first + i >= vocab) continue;
+                if constexpr (kBytes == 4) w[i] = reinterpret_cast<const uint32_t*>(base)[first + i];
+                else {
+                    const uint32_t v = reinterpret_cast<const uint16_t*>(base)[first + i];
+                    w[i / 2] = i % 2 ? (w[i / 2] & 0xffffu) | v << 16 : (w[i / 2] & 0xffff0000u) | v;
+                }
+            }
         }
-        return first;
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    // its values, minus infinity for NaN
+    static __device__ __forceinline__ void values_of(const uint4& u, float (&v)[kValues]) {
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) v[i] = fmaxf(Chunk<T>::at(u, i), -INFINITY);
     }
 };
+// f(chunk, its values) for the chunks [begin, end), every STEP-th per thread, several loads on their way.  All threads go through all of it: behind the end, chunks of NaN.
+template <typename T, int STEP, int kAhead = 2, typename F> __device__ __forceinline__ void for_chunks(const Row<T>& x, int begin, int end, const F& f) {
+    for (int c0 = begin; c0 < end; c0 += kAhead * STEP) {
+        uint4 u[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) u[i] = x.load(c0 + i * STEP + static_cast<int>(threadIdx.x), end);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (c0 + i * STEP >= end) break;
+            float v[Row<T>::kValues];
+            Row<T>::values_of(u[i], v);
+            f(c0 + i * STEP + static_cast<int>(threadIdx.x), v);
+        }
+    }
+}
 
-// 2^y, y <= 0, times 2^kUnit, rounded: 2^f for |f| <= 1/2 by its series to the eleventh power (the rest is below 7e-15), the exponent added, the fraction
-// rounded off by adding 2^52.
-__device__ __forceinline__ uint64_t weight_of(double y) {
-    if (!(y >= -(kUnit + 1.0))) return 0;
-    const double n = rint(y), f = (y - n) * 0.69314718055994530942;
-    double p = 1.0 / 39916800.0;
-    p = __builtin_fma(p, f, 1.0 / 3628800.0);
-    p = __builtin_fma(p, f, 1.0 / 362880.0);
-    p = __builtin_fma(p, f, 1.0 / 40320.0);
-    p = __builtin_fma(p, f, 1.0 / 5040.0);
-    p = __builtin_fma(p, f, 1.0 / 720.0);
-    p = __builtin_fma(p, f, 1.0 / 120.0);
-    p = __builtin_fma(p, f, 1.0 / 24.0);
-    p = __builtin_fma(p, f, 1.0 / 6.0);
-    p = __builtin_fma(p, f, 0.5);
+// 2^y, y <= 0 (and above -2^30: below, anything), times 2^kUnit, rounded.  The nearest integer to y falls out of adding 1.5 * 2^52; 2^f for the rest, |f| <= 1/2, by the
+// polynomial of degree 10 through it at Chebyshev's points (within 3e-16); the integer goes to the exponent, and adding 2^52 rounds the fraction off.  Additions and fused
+// products alone, which have four times the rate of the instructions that round, convert and scale (832 rows of 32000 without cuts: 74 us with those), without branches, so that
+// a chunk's values go side by side.
+__device__ __forceinline__ uint64_t weight_at(double y) {
+    const double shifted = y + 0x1.8p52, f = y - (shifted - 0x1.8p52);
+    double p = 7.072585949269223e-09;
+    p = __builtin_fma(p, f, 1.0208690299958306e-07);
+    p = __builtin_fma(p, f, 1.321544258792169e-06);
+    p = __builtin_fma(p, f, 1.5252657260200837e-05);
+    p = __builtin_fma(p, f, 0.0001540353044173605);
+    p = __builtin_fma(p, f, 0.0013333558230164974);
+    p = __builtin_fma(p, f, 0.009618129107606888);
+    p = __builtin_fma(p, f, 0.05550410866444772);
+    p = __builtin_fma(p, f, 0.24022650695910097);
+    p = __builtin_fma(p, f, 0.69314718055995);
     p = __builtin_fma(p, f, 1.0);
-    p = __builtin_fma(p, f, 1.0);
-    const double scaled = __longlong_as_double(__double_as_longlong(p) + static_cast<long long>(static_cast<int>(n) + kUnit) * (1ll << 52));
+    const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(p));
+    const uint32_t high = static_cast<uint32_t>(bits >> 32) + ((static_cast<uint32_t>(__double_as_longlong(shifted)) + kUnit) << 20);
+    const double scaled = __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(bits)));
     return static_cast<uint64_t>(__double_as_longlong(scaled + 0x1p52)) & 0x000fffffffffffffull;
 }
 
@@ -128,20 +159,42 @@ __device__ __forceinline__ uint64_t share_up(uint64_t fraction, uint64_t of) {  
 }
 
 struct Params {
-    double most, factor, per_bin;               // the largest logit; base-2 exponent per unit of distance; bins per unit of it
+    double factor;                              // base-2 exponent per unit of distance from the largest logit
+    float most, per_bin, near;                  // the largest logit; bins per unit of distance; distance behind which weights are none
     uint64_t least_weight;                      // of min_p
     float temperature, top_p;
     int top_k;
-    bool greedy, cut;                           // the largest logit is the token; top-k or top-p leave something out
+    bool greedy, cut, few;                      // the largest logit is the token; top-k or top-p leave something out; a small top-k
     uint64_t best;
 };
-
-// a value's base-2 exponent, zero or below (plus infinity as the largest: the others have minus infinity)
-__device__ __forceinline__ double exponent_of(const Params& p, float x) { return x == p.most ? 0.0 : (static_cast<double>(x) - p.most) * p.factor; }
-__device__ __forceinline__ int bin_of(const Params& p, double y) { return static_cast<int>(fmin(-y * p.per_bin, kBins - 1.0)); }
-
+// all bits or none: a mask where a choice would be a branch around what is chosen, and a chunk's values would go one after the other
+__device__ __forceinline__ uint64_t only(bool v) { return ~(static_cast<uint64_t>(v) - 1); }
+// (plus infinity as the largest: it has no distance from itself, the others an infinite one)
+__device__ __forceinline__ float distance(const Params& p, float x) { return x == p.most ? 0.0f : p.most - x; }
+__device__ __forceinline__ bool weighs(const Params& p, float x) { return distance(p, x) <= p.near; }
+__device__ __forceinline__ int bin_of(const Params& p, float x) { return static_cast<int>(fminf(distance(p, x) * p.per_bin, kBins - 1.0f)); }
+__device__ __forceinline__ uint64_t weight_of(const Params& p, float x) {
+    const double d = x == p.most ? 0.0 : static_cast<double>(x) - static_cast<double>(p.most);
+    return weight_at(d * p.factor) & only(weighs(p, x));
+}
+// what the caller asks of the row
+struct Asked { float temperature, top_p, min_p, uniform; int top_k; };
+__device__ __forceinline__ Asked asked_of(const SampleArgs& a, int row) {
+    return Asked{a.temperature ? a.temperature[row] : a.temperature_all, a.top_p ? a.top_p[row] : a.top_p_all, a.min_p ? a.min_p[row] : a.min_p_all, a.uniform[row],
+                 a.top_k ? a.top_k[row] : a.top_k_all};
+}
+__device__ __forceinline__ Params params_of(const Asked& asked, int vocab, uint64_t best, uint32_t least);
+// the largest and least of a wave's values, for all its lanes
+__device__ __forceinline__ void wave_extremes(uint64_t& best, uint32_t& least) {
+#pragma unroll
+    for (int i = 32; i > 0; i /= 2) {
+        const uint64_t b = __shfl_xor(static_cast<unsigned long long>(best), i);
+        best = b > best ? b : best;
+        least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), i)));
+    }
+}
 // the row's parameters, by a wave from what the slices left
-__device__ __forceinline__ Params params_of(const SampleArgs& a, int row) {
+__device__ __forceinline__ Params slices_params(const SampleArgs& a, int row, const Asked& asked) {
     const int lane = threadIdx.x & 63;
     uint64_t best = 0;
     uint32_t least = 0xffffffffu;
@@ -150,117 +203,127 @@ __device__ __forceinline__ Params params_of(const SampleArgs& a, int row) {
         best = b > best ? b : best;
         least = min(least, a.least[static_cast<size_t>(row) * a.slices + i]);
     }
-#pragma unroll
-    for (int i = 32; i > 0; i /= 2) {
-        const uint64_t b = __shfl_xor(static_cast<unsigned long long>(best), i);
-        best = b > best ? b : best;
-        least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), i)));
-    }
+    wave_extremes(best, least);
+    return params_of(asked, a.vocab, best, least);
+}
+__device__ __forceinline__ Params params_of(const Asked& asked, int vocab, uint64_t best, uint32_t least) {
     Params p;
     p.best = best;
     p.most = of_key(static_cast<uint32_t>(best >> 32));
-    p.temperature = a.temperature ? a.temperature[row] : a.temperature_all;
-    p.top_k = a.top_k ? a.top_k[row] : a.top_k_all;
-    p.top_p = a.top_p ? a.top_p[row] : a.top_p_all;
-    const float min_p = a.min_p ? a.min_p[row] : a.min_p_all;
+    p.temperature = asked.temperature;
+    p.top_k = asked.top_k;
+    p.top_p = asked.top_p;
+    const float min_p = asked.min_p;
     p.least_weight = min_p > 0.0f ? static_cast<uint64_t>(ceil(static_cast<double>(fminf(min_p, 1.0f)) * 0x1p43)) : 0;
     if (p.least_weight == 0) p.least_weight = 1;                              // (weights of nothing are never kept)
     p.greedy = !(p.temperature > 0.0f) || p.top_k == 1 || static_cast<uint32_t>(best >> 32) == kNone;
-    p.cut = (p.top_k > 0 && p.top_k < a.vocab) || p.top_p < 1.0f;
+    p.few = p.top_k > 0 && p.top_k <= kFew && p.top_k < vocab;
+    p.cut = (p.top_k > 0 && p.top_k < vocab) || p.top_p < 1.0f;
     p.factor = 1.44269504088896340736 / static_cast<double>(p.temperature);
-    const double y = exponent_of(p, of_key(least)), range = fmin(fmax(-y, 0x1p-40), kUnit + 2.0);           // (of values in a row that have weights)
-    p.per_bin = kBins / range;
+    // (weights below 2^-44 are none; in the last step of a float's more)
+    p.near = static_cast<float>(fmin((kUnit + 1.5) / p.factor, static_cast<double>(FLT_MAX)));
+    const float span = fmaxf(fminf(distance(p, of_key(least)), p.near), FLT_MIN);
+    p.per_bin = fminf(kBins / span, FLT_MAX);
     return p;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_extremes_kernel(const SampleArgs a) {
-    __shared__ uint64_t bests[kThreads / 64];
-    __shared__ uint32_t leasts[kThreads / 64];
-    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
-    for (int i = slice * kThreads + tid; i < kBins; i += a.slices * kThreads) {              // for the next launch
-        a.mass[static_cast<size_t>(row) * kBins + i] = 0;
-        a.count[static_cast<size_t>(row) * kBins + i] = 0;
-    }
-    if (slice == 0 && tid == 0) a.listed_count[row] = 0;
-    const Row<T> x(a, row);
-    const int end = min((slice + 1) * a.slice_chunks, x.chunks());
-    uint64_t best = place_key(kNone, 0x7fffffff);
-    uint32_t least = 0xffffffffu;
-    for (int c = slice * a.slice_chunks + tid; c < end; c += kThreads) {
-        uint32_t key[Row<T>::kValues];
-        const int first = x.keys(c, key);
+__device__ __forceinline__ void add_to(uint64_t* at, uint64_t v) { atomicAdd(reinterpret_cast<unsigned long long*>(at), static_cast<unsigned long long>(v)); }
+
+// the largest and least values of the chunks [begin, end)
+template <typename T, int STEP> __device__ __forceinline__ void extremes(const Row<T>& x, int begin, int end, uint64_t& best, uint32_t& least) {
+    float most = -INFINITY, low = INFINITY;
+    int at = 0x7fffffff;
+    for_chunks<T, STEP, 4>(x, begin, end, [&](int c, const float (&v)[Row<T>::kValues]) {
+        float here = v[0];
 #pragma unroll
-        for (int i = 0; i < Row<T>::kValues; ++i) {
-            const uint64_t k = place_key(key[i], first + i);
-            if (key[i] != kNone) {
-                best = k > best ? k : best;
-                least = min(least, key[i]);
+        for (int i = 1; i < Row<T>::kValues; ++i) here = fmaxf(here, v[i]);
+#pragma unroll
+        for (int i = 0; i < Row<T>::kValues; ++i) low = fminf(low, v[i] == -INFINITY ? INFINITY : v[i]);
+        if (here > most) {                                                    // (a thread's chunks come in their order)
+            most = here;
+#pragma unroll
+            for (int i = Row<T>::kValues - 1; i >= 0; --i) at = v[i] == here ? x.first_of(c) + i : at;
+        }
+    });
+    if (most > -INFINITY) {
+        const uint64_t k = place_key(order_key(most), at);
+        best = k > best ? k : best;
+        least = min(least, order_key(low));
+    }
+}
+
+// Whether the histogram of a small top-k takes a chunk's largest value alone: where k of them lie, k values do at least, and should there be fewer than k chunks with any value
+// that is not masked, the list holds all of them.
+template <typename T> __device__ __forceinline__ bool by_chunk(const Params& p) { return p.few && p.top_k <= kListed / Row<T>::kValues; }
+
+// the chunks' values into a histogram in LDS
+template <typename T, int STEP> __device__ __forceinline__ void fill(const Row<T>& x, const Params& p, int begin, int end, uint64_t* mass, uint32_t* count) {
+    if (by_chunk<T>(p)) {
+        for_chunks<T, STEP, 4>(x, begin, end, [&](int, const float (&v)[Row<T>::kValues]) {
+            float most = v[0];
+#pragma unroll
+            for (int i = 1; i < Row<T>::kValues; ++i) most = fmaxf(most, v[i]);
+            if (weighs(p, most)) atomicAdd(count + bin_of(p, most), 1u);
+        });
+        return;
+    }
+    if (p.few) {
+        for_chunks<T, STEP, 4>(x, begin, end, [&](int, const float (&v)[Row<T>::kValues]) {
+            int bin[Row<T>::kValues];
+#pragma unroll
+            for (int i = 0; i < Row<T>::kValues; ++i) bin[i] = weighs(p, v[i]) ? bin_of(p, v[i]) : -1;
+#pragma unroll
+            for (int i = 0; i < Row<T>::kValues; ++i)
+                if (bin[i] >= 0) atomicAdd(count + bin[i], 1u);
+        });
+        return;
+    }
+    for_chunks<T, STEP>(x, begin, end, [&](int, const float (&v)[Row<T>::kValues]) {
+        uint64_t w[Row<T>::kValues];
+#pragma unroll
+        for (int i = 0; i < Row<T>::kValues; ++i) w[i] = weight_of(p, v[i]);
+#pragma unroll
+        for (int i = 0; i < Row<T>::kValues; ++i)
+            if (w[i]) {
+                const int bin = bin_of(p, v[i]);
+                add_to(mass + bin, w[i]);
+                atomicAdd(count + bin, 1u);
             }
-        }
-    }
-#pragma unroll
-    for (int i = 32; i > 0; i /= 2) {
-        const uint64_t b = __shfl_xor(static_cast<unsigned long long>(best), i);
-        best = b > best ? b : best;
-        least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), i)));
-    }
-    if ((tid & 63) == 0) { bests[tid >> 6] = best; leasts[tid >> 6] = least; }
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kThreads / 64; ++w) {
-            best = bests[w] > best ? bests[w] : best;
-            least = min(least, leasts[w]);
-        }
-        a.best[static_cast<size_t>(row) * a.slices + slice] = best;
-        a.least[static_cast<size_t>(row) * a.slices + slice] = least;
-    }
+    });
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_histogram_kernel(const SampleArgs a) {
-    __shared__ uint64_t mass[kBins];
-    __shared__ uint32_t count[kBins];
-    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
-    const Params p = params_of(a, row);
-    if (p.greedy || !p.cut) return;
-    for (int i = tid; i < kBins; i += kThreads) { mass[i] = 0; count[i] = 0; }
-    __syncthreads();
-    const Row<T> x(a, row);
-    const int end = min((slice + 1) * a.slice_chunks, x.chunks());
-    for (int c = slice * a.slice_chunks + tid; c < end; c += kThreads) {
-        uint32_t key[Row<T>::kValues];
-        x.keys(c, key);
-#pragma unroll
-        for (int i = 0; i < Row<T>::kValues; ++i) {
-            if (key[i] == kNone) continue;
-            const double y = exponent_of(p, of_key(key[i]));
-            const uint64_t w = weight_of(y);
-            if (w == 0) continue;
-            const int bin = bin_of(p, y);
-            atomicAdd(reinterpret_cast<unsigned long long*>(&mass[bin]), static_cast<unsigned long long>(w));
-            atomicAdd(&count[bin], 1u);
-        }
-    }
-    __syncthreads();
-    for (int i = tid; i < kBins; i += kThreads)
-        if (count[i]) {
-            atomicAdd(reinterpret_cast<unsigned long long*>(a.mass + static_cast<size_t>(row) * kBins + i), static_cast<unsigned long long>(mass[i]));
-            atomicAdd(a.count + static_cast<size_t>(row) * kBins + i, count[i]);
-        }
-}
-
+// the sum over the lanes up to this one: shifts within 16 lanes, then the ends of 16 and of 32 lanes to those behind
 __device__ __forceinline__ uint64_t lanes_until(uint64_t v) {
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) {
-        const uint64_t before = __shfl_up(static_cast<unsigned long long>(v), i);
-        if ((threadIdx.x & 63) >= i) v += before;
+#define PLLM_STEP(ctrl, rows)                                                                                                                          \
+    {                                                                                                                                                  \
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(v), ctrl, rows, 0xf, false);                                          \
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(v >> 32), ctrl, rows, 0xf, false);                                    \
+        v += static_cast<uint64_t>(hi) << 32 | lo;                                                                                                     \
     }
+    PLLM_STEP(0x111, 0xf)
+    PLLM_STEP(0x112, 0xf)
+    PLLM_STEP(0x114, 0xf)
+    PLLM_STEP(0x118, 0xf)
+    PLLM_STEP(0x142, 0xa)
+    PLLM_STEP(0x143, 0xc)
+#undef PLLM_STEP
     return v;
 }
-// the sum over the threads up to this one, and over all in `total`; `parts` [THREADS / 64], free again behind the next barrier
+__device__ __forceinline__ uint64_t lanes_sum(uint64_t v) {
+    v = lanes_until(v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), 63), hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), 63);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+// a wave's values (all lanes take part) to one place in LDS, the lanes' (64 chunks of one stretch) first together: one by one they wait for each other (a pass over 832 rows of 32000
+// 57 us)
+__device__ __forceinline__ void add_all(uint64_t* at, uint64_t v) {
+    v = lanes_sum(v);
+    if ((threadIdx.x & 63) == 0 && v) add_to(at, v);
+}
+// the sum over the threads up to this one, and over all in `total`; `parts` [THREADS / 64]
 template <int THREADS> __device__ __forceinline__ uint64_t threads_until(uint64_t v, uint64_t* parts, uint64_t& total) {
     v = lanes_until(v);
+    __syncthreads();
     if ((threadIdx.x & 63) == 63) parts[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t before = 0, all = 0;
@@ -272,8 +335,20 @@ template <int THREADS> __device__ __forceinline__ uint64_t threads_until(uint64_
     total = all;
     return before + v;
 }
+// the sum over the workgroup, for all threads
+template <int THREADS> __device__ __forceinline__ uint64_t all_sum(uint64_t v, uint64_t* parts) {
+    v = lanes_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) v += parts[w];
+    return v;
+}
 
-// Where the cuts lie.  Bins below `low` are kept whole (as far as min_p goes), those of [low, high] hold the last one that top-p keeps, bin `last` the k-th.
+// Where the cuts lie.  Bins below `low` are kept whole (as far as min_p goes), those of [low, high] hold the last one that top-p keeps, bin `last` the k-th.  A
+// small top-k: low 0, high and last the k-th's bin.
 struct Cuts {
     int low, high, last;                        // last: -1 without a cut by top-k; low: kBins without any cut
     uint64_t before_low, before_last, total;    // sums of weights
@@ -281,26 +356,25 @@ struct Cuts {
 };
 // By a workgroup, from the row's histogram.
 template <int THREADS>
-__device__ __forceinline__ void find_cuts(const SampleArgs& a, int row, const Params& p, Cuts& out, uint64_t* parts) {
+__device__ __forceinline__ void find_cuts(const uint64_t* masses_of, const uint32_t* counts_of, const Params& p, Cuts& out, uint64_t* parts) {
     constexpr int kPer = kBins / THREADS;
     const int tid = threadIdx.x;
     uint64_t mass[kPer], masses = 0;
     uint32_t count[kPer], counts = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        mass[i] = a.mass[static_cast<size_t>(row) * kBins + kPer * tid + i];
-        count[i] = a.count[static_cast<size_t>(row) * kBins + kPer * tid + i];
+        mass[i] = p.few ? 0 : masses_of[kPer * tid + i];
+        count[i] = counts_of[kPer * tid + i];
         masses += mass[i];
         counts += count[i];
     }
-    uint64_t total, everyone;
-    const uint64_t mass0 = threads_until<THREADS>(masses, parts, total) - masses;
-    __syncthreads();
+    uint64_t total = 0, everyone;
+    const uint64_t mass0 = p.few ? 0 : threads_until<THREADS>(masses, parts, total) - masses;
     const uint64_t count0 = threads_until<THREADS>(counts, parts, everyone) - counts;
-    if (tid == 0) { out.low = kBins; out.high = kBins; out.last = -1; out.before_low = 0; out.before_last = 0; out.total = total; out.need = 0; }
+    if (tid == 0) { out.low = p.few ? 0 : kBins; out.high = p.few ? kBins - 1 : kBins; out.last = p.few ? kBins - 1 : -1; out.before_low = 0; out.before_last = 0; out.total = total; out.need = 0; }
     __syncthreads();
     const uint64_t k = p.top_k > 0 ? static_cast<uint64_t>(p.top_k) : ~uint64_t{0};
-    if (everyone > k) {
+    if (p.few ? everyone >= k : everyone > k) {
         uint64_t c = count0, m = mass0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
@@ -309,12 +383,14 @@ __device__ __forceinline__ void find_cuts(const SampleArgs& a, int row, const Pa
                 out.before_last = m;
                 out.need = static_cast<uint32_t>(k - c);
                 out.total = m + mass[i];                                      // what the first k add up to, at most
+                if (p.few) out.high = kPer * tid + i;
             }
             c += count[i];
             m += mass[i];
         }
         __syncthreads();
     }
+    if (p.few) return;
     if (p.top_p < 1.0f) {
         const uint64_t f = p.top_p > 0.0f ? fraction(p.top_p) : 0, upper = out.total, lower = out.last >= 0 ? out.before_last + 1 : upper;
         const uint64_t first = share_up(f, lower) > 0 ? share_up(f, lower) : 1, second = share_up(f, upper) > 0 ? share_up(f, upper) : 1;
@@ -333,244 +409,550 @@ __device__ __forceinline__ void find_cuts(const SampleArgs& a, int row, const Pa
     __syncthreads();
 }
 
+// A chunk's values: those of the cuts' bins to the list in LDS, of those above them the sum of weights.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_masses_kernel(const SampleArgs a) {
-    __shared__ uint64_t parts[kThreads / 64];
-    __shared__ Cuts cuts;
-    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
-    const Params p = params_of(a, row);
-    if (p.greedy) return;
-    int low = kBins, high = kBins, last = -1;
-    if (p.cut) {
-        find_cuts<kThreads>(a, row, p, cuts, parts);
-        low = cuts.low; high = cuts.high; last = cuts.last;
+__device__ __forceinline__ uint64_t sort_out(const Params& p, const float (&v)[Row<T>::kValues], int first, int low, int high, int last, uint64_t* list, uint32_t* listed) {
+    if (p.few) {
+        float most = v[0];
+#pragma unroll
+        for (int i = 1; i < Row<T>::kValues; ++i) most = fmaxf(most, v[i]);
+        if (weighs(p, most) && bin_of(p, most) <= high) {
+#pragma unroll
+            for (int i = 0; i < Row<T>::kValues; ++i)
+                if (weighs(p, v[i]) && bin_of(p, v[i]) <= high) {
+                    const uint32_t at = atomicAdd(listed, 1u);
+                    if (at < kListed) list[at] = place_key(order_key(v[i]), first + i);
+                }
+        }
+        return 0;
     }
-    const Row<T> x(a, row);
-    const int end = min((slice + 1) * a.slice_chunks, x.chunks());
     uint64_t sum = 0;
-    for (int c = slice * a.slice_chunks + tid; c < end; c += kThreads) {
-        uint32_t key[Row<T>::kValues];
-        const int first = x.keys(c, key);
+    bool any = false, certain = false;
+    int bin[Row<T>::kValues];
+#pragma unroll
+    for (int i = 0; i < Row<T>::kValues; ++i) {
+        bin[i] = weighs(p, v[i]) ? bin_of(p, v[i]) : 0x7fffffff;
+        certain |= bin[i] < low;
+        any |= (bin[i] >= low && bin[i] <= high) || bin[i] == last;
+    }
+    if (certain) {
 #pragma unroll
         for (int i = 0; i < Row<T>::kValues; ++i) {
-            if (key[i] == kNone) continue;
-            const double y = exponent_of(p, of_key(key[i]));
-            const int bin = bin_of(p, y);
-            if (bin > high && bin != last) continue;
-            const uint64_t w = weight_of(y);
-            if (w == 0) continue;
-            if (bin < low) {
-                if (w >= p.least_weight) sum += w;
-            } else {
-                const uint32_t at = atomicAdd(a.listed_count + row, 1u);
-                if (at < kListed) a.listed[static_cast<size_t>(row) * kListed + at] = place_key(key[i], first + i);
-            }
+            const uint64_t w = weight_of(p, v[i]);
+            sum += w & only(bin[i] < low) & only(w >= p.least_weight);
         }
     }
+    if (any)
 #pragma unroll
-    for (int i = 32; i > 0; i /= 2) sum += __shfl_xor(static_cast<unsigned long long>(sum), i);
-    __syncthreads();
-    if ((tid & 63) == 0) parts[tid >> 6] = sum;
-    __syncthreads();
-    if (tid == 0) a.masses[static_cast<size_t>(row) * a.slices + slice] = (parts[0] + parts[1]) + (parts[2] + parts[3]);
+        for (int i = 0; i < Row<T>::kValues; ++i)
+            if ((bin[i] >= low && bin[i] <= high) || bin[i] == last) {
+                const uint32_t at = atomicAdd(listed, 1u);
+                if (at < kListed) list[at] = place_key(order_key(v[i]), first + i);
+            }
+    return sum;
 }
 
-// the sum over the workgroup, for all threads
-template <int THREADS> __device__ __forceinline__ void all_sum(uint64_t& v, uint64_t* parts) {
-#pragma unroll
-    for (int i = 32; i > 0; i /= 2) v += __shfl_xor(static_cast<unsigned long long>(v), i);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0;
-    for (int w = 0; w < THREADS / 64; ++w) v += parts[w];
-}
-
-template <typename T>
-__global__ __launch_bounds__(kLastThreads) void sample_token_kernel(const SampleArgs a) {
-    constexpr int kPer = kListed / kLastThreads, kValues = Row<T>::kValues;
-    __shared__ uint64_t list[kListed];
-    __shared__ uint64_t parts[kLastThreads / 64];
-    __shared__ Cuts cuts;
-    __shared__ uint64_t found[3];
-    __shared__ int chosen;
-    const int row = blockIdx.x, tid = threadIdx.x;
-    const Params p = params_of(a, row);
-    if (p.greedy) {
-        if (tid == 0) a.tokens[row] = static_cast<uint32_t>(p.best >> 32) == kNone ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(p.best));
+// Values of LDS in falling order, n a power of two; up to 128 by one wave, without barriers.
+template <int THREADS> __device__ __forceinline__ void sort_falling(uint64_t* list, int n) {
+    auto stage = [&](int size, int step, int i) {
+        const int low = 2 * i - (i & (step - 1)), high = low + step;
+        const uint64_t u = list[low], v = list[high];
+        if ((u < v) == ((low & size) == 0)) { list[low] = v; list[high] = u; }
+    };
+    if (n <= 128) {
+        if (threadIdx.x < 64)
+            for (int size = 2; size <= n; size *= 2)
+                for (int step = size / 2; step > 0; step /= 2) {
+                    if (static_cast<int>(threadIdx.x) < n / 2) stage(size, step, threadIdx.x);
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();                          // (one wave's LDS operations take effect in order)
+                }
+        __syncthreads();
         return;
     }
-    const Row<T> x(a, row);
-    uint64_t last_kept = 0;                                                   // place key of the last value that is kept
-    uint32_t listed = 0;
-    if (p.cut) {
-        find_cuts<kLastThreads>(a, row, p, cuts, parts);
-        listed = a.listed_count[row];
+    for (int size = 2; size <= n; size *= 2)
+        for (int step = size / 2; step > 0; step /= 2) {
+            for (int i = threadIdx.x; i < n / 2; i += THREADS) stage(size, step, i);
+            __syncthreads();
+        }
+}
+
+template <int THREADS> struct Choice {           // LDS of the last step
+    uint64_t list[kListed];
+    uint64_t sums[kBins];                       // of bins, of parts of a bin, of stretches
+    uint64_t few[kTied];
+    uint64_t parts[THREADS / 64];
+    uint64_t found[3];
+    Cuts cuts;
+    uint32_t fews;
+};
+static_assert(kMostStretches <= kBins, "stretches have a place each in sums");
+
+// From sums [n] (n a multiple of THREADS or fewer) the first whose running sum reaches `least`: number and the sum in front of it, for all threads.
+template <int THREADS> __device__ __forceinline__ int reach(Choice<THREADS>& s, int n, uint64_t least, uint64_t& before) {
+    constexpr int kPer = kBins / THREADS;
+    uint64_t v[kPer], mine = 0, total;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int at = kPer * static_cast<int>(threadIdx.x) + i;
+        v[i] = at < n ? s.sums[at] : 0;
+        mine += v[i];
     }
-    const bool bounded = p.cut && cuts.low < kBins;
-    auto weight_key = [&](uint64_t key) { return weight_of(exponent_of(p, of_key(static_cast<uint32_t>(key >> 32)))); };
-    auto bin_key = [&](uint64_t key) { return bin_of(p, exponent_of(p, of_key(static_cast<uint32_t>(key >> 32)))); };
-    if (bounded && listed <= kListed) {
-        // the listed values in order, falling
-        int n = 64;
-        while (n < static_cast<int>(listed)) n *= 2;
-        for (int i = tid; i < n; i += kLastThreads) list[i] = i < static_cast<int>(listed) ? a.listed[static_cast<size_t>(row) * kListed + i] : 0;
-        __syncthreads();
-        for (int size = 2; size <= n; size *= 2)
-            for (int step = size / 2; step > 0; step /= 2) {
-                for (int i = tid; i < n / 2; i += kLastThreads) {
-                    const int low = 2 * i - (i & (step - 1)), high = low + step;
-                    const uint64_t u = list[low], v = list[high];
-                    if ((u < v) == ((low & size) == 0)) { list[low] = v; list[high] = u; }
-                }
-                __syncthreads();
-            }
-        // sums of their weights in that order; those of bin `last` apart
-        uint64_t w[kPer], mine = 0, in_last = 0;
-        int at_last[kPer];
+    uint64_t until = threads_until<THREADS>(mine, s.parts, total) - mine;
+    if (until < least && until + mine >= least) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const int at = kPer * tid + i;
-            const bool there = at < static_cast<int>(listed);
-            w[i] = there ? weight_key(list[at]) : 0;
-            at_last[i] = there && cuts.last >= 0 && bin_key(list[at]) == cuts.last;
-            mine += w[i];
-            in_last += at_last[i];
+            if (until < least && until + v[i] >= least) { s.found[0] = kPer * threadIdx.x + i; s.found[1] = until; }
+            until += v[i];
         }
-        uint64_t total, total_last;
-        uint64_t until = threads_until<kLastThreads>(mine, parts, total) - mine;
+    }
+    __syncthreads();
+    before = s.found[1];
+    return static_cast<int>(s.found[0]);
+}
+
+// Of the listed values of a bin, in falling order of their places: the first one at which the sum (of weights, or of ones) reaches `least`.  The bin is cut in kBins parts
+// once more; what is left in a part is equal values mostly.
+template <int THREADS, typename Weight>
+__device__ __forceinline__ uint64_t resolve(Choice<THREADS>& s, const Params& p, int listed, int bin, uint64_t least, const Weight& weight) {
+    const int tid = threadIdx.x;
+    auto place_of = [&](uint64_t key, int& part) {                             // its bin, and its part of it
+        const float x = of_key(static_cast<uint32_t>(key >> 32));
+        const int b = bin_of(p, x);
+        // (fused by name: left to the compiler, one loop had the product rounded and the other not, and looked for a value in the neighbouring part)
+        const float inside = __builtin_fmaf(distance(p, x), p.per_bin, -static_cast<float>(b));
+        part = static_cast<int>(fminf(fmaxf(inside * kBins, 0.0f), kBins - 1.0f));
+        return b;
+    };
+    __syncthreads();
+    for (int i = tid; i < kBins; i += THREADS) s.sums[i] = 0;
+    if (tid == 0) s.fews = 0;
+    __syncthreads();
+    for (int i = tid; i < listed; i += THREADS) {
+        int part;
+        if (place_of(s.list[i], part) == bin) add_to(&s.sums[part], weight(s.list[i]));
+    }
+    __syncthreads();
+    uint64_t before;
+    const int of = reach<THREADS>(s, kBins, least, before);
+    for (int i = tid; i < listed; i += THREADS) {
+        int part;
+        if (place_of(s.list[i], part) == bin && part == of) {
+            const uint32_t at = atomicAdd(&s.fews, 1u);
+            if (at < kTied) s.few[at] = s.list[i];
+        }
+    }
+    __syncthreads();
+    const int n = static_cast<int>(s.fews);
+    if (n > kTied) return 0;                                                  // (no place: the caller goes by the row)
+    if (n <= 64) {                                                            // each against all
+        const uint64_t mine = tid < n ? s.few[tid] : 0, w = tid < n ? weight(mine) : 0;
+        uint64_t sum = before;
+        if (tid < n) {
+            for (int i = 0; i < n; ++i) sum += s.few[i] > mine ? weight(s.few[i]) : 0;
+            if (sum < least && sum + w >= least) s.found[2] = mine;
+        }
         __syncthreads();
-        uint64_t rank = threads_until<kLastThreads>(in_last, parts, total_last) - in_last;
-        if (tid == 0) { found[0] = 0; found[1] = 0; found[2] = 0; }
+        return s.found[2];
+    }
+    int size = 128;
+    while (size < n) size *= 2;
+    for (int i = n + tid; i < size; i += THREADS) s.few[i] = 0;
+    __syncthreads();
+    sort_falling<THREADS>(s.few, size);
+    for (int i = tid; i < kTied; i += THREADS) s.sums[i] = i < n ? weight(s.few[i]) : 0;
+    __syncthreads();
+    uint64_t in_front;
+    const int at = reach<THREADS>(s, kTied, least - before, in_front);
+    return s.few[at];
+}
+
+// The last step, by a workgroup: the token.  The listed values are in s.list, unordered, `listed` of them (more than the list holds: bisection); certain(i) is what is
+// kept for certain of stretch i (kStretch chunks).
+template <typename T, int THREADS, typename Certain>
+__device__ __forceinline__ int64_t choose(const Row<T>& x, const Params& p, Choice<THREADS>& s, int listed, float u, const Certain& certain) {
+    constexpr int kValues = Row<T>::kValues;
+    const int tid = threadIdx.x, stretches = (x.chunks() + kStretch - 1) / kStretch;
+    const uint64_t u_fraction = fraction(u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f), p_fraction = p.top_p > 0.0f ? fraction(p.top_p) : 0;
+    const Cuts cuts = s.cuts;
+    const bool bounded = p.cut && cuts.low < kBins;
+    bool ordered = bounded && listed <= kListed;
+    auto weight_key = [&](uint64_t key) { return weight_of(p, of_key(static_cast<uint32_t>(key >> 32))); };
+    auto bin_key = [&](uint64_t key) { return bin_of(p, of_key(static_cast<uint32_t>(key >> 32))); };
+    auto one = [](uint64_t) { return uint64_t{1}; };
+    uint64_t last_kept = 0;                                                   // place key of the last value that is kept
+    if (ordered && p.few && listed <= kDirect) {
+        // everything that is kept is in a short list: each against all, in the order of the values and in that of the indexes
+        uint64_t key = 0, w = 0, before = 0;
+        int rank = 0;
+        if (tid < listed) {
+            key = s.list[tid];
+            w = weight_key(key);
+            s.few[tid] = w;
+        }
         __syncthreads();
-        uint64_t sums[kPer];
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) { until += w[i]; sums[i] = until; }
-        if (cuts.last >= 0) {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                if (at_last[i] && ++rank == 1) found[0] = sums[i] - w[i];     // in front of the bin
-                if (at_last[i] && rank == cuts.need) { found[1] = sums[i]; found[2] = list[kPer * tid + i]; }
+        if (tid < listed)
+            for (int i = 0; i < listed; ++i) {
+                const bool above = s.list[i] > key;
+                rank += above;
+                before += above ? s.few[i] : 0;
             }
-            __syncthreads();
-        }
-        last_kept = found[2];
-        if (p.top_p < 1.0f) {
-            const uint64_t all = cuts.last >= 0 ? cuts.before_last + found[1] - found[0] : cuts.total;
-            const uint64_t share = share_up(p.top_p > 0.0f ? fraction(p.top_p) : 0, all), least = (share > 0 ? share : 1) - cuts.before_low;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (w[i] && sums[i] - w[i] < least && sums[i] >= least) found[2] = list[kPer * tid + i];
-            __syncthreads();
-            last_kept = found[2];
-        }
-    } else if (bounded) {
-        // more values in the cuts' bins than the list holds, many of them equal: bisection over their places, a pass over the row each
-        auto pass = [&](uint64_t from, int low, int high, bool counts) {
+        bool stays = tid < listed && rank < p.top_k;
+        const uint64_t all = all_sum<THREADS>(stays ? w : 0, s.parts), share = share_up(p_fraction, all);
+        stays &= (!(p.top_p < 1.0f) || rank == 0 || before < share) && w >= p.least_weight;
+        const uint64_t total = all_sum<THREADS>(stays ? w : 0, s.parts), target = __umul64hi(u_fraction, total);
+        if (tid < listed) s.few[tid] = stays ? w : 0;
+        __syncthreads();
+        if (stays) {
             uint64_t sum = 0;
-            for (int c = tid; c < x.chunks(); c += kLastThreads) {
-                uint32_t key[kValues];
-                const int first = x.keys(c, key);
+            for (int i = 0; i < listed; ++i) sum += static_cast<uint32_t>(s.list[i]) > static_cast<uint32_t>(key) ? s.few[i] : 0;             // (complements)
+            if (sum <= target && sum + w > target) s.found[2] = ~static_cast<uint32_t>(key);
+        }
+        __syncthreads();
+        return static_cast<int64_t>(s.found[2]);
+    }
+    if (ordered) {
+        uint64_t all = cuts.total;                                            // what the first k add up to
+        int last = cuts.last;
+        uint64_t need = cuts.need;
+        if (p.few) {
+            // (the histogram may have had the chunks' largest values alone)
+            need = 0;
+            if (listed > p.top_k) {
+                uint64_t before;
+                __syncthreads();
+                for (int i = tid; i < kBins; i += THREADS) s.sums[i] = 0;
+                __syncthreads();
+                for (int i = tid; i < listed; i += THREADS) add_to(&s.sums[bin_key(s.list[i])], 1);
+                __syncthreads();
+                last = reach<THREADS>(s, kBins, p.top_k, before);
+                need = p.top_k - before;
+            } else {                                                          // all of them: down to the least
+                if (tid == 0) s.found[2] = ~uint64_t{0};
+                __syncthreads();
+                for (int i = tid; i < listed; i += THREADS) atomicMin(reinterpret_cast<unsigned long long*>(&s.found[2]), static_cast<unsigned long long>(s.list[i]));
+                __syncthreads();
+                last_kept = s.found[2];
+            }
+        }
+        if (last >= 0 && need > 0) {
+            last_kept = resolve<THREADS>(s, p, listed, last, need, one);
+            ordered = last_kept != 0;
+        }
+        if (ordered && p.top_p < 1.0f) {
+            if (cuts.last >= 0) {
+                uint64_t sum = 0;
+                for (int i = tid; i < listed; i += THREADS) sum += s.list[i] >= last_kept && (p.few || bin_key(s.list[i]) == cuts.last) ? weight_key(s.list[i]) : 0;
+                all = all_sum<THREADS>(sum, s.parts) + cuts.before_last;
+            }
+            const uint64_t share = share_up(p_fraction, all), least = (share > 0 ? share : 1) - cuts.before_low;
+            int bin = cuts.low;
+            uint64_t before = 0;
+            if (cuts.low != cuts.high) {
+                __syncthreads();
+                for (int i = tid; i < kBins; i += THREADS) s.sums[i] = 0;
+                __syncthreads();
+                for (int i = tid; i < listed; i += THREADS) {
+                    const int b = bin_key(s.list[i]);
+                    if (b <= cuts.high) add_to(&s.sums[b], weight_key(s.list[i]));
+                }
+                __syncthreads();
+                bin = reach<THREADS>(s, kBins, least, before);
+            }
+            last_kept = resolve<THREADS>(s, p, listed, bin, least - before, weight_key);
+            ordered = last_kept != 0;
+        }
+    }
+    if (bounded && !ordered) {
+        last_kept = 0;
+        // more values at the cuts than the list holds, many of them equal: by the digits of their places, from the first on, a pass over the row for each of eight
+        auto reached = [&](uint64_t least, bool counts) {                      // the place of the value at which the sum reaches `least`
+            uint64_t place = 0;
+            for (int shift = 56; shift >= 0; shift -= 8) {
+                __syncthreads();
+                for (int i = tid; i < 256; i += THREADS) s.sums[i] = 0;
+                __syncthreads();
+                for_chunks<T, THREADS>(x, 0, x.chunks(), [&](int c, const float (&v)[kValues]) {
+                    // (neighbours mostly have one digit: their sum in one addition)
+                    uint64_t sum = 0;
+                    int digit = 0;
+#pragma unroll
+                    for (int i = 0; i < kValues; ++i) {
+                        const uint64_t key = place_key(order_key(v[i]), x.first_of(c) + i), w = weight_of(p, v[i]);
+                        if (w == 0 || (shift < 56 && (key >> shift >> 8) != (place >> shift >> 8))) continue;
+                        const int its = 255 - static_cast<int>(key >> shift & 255);          // falling
+                        if (sum && its != digit) { add_to(&s.sums[digit], sum); sum = 0; }
+                        digit = its;
+                        sum += counts ? 1 : w;
+                    }
+                    const int first = __builtin_amdgcn_readfirstlane(digit);
+                    if (__ballot(digit == first) == ~0ull) {                  // (all 64 lanes)
+                        sum = lanes_sum(sum);
+                        if (sum && (tid & 63) == 0) add_to(&s.sums[first], sum);
+                    } else if (sum) add_to(&s.sums[digit], sum);
+                });
+                __syncthreads();
+                uint64_t before;
+                const int its = reach<THREADS>(s, 256, least, before);
+                least -= before;
+                place |= static_cast<uint64_t>(255 - its) << shift;
+            }
+            return place;
+        };
+        auto whole = [&](uint64_t from, bool counts) {
+            uint64_t sum = 0;
+            for_chunks<T, THREADS>(x, 0, x.chunks(), [&](int c, const float (&v)[kValues]) {
 #pragma unroll
                 for (int i = 0; i < kValues; ++i) {
-                    if (key[i] == kNone || place_key(key[i], first + i) < from) continue;
-                    const double y = exponent_of(p, of_key(key[i]));
-                    const int bin = bin_of(p, y);
-                    if (bin < low || bin > high) continue;
-                    const uint64_t w = weight_of(y);
+                    const uint64_t w = place_key(order_key(v[i]), x.first_of(c) + i) < from ? 0 : weight_of(p, v[i]);
                     sum += counts ? (w != 0) : w;
                 }
-            }
-            all_sum<kLastThreads>(sum, parts);
-            return sum;
+            });
+            return all_sum<THREADS>(sum, s.parts);
         };
-        auto bisect = [&](uint64_t least, int low, int high, bool counts) {    // the largest place from which on there is as much
-            uint64_t from = 0;
-            for (uint64_t bit = uint64_t{1} << 63; bit; bit >>= 1)
-                if (pass(from | bit, low, high, counts) >= least) from |= bit;
-            return from;
-        };
-        uint64_t all = cuts.total;
-        if (cuts.last >= 0) {
-            last_kept = bisect(cuts.need, cuts.last, cuts.last, true);
-            all = cuts.before_last + pass(last_kept, cuts.last, cuts.last, false);
-        }
+        if (p.top_k > 0 && whole(0, true) > static_cast<uint64_t>(p.top_k)) last_kept = reached(p.top_k, true);
         if (p.top_p < 1.0f) {
-            const uint64_t share = share_up(p.top_p > 0.0f ? fraction(p.top_p) : 0, all);
-            last_kept = bisect((share > 0 ? share : 1) - cuts.before_low, cuts.low, cuts.high, false);
+            const uint64_t share = share_up(p_fraction, whole(last_kept, false));
+            last_kept = reached(share > 0 ? share : 1, false);
         }
     }
-    // sums of the slices: what was kept for certain and the listed values that are
+    // what is kept of each stretch: for certain, and of the listed values
     auto kept = [&](uint64_t key, uint64_t w) { return key >= last_kept && w >= p.least_weight; };
-    auto slice_sum = [&](int slice) { return a.masses[static_cast<size_t>(row) * a.slices + slice]; };
-    __shared__ uint64_t sums[kLastThreads];                                   // (at most so many slices)
-    for (int i = tid; i < a.slices; i += kLastThreads) sums[i] = slice_sum(i);
     __syncthreads();
-    auto add = [&](uint64_t key, uint64_t w) {
-        const int slice = (static_cast<int>(~static_cast<uint32_t>(key)) + x.skew) / kValues / a.slice_chunks;
-        atomicAdd(reinterpret_cast<unsigned long long*>(&sums[slice]), static_cast<unsigned long long>(w));
-    };
-    if (bounded && listed <= kListed) {
-        for (int i = tid; i < static_cast<int>(listed); i += kLastThreads) {
-            const uint64_t w = weight_key(list[i]);
-            if (kept(list[i], w)) add(list[i], w);
+    for (int i = tid; i < stretches; i += THREADS) s.sums[i] = p.few ? 0 : certain(i);
+    __syncthreads();
+    if (ordered) {
+        for (int i = tid; i < listed; i += THREADS) {
+            const uint64_t key = s.list[i], w = weight_key(key);
+            if (kept(key, w)) add_to(&s.sums[(static_cast<int>(~static_cast<uint32_t>(key)) + x.skew) / kValues / kStretch], w);
         }
     } else if (bounded) {
-        for (int c = tid; c < x.chunks(); c += kLastThreads) {
-            uint32_t key[kValues];
-            const int first = x.keys(c, key);
+        for_chunks<T, THREADS>(x, 0, x.chunks(), [&](int c, const float (&v)[kValues]) {
+            uint64_t sum = 0;
 #pragma unroll
             for (int i = 0; i < kValues; ++i) {
-                if (key[i] == kNone) continue;
-                const uint64_t place = place_key(key[i], first + i), w = weight_key(place);
-                if (bin_key(place) >= cuts.low && kept(place, w)) add(place, w);
+                const uint64_t w = weight_of(p, v[i]);
+                if (w && bin_of(p, v[i]) >= cuts.low && kept(place_key(order_key(v[i]), x.first_of(c) + i), w)) sum += w;
             }
-        }
+            add_all(&s.sums[c / kStretch], sum);
+        });
     }
     __syncthreads();
-    const uint64_t mine = tid < a.slices ? sums[tid] : 0;
-    uint64_t total;
-    const uint64_t until = threads_until<kLastThreads>(mine, parts, total);
-    const float u = a.uniform[row];
-    const uint64_t target = __umul64hi(fraction(u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f), total);         // the token's sum is the first above it
-    if (until - mine <= target && until > target) { chosen = tid; found[0] = until - mine; }
-    __syncthreads();
-    const int begin = chosen * a.slice_chunks, end = min(begin + a.slice_chunks, x.chunks());
-    uint64_t before = found[0];
-    for (int c0 = begin; c0 < end; c0 += kLastThreads) {
-        uint32_t key[kValues];
-        uint64_t w[kValues], own = 0;
-        int first = 0;
-#pragma unroll
-        for (int i = 0; i < kValues; ++i) w[i] = 0;
-        if (c0 + tid < end) {
-            first = x.keys(c0 + tid, key);
-#pragma unroll
-            for (int i = 0; i < kValues; ++i) {
-                if (key[i] == kNone) continue;
-                const uint64_t place = place_key(key[i], first + i), v = weight_key(place);
-                w[i] = kept(place, v) ? v : 0;
-                own += w[i];
+    uint64_t total = 0;
+    for (int i = tid; i < stretches; i += THREADS) total += s.sums[i];
+    total = all_sum<THREADS>(total, s.parts);
+    const uint64_t target = __umul64hi(u_fraction, total);                    // the token's sum is the first above it
+    uint64_t before;
+    const int stretch = reach<THREADS>(s, stretches, target + 1, before);
+    if (ordered && p.few) {
+        // everything that is kept is in the list: the stretch's in rising order of their indexes, each against all (a stretch with more is looked at in the row)
+        if (tid == 0) s.fews = 0;
+        __syncthreads();
+        for (int i = tid; i < listed; i += THREADS) {
+            const uint64_t key = s.list[i];
+            if ((static_cast<int>(~static_cast<uint32_t>(key)) + x.skew) / kValues / kStretch == stretch && kept(key, weight_key(key))) {
+                const uint32_t at = atomicAdd(&s.fews, 1u);
+                if (at < kTied) s.few[at] = key;
             }
         }
-        uint64_t here;
         __syncthreads();
-        uint64_t sum = before + threads_until<kLastThreads>(own, parts, here) - own;
+        const int n = static_cast<int>(s.fews);
+        if (n <= 64) {
+            if (tid < n) {
+                const uint64_t mine = s.few[tid];
+                uint64_t sum = before;
+                for (int i = 0; i < n; ++i) sum += static_cast<uint32_t>(s.few[i]) > static_cast<uint32_t>(mine) ? weight_key(s.few[i]) : 0;      // (complements)
+                if (sum <= target && sum + weight_key(mine) > target) s.found[2] = ~static_cast<uint32_t>(mine);
+            }
+            __syncthreads();
+            return static_cast<int64_t>(s.found[2]);
+        }
+    }
+    const int begin = stretch * kStretch, end = min(begin + kStretch, x.chunks());
+    static_assert(kStretch % THREADS == 0, "whole passes");
+    for (int c0 = begin; c0 < end; c0 += THREADS) {
+        float v[kValues];
+        uint64_t w[kValues], own = 0, here;
+        Row<T>::values_of(x.load(c0 + tid, end), v);
+        const int first = x.first_of(c0 + tid);
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) {
+            w[i] = weight_of(p, v[i]);
+            w[i] = kept(place_key(order_key(v[i]), first + i), w[i]) ? w[i] : 0;
+            own += w[i];
+        }
+        uint64_t sum = before + threads_until<THREADS>(own, s.parts, here) - own;
         if (sum <= target && sum + own > target) {
 #pragma unroll
             for (int i = 0; i < kValues; ++i) {
-                if (sum <= target && sum + w[i] > target) a.tokens[row] = first + i;
+                if (sum <= target && sum + w[i] > target) s.found[2] = static_cast<uint64_t>(first + i);
                 sum += w[i];
             }
         }
         before += here;
         if (before > target) break;                                           // (all threads alike)
     }
+    __syncthreads();
+    return static_cast<int64_t>(s.found[2]);
+}
+
+__device__ __forceinline__ int64_t greedy_token(uint64_t best) { return static_cast<uint32_t>(best >> 32) == kNone ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(best)); }
+
+// ---- few rows: slices ---------------------------------------------------------------------------------------------------
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_extremes_kernel(const SampleArgs a) {
+    __shared__ uint64_t bests[kThreads / 64];
+    __shared__ uint32_t leasts[kThreads / 64];
+    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
+    for (int i = slice * kThreads + tid; i < kBins; i += a.slices * kThreads) {              // for the next launch
+        a.mass[static_cast<size_t>(row) * kBins + i] = 0;
+        a.count[static_cast<size_t>(row) * kBins + i] = 0;
+    }
+    if (slice == 0 && tid == 0) a.listed_count[row] = 0;
+    const Row<T> x(a, row);
+    uint64_t best = place_key(kNone, 0x7fffffff);
+    uint32_t least = 0xffffffffu;
+    extremes<T, kThreads>(x, slice * a.slice_chunks, min((slice + 1) * a.slice_chunks, x.chunks()), best, least);
+    wave_extremes(best, least);
+    if ((tid & 63) == 0) { bests[tid >> 6] = best; leasts[tid >> 6] = least; }
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < kThreads / 64; ++w) {
+            best = bests[w] > best ? bests[w] : best;
+            least = min(least, leasts[w]);
+        }
+        a.best[static_cast<size_t>(row) * a.slices + slice] = best;
+        a.least[static_cast<size_t>(row) * a.slices + slice] = least;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_histogram_kernel(const SampleArgs a) {
+    __shared__ uint64_t mass[kBins];
+    __shared__ uint32_t count[kBins];
+    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
+    const Params p = slices_params(a, row, asked_of(a, row));
+    if (p.greedy || !p.cut) return;
+    for (int i = tid; i < kBins; i += kThreads) { mass[i] = 0; count[i] = 0; }
+    __syncthreads();
+    const Row<T> x(a, row);
+    fill<T, kThreads>(x, p, slice * a.slice_chunks, min((slice + 1) * a.slice_chunks, x.chunks()), mass, count);
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kThreads)
+        if (count[i]) {
+            if (!p.few) add_to(a.mass + static_cast<size_t>(row) * kBins + i, mass[i]);
+            atomicAdd(a.count + static_cast<size_t>(row) * kBins + i, count[i]);
+        }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_masses_kernel(const SampleArgs a) {
+    __shared__ uint64_t list[kListed], parts[kThreads / 64], sums[kMostStretches];
+    __shared__ Cuts cuts;
+    __shared__ uint32_t listed, at;
+    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
+    const Params p = slices_params(a, row, asked_of(a, row));
+    if (p.greedy) return;
+    if (tid == 0) listed = 0;
+    for (int i = tid; i < kMostStretches; i += kThreads) sums[i] = 0;
+    int low = kBins, high = kBins, last = -1;
+    if (p.cut) {
+        find_cuts<kThreads>(a.mass + static_cast<size_t>(row) * kBins, a.count + static_cast<size_t>(row) * kBins, p, cuts, parts);
+        low = cuts.low; high = cuts.high; last = cuts.last;
+    }
+    __syncthreads();
+    const Row<T> x(a, row);
+    const int begin = slice * a.slice_chunks, end = min(begin + a.slice_chunks, x.chunks());
+    for_chunks<T, kThreads>(x, begin, end, [&](int c, const float (&v)[Row<T>::kValues]) {
+        const uint64_t sum = sort_out<T>(p, v, x.first_of(c), low, high, last, list, &listed);
+        if (!p.few) add_all(&sums[(c - begin) / kStretch], sum);
+    });
+    __syncthreads();
+    const int stretches = (end - begin + kStretch - 1) / kStretch;            // (slices are whole stretches)
+    if (!p.few)
+        for (int i = tid; i < stretches; i += kThreads) a.masses[static_cast<size_t>(row) * a.stretches + begin / kStretch + i] = sums[i];
+    if (listed == 0) return;
+    if (tid == 0) at = atomicAdd(a.listed_count + row, listed);               // (more than the list holds is more than that here too)
+    __syncthreads();
+    for (int i = tid; i < static_cast<int>(min(listed, static_cast<uint32_t>(kListed))); i += kThreads)
+        if (at + i < kListed) a.listed[static_cast<size_t>(row) * kListed + at + i] = list[i];
+}
+
+template <typename T>
+__global__ __launch_bounds__(kLastThreads) void sample_token_kernel(const SampleArgs a) {
+    __shared__ Choice<kLastThreads> s;
+    const int row = blockIdx.x, tid = threadIdx.x;
+    const Asked asked = asked_of(a, row);
+    const Params p = slices_params(a, row, asked);
+    if (p.greedy) {
+        if (tid == 0) a.tokens[row] = greedy_token(p.best);
+        return;
+    }
+    int listed = 0;
+    if (p.cut) {
+        listed = static_cast<int>(a.listed_count[row]);
+        for (int i = tid; i < min(listed, kListed); i += kLastThreads) s.list[i] = a.listed[static_cast<size_t>(row) * kListed + i];
+        find_cuts<kLastThreads>(a.mass + static_cast<size_t>(row) * kBins, a.count + static_cast<size_t>(row) * kBins, p, s.cuts, s.parts);
+    }
+    __syncthreads();
+    const int64_t token = choose<T, kLastThreads>(Row<T>(a, row), p, s, listed, asked.uniform, [&](int i) { return a.masses[static_cast<size_t>(row) * a.stretches + i]; });
+    if (tid == 0) a.tokens[row] = token;
+}
+
+// ---- many rows: a workgroup each ----------------------------------------------------------------------------------------
+
+template <typename T>
+__global__ __launch_bounds__(kRowThreads, 5) void sample_row_kernel(const SampleArgs a) {
+    __shared__ Choice<kRowThreads> s;
+    __shared__ uint32_t count[kBins], leasts[kRowThreads / 64], listed;
+    __shared__ uint64_t sums[kMostStretches];
+    const int row = blockIdx.x, tid = threadIdx.x;
+    const Row<T> x(a, row);
+    const Asked asked = asked_of(a, row);                                     // (on its way beside the row)
+    const int chunks = x.chunks();
+    uint64_t best = place_key(kNone, 0x7fffffff);
+    uint32_t least = 0xffffffffu;
+    extremes<T, kRowThreads>(x, 0, chunks, best, least);
+    wave_extremes(best, least);
+    if ((tid & 63) == 0) { s.parts[tid >> 6] = best; leasts[tid >> 6] = least; }
+    if (tid == 0) listed = 0;
+    for (int i = tid; i < kBins; i += kRowThreads) { s.sums[i] = 0; count[i] = 0; }
+    for (int i = tid; i < kMostStretches; i += kRowThreads) sums[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kRowThreads / 64; ++w) {
+        best = s.parts[w] > best ? s.parts[w] : best;
+        least = min(least, leasts[w]);
+    }
+    const Params p = params_of(asked, a.vocab, best, least);
+    if (p.greedy) {
+        if (tid == 0) a.tokens[row] = greedy_token(p.best);
+        return;
+    }
+    int low = kBins, high = kBins, last = -1;
+    __syncthreads();
+    if (p.cut) {
+        fill<T, kRowThreads>(x, p, 0, chunks, s.sums, count);
+        __syncthreads();
+        find_cuts<kRowThreads>(s.sums, count, p, s.cuts, s.parts);
+        low = s.cuts.low; high = s.cuts.high; last = s.cuts.last;
+    }
+    for_chunks<T, kRowThreads>(x, 0, chunks, [&](int c, const float (&v)[Row<T>::kValues]) {
+        const uint64_t sum = sort_out<T>(p, v, x.first_of(c), low, high, last, s.list, &listed);
+        if (!p.few) add_all(&sums[c / kStretch], sum);
+    });
+    __syncthreads();
+    const int64_t token = choose<T, kRowThreads>(x, p, s, static_cast<int>(listed), asked.uniform, [&](int i) { return sums[i]; });
+    if (tid == 0) a.tokens[row] = token;
 }
 
 template <typename T> int launch(const SampleArgs& a, hipStream_t stream) {
     const dim3 grid(a.slices, a.rows);
+    if (a.slices == 0) {
+        hipLaunchKernelGGL((sample_row_kernel<T>), dim3(a.rows), dim3(kRowThreads), 0, stream, a);
+        return hipGetLastError() == hipSuccess ? PLLM_OK : PLLM_ERR_LAUNCH;
+    }
     hipLaunchKernelGGL((sample_extremes_kernel<T>), grid, dim3(kThreads), 0, stream, a);
     const bool cut = a.top_k || a.top_p || (a.top_k_all > 0 && a.top_k_all < a.vocab) || a.top_p_all < 1.0f;
     if (cut) hipLaunchKernelGGL((sample_histogram_kernel<T>), grid, dim3(kThreads), 0, stream, a);
@@ -579,21 +961,26 @@ template <typename T> int launch(const SampleArgs& a, hipStream_t stream) {
     return hipGetLastError() == hipSuccess ? PLLM_OK : PLLM_ERR_LAUNCH;
 }
 
-struct Layout { int slices, slice_chunks; size_t best, least, masses, mass, count, listed, listed_count, bytes; };
+struct Layout { int slices, slice_chunks, stretches; size_t best, least, masses, mass, count, listed, listed_count, bytes; };
 Layout layout_of(int64_t rows, int64_t vocab, int dtype) {
     const int values = dtype == PLLM_F32 ? 4 : 8;
     const int64_t chunks = (vocab + 2 * values - 2) / values;                 // (a row may begin inside a chunk)
-    // as many slices as give the machine about four workgroups per compute unit, none of fewer than two chunks per thread
-    const int64_t most = std::min<int64_t>((chunks + 2 * kThreads - 1) / (2 * kThreads), kLastThreads);
-    const int64_t slices = std::max<int64_t>(1, std::min(most, (1024 + rows - 1) / rows));
+    // A workgroup per row where there are more rows than compute units, or rows of a few chunks per thread.  Otherwise as many slices as give the machine about four workgroups
+    // per compute unit, none of fewer than two chunks per thread.
     Layout l{};
-    l.slice_chunks = static_cast<int>((chunks + slices - 1) / slices);
-    l.slices = static_cast<int>((chunks + l.slice_chunks - 1) / l.slice_chunks);
+    if (rows >= compute_units() || chunks <= 2 * kRowThreads) {
+        l.bytes = 256;
+        return l;
+    }
+    const int64_t stretches = (chunks + kStretch - 1) / kStretch, slices = std::min(stretches, (4 * compute_units() + rows - 1) / rows), each = (stretches + slices - 1) / slices;
+    l.stretches = static_cast<int>(stretches);
+    l.slice_chunks = static_cast<int>(each * kStretch);
+    l.slices = static_cast<int>((stretches + each - 1) / each);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += align256(bytes); return here; };
     l.best = take(rows * l.slices * 8);
     l.least = take(rows * l.slices * 4);
-    l.masses = take(rows * l.slices * 8);
+    l.masses = take(rows * l.stretches * 8);
     l.mass = take(rows * kBins * 8);
     l.count = take(rows * kBins * 4);
     l.listed = take(rows * kListed * 8);
@@ -635,7 +1022,7 @@ int pllm_sample_tokens(const void* logits, int64_t stride, int dtype, const floa
     a.best = reinterpret_cast<uint64_t*>(ws + l.best); a.least = reinterpret_cast<uint32_t*>(ws + l.least); a.masses = reinterpret_cast<uint64_t*>(ws + l.masses);
     a.mass = reinterpret_cast<uint64_t*>(ws + l.mass); a.count = reinterpret_cast<uint32_t*>(ws + l.count);
     a.listed = reinterpret_cast<uint64_t*>(ws + l.listed); a.listed_count = reinterpret_cast<uint32_t*>(ws + l.listed_count);
-    a.rows = static_cast<int>(rows); a.vocab = static_cast<int>(vocab); a.slices = l.slices; a.slice_chunks = l.slice_chunks;
+    a.rows = static_cast<int>(rows); a.vocab = static_cast<int>(vocab); a.slices = l.slices; a.slice_chunks = l.slice_chunks; a.stretches = l.stretches;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == PLLM_F32) return launch<float>(a, st);
     return dtype == PLLM_F16 ? launch<F16>(a, st) : launch<B16>(a, st);
