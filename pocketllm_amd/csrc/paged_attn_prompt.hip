@@ -53,6 +53,8 @@ struct PagedPromptArgs {
     float scale;                                // base 2
     int few_rows;                               // sequences of so many query rows or fewer are another kernel's
     int even;                                   // (trees) without cu_steps: new tokens of every sequence
+    int deal;                                   // (trees in runs) compute units that a head has its share of
+    int2* plan;                                 // (trees in runs) [seqs]: number of the sequence's first unit, runs of each of its blocks
     int runs, tokens, seqs, heads, kv_heads, page_shift, pool, width, slots;
 };
 
@@ -127,6 +129,65 @@ __device__ __forceinline__ bool find_block(const PagedPromptArgs& a, int index, 
     return false;
 }
 
+// Trees in runs: the keys of a sequence's blocks are cut in runs by its own length, all runs of about the same length.  A unit is a run of a block.  Where a head has clearly fewer
+// blocks than its share of the compute units (a.deal), runs are the shortest with which its units are no more than that: all of them run at once.  Otherwise none is
+// longer than the mean of three quarters of a.deal, so that units are no more than the blocks and these together, and the longest come first.
+struct Unit { int s, block, run, runs, tiles, first; };                       // sequence, block, run of how many, tiles of a run, number of the sequence's first unit
+template <int ROWS>
+__device__ __forceinline__ bool find_unit(const PagedPromptArgs& a, int index, int group, Unit& u) {
+    constexpr int kLeastTiles = 4, kMostRuns = 64;                            // (the kernel that joins the runs has a lane for each)
+    const int lane = threadIdx.x & 63;
+    int blocks = 0, tiles = 0;                                                // of the lane's sequence
+    if (lane <= a.seqs) {
+        const int offset = offset_of<true>(a, lane), n = max((lane == a.seqs ? a.tokens : offset_of<true>(a, lane + 1)) - offset, 0);
+        const int rows = lane < a.seqs && n * group <= a.few_rows ? 0 : n * group;
+        blocks = (rows + ROWS - 1) / ROWS;
+        if (lane < a.seqs && blocks > 0) tiles = (paged_length(a.lengths[lane], a.width, a.page_shift) + kTile - 1) / kTile;
+    }
+    // (counts far below 2^24, the same float arithmetic in every workgroup; a rounding that leaves a run a tile longer than `longest` does no harm)
+    auto all = [&](float count) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(group_sum<64>(count)))); };
+    auto runs_of = [&](int longest) { return fmaxf(ceilf(static_cast<float>(tiles) * (1.0f / static_cast<float>(longest))), 1.0f); };
+    const float work = all(static_cast<float>(blocks) * static_cast<float>(tiles)), count = all(static_cast<float>(blocks));
+    const int most = __builtin_amdgcn_readfirstlane(static_cast<int>(group_max<64>(static_cast<float>(tiles))));
+    const bool at_once = 2.0f * count <= static_cast<float>(a.deal);
+    const float share = at_once ? static_cast<float>(a.deal) - count : 0.75f * static_cast<float>(a.deal);
+    int longest = static_cast<int>(ceilf(work / share * 1.0001f));            // (enough: cutting adds a unit per block at most)
+    if (at_once) {
+        int low = static_cast<int>(work / static_cast<float>(a.deal));
+        while (low + 1 < longest) {
+            const int middle = (low + longest) / 2;
+            if (all(static_cast<float>(blocks) * runs_of(middle)) <= static_cast<float>(a.deal)) longest = middle;
+            else low = middle;
+        }
+    }
+    longest = max(max(longest, most / kMostRuns + 1), kLeastTiles);
+    const int runs = static_cast<int>(runs_of(longest)), length = (tiles + runs - 1) / runs, units = blocks * runs;
+    int mine = units, place = index;
+    if (index >= static_cast<int>(all(static_cast<float>(units)))) return false;
+    if (!at_once) {
+        auto seeing = [&](int t) { return length >= t ? units : 0; };
+        auto all_seeing = [&](int t) { return static_cast<int>(all(static_cast<float>(seeing(t)))); };
+        int low = 0, high = longest + 1;
+        while (low < high) {                                                  // the most tiles that more than `index` units have
+            const int middle = (low + high + 1) / 2;
+            if (all_seeing(middle) > index) low = middle;
+            else high = middle - 1;
+        }
+        mine = seeing(low) - seeing(low + 1);
+        place = index - all_seeing(low + 1);
+    }
+    const int until = lanes_until(mine);
+    const uint64_t behind = __ballot(until > place);
+    u.s = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(behind)) - 1);
+    u.runs = __builtin_amdgcn_readlane(runs, u.s);
+    u.tiles = __builtin_amdgcn_readlane(length, u.s);
+    const int within = place - __builtin_amdgcn_readlane(until - mine, u.s);
+    u.block = within / u.runs;
+    u.run = within % u.runs;
+    u.first = index - within;
+    return true;
+}
+
 // TREE: the new tokens are nodes of a tree; the tiles that hold some of their keys are masked by the nodes' ancestors
 template <bool BF16, int D, bool RUNS, bool SPLIT, bool TREE>
 __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPromptArgs a) {
@@ -146,8 +207,21 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     const int place = SPLIT ? wave & 3 : wave, second = SPLIT ? wave >> 2 : 0;                // the wave's rows, the half of a tile's keys
     const int kvh = blockIdx.x, group = a.heads / a.kv_heads;
     // rows of one key/value head: token * group + head in the group; the tokens behind the last sequence are one more, without keys
+    constexpr bool kDealt = TREE && RUNS;
     int s = 0, row0 = 0;
-    if (!find_block<kRows, TREE>(a, blockIdx.z, group, s, row0)) return;
+    Unit unit{};
+    if constexpr (kDealt) {
+        if (!find_unit<kRows>(a, blockIdx.z, group, unit)) return;
+        // (all lanes alike, which the compiler does not see behind the branch: addresses would be every lane's)
+        unit.block = __builtin_amdgcn_readfirstlane(unit.block);
+        unit.run = __builtin_amdgcn_readfirstlane(unit.run);
+        unit.runs = __builtin_amdgcn_readfirstlane(unit.runs);
+        unit.tiles = __builtin_amdgcn_readfirstlane(unit.tiles);
+        unit.s = __builtin_amdgcn_readfirstlane(unit.s);
+        s = unit.s;
+        row0 = unit.block * kRows;
+        if (kvh == 0 && unit.block == 0 && unit.run == 0 && tid == 0) a.plan[s] = make_int2(unit.first, unit.runs);
+    } else if (!find_block<kRows, TREE>(a, blockIdx.z, group, s, row0)) return;
     const bool tail = s == a.seqs;
     const int offset = offset_of<TREE>(a, s), n = (tail ? a.tokens : offset_of<TREE>(a, s + 1)) - offset;
     const int rows = n * group;                                               // (fits: the host's check)
@@ -160,8 +234,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     const int past = tree_past(given, n);                                     // (TREE)
     const int all_tiles = (visible(min(rows, row0 + kRows) - 1) + kTile - 1) / kTile;
     // this workgroup's tiles: t0 .. end - 1
-    const int run = RUNS ? (all_tiles + static_cast<int>(gridDim.y) - 1) / static_cast<int>(gridDim.y) : all_tiles, t0 = RUNS ? min(static_cast<int>(blockIdx.y) * run, all_tiles) : 0;
-    const int end = RUNS ? min(t0 + run, all_tiles) : all_tiles, tiles = end - t0;
+    const int run = kDealt ? unit.tiles : (RUNS ? (all_tiles + static_cast<int>(gridDim.y) - 1) / static_cast<int>(gridDim.y) : all_tiles);
+    const int t0 = RUNS ? min((kDealt ? unit.run : static_cast<int>(blockIdx.y)) * run, all_tiles) : 0;
+    const int end = kDealt && unit.run == unit.runs - 1 ? all_tiles : (RUNS ? min(t0 + run, all_tiles) : all_tiles), tiles = end - t0;
     const int full = (TREE ? clamp_int(past, 0, visible(row0)) : visible(row0)) / kTile;     // tiles that every row of the workgroup sees whole
     const int w0 = row0 + 32 * place, my_row = min(w0 + r, rows - 1);
     const int limit = visible(my_row);
@@ -361,6 +436,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
             if (!PLAIN && tid == 0) nan_values[(t + 2) & 3] = 0;              // read two steps ago, written in the next
             store_keys(t + 2, half, keys_at.here, key_raw, key_scale);
             store_values(plain, t + 1, half ^ 1, values_here, value_raw, value_scale);
+            // (before what `checked` branches on: behind it the compiler puts this load after the products, and the next step waits for it at its very beginning)
+            const int entry_ahead = entry(min(t + 5, last));
             value_raw = load_values(min(t + 2, last), keys_at);
             key_raw = load_keys(min(t + 3, last), next_at);
             key_scale = a.key_scales[next_at.at];
@@ -369,7 +446,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
             values_here = keys_at.here;
             keys_at = next_at;
             next_at = checked(min(t + 4, last), entry_next);
-            entry_next = entry(min(t + 5, last));
+            entry_next = entry_ahead;
         };
         const int seen = limit - kTile * t - 32 * second - 4 * h;
         uint32_t bits[2] = {};                                                // (TREE) of the lane's keys from its first on
@@ -519,10 +596,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
                 for (int i = 0; i < 4; ++i) o[u][4 * g + i] = __builtin_fmaf(o[u][4 * g + i], mine_by, with[i] * theirs_by);
             }
     }
-    if constexpr (RUNS) {
+    if (RUNS && !(kDealt && unit.runs == 1)) {
         // one of several runs of the block's keys: sums and statistics as they are, for the kernel that brings them together
         if (w0 + r < rows) {
-            const size_t row = (static_cast<size_t>(blockIdx.y) * a.tokens + offset + my_row / group) * a.heads + kvh * group + my_row % group;
+            const size_t row = kDealt ? (static_cast<size_t>(blockIdx.z) * a.kv_heads + kvh) * kRows + 32 * place + r
+                                      : (static_cast<size_t>(blockIdx.y) * a.tokens + offset + my_row / group) * a.heads + kvh * group + my_row % group;
             if (h == 0) a.stats[row] = make_float2(m, den);
 #pragma unroll
             for (int u = 0; u < kDimTiles; ++u)
@@ -586,7 +664,48 @@ __global__ __launch_bounds__(256) void paged_prompt_merge_kernel(const PagedProm
     else *out = static_cast<uint16_t>(half_pair<BF16>(total[0] * inv, 0.0f));
 }
 
-constexpr int kTreeFewRows = 64;
+// The same for trees, whose blocks have as many runs as their sequence's length asks for: a wave per query row.
+template <bool BF16, int D, int ROWS>
+__global__ __launch_bounds__(256) void paged_tree_merge_kernel(const PagedPromptArgs a) {
+    constexpr int kPer = D / 64, kBatch = 4;
+    const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads, row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, group = a.heads / a.kv_heads;
+    if (row >= rows) return;
+    const int token = static_cast<int>(row / a.heads), head = static_cast<int>(row % a.heads);
+    const int s = a.cu_steps ? paged_sequence(a.cu_steps, a.tokens, a.seqs + 1, 1, 0, token) : token / a.even;
+    if (s >= a.seqs) return;
+    const int offset = offset_of<true>(a, s), n = offset_of<true>(a, s + 1) - offset;
+    if (token >= offset + n || n * group <= a.few_rows) return;               // (rows of no sequence, of the other kernel)
+    const int2 plan = a.plan[s];
+    // (offsets that fall leave sequences without a unit: nothing of theirs is read outside what there is)
+    if (plan.y <= 1 || plan.y > 64 || plan.x < 0 || plan.x >= a.slots) return;
+    const int in_sequence = (token - offset) * group + head % group, unit = plan.x + in_sequence / ROWS * plan.y, kvh = head / group;
+    if (unit + plan.y > a.slots) return;
+    auto at = [&](int run) { return (static_cast<size_t>(unit + run) * a.kv_heads + kvh) * ROWS + in_sequence % ROWS; };
+    const float2 mine = lane < plan.y ? a.stats[at(lane)] : make_float2(-FLT_MAX, 0.0f);                     // (at most 64 runs)
+    const float top = group_max<64>(mine.x), factor = __builtin_amdgcn_exp2f(mine.x - top), den = group_sum<64>(mine.y * factor);
+    float total[kPer] = {};
+    for (int i0 = 0; i0 < plan.y; i0 += kBatch) {
+        float v[kBatch][kPer];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) v[i][j] = a.sums[at(min(i0 + i, plan.y - 1)) * D + kPer * lane + j];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (i0 + i >= plan.y) break;
+            const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(factor), i0 + i));
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) total[j] = __builtin_fmaf(v[i][j], f, total[j]);
+        }
+    }
+    const float inv = den == 0.0f ? 0.0f : 2.0f / den;
+    uint16_t* out = a.out + row * D + kPer * lane;
+    if constexpr (kPer == 2) *reinterpret_cast<uint32_t*>(out) = half_pair<BF16>(total[0] * inv, total[1] * inv);
+    else *out = static_cast<uint16_t>(half_pair<BF16>(total[0] * inv, 0.0f));
+}
+
+constexpr int kTreeFewRows = 64, kTreeFewKeys = 1 << 18;
 
 template <bool BF16, int D, bool TREE>
 int launch(const PagedPromptArgs& a, bool split, hipStream_t stream) {
@@ -599,11 +718,15 @@ int launch(const PagedPromptArgs& a, bool split, hipStream_t stream) {
     if (!grant_dynamic_smem(reinterpret_cast<const void*>(kernel), smem + (TREE ? 18432 : 8192), granted[2 * runs + split])) return PLLM_ERR_LAUNCH;
     // Runs before blocks: indexes without a block come last.  Workgroups go to the shader engines in turn, those that end at once too, and an engine that got more
     // of the others than it has compute units works a second round (128 tokens behind 30000 positions in blocks of half the rows 213 -> 117 us).
-    hipLaunchKernelGGL(kernel, dim3(a.kv_heads, a.runs, a.slots), dim3(kThreads), smem, stream, a);
+    hipLaunchKernelGGL(kernel, dim3(a.kv_heads, TREE ? 1 : a.runs, a.slots), dim3(kThreads), smem, stream, a);
     if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
     if (a.sums) {
         const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
-        hipLaunchKernelGGL((paged_prompt_merge_kernel<BF16, D>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream, a);
+        const dim3 row_grid(static_cast<unsigned>((rows + 3) / 4));
+        if constexpr (TREE) {
+            if (split) hipLaunchKernelGGL((paged_tree_merge_kernel<BF16, D, kBlockRows / 2>), row_grid, dim3(256), 0, stream, a);
+            else hipLaunchKernelGGL((paged_tree_merge_kernel<BF16, D, kBlockRows>), row_grid, dim3(256), 0, stream, a);
+        } else hipLaunchKernelGGL((paged_prompt_merge_kernel<BF16, D>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream, a);
         if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
     }
     return PLLM_OK;
@@ -641,7 +764,7 @@ int few_rows(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
     return rows < group ? 0 : static_cast<int>(rows);
 }
 
-struct Parts { int runs, few; bool split; size_t run_bytes, few_bytes; };
+struct Parts { int runs, few; bool split; size_t run_bytes, few_bytes; int units, deal; };
 Parts parts_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions, int few) {
     Parts p{};
     const int64_t rows = tokens * (heads / kv_heads);
@@ -663,17 +786,41 @@ Parts parts_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, in
 }
 
 
-// Trees of the same number of nodes: whether the decode kernel takes them.
+// Whether the decode kernel takes trees, all of the same number of nodes: few rows, or so few keys before them that its shorter way to the first product counts (one
+// tree of 26 nodes of 48 and 8 heads behind 4000 positions 18.6 us, by units 28; behind 100000 positions 16 nodes 90, by units 82).
 bool few_nodes(int64_t nodes, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
     const int64_t rows = nodes * (heads / kv_heads);
-    return nodes <= 64 && rows <= kTreeFewRows && paged_decode_parts_bytes(seqs, rows, kv_heads, head_dim, positions) <= (size_t{1} << 30);
+    if (nodes > 64 || (rows > kTreeFewRows && (rows + 31) / 32 * seqs * kv_heads * positions > kTreeFewKeys)) return false;
+    return paged_decode_parts_bytes(seqs, rows, kv_heads, head_dim, positions) <= (size_t{1} << 30);
 }
+size_t unit_bytes(int64_t units, int64_t kv_heads, int64_t rows, int64_t head_dim) { return align256(units * kv_heads * rows * head_dim * sizeof(float)); }
+// Up to 63 sequences: all of them by units (a kernel of its own for those of few rows, as prompts have, costs more than it saves: 32 of up to 26 nodes behind up to 8191
+// positions 182 -> 135 us, 8 of up to 16 behind up to 8000 68 -> 43).  More: whole blocks, in the order of the sequences.
+// Blocks of half the rows where a sequence's rows fill them so much better that the smaller products' extra copies are paid for.
 Parts tree_parts(int64_t tokens, int64_t seqs, bool even, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
-    if (!even) return parts_of(tokens, seqs, heads, kv_heads, head_dim, positions, few_rows(tokens, seqs, heads, kv_heads, head_dim, positions));
+    const int64_t group = heads / kv_heads, rows = tokens * group, each = std::max<int64_t>(rows / seqs, 1);
     Parts p{};
-    if (!few_nodes(tokens / seqs, seqs, heads, kv_heads, head_dim, positions)) return parts_of(tokens, seqs, heads, kv_heads, head_dim, positions, 0);
-    p.few = static_cast<int>(tokens / seqs * (heads / kv_heads));
-    p.few_bytes = paged_decode_parts_bytes(seqs, p.few, kv_heads, head_dim, positions);
+    if (even && few_nodes(tokens / seqs, seqs, heads, kv_heads, head_dim, positions)) {
+        p.few = static_cast<int>(each);
+        p.few_bytes = paged_decode_parts_bytes(seqs, p.few, kv_heads, head_dim, positions);
+        return p;
+    }
+    p.runs = 1;
+    p.split = 5 * ((each + kBlockRows / 2 - 1) / (kBlockRows / 2)) <= 8 * ((each + kBlockRows - 1) / kBlockRows);
+    const int64_t block = p.split ? kBlockRows / 2 : kBlockRows;
+    if (seqs < 64) {
+        const int64_t blocks = blocks_of(rows, seqs, 0, static_cast<int>(block)) + 1, deal = std::max<int64_t>(compute_units() / kv_heads, 1), units = blocks + deal + 1;
+        const size_t bytes = unit_bytes(units, kv_heads, block, head_dim) + align256(units * kv_heads * block * sizeof(float2)) + align256(seqs * sizeof(int2));
+        if (blocks * kv_heads <= 4 * compute_units() && bytes <= (size_t{1} << 30)) {
+            p.runs = 2;                                                       // (some number of them)
+            p.deal = static_cast<int>(deal);
+            p.units = static_cast<int>(units);
+            p.run_bytes = bytes;
+        }
+    } else if (!even) {
+        p.few = few_rows(tokens, seqs, heads, kv_heads, head_dim, positions);
+        p.few_bytes = p.few > 0 ? paged_decode_parts_bytes(seqs, p.few, kv_heads, head_dim, positions) : 0;
+    }
     return p;
 }
 
@@ -697,7 +844,7 @@ int attention(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pag
     const Parts parts = tree ? tree_parts(tokens, seqs, cu_steps == nullptr, heads, kv_heads, head_dim, positions)
                              : parts_of(tokens, seqs, heads, kv_heads, head_dim, positions, few_rows(tokens, seqs, heads, kv_heads, head_dim, positions));
     // (the rows behind the last sequence: what is left of the whole blocks, and one more)
-    const int64_t rows = tokens * (heads / kv_heads), slots = blocks_of(rows, seqs, parts.few, parts.split ? kBlockRows / 2 : kBlockRows) + 1;
+    const int64_t rows = tokens * (heads / kv_heads), slots = parts.units > 0 ? parts.units : blocks_of(rows, seqs, parts.few, parts.split ? kBlockRows / 2 : kBlockRows) + 1;
     if (rows > 0x3fffffff || slots > 0xffff) return PLLM_ERR_UNSUPPORTED;
     const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) | reinterpret_cast<uintptr_t>(out) |
                            reinterpret_cast<uintptr_t>(workspace);
@@ -720,8 +867,15 @@ int attention(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pag
     a.few_rows = parts.few;
     a.even = cu_steps ? 0 : static_cast<int>(tokens / seqs);
     if (a.runs > 1) {
-        a.sums = static_cast<float*>(workspace);
-        a.stats = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) + align256(static_cast<size_t>(a.runs) * tokens * heads * head_dim * sizeof(float)));
+        unsigned char* const at = static_cast<unsigned char*>(workspace);
+        a.sums = reinterpret_cast<float*>(at);
+        if (parts.units > 0) {
+            const int64_t block = parts.split ? kBlockRows / 2 : kBlockRows;
+            const size_t sums = unit_bytes(parts.units, kv_heads, block, head_dim);
+            a.stats = reinterpret_cast<float2*>(at + sums);
+            a.plan = reinterpret_cast<int2*>(at + sums + align256(parts.units * kv_heads * block * sizeof(float2)));
+            a.deal = parts.deal;
+        } else a.stats = reinterpret_cast<float2*>(at + align256(static_cast<size_t>(a.runs) * tokens * heads * head_dim * sizeof(float)));
     }
     if (cu_steps || a.few_rows == 0) {                                        // (otherwise every row is the decode kernel's)
         int status;
