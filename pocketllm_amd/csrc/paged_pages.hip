@@ -27,15 +27,16 @@ struct CompactArgs {
     int even, most, kv_heads, pool, width, page_shift;
 };
 
+constexpr int kCompactThreads = 128;
 template <int D>
-__global__ __launch_bounds__(256) void paged_compact_kernel(const Layers layers, const CompactArgs a) {
-    constexpr int kMostPage = 128;
-    __shared__ int nodes[kTreeNodes];
-    __shared__ int source_page[kMostPage];
-    __shared__ float ratio[kMostPage];
-    __shared__ __align__(16) uint8_t rows[kMostPage * D];
-    __shared__ int good, moves;
-    __shared__ float new_scale, old_ratio;
+__global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const Layers layers, const CompactArgs a) {
+    constexpr int kThreads = kCompactThreads;
+    // of token j of the path: its node; pages and scales of its source and its destination.  All of them at once (a page's own is not changed before its turn, and no later
+    // page's source): one after the other each page waits for its own loads
+    __shared__ int nodes[kTreeNodes], source_page[kTreeNodes], target_page[kTreeNodes];
+    __shared__ float ratio[kTreeNodes], target_scale[kTreeNodes];
+    extern __shared__ __align__(16) uint8_t rows[];                           // [tokens that a page takes of a path][D]
+    __shared__ int good;
     const int tid = threadIdx.x, kind = blockIdx.x & 1, head = blockIdx.x >> 1, s = blockIdx.y;
     const Layer& layer = layers.layer[blockIdx.z];
     uint8_t* const pages = kind ? layer.value_pages : layer.key_pages;
@@ -49,76 +50,82 @@ __global__ __launch_bounds__(256) void paged_compact_kernel(const Layers layers,
     const int64_t first64 = static_cast<int64_t>(a.lengths[s]) - n;
     if (count0 == 0 || first64 < -kTreeNodes || first64 >= static_cast<int64_t>(a.width) << a.page_shift) return;
     const int first = static_cast<int>(first64);
+    const int32_t* table = a.table + static_cast<size_t>(s) * a.table_stride;
     if (tid == 0) good = count0;
     __syncthreads();
-    for (int j = tid; j < count0; j += 256) {
+    for (int j = tid; j < count0; j += kThreads) {
         const int32_t* kept = a.kept + static_cast<size_t>(s) * a.most;
         const int node = kept[j], before = j ? kept[j - 1] : -1;
+        if (node <= before || before < (j ? 0 : -1) || node >= n) {
+            atomicMin(&good, j);                                              // from here on it is no path
+            continue;
+        }
+        const int source = paged_page(table, first + node, a.width, a.page_shift, a.pool), target = paged_page(table, first + j, a.width, a.page_shift, a.pool);
         nodes[j] = node;
-        if (node <= before || before < (j ? 0 : -1) || node >= n) atomicMin(&good, j);       // from here on it is no path
+        source_page[j] = source;
+        target_page[j] = target;
+        ratio[j] = source < 0 ? 0.0f : scales[static_cast<size_t>(source) * a.kv_heads + head];
+        target_scale[j] = target < 0 ? 0.0f : scales[static_cast<size_t>(target) * a.kv_heads + head];
     }
     __syncthreads();
     const int count = good;
     if (count == 0) return;
-    const int32_t* table = a.table + static_cast<size_t>(s) * a.table_stride;
     const size_t head_bytes = static_cast<size_t>(D) << a.page_shift;
     const int last_page = (first + count - 1) >> a.page_shift;
     for (int p = max(first, 0) >> a.page_shift; p <= last_page && p < a.width; ++p) {
         const int page0 = p << a.page_shift, from = max(max(first, 0), page0), to = min(first + count, page0 + page_tokens);
-        const int tokens = to - from, j0 = from - first;                      // nodes[j0 ..] go to slots from - page0 ..
+        const int tokens = to - from, j0 = from - first, held = from - page0; // nodes[j0 ..] go to slots `held` ..
         if (tokens <= 0 || nodes[j0 + tokens - 1] == j0 + tokens - 1) continue;              // (all of them where they are)
-        const int page = paged_page(table, page0, a.width, a.page_shift, a.pool);
+        const int page = target_page[j0];
         if (page < 0) continue;
+        const float own = target_scale[j0];
+        bool moves = false;
+        float most = held > 0 ? own : 0.0f;
+        for (int t = tid & 63; t < tokens; t += 64) {                         // (every wave for itself)
+            moves |= source_page[j0 + t] >= 0;
+            most = fmaxf(most, ratio[j0 + t]);
+        }
+        if (!__any(moves)) continue;
+        most = group_max<64>(most);
+        const float old_ratio = own == most ? 1.0f : own / most;
         const size_t at = static_cast<size_t>(page) * a.kv_heads + head;
-        if (tid == 0) moves = 0;
-        __syncthreads();
-        if (tid < tokens) {
-            const int source = paged_page(table, first + nodes[j0 + tid], a.width, a.page_shift, a.pool);
-            source_page[tid] = source;
-            ratio[tid] = source < 0 ? 0.0f : scales[static_cast<size_t>(source) * a.kv_heads + head];
-            if (source >= 0) moves = 1;
-        }
-        __syncthreads();
-        const float own = scales[at];
-        if (!moves) { __syncthreads(); continue; }
-        if (tid < 64) {
-            float most = from > page0 ? own : 0.0f;
-            for (int t = tid; t < tokens; t += 64) most = fmaxf(most, ratio[t]);
-            most = group_max<64>(most);
-            if (tid == 0) { new_scale = most; old_ratio = own == most ? 1.0f : own / most; }
-        }
-        __syncthreads();
-        if (tid < tokens) ratio[tid] = ratio[tid] == new_scale ? 1.0f : ratio[tid] / new_scale;
-        __syncthreads();
         uint8_t* const codes = pages + at * head_bytes;
+        auto factor = [&](int t) { return ratio[j0 + t] == most ? 1.0f : ratio[j0 + t] / most; };
         // the rows, scaled, to LDS: [token][D]
         if (!kind) {
-            for (int i = tid; i < tokens * (D / 16); i += 256) {
-                const int t = i / (D / 16), piece = i % (D / 16), source = source_page[t];
+            for (int i = tid; i < tokens * (D / 16); i += kThreads) {
+                const int t = i / (D / 16), piece = i % (D / 16), source = source_page[j0 + t];
                 if (source < 0) continue;
                 const int slot = (first + nodes[j0 + t]) & (page_tokens - 1);
                 uint4 w = *reinterpret_cast<const uint4*>(pages + (static_cast<size_t>(source) * a.kv_heads + head) * head_bytes + static_cast<size_t>(slot) * D + 16 * piece);
-                const float r = ratio[t];
+                const float r = factor(t);
                 if (r != 1.0f) w = make_uint4(scaled_codes(w.x, r), scaled_codes(w.y, r), scaled_codes(w.z, r), scaled_codes(w.w, r));
                 *reinterpret_cast<uint4*>(rows + t * D + 16 * piece) = w;
             }
         } else {
-            for (int i = tid; i < tokens * D; i += 256) {
-                const int t = i / D, d = i % D, source = source_page[t];
-                if (source < 0) continue;
-                const int slot = (first + nodes[j0 + t]) & (page_tokens - 1);
-                uint32_t w = pages[(static_cast<size_t>(source) * a.kv_heads + head) * head_bytes + (static_cast<size_t>(d) << a.page_shift) + slot];
-                const float r = ratio[t];
-                if (r != 1.0f) w = scaled_codes(w, r) & 0xffu;
-                rows[t * D + d] = static_cast<uint8_t>(w);
+            constexpr int kAtOnce = 8;                                        // requests on their way
+            for (int i0 = tid; i0 < tokens * D; i0 += kAtOnce * kThreads) {
+                uint32_t w[kAtOnce];
+                float r[kAtOnce];
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) {
+                    const int i = min(i0 + u * kThreads, tokens * D - 1), t = i / D, d = i % D, source = max(source_page[j0 + t], 0);
+                    const int slot = (first + nodes[j0 + t]) & (page_tokens - 1);
+                    r[u] = factor(t);
+                    w[u] = pages[(static_cast<size_t>(source) * a.kv_heads + head) * head_bytes + (static_cast<size_t>(d) << a.page_shift) + slot];
+                }
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) {
+                    const int i = i0 + u * kThreads;
+                    if (i < tokens * D) rows[i] = static_cast<uint8_t>(r[u] != 1.0f ? scaled_codes(w[u], r[u]) : w[u]);
+                }
             }
         }
         __syncthreads();
-        const int held = from - page0;
         if (held > 0 && old_ratio != 1.0f) {                                  // what the page keeps, on the larger scale
             const float r = old_ratio;
             const int across = (held + 15) / 16, pieces = kind ? D * across : held * (D / 16);
-            for (int i = tid; i < pieces; i += 256) {
+            for (int i = tid; i < pieces; i += kThreads) {
                 uint4* piece = reinterpret_cast<uint4*>(kind ? codes + (static_cast<size_t>(i / across) << a.page_shift) + 16 * (i % across) : codes + 16 * i);
                 const int keep = kind ? held - 16 * (i % across) : 16;
                 const uint4 w = *piece;
@@ -128,14 +135,14 @@ __global__ __launch_bounds__(256) void paged_compact_kernel(const Layers layers,
             }
             __syncthreads();                                                  // (older and new values share 16 bytes)
         }
-        if (tid == 0) scales[at] = new_scale;
+        if (tid == 0) scales[at] = most;
         if (!kind) {
-            for (int i = tid; i < tokens * (D / 16); i += 256)
-                if (source_page[i / (D / 16)] >= 0) *reinterpret_cast<uint4*>(codes + held * D + 16 * i) = *reinterpret_cast<const uint4*>(rows + 16 * i);
+            for (int i = tid; i < tokens * (D / 16); i += kThreads)
+                if (source_page[j0 + i / (D / 16)] >= 0) *reinterpret_cast<uint4*>(codes + held * D + 16 * i) = *reinterpret_cast<const uint4*>(rows + 16 * i);
         } else {
-            for (int i = tid; i < tokens * D; i += 256) {
+            for (int i = tid; i < tokens * D; i += kThreads) {
                 const int t = i % tokens, d = i / tokens;
-                if (source_page[t] >= 0) codes[(static_cast<size_t>(d) << a.page_shift) + held + t] = rows[t * D + d];
+                if (source_page[j0 + t] >= 0) codes[(static_cast<size_t>(d) << a.page_shift) + held + t] = rows[t * D + d];
             }
         }
         __syncthreads();
@@ -280,6 +287,105 @@ __global__ __launch_bounds__(1024) void paged_fork_deal_kernel(const ForkArgs a)
     if (tid == 0) *a.given = min(given, wanted);
 }
 
+// The three steps above in one launch, for pools whose counts fit LDS: two words a page.  Requests for four entries a thread are on their way at a time.
+constexpr int kPoolInLds = 16384;
+__global__ __launch_bounds__(1024) void paged_fork_small_kernel(const ForkArgs a) {
+    extern __shared__ int32_t counts[];                                       // [pool] holders, [pool] lowest new row that keeps the page in part
+    __shared__ int parts[16];
+    constexpr int kAtOnce = 4;
+    int32_t* const uses = counts;
+    int32_t* const first = counts + a.pool;
+    const int tid = threadIdx.x;
+    for (int p0 = tid; p0 < a.pool; p0 += kAtOnce * 1024) {
+        int v[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) v[i] = a.uses[min(p0 + 1024 * i, a.pool - 1)];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            if (p0 + 1024 * i < a.pool) {
+                uses[p0 + 1024 * i] = v[i];
+                first[p0 + 1024 * i] = 0x7fffffff;
+            }
+    }
+    __syncthreads();
+    const int held = a.seqs * a.width, entries = (a.seqs + a.rows) * a.width; // (fit: the host's check)
+    for (int at0 = tid; at0 < entries; at0 += kAtOnce * 1024) {
+        int page[kAtOnce], what[kAtOnce], row[kAtOnce];                       // what: -1 a holder less, 1 a holder more, 0 kept in part, 2 nothing
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int index = at0 + 1024 * i;
+            what[i] = 2;
+            page[i] = -1;
+            row[i] = 0;
+            if (index < held) {
+                what[i] = -1;
+                page[i] = fork_entry(a, index / a.width, index % a.width);
+            } else if (index < entries) {
+                const int r = (index - held) / a.width, at = (index - held) % a.width;
+                const ForkRow f = fork_row(a, r);
+                if (f.source >= 0 && (at < f.full || (at == f.full && f.some))) {
+                    what[i] = at < f.full ? 1 : 0;
+                    page[i] = fork_entry(a, f.source, at);
+                    row[i] = r;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (page[i] < 0) continue;
+            if (what[i] == 0) atomicMin(first + page[i], row[i]);
+            else if (what[i] != 2) atomicAdd(uses + page[i], what[i]);
+        }
+    }
+    __syncthreads();
+    int wanted = 0;
+    for (int r0 = 0; r0 < a.rows; r0 += 1024) {
+        const int r = r0 + tid;
+        int wants = 0, copied = -1, stays = -1;
+        if (r < a.rows) {
+            const ForkRow f = fork_row(a, r);
+            wants = f.last - f.full - (f.some ? 1 : 0);
+            const int page = f.some ? fork_entry(a, f.source, f.full) : -1;
+            if (page >= 0) {
+                if (first[page] == r && uses[page] <= 0) stays = page;
+                else { copied = page; ++wants; }
+            }
+            a.copies[r] = copied;
+        }
+        if (stays >= 0) first[stays] = -1;                                    // (rows of this page read either: neither is their own number)
+        int all;
+        const int until = threads_until(wants, parts, all);
+        if (r < a.rows) a.start[r] = wanted + until - wants;
+        wanted += all;
+    }
+    __syncthreads();
+    int given = 0;
+    constexpr int kPer = 4;
+    for (int p0 = 0; p0 < a.pool; p0 += 1024 * kPer) {
+        int holders[kPer], free = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int p = p0 + kPer * tid + i;
+            holders[i] = p < a.pool ? max(uses[p], 0) + (first[p] < 0) : 1;
+            free += holders[i] == 0;
+        }
+        int all;
+        int rank = given + threads_until(free, parts, all) - free;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int p = p0 + kPer * tid + i;
+            if (p >= a.pool) break;
+            if (holders[i] == 0 && rank++ < wanted) {
+                a.fresh[rank - 1] = p;
+                holders[i] = 1;
+            }
+            a.new_uses[p] = holders[i];
+        }
+        given += all;
+    }
+    if (tid == 0) *a.given = min(given, wanted);
+}
+
 // Blocks of 256 entries of a row's table first, then a row's copies: blocks of 16 KB of keys or values of a layer.
 __global__ __launch_bounds__(256) void paged_fork_rows_kernel(const Layers layers, const ForkArgs a, int table_blocks, int copy_blocks) {
     const int r = blockIdx.x, block = blockIdx.y, tid = threadIdx.x;
@@ -382,8 +488,10 @@ int pllm_paged_cache_compact(void* const* caches, int64_t layers, int64_t pool, 
     for (int64_t from = 0; from < layers; from += kLayers) {
         const int64_t count = std::min<int64_t>(layers - from, kLayers);
         const dim3 grid(static_cast<unsigned>(2 * kv_heads), static_cast<unsigned>(seqs), static_cast<unsigned>(count));
-        if (head_dim == 128) hipLaunchKernelGGL((paged_compact_kernel<128>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), some_layers(caches, from, count), a);
-        else hipLaunchKernelGGL((paged_compact_kernel<64>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), some_layers(caches, from, count), a);
+        // (LDS for what a path can take of a page, so that many workgroups fit a compute unit)
+        const size_t lds = static_cast<size_t>(std::min(most, page_tokens) * head_dim);
+        if (head_dim == 128) hipLaunchKernelGGL((paged_compact_kernel<128>), grid, dim3(kCompactThreads), lds, static_cast<hipStream_t>(stream), some_layers(caches, from, count), a);
+        else hipLaunchKernelGGL((paged_compact_kernel<64>), grid, dim3(kCompactThreads), lds, static_cast<hipStream_t>(stream), some_layers(caches, from, count), a);
     }
     return hipGetLastError() == hipSuccess ? PLLM_OK : PLLM_ERR_LAUNCH;
 }
@@ -415,9 +523,16 @@ int pllm_paged_cache_fork(void* const* caches, int64_t layers, int64_t pool, int
                ints(l.given), static_cast<int>(seqs), static_cast<int>(rows), static_cast<int>(table_width), static_cast<int>(pool), shift_of(page_tokens), static_cast<int>(kv_heads),
                static_cast<int>(head_dim)};
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(paged_fork_begin_kernel, dim3(static_cast<unsigned>((pool + 255) / 256)), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(paged_fork_count_kernel, dim3(static_cast<unsigned>(table_blocks), static_cast<unsigned>(seqs + rows)), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(paged_fork_deal_kernel, dim3(1), dim3(1024), 0, st, a);
+    static SmemGrant granted;
+    const size_t lds = 2 * sizeof(int32_t) * static_cast<size_t>(pool);
+    if (pool <= kPoolInLds && (seqs + rows) * table_width <= (1 << 17)) {
+        if (!grant_dynamic_smem(reinterpret_cast<const void*>(paged_fork_small_kernel), lds, granted)) return PLLM_ERR_LAUNCH;
+        hipLaunchKernelGGL(paged_fork_small_kernel, dim3(1), dim3(1024), lds, st, a);
+    } else {
+        hipLaunchKernelGGL(paged_fork_begin_kernel, dim3(static_cast<unsigned>((pool + 255) / 256)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(paged_fork_count_kernel, dim3(static_cast<unsigned>(table_blocks), static_cast<unsigned>(seqs + rows)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(paged_fork_deal_kernel, dim3(1), dim3(1024), 0, st, a);
+    }
     for (int64_t from = 0; from < layers; from += kLayers) {
         const int64_t count = std::min<int64_t>(layers - from, kLayers), tables = from == 0 ? table_blocks : 0;
         hipLaunchKernelGGL(paged_fork_rows_kernel, dim3(static_cast<unsigned>(rows), static_cast<unsigned>(tables + 2 * count * copy_blocks)), dim3(256), 0, st,
