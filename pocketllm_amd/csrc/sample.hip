@@ -163,7 +163,7 @@ struct Params {
     float most, per_bin, near;                  // the largest logit; bins per unit of distance; distance behind which weights are none
     uint64_t least_weight;                      // of min_p
     float temperature, top_p;
-    int top_k;
+    int top_k, index_shift;                     // index_shift: binary digits of an index behind the first ten
     bool greedy, cut, few;                      // the largest logit is the token; top-k or top-p leave something out; a small top-k
     uint64_t best;
 };
@@ -217,6 +217,7 @@ __device__ __forceinline__ Params params_of(const Asked& asked, int vocab, uint6
     p.least_weight = min_p > 0.0f ? static_cast<uint64_t>(ceil(static_cast<double>(fminf(min_p, 1.0f)) * 0x1p43)) : 0;
     if (p.least_weight == 0) p.least_weight = 1;                              // (weights of nothing are never kept)
     p.greedy = !(p.temperature > 0.0f) || p.top_k == 1 || static_cast<uint32_t>(best >> 32) == kNone;
+    p.index_shift = max(32 - __clz(vocab) - 10, 0);
     p.few = p.top_k > 0 && p.top_k <= kFew && p.top_k < vocab;
     p.cut = (p.top_k > 0 && p.top_k < vocab) || p.top_p < 1.0f;
     p.factor = 1.44269504088896340736 / static_cast<double>(p.temperature);
@@ -543,13 +544,34 @@ __device__ __forceinline__ uint64_t resolve(Choice<THREADS>& s, const Params& p,
         }
     }
     __syncthreads();
-    const int n = static_cast<int>(s.fews);
+    int n = static_cast<int>(s.fews);
     if (n > kTied) return 0;                                                  // (no place: the caller goes by the row)
+    least -= before;
+    if (n > 64) {
+        // many of them: of equal ones the stretch of indexes first (bf16 logits, 96 rows of 200064 with top-p: sorted, the last launch 26 us)
+        static_assert(kTied <= THREADS, "a value per thread");
+        const uint64_t mine = tid < n ? s.few[tid] : s.few[0];
+        if (__syncthreads_and(static_cast<uint32_t>(mine >> 32) == static_cast<uint32_t>(s.few[0] >> 32))) {
+            const int span = static_cast<int>(~static_cast<uint32_t>(mine)) >> p.index_shift;                // (below kBins, rising where places fall)
+            for (int i = tid; i < kBins; i += THREADS) s.sums[i] = 0;
+            if (tid == 0) s.fews = 0;
+            __syncthreads();
+            if (tid < n) add_to(&s.sums[span], weight(mine));
+            __syncthreads();
+            const int its = reach<THREADS>(s, kBins, least, before);
+            if (tid < n && span == its) s.few[atomicAdd(&s.fews, 1u)] = mine;
+            __syncthreads();
+            n = static_cast<int>(s.fews);
+            least -= before;
+        }
+    }
     if (n <= 64) {                                                            // each against all
         const uint64_t mine = tid < n ? s.few[tid] : 0, w = tid < n ? weight(mine) : 0;
-        uint64_t sum = before;
+        if (tid < 64) s.sums[tid] = w;
+        __syncthreads();
+        uint64_t sum = 0;
         if (tid < n) {
-            for (int i = 0; i < n; ++i) sum += s.few[i] > mine ? weight(s.few[i]) : 0;
+            for (int i = 0; i < n; ++i) sum += s.sums[i] & only(s.few[i] > mine);
             if (sum < least && sum + w >= least) s.found[2] = mine;
         }
         __syncthreads();
@@ -562,8 +584,7 @@ __device__ __forceinline__ uint64_t resolve(Choice<THREADS>& s, const Params& p,
     sort_falling<THREADS>(s.few, size);
     for (int i = tid; i < kTied; i += THREADS) s.sums[i] = i < n ? weight(s.few[i]) : 0;
     __syncthreads();
-    uint64_t in_front;
-    const int at = reach<THREADS>(s, kTied, least - before, in_front);
+    const int at = reach<THREADS>(s, kTied, least, before);
     return s.few[at];
 }
 
@@ -583,31 +604,42 @@ __device__ __forceinline__ int64_t choose(const Row<T>& x, const Params& p, Choi
     uint64_t last_kept = 0;                                                   // place key of the last value that is kept
     if (ordered && p.few && listed <= kDirect) {
         // everything that is kept is in a short list: each against all, in the order of the values and in that of the indexes
+        constexpr int kAtOnce = 8;                                            // (LDS reads on their way; one after the other 60 values took 4 us)
+        const int padded = (listed + kAtOnce - 1) & -kAtOnce;
         uint64_t key = 0, w = 0, before = 0;
         int rank = 0;
-        if (tid < listed) {
-            key = s.list[tid];
-            w = weight_key(key);
+        if (tid < padded) {
+            key = tid < listed ? s.list[tid] : 0;
+            w = tid < listed ? weight_key(key) : 0;
             s.few[tid] = w;
+            if (tid >= listed) s.list[tid] = 0;
         }
         __syncthreads();
-        if (tid < listed)
-            for (int i = 0; i < listed; ++i) {
-                const bool above = s.list[i] > key;
-                rank += above;
-                before += above ? s.few[i] : 0;
+        for (int i0 = 0; i0 < padded; i0 += kAtOnce) {
+            uint64_t other[kAtOnce], its[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) { other[i] = s.list[i0 + i]; its[i] = s.few[i0 + i]; }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                rank += other[i] > key;
+                before += its[i] & only(other[i] > key);
             }
+        }
         bool stays = tid < listed && rank < p.top_k;
         const uint64_t all = all_sum<THREADS>(stays ? w : 0, s.parts), share = share_up(p_fraction, all);
         stays &= (!(p.top_p < 1.0f) || rank == 0 || before < share) && w >= p.least_weight;
         const uint64_t total = all_sum<THREADS>(stays ? w : 0, s.parts), target = __umul64hi(u_fraction, total);
-        if (tid < listed) s.few[tid] = stays ? w : 0;
+        if (tid < padded) s.few[tid] = stays ? w : 0;
         __syncthreads();
-        if (stays) {
-            uint64_t sum = 0;
-            for (int i = 0; i < listed; ++i) sum += static_cast<uint32_t>(s.list[i]) > static_cast<uint32_t>(key) ? s.few[i] : 0;             // (complements)
-            if (sum <= target && sum + w > target) s.found[2] = ~static_cast<uint32_t>(key);
+        uint64_t sum = 0;
+        for (int i0 = 0; i0 < padded; i0 += kAtOnce) {
+            uint64_t other[kAtOnce], its[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) { other[i] = s.list[i0 + i]; its[i] = s.few[i0 + i]; }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) sum += its[i] & only(static_cast<uint32_t>(other[i]) > static_cast<uint32_t>(key));                 // (complements)
         }
+        if (stays && sum <= target && sum + w > target) s.found[2] = ~static_cast<uint32_t>(key);
         __syncthreads();
         return static_cast<int64_t>(s.found[2]);
     }
@@ -893,7 +925,9 @@ __global__ __launch_bounds__(kLastThreads) void sample_token_kernel(const Sample
     if (p.cut) {
         listed = static_cast<int>(a.listed_count[row]);
         for (int i = tid; i < min(listed, kListed); i += kLastThreads) s.list[i] = a.listed[static_cast<size_t>(row) * kListed + i];
-        find_cuts<kLastThreads>(a.mass + static_cast<size_t>(row) * kBins, a.count + static_cast<size_t>(row) * kBins, p, s.cuts, s.parts);
+        // (the list of a small top-k is cut by itself)
+        if (!p.few) find_cuts<kLastThreads>(a.mass + static_cast<size_t>(row) * kBins, a.count + static_cast<size_t>(row) * kBins, p, s.cuts, s.parts);
+        else if (tid == 0) s.cuts = Cuts{0, kBins - 1, kBins - 1, 0, 0, 0, 0};
     }
     __syncthreads();
     const int64_t token = choose<T, kLastThreads>(Row<T>(a, row), p, s, listed, asked.uniform, [&](int i) { return a.masses[static_cast<size_t>(row) * a.stretches + i]; });
