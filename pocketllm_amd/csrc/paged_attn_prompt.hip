@@ -13,9 +13,14 @@
 //
 // SPLIT, for calls of few blocks: 128 rows, waves 4 to 7 have those of 0 to 3 and the other 32 keys of every tile, and what they leave meets in LDS at the end.
 //
-// Bound: 4 D operations per row and key.  8192 tokens of 48 and 8 heads, 825 G operations: 793 us, 1040 T/s, where a large matrix product of the library
+// Bound: 4 D operations per row and key.  8192 tokens of 48 and 8 heads, 825 G operations: 777 us, 1060 T/s, where a large matrix product of the library
 // reaches 1155; what is between is the softmax's vector instructions (48 % of the cycles, the matrix unit 47 %: the two waves of a SIMD overlap them in
 // part) and the barrier of each tile.
+//
+// TREE: the new tokens are nodes of a drafted tree.  A node's ancestors are four 64-bit masks, walked up once per workgroup; tiles before the tree go as they do for prompts,
+// those that hold a node's key are masked by 64 bits of them per row.  Keys are cut in runs by units, below.  32 trees of 26 nodes of 48 and 8 heads behind up to 8191 positions,
+// 82 G operations, 170 us; five of up to 200 nodes of 64 and 8 heads behind up to 30000, 402 G, 508 us (790 T/s).  What is between that and prompts' rate: rows that do not fill
+// their block (156 of 256 at 26 nodes), about 12 us of a unit before its first and around its masked tiles, and 6 to 14 for the runs' sums.
 #include "paged_attention.h"
 #include "paged_device.h"
 
@@ -705,8 +710,6 @@ __global__ __launch_bounds__(256) void paged_tree_merge_kernel(const PagedPrompt
     else *out = static_cast<uint16_t>(half_pair<BF16>(total[0] * inv, 0.0f));
 }
 
-constexpr int kTreeFewRows = 64, kTreeFewKeys = 1 << 18;
-
 template <bool BF16, int D, bool TREE>
 int launch(const PagedPromptArgs& a, bool split, hipStream_t stream) {
     static SmemGrant granted[4];
@@ -785,9 +788,9 @@ Parts parts_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, in
     return p;
 }
 
-
 // Whether the decode kernel takes trees, all of the same number of nodes: few rows, or so few keys before them that its shorter way to the first product counts (one
 // tree of 26 nodes of 48 and 8 heads behind 4000 positions 18.6 us, by units 28; behind 100000 positions 16 nodes 90, by units 82).
+constexpr int kTreeFewRows = 64, kTreeFewKeys = 1 << 18;
 bool few_nodes(int64_t nodes, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
     const int64_t rows = nodes * (heads / kv_heads);
     if (nodes > 64 || (rows > kTreeFewRows && (rows + 31) / 32 * seqs * kv_heads * positions > kTreeFewKeys)) return false;

@@ -13,7 +13,9 @@
 //      to kFew everything above the cut goes to the list, and no other value's weight is ever formed
 //   4. the list in order, the cuts in it, the stretch of the row that the token lies in, the token
 // Many rows: a workgroup each, one launch.  Few rows: four launches, the first three over slices of the rows.
-// Bound: bytes (the row once from memory, then from the caches) and the 64-bit exponential, about 20 instructions a value, where there is no small top-k.
+// Bound: where there is no small top-k, the 64-bit exponential in two passes (about 44 instructions a value in all, those in 64 bits at half the rate): 832 rows of 32000 bf16 logits
+// with cuts by top-p, min_p and top-k 81 us, 96 rows of 200064 in four launches 83, for bytes of 10 and 7.5.  With one, the bytes and, for a single row, the launches one after
+// the other: 200064 fp32 logits 21 us (3.1 + 5.3 + 6.1 + 7.1 of the launches; in one workgroup the row alone takes longer).
 #include "pllm_device.h"
 #include "pllm_internal.h"
 
@@ -131,8 +133,8 @@ template <typename T, int STEP, int kAhead = 2, typename F> __device__ __forcein
 
 // 2^y, y <= 0 (and above -2^30: below, anything), times 2^kUnit, rounded.  The nearest integer to y falls out of adding 1.5 * 2^52; 2^f for the rest, |f| <= 1/2, by the
 // polynomial of degree 10 through it at Chebyshev's points (within 3e-16); the integer goes to the exponent, and adding 2^52 rounds the fraction off.  Additions and fused
-// products alone, which have four times the rate of the instructions that round, convert and scale (832 rows of 32000 without cuts: 74 us with those), without branches, so that
-// a chunk's values go side by side.
+// products alone, which have four times the rate of the instructions that round, convert and scale (832 rows of 32000 without cuts: 73.5 us with those, 71.5 so), without
+// branches, so that a chunk's values go side by side.
 __device__ __forceinline__ uint64_t weight_at(double y) {
     const double shifted = y + 0x1.8p52, f = y - (shifted - 0x1.8p52);
     double p = 7.072585949269223e-09;
@@ -315,8 +317,8 @@ __device__ __forceinline__ uint64_t lanes_sum(uint64_t v) {
     const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), 63), hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), 63);
     return static_cast<uint64_t>(hi) << 32 | lo;
 }
-// a wave's values (all lanes take part) to one place in LDS, the lanes' (64 chunks of one stretch) first together: one by one they wait for each other (a pass over 832 rows of 32000
-// 57 us)
+// a wave's values (all lanes take part, with 64 chunks of one stretch) to one place in LDS, the lanes' first together (the time is that of an atomic per lane, which the compiler
+// joins where it sees that the place is one)
 __device__ __forceinline__ void add_all(uint64_t* at, uint64_t v) {
     v = lanes_sum(v);
     if ((threadIdx.x & 63) == 0 && v) add_to(at, v);
@@ -548,7 +550,8 @@ __device__ __forceinline__ uint64_t resolve(Choice<THREADS>& s, const Params& p,
     if (n > kTied) return 0;                                                  // (no place: the caller goes by the row)
     least -= before;
     if (n > 64) {
-        // many of them: of equal ones the stretch of indexes first (bf16 logits, 96 rows of 200064 with top-p: sorted, the last launch 26 us)
+        // many of them: of equal ones the stretch of indexes first (bf16 logits, 96 rows of 200064 with top-p: the last launch 26 us
+        // if they are sorted, 21 so)
         static_assert(kTied <= THREADS, "a value per thread");
         const uint64_t mine = tid < n ? s.few[tid] : s.few[0];
         if (__syncthreads_and(static_cast<uint32_t>(mine >> 32) == static_cast<uint32_t>(s.few[0] >> 32))) {

@@ -928,7 +928,7 @@ def draft_tree_accept_forward(parents: torch.Tensor, drafted: torch.Tensor, samp
     [tokens] what the model gives behind each of them, lengths int32 [seqs] with the tree's nodes; cu_steps int32 [seqs + 1] (None: tokens / seqs each).
     Returns (kept int32 [seqs, most] the path's nodes and -1 behind them, counts int32 [seqs], tokens int64 [seqs] what is sampled at its last node, lengths int32 [seqs] with
     the path alone).  most, 1 to 256: nodes at which a path ends (default: those of a tree; with cu_steps 256).  A sequence without nodes: 0 and token -1; nodes from the
-    257th on are not looked at."""
+    257th on are not looked at.  Tokens are compared as numbers, also -1, which sample_tokens_forward gives for a row without a token."""
     what = "draft_tree_accept"
     made = _bindings.draft_tree_accept("draft_tree_accept_forward", parents, drafted, sampled, lengths, cu_steps, most)
     if made is not None:
@@ -975,7 +975,8 @@ def paged_cache_compact_forward(layers, block_table: torch.Tensor, lengths: torc
     """The keys and values of the accepted path of each sequence's drafted tree to the places right behind the past, in every layer's cache, in place: with n new tokens in
     lengths[s] positions (steps: n, or cu_steps int32 [seqs + 1]) token lengths[s] - n + kept[s, j] becomes token lengths[s] - n + j for j < counts[s].
     layers: a list of (key_pages, value_pages, key_scales, value_scales), one launch for up to 64 of them; block_table int32 [seqs, pages]; lengths
-    as they were before acceptance; kept int32 [seqs, most], counts int32 [seqs] as draft_tree_accept_forward gives them (a row that stops rising or leaves the tree ends there).
+    as they were before acceptance; kept int32 [seqs, most], counts int32 [seqs] as draft_tree_accept_forward gives them (a row that stops rising or leaves the tree ends there; a
+    tree of more than 256 nodes stays as it is).
     The scale of a page that tokens move to becomes the largest that its content had, and codes are scaled down to it.  As in paged_kv_append_forward what
     a call writes has pages of its own.  What lies behind a path stays as it is, or as it was moved over."""
     what = "paged_cache_compact"

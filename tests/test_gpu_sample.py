@@ -176,3 +176,44 @@ def test_captured_and_replayed_on_two_streams():
             want = call()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("count", [60, 65, 300, 512, 513, 1500, 2049])
+def test_cuts_inside_equal_logits(count, apart, dtype):
+    """So many equal values at a cut, one beside the other or all over the row, some of them kept."""
+    vocab, g = 20000, torch.Generator().manual_seed(count)
+    for rows, wide in ((3, vocab), (3, 3200)):                                # in slices; a workgroup per row
+        x = (torch.randn(rows, wide, generator=g) * 0.3 - 4).to(dtype)
+        x[:, wide // 2:wide // 2 + 20] = (torch.rand(20, generator=g) + 1).to(dtype)
+        at = torch.randperm(wide // 2, generator=g)[:count] if apart else torch.arange(100, 100 + count)
+        if count > wide // 2 - 100:
+            continue
+        x[:, at] = 0.25
+        u = uniforms(rows, count)
+        keep = 20 + count // 3
+        check(x, u, top_k=keep)
+        check(x, u, top_k=keep, top_p=0.77)
+        # what the 20 and a third of the equal ones have of everything, between two of them
+        w = np.exp(x[0].double().numpy() - x[0].double().max().item())
+        level = np.exp(0.25 - x[0].double().max().item())
+        share = (w[x[0].double().numpy() > 0.25].sum() + (keep - 20 + 0.4) * level) / w.sum()
+        check(x[:1].repeat(rows, 1), u, top_p=float(share))
+
+
+@pytest.mark.parametrize("count,levels", [(90, 5), (400, 7), (500, 16), (700, 5)])
+def test_cuts_among_neighbouring_floats(count, levels):
+    """Values that differ by single steps of a float32, more of them in one part of a bin than are compared one with another, and more than are ordered."""
+    vocab, g = 9000, torch.Generator().manual_seed(count)
+    x = torch.rand(2, vocab, generator=g) * 4 - 30
+    x[:, :3] = torch.tensor([0.0, -0.5, -1.0])
+    near = torch.tensor(-5.0)
+    steps = near + torch.arange(levels) * 2.0 ** -21                          # (a step of float32 from 4 to 8)
+    at = torch.randperm(vocab - 3, generator=g)[:count] + 3
+    x[:, at] = steps[torch.randint(levels, (count,), generator=g)]
+    u = uniforms(2, count)
+    w = np.exp(x[0].double().numpy())
+    check(x[:1].repeat(2, 1), u, top_p=float((w[:3].sum() + (count // 2 + 0.4) * np.exp(-5.0)) / w.sum()))
+    check(x, u, top_k=3 + count // 2)
+    check(x, u, top_k=3 + count // 2, top_p=0.9, temperature=1.5)

@@ -59,6 +59,31 @@ def test_many_sequences_of_few_nodes():
     check(cache, nodes, 2, torch.float16, [random_tree(rng, n) if n else [] for n in nodes], tail=1)
 
 
+@pytest.mark.parametrize("seqs,nodes,heads,dim,past,dtype", [
+    (66, 26, 6, 128, 900, torch.bfloat16), (64, 12, 16, 64, 1000, torch.float16), (70, 80, 1, 64, 2000, torch.bfloat16), (65, 100, 3, 128, 64, torch.float16),
+])
+def test_many_sequences_of_many_rows(seqs, nodes, heads, dim, past, dtype):
+    """64 sequences and more: blocks and halves of blocks in the order of the sequences, of the same number of nodes and of any."""
+    rng = np.random.default_rng(seqs)
+    cache = Cache([int(p) + nodes for p in rng.integers(0, past, seqs)], 1, dim, 64, seed=seqs)
+    check(cache, [nodes] * seqs, heads, dtype, [random_tree(rng, nodes) for _ in range(seqs)], ragged=False)
+    some = [int(n) for n in rng.integers(0, nodes + 1, seqs)]
+    check(cache, some, heads, dtype, [random_tree(rng, n) if n else [] for n in some], tail=5)
+
+
+@pytest.mark.parametrize("nodes,pasts,heads,kv_heads,dim,dtype", [
+    ([70, 200, 0, 100, 5, 256], [3000, 700, 10, 0, 1900, 64], 32, 32, 64, torch.bfloat16),       # more units than run at once, some sequences in runs
+    ([100, 30, 90], [900, 2500, 64], 48, 16, 128, torch.float16),
+    ([70, 5], [300, 130], 260, 260, 64, torch.bfloat16),                      # more heads than compute units
+    ([66], [100000], 1, 1, 64, torch.float16),                                # as many runs as a block has
+    ([70, 66], [20000, 9], 2, 1, 128, torch.bfloat16),
+])
+def test_keys_cut_in_runs(nodes, pasts, heads, kv_heads, dim, dtype):
+    rng = np.random.default_rng(heads)
+    cache = Cache([p + n for p, n in zip(pasts, nodes)], kv_heads, dim, 64, seed=heads)
+    check(cache, nodes, heads, dtype, [random_tree(rng, n) if n else [] for n in nodes], tail=2)
+
+
 @pytest.mark.parametrize("n", [10, 70])
 def test_a_chain_is_the_causal_form(n):
     """The nodes one after the other: what the prompt and the decode form give, within both kernels' roundings against the float64 form."""

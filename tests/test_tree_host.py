@@ -212,6 +212,7 @@ def test_c_entries_refuse_before_anything_is_launched():
     for name in ("uses", "sources", "reserve", "new_table", "new_uses", "missing"):
         assert fork(**{name: None}) == invalid
     assert fork(rows=0) == invalid and fork(rows=65535) == unsupported
+    assert fork(rows=60000, width=40000, table_stride=40000) == unsupported      # (more pages than 32 bits count)
     assert fork(need=lib.pllm_paged_cache_fork_workspace_bytes(2, 4) - 1) == workspace and fork(ws=None) == workspace
 
     def sample(**kw):
