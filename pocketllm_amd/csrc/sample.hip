@@ -7,20 +7,22 @@
 // u in 10^9 (float32 weights and sums: one in a hundred).  Weights below 2^-44 are none.
 //
 // Nothing is sorted but a few hundred values:
-//   1. the row's largest and least values
+//   1. the row's largest value, and about the least
 //   2. a histogram over the distance from the largest, linear from it to the least value or to where weights end: values per bin and, without a small top-k, weights
 //   3. in it the bins that the cuts of top-k and top-p lie in; the values of these bins to a list, of those above them only the sum of weights.  With a top-k of up
 //      to kFew everything above the cut goes to the list, and no other value's weight is ever formed
 //   4. the list in order, the cuts in it, the stretch of the row that the token lies in, the token
 // Many rows: a workgroup each, one launch.  Few rows: four launches, the first three over slices of the rows.
-// Bound: where there is no small top-k, the 64-bit exponential in two passes (about 44 instructions a value in all, those in 64 bits at half the rate): 832 rows of 32000 bf16 logits
-// with cuts by top-p, min_p and top-k 81 us, 96 rows of 200064 in four launches 83, for bytes of 10 and 7.5.  With one, the bytes and, for a single row, the launches one after
-// the other: 200064 fp32 logits 21 us (3.1 + 5.3 + 6.1 + 7.1 of the launches; in one workgroup the row alone takes longer).
+// Bound: where there is no small top-k, the 64-bit exponential in two passes (about 100 instructions a value in all, of 16 cycles for a wave; the vector units are busy for 60 % of the
+// time, the rest is launches, chains of loads and barriers around the cuts, and rows that do not divide among the units): 832 rows of 32000 fp16 logits, all with top-p, 103 us,
+// of mixed parameters 75, 96 rows of 200064 in four launches 71, for bytes of 10 and 7.5.  With one, the bytes and, for a single row, the launches one after the other:
+// 200064 fp32 logits 21 us (3.1 + 5.3 + 5.9 + 7.4 of the launches; in one workgroup the row alone takes longer).
 #include "pllm_device.h"
 #include "pllm_internal.h"
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 namespace pllm {
 namespace {
@@ -31,6 +33,7 @@ constexpr int kDirect = 128;                    // listed values up to which eac
 constexpr int kFew = kListed / 2;               // top-k up to which everything that is kept goes to the list
 constexpr int kUnit = 43;                       // binary digits of a weight
 constexpr int kThreads = 256, kRowThreads = 512, kLastThreads = 512;
+constexpr int kAhead = 2;                       // chunks of a thread on their way while as many are worked on
 constexpr int kStretch = 512, kMostStretches = (1 << 20) / 4 / kStretch + 1;               // chunks whose kept weights are summed up together; of a row
 
 struct SampleArgs {
@@ -39,7 +42,7 @@ struct SampleArgs {
     const float* temperature; const int32_t* top_k; const float* top_p; const float* min_p;             // per row, or null: the values below for all
     float temperature_all; int top_k_all; float top_p_all, min_p_all;
     int64_t* tokens;
-    uint64_t* best; uint32_t* least;            // [rows][slices]: order key of the largest value, then the complement of its index; order key of the least
+    uint64_t* best; uint32_t* least;            // [rows][slices]: order key of the largest value, then the complement of its chunk's number; order key of about the least
     uint64_t* masses;                           // [rows][stretches] of what is kept for certain
     uint64_t* mass; uint32_t* count;            // [rows][kBins]
     uint64_t* listed; uint32_t* listed_count;   // [rows][kListed], [rows]: order key and complement of the index
@@ -64,6 +67,8 @@ template <> struct Chunk<float> {
 };
 struct F16 {};
 struct B16 {};
+typedef _Float16 Half2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ Half2 half2_of(uint32_t w) { return __builtin_bit_cast(Half2, w); }
 template <> struct Chunk<F16> {
     static constexpr int kValues = 8;
     static __device__ __forceinline__ float at(const uint4& u, int i) {
@@ -109,33 +114,65 @@ template <typename T> struct Row {
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
+    // the largest of a chunk's values (NaN or minus infinity if there is none)
+    static __device__ __forceinline__ float most_of(const uint4& u) {
+        if constexpr (std::is_same_v<T, F16>) {
+            const Half2 m = __builtin_elementwise_max(__builtin_elementwise_max(half2_of(u.x), half2_of(u.y)), __builtin_elementwise_max(half2_of(u.z), half2_of(u.w)));
+            return fmaxf(static_cast<float>(m[0]), static_cast<float>(m[1]));
+        } else {
+            float m = Chunk<T>::at(u, 0);
+#pragma unroll
+            for (int i = 1; i < kValues; ++i) m = fmaxf(m, Chunk<T>::at(u, i));
+            return m;
+        }
+    }
+    // the least, minus infinity among them
+    static __device__ __forceinline__ float least_of(const uint4& u) {
+        if constexpr (std::is_same_v<T, F16>) {
+            const Half2 m = __builtin_elementwise_min(__builtin_elementwise_min(half2_of(u.x), half2_of(u.y)), __builtin_elementwise_min(half2_of(u.z), half2_of(u.w)));
+            return fminf(static_cast<float>(m[0]), static_cast<float>(m[1]));
+        } else {
+            float m = Chunk<T>::at(u, 0);
+#pragma unroll
+            for (int i = 1; i < kValues; ++i) m = fminf(m, Chunk<T>::at(u, i));
+            return m;
+        }
+    }
     // its values, minus infinity for NaN
     static __device__ __forceinline__ void values_of(const uint4& u, float (&v)[kValues]) {
 #pragma unroll
         for (int i = 0; i < kValues; ++i) v[i] = fmaxf(Chunk<T>::at(u, i), -INFINITY);
     }
 };
-// f(chunk, its values) for the chunks [begin, end), every STEP-th per thread, several loads on their way.  All threads go through all of it: behind the end, chunks of NaN.
-template <typename T, int STEP, int kAhead = 2, typename F> __device__ __forceinline__ void for_chunks(const Row<T>& x, int begin, int end, const F& f) {
-    for (int c0 = begin; c0 < end; c0 += kAhead * STEP) {
-        uint4 u[kAhead];
+// The next chunks of a thread, every STEP-th, on their way.
+template <typename T, int STEP, int COUNT> struct Ahead {
+    uint4 u[COUNT];
+    __device__ __forceinline__ Ahead(const Row<T>& x, int c0, int end) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) u[i] = x.load(c0 + i * STEP + static_cast<int>(threadIdx.x), end);
+        for (int i = 0; i < COUNT; ++i) u[i] = x.load(c0 + i * STEP + static_cast<int>(threadIdx.x), end);
+    }
+};
+// f(number, chunk) for the chunks [begin, end), every STEP-th per thread; `first` are those from `begin` on.  All threads go through all of it: behind the end, chunks of NaN.
+template <typename T, int STEP, int COUNT, typename F> __device__ __forceinline__ void for_chunks(const Row<T>& x, Ahead<T, STEP, COUNT> first, int begin, int end, const F& f) {
+    for (int c0 = begin; c0 < end; c0 += COUNT * STEP) {
+        const Ahead<T, STEP, COUNT> next(x, c0 + COUNT * STEP, end);
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
+        for (int i = 0; i < COUNT; ++i) {
             if (c0 + i * STEP >= end) break;
-            float v[Row<T>::kValues];
-            Row<T>::values_of(u[i], v);
-            f(c0 + i * STEP + static_cast<int>(threadIdx.x), v);
+            f(c0 + i * STEP + static_cast<int>(threadIdx.x), first.u[i]);
         }
+        first = next;
     }
 }
+template <typename T, int STEP, typename F> __device__ __forceinline__ void for_chunks(const Row<T>& x, int begin, int end, const F& f) {
+    for_chunks<T, STEP, 1>(x, Ahead<T, STEP, 1>(x, begin, end), begin, end, f);
+}
 
-// 2^y, y <= 0 (and above -2^30: below, anything), times 2^kUnit, rounded.  The nearest integer to y falls out of adding 1.5 * 2^52; 2^f for the rest, |f| <= 1/2, by the
-// polynomial of degree 10 through it at Chebyshev's points (within 3e-16); the integer goes to the exponent, and adding 2^52 rounds the fraction off.  Additions and fused
-// products alone, which have four times the rate of the instructions that round, convert and scale (832 rows of 32000 without cuts: 73.5 us with those, 71.5 so), without
-// branches, so that a chunk's values go side by side.
-__device__ __forceinline__ uint64_t weight_at(double y) {
+// 2^y, y <= 0 (and above -900: below, anything), times 2^kUnit.  The nearest integer to y falls out of adding 1.5 * 2^52; 2^f for the rest, |f| <= 1/2, by the polynomial
+// of degree 10 through it at Chebyshev's points (within 3e-16); the integer goes to the exponent.  Additions and fused products alone, which have four times the rate of
+// the instructions that round, convert and scale, and no branches, so that a chunk's values go side by side.  The last digit is set: it stands far behind the point, and no
+// weight lies in the middle between two integers, where rounding would go by the sum that it is added to.
+__device__ __forceinline__ double exponential(double y) {
     const double shifted = y + 0x1.8p52, f = y - (shifted - 0x1.8p52);
     double p = 7.072585949269223e-09;
     p = __builtin_fma(p, f, 1.0208690299958306e-07);
@@ -150,9 +187,17 @@ __device__ __forceinline__ uint64_t weight_at(double y) {
     p = __builtin_fma(p, f, 1.0);
     const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(p));
     const uint32_t high = static_cast<uint32_t>(bits >> 32) + ((static_cast<uint32_t>(__double_as_longlong(shifted)) + kUnit) << 20);
-    const double scaled = __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(bits)));
-    return static_cast<uint64_t>(__double_as_longlong(scaled + 0x1p52)) & 0x000fffffffffffffull;
+    return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(bits) | 1));
 }
+// v, or next to nothing, which adds nothing to a sum of integers.  (A mask on half a number: a choice would become a branch around what is chosen.)
+__device__ __forceinline__ double only_if(bool keep, double v) {
+    const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(v));
+    const uint32_t high = static_cast<uint32_t>(bits >> 32) & (0u - static_cast<uint32_t>(keep));
+    return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(bits)));
+}
+// A sum of up to 256 weights begins at 2^52, where a number's last digit is 1: every addition rounds the weight that it adds to an integer, and nothing else.
+constexpr double kNoWeight = 0x1p52;
+__device__ __forceinline__ uint64_t whole_of(double sum) { return static_cast<uint64_t>(__double_as_longlong(sum)) & 0x000fffffffffffffull; }
 
 // a number of [0, 1) as a 64-bit fraction
 __device__ __forceinline__ uint64_t fraction(float v) { return static_cast<uint64_t>(static_cast<double>(v) * 0x1p64); }
@@ -164,21 +209,22 @@ struct Params {
     double factor;                              // base-2 exponent per unit of distance from the largest logit
     float most, per_bin, near;                  // the largest logit; bins per unit of distance; distance behind which weights are none
     uint64_t least_weight;                      // of min_p
+    double least_before;                        // of a weight that rounds to no less
     float temperature, top_p;
     int top_k, index_shift;                     // index_shift: binary digits of an index behind the first ten
-    bool greedy, cut, few;                      // the largest logit is the token; top-k or top-p leave something out; a small top-k
+    bool greedy, cut, few, counts;              // the largest logit is the token; top-k or top-p leave something out; a small top-k; another one
     uint64_t best;
 };
 // all bits or none: a mask where a choice would be a branch around what is chosen, and a chunk's values would go one after the other
 __device__ __forceinline__ uint64_t only(bool v) { return ~(static_cast<uint64_t>(v) - 1); }
-// (plus infinity as the largest: it has no distance from itself, the others an infinite one)
-__device__ __forceinline__ float distance(const Params& p, float x) { return x == p.most ? 0.0f : p.most - x; }
+// (plus infinity as the largest: it has no distance from itself, the others an infinite one; a difference that is no number is none)
+__device__ __forceinline__ float distance(const Params& p, float x) { return fmaxf(p.most - x, 0.0f); }
 __device__ __forceinline__ bool weighs(const Params& p, float x) { return distance(p, x) <= p.near; }
 __device__ __forceinline__ int bin_of(const Params& p, float x) { return static_cast<int>(fminf(distance(p, x) * p.per_bin, kBins - 1.0f)); }
-__device__ __forceinline__ uint64_t weight_of(const Params& p, float x) {
-    const double d = x == p.most ? 0.0 : static_cast<double>(x) - static_cast<double>(p.most);
-    return weight_at(d * p.factor) & only(weighs(p, x));
+__device__ __forceinline__ double weight_before(const Params& p, float x) {                   // (anything where x does not weigh)
+    return exponential(fmin(static_cast<double>(x) - static_cast<double>(p.most), 0.0) * p.factor);
 }
+__device__ __forceinline__ uint64_t weight_of(const Params& p, float x) { return whole_of(kNoWeight + only_if(weighs(p, x), weight_before(p, x))); }
 // what the caller asks of the row
 struct Asked { float temperature, top_p, min_p, uniform; int top_k; };
 __device__ __forceinline__ Asked asked_of(const SampleArgs& a, int row) {
@@ -218,9 +264,11 @@ __device__ __forceinline__ Params params_of(const Asked& asked, int vocab, uint6
     const float min_p = asked.min_p;
     p.least_weight = min_p > 0.0f ? static_cast<uint64_t>(ceil(static_cast<double>(fminf(min_p, 1.0f)) * 0x1p43)) : 0;
     if (p.least_weight == 0) p.least_weight = 1;                              // (weights of nothing are never kept)
+    p.least_before = static_cast<double>(p.least_weight) - 0.5;
     p.greedy = !(p.temperature > 0.0f) || p.top_k == 1 || static_cast<uint32_t>(best >> 32) == kNone;
     p.index_shift = max(32 - __clz(vocab) - 10, 0);
     p.few = p.top_k > 0 && p.top_k <= kFew && p.top_k < vocab;
+    p.counts = p.top_k > kFew && p.top_k < vocab;
     p.cut = (p.top_k > 0 && p.top_k < vocab) || p.top_p < 1.0f;
     p.factor = 1.44269504088896340736 / static_cast<double>(p.temperature);
     // (weights below 2^-44 are none; in the last step of a float's more)
@@ -232,21 +280,17 @@ __device__ __forceinline__ Params params_of(const Asked& asked, int vocab, uint6
 
 __device__ __forceinline__ void add_to(uint64_t* at, uint64_t v) { atomicAdd(reinterpret_cast<unsigned long long*>(at), static_cast<unsigned long long>(v)); }
 
-// the largest and least values of the chunks [begin, end)
+// The largest value of the chunks [begin, end), with the complement of its chunk's number, and about the least one: of chunks with masked values their largest, so that a mask
+// here and there does not stretch the histogram (whose last bin takes all that is farther away).
 template <typename T, int STEP> __device__ __forceinline__ void extremes(const Row<T>& x, int begin, int end, uint64_t& best, uint32_t& least) {
     float most = -INFINITY, low = INFINITY;
     int at = 0x7fffffff;
-    for_chunks<T, STEP, 4>(x, begin, end, [&](int c, const float (&v)[Row<T>::kValues]) {
-        float here = v[0];
-#pragma unroll
-        for (int i = 1; i < Row<T>::kValues; ++i) here = fmaxf(here, v[i]);
-#pragma unroll
-        for (int i = 0; i < Row<T>::kValues; ++i) low = fminf(low, v[i] == -INFINITY ? INFINITY : v[i]);
-        if (here > most) {                                                    // (a thread's chunks come in their order)
-            most = here;
-#pragma unroll
-            for (int i = Row<T>::kValues - 1; i >= 0; --i) at = v[i] == here ? x.first_of(c) + i : at;
-        }
+    for_chunks<T, STEP, kAhead>(x, Ahead<T, STEP, kAhead>(x, begin, end), begin, end, [&](int c, const uint4& u) {
+        const float here = Row<T>::most_of(u), lowest = Row<T>::least_of(u);
+        const bool larger = here > most;                                      // (a thread's chunks come in their order)
+        most = larger ? here : most;
+        at = larger ? c : at;
+        low = fminf(low, lowest > -INFINITY ? lowest : (here > -INFINITY ? here : INFINITY));
     });
     if (most > -INFINITY) {
         const uint64_t k = place_key(order_key(most), at);
@@ -260,18 +304,18 @@ template <typename T, int STEP> __device__ __forceinline__ void extremes(const R
 template <typename T> __device__ __forceinline__ bool by_chunk(const Params& p) { return p.few && p.top_k <= kListed / Row<T>::kValues; }
 
 // the chunks' values into a histogram in LDS
-template <typename T, int STEP> __device__ __forceinline__ void fill(const Row<T>& x, const Params& p, int begin, int end, uint64_t* mass, uint32_t* count) {
+template <typename T, int STEP> __device__ __forceinline__ void fill(const Row<T>& x, const Ahead<T, STEP, kAhead>& ahead, const Params& p, int begin, int end, uint64_t* mass, uint32_t* count) {
     if (by_chunk<T>(p)) {
-        for_chunks<T, STEP, 4>(x, begin, end, [&](int, const float (&v)[Row<T>::kValues]) {
-            float most = v[0];
-#pragma unroll
-            for (int i = 1; i < Row<T>::kValues; ++i) most = fmaxf(most, v[i]);
+        for_chunks<T, STEP, kAhead>(x, ahead, begin, end, [&](int, const uint4& u) {
+            const float most = fmaxf(Row<T>::most_of(u), -INFINITY);
             if (weighs(p, most)) atomicAdd(count + bin_of(p, most), 1u);
         });
         return;
     }
     if (p.few) {
-        for_chunks<T, STEP, 4>(x, begin, end, [&](int, const float (&v)[Row<T>::kValues]) {
+        for_chunks<T, STEP, kAhead>(x, ahead, begin, end, [&](int, const uint4& u) {
+            float v[Row<T>::kValues];
+            Row<T>::values_of(u, v);
             int bin[Row<T>::kValues];
 #pragma unroll
             for (int i = 0; i < Row<T>::kValues; ++i) bin[i] = weighs(p, v[i]) ? bin_of(p, v[i]) : -1;
@@ -281,16 +325,20 @@ template <typename T, int STEP> __device__ __forceinline__ void fill(const Row<T
         });
         return;
     }
-    for_chunks<T, STEP>(x, begin, end, [&](int, const float (&v)[Row<T>::kValues]) {
+    for_chunks<T, STEP, kAhead>(x, ahead, begin, end, [&](int, const uint4& u) {
+        float v[Row<T>::kValues];
+        Row<T>::values_of(u, v);
         uint64_t w[Row<T>::kValues];
 #pragma unroll
         for (int i = 0; i < Row<T>::kValues; ++i) w[i] = weight_of(p, v[i]);
+#pragma unroll
+        for (int i = 0; i < Row<T>::kValues; ++i) asm volatile("" : "+v"(w[i]));              // (formed side by side, not each behind the last one's addition)
 #pragma unroll
         for (int i = 0; i < Row<T>::kValues; ++i)
             if (w[i]) {
                 const int bin = bin_of(p, v[i]);
                 add_to(mass + bin, w[i]);
-                atomicAdd(count + bin, 1u);
+                if (p.counts) atomicAdd(count + bin, 1u);
             }
     });
 }
@@ -317,11 +365,22 @@ __device__ __forceinline__ uint64_t lanes_sum(uint64_t v) {
     const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), 63), hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), 63);
     return static_cast<uint64_t>(hi) << 32 | lo;
 }
-// a wave's values (all lanes take part, with 64 chunks of one stretch) to one place in LDS, the lanes' first together (the time is that of an atomic per lane, which the compiler
-// joins where it sees that the place is one)
+// A wave's sums of a chunk's weights (64 chunks of one stretch; all lanes take part) to one place in LDS, first together, by halves of 24 binary digits: sums of eight weights
+// stay below 2^47, 64 of either half below 2^32, and half as many instructions as with 64 digits are about a sixth of what a chunk takes.
 __device__ __forceinline__ void add_all(uint64_t* at, uint64_t v) {
-    v = lanes_sum(v);
-    if ((threadIdx.x & 63) == 0 && v) add_to(at, v);
+    if (!__any(v != 0)) return;
+    uint32_t low = static_cast<uint32_t>(v) & 0xffffffu, high = static_cast<uint32_t>(v >> 24);
+#define PLLM_STEP(ctrl, rows)                                                                                                                          \
+    low += __builtin_amdgcn_update_dpp(0, low, ctrl, rows, 0xf, false);                                                                                \
+    high += __builtin_amdgcn_update_dpp(0, high, ctrl, rows, 0xf, false);
+    PLLM_STEP(0x111, 0xf)
+    PLLM_STEP(0x112, 0xf)
+    PLLM_STEP(0x114, 0xf)
+    PLLM_STEP(0x118, 0xf)
+    PLLM_STEP(0x142, 0xa)
+    PLLM_STEP(0x143, 0xc)
+#undef PLLM_STEP
+    if ((threadIdx.x & 63) == 63) add_to(at, (static_cast<uint64_t>(high) << 24) + low);
 }
 // the sum over the threads up to this one, and over all in `total`; `parts` [THREADS / 64]
 template <int THREADS> __device__ __forceinline__ uint64_t threads_until(uint64_t v, uint64_t* parts, uint64_t& total) {
@@ -357,27 +416,33 @@ struct Cuts {
     uint64_t before_low, before_last, total;    // sums of weights
     uint32_t need;                              // of bin `last`
 };
-// By a workgroup, from the row's histogram.
-template <int THREADS>
-__device__ __forceinline__ void find_cuts(const uint64_t* masses_of, const uint32_t* counts_of, const Params& p, Cuts& out, uint64_t* parts) {
-    constexpr int kPer = kBins / THREADS;
-    const int tid = threadIdx.x;
-    uint64_t mass[kPer], masses = 0;
-    uint32_t count[kPer], counts = 0;
+// A thread's part of a row's histogram.
+template <int THREADS> struct Bins {
+    static constexpr int kPer = kBins / THREADS;
+    uint64_t mass[kPer];
+    uint32_t count[kPer];
+    __device__ __forceinline__ Bins(const uint64_t* masses, const uint32_t* counts) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        mass[i] = p.few ? 0 : masses_of[kPer * tid + i];
-        count[i] = counts_of[kPer * tid + i];
-        masses += mass[i];
-        counts += count[i];
+        for (int i = 0; i < kPer; ++i) { mass[i] = masses[kPer * threadIdx.x + i]; count[i] = counts[kPer * threadIdx.x + i]; }
     }
+};
+// By a workgroup, from the row's histogram (whose weights are zero with a small top-k, and values without a top-k).
+template <int THREADS>
+__device__ __forceinline__ void find_cuts(const Bins<THREADS>& bins, const Params& p, Cuts& out, uint64_t* parts) {
+    constexpr int kPer = Bins<THREADS>::kPer;
+    const int tid = threadIdx.x;
+    const auto& mass = bins.mass;
+    const auto& count = bins.count;
+    uint64_t masses = 0, counts = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) { masses += mass[i]; counts += count[i]; }
     uint64_t total = 0, everyone;
-    const uint64_t mass0 = p.few ? 0 : threads_until<THREADS>(masses, parts, total) - masses;
+    const uint64_t mass0 = threads_until<THREADS>(masses, parts, total) - masses;
     const uint64_t count0 = threads_until<THREADS>(counts, parts, everyone) - counts;
     if (tid == 0) { out.low = p.few ? 0 : kBins; out.high = p.few ? kBins - 1 : kBins; out.last = p.few ? kBins - 1 : -1; out.before_low = 0; out.before_last = 0; out.total = total; out.need = 0; }
     __syncthreads();
-    const uint64_t k = p.top_k > 0 ? static_cast<uint64_t>(p.top_k) : ~uint64_t{0};
-    if (p.few ? everyone >= k : everyone > k) {
+    const uint64_t k = static_cast<uint64_t>(p.top_k);
+    if (p.few ? everyone >= k : p.counts && everyone > k) {
         uint64_t c = count0, m = mass0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
@@ -414,12 +479,12 @@ __device__ __forceinline__ void find_cuts(const uint64_t* masses_of, const uint3
 
 // A chunk's values: those of the cuts' bins to the list in LDS, of those above them the sum of weights.
 template <typename T>
-__device__ __forceinline__ uint64_t sort_out(const Params& p, const float (&v)[Row<T>::kValues], int first, int low, int high, int last, uint64_t* list, uint32_t* listed) {
+__device__ __forceinline__ uint64_t sort_out(const Params& p, const uint4& u, int first, int low, int high, int last, uint64_t* list, uint32_t* listed) {
+    float v[Row<T>::kValues];
     if (p.few) {
-        float most = v[0];
-#pragma unroll
-        for (int i = 1; i < Row<T>::kValues; ++i) most = fmaxf(most, v[i]);
+        const float most = fmaxf(Row<T>::most_of(u), -INFINITY);
         if (weighs(p, most) && bin_of(p, most) <= high) {
+            Row<T>::values_of(u, v);
 #pragma unroll
             for (int i = 0; i < Row<T>::kValues; ++i)
                 if (weighs(p, v[i]) && bin_of(p, v[i]) <= high) {
@@ -429,30 +494,37 @@ __device__ __forceinline__ uint64_t sort_out(const Params& p, const float (&v)[R
         }
         return 0;
     }
-    uint64_t sum = 0;
+    Row<T>::values_of(u, v);
+    // (bins as float numbers, whole ones where they are compared with `place`; the last bin has no end)
+    const float from = low < kBins ? static_cast<float>(low) : INFINITY, to = high < kBins - 1 ? static_cast<float>(high + 1) : INFINITY;
+    const float last_from = last >= 0 ? static_cast<float>(last) : INFINITY, last_to = last < kBins - 1 ? static_cast<float>(last + 1) : INFINITY;
     bool any = false, certain = false;
-    int bin[Row<T>::kValues];
+    bool above[Row<T>::kValues], inside[Row<T>::kValues];
 #pragma unroll
     for (int i = 0; i < Row<T>::kValues; ++i) {
-        bin[i] = weighs(p, v[i]) ? bin_of(p, v[i]) : 0x7fffffff;
-        certain |= bin[i] < low;
-        any |= (bin[i] >= low && bin[i] <= high) || bin[i] == last;
+        const float d = distance(p, v[i]), place = d * p.per_bin;
+        const bool here = d <= p.near;
+        above[i] = here && place < from;
+        inside[i] = here && ((place >= from && place < to) || (place >= last_from && place < last_to));
+        certain |= above[i];
+        any |= inside[i];
     }
+    double sum = kNoWeight;
     if (certain) {
 #pragma unroll
         for (int i = 0; i < Row<T>::kValues; ++i) {
-            const uint64_t w = weight_of(p, v[i]);
-            sum += w & only(bin[i] < low) & only(w >= p.least_weight);
+            const double w = weight_before(p, v[i]);
+            sum += only_if(above[i] && w >= p.least_before, w);
         }
     }
     if (any)
 #pragma unroll
         for (int i = 0; i < Row<T>::kValues; ++i)
-            if ((bin[i] >= low && bin[i] <= high) || bin[i] == last) {
+            if (inside[i]) {
                 const uint32_t at = atomicAdd(listed, 1u);
                 if (at < kListed) list[at] = place_key(order_key(v[i]), first + i);
             }
-    return sum;
+    return whole_of(sum);
 }
 
 // Values of LDS in falling order, n a power of two; up to 128 by one wave, without barriers.
@@ -547,26 +619,33 @@ __device__ __forceinline__ uint64_t resolve(Choice<THREADS>& s, const Params& p,
     }
     __syncthreads();
     int n = static_cast<int>(s.fews);
-    if (n > kTied) return 0;                                                  // (no place: the caller goes by the row)
     least -= before;
     if (n > 64) {
-        // many of them: of equal ones the stretch of indexes first (bf16 logits, 96 rows of 200064 with top-p: the last launch 26 us
-        // if they are sorted, 21 so)
-        static_assert(kTied <= THREADS, "a value per thread");
-        const uint64_t mine = tid < n ? s.few[tid] : s.few[0];
-        if (__syncthreads_and(static_cast<uint32_t>(mine >> 32) == static_cast<uint32_t>(s.few[0] >> 32))) {
-            const int span = static_cast<int>(~static_cast<uint32_t>(mine)) >> p.index_shift;                // (below kBins, rising where places fall)
+        // many of them: of equal ones the stretch of indexes first (bf16 logits, 96 rows of 200064, mixed: the last launch 26 us
+        // if they are sorted, 20 so)
+        const uint32_t value = static_cast<uint32_t>(s.few[0] >> 32);
+        auto in_part = [&](uint64_t key) { int part; return place_of(key, part) == bin && part == of; };
+        bool others = false;
+        for (int i = tid; i < listed; i += THREADS) others |= static_cast<uint32_t>(s.list[i] >> 32) != value && in_part(s.list[i]);
+        if (!__syncthreads_or(others)) {
+            auto span = [&](uint64_t key) { return static_cast<int>(~static_cast<uint32_t>(key)) >> p.index_shift; };           // (below kBins, rising where places fall)
             for (int i = tid; i < kBins; i += THREADS) s.sums[i] = 0;
             if (tid == 0) s.fews = 0;
             __syncthreads();
-            if (tid < n) add_to(&s.sums[span], weight(mine));
+            for (int i = tid; i < listed; i += THREADS)
+                if (in_part(s.list[i])) add_to(&s.sums[span(s.list[i])], weight(s.list[i]));
             __syncthreads();
             const int its = reach<THREADS>(s, kBins, least, before);
-            if (tid < n && span == its) s.few[atomicAdd(&s.fews, 1u)] = mine;
+            for (int i = tid; i < listed; i += THREADS)
+                if (in_part(s.list[i]) && span(s.list[i]) == its) {
+                    const uint32_t at = atomicAdd(&s.fews, 1u);
+                    if (at < kTied) s.few[at] = s.list[i];
+                }
             __syncthreads();
             n = static_cast<int>(s.fews);
             least -= before;
         }
+        if (n > kTied) return 0;                                              // (no place: the caller goes by the row)
     }
     if (n <= 64) {                                                            // each against all
         const uint64_t mine = tid < n ? s.few[tid] : 0, w = tid < n ? weight(mine) : 0;
@@ -707,7 +786,9 @@ __device__ __forceinline__ int64_t choose(const Row<T>& x, const Params& p, Choi
                 __syncthreads();
                 for (int i = tid; i < 256; i += THREADS) s.sums[i] = 0;
                 __syncthreads();
-                for_chunks<T, THREADS>(x, 0, x.chunks(), [&](int c, const float (&v)[kValues]) {
+                for_chunks<T, THREADS>(x, 0, x.chunks(), [&](int c, const uint4& u) {
+                    float v[kValues];
+                    Row<T>::values_of(u, v);
                     // (neighbours mostly have one digit: their sum in one addition)
                     uint64_t sum = 0;
                     int digit = 0;
@@ -736,7 +817,9 @@ __device__ __forceinline__ int64_t choose(const Row<T>& x, const Params& p, Choi
         };
         auto whole = [&](uint64_t from, bool counts) {
             uint64_t sum = 0;
-            for_chunks<T, THREADS>(x, 0, x.chunks(), [&](int c, const float (&v)[kValues]) {
+            for_chunks<T, THREADS>(x, 0, x.chunks(), [&](int c, const uint4& u) {
+float v[kValues];
+Row<T>::values_of(u, v);
 #pragma unroll
                 for (int i = 0; i < kValues; ++i) {
                     const uint64_t w = place_key(order_key(v[i]), x.first_of(c) + i) < from ? 0 : weight_of(p, v[i]);
@@ -762,7 +845,9 @@ __device__ __forceinline__ int64_t choose(const Row<T>& x, const Params& p, Choi
             if (kept(key, w)) add_to(&s.sums[(static_cast<int>(~static_cast<uint32_t>(key)) + x.skew) / kValues / kStretch], w);
         }
     } else if (bounded) {
-        for_chunks<T, THREADS>(x, 0, x.chunks(), [&](int c, const float (&v)[kValues]) {
+        for_chunks<T, THREADS>(x, 0, x.chunks(), [&](int c, const uint4& u) {
+            float v[kValues];
+            Row<T>::values_of(u, v);
             uint64_t sum = 0;
 #pragma unroll
             for (int i = 0; i < kValues; ++i) {
@@ -804,7 +889,6 @@ __device__ __forceinline__ int64_t choose(const Row<T>& x, const Params& p, Choi
         }
     }
     const int begin = stretch * kStretch, end = min(begin + kStretch, x.chunks());
-    static_assert(kStretch % THREADS == 0, "whole passes");
     for (int c0 = begin; c0 < end; c0 += THREADS) {
         float v[kValues];
         uint64_t w[kValues], own = 0, here;
@@ -831,7 +915,18 @@ __device__ __forceinline__ int64_t choose(const Row<T>& x, const Params& p, Choi
     return static_cast<int64_t>(s.found[2]);
 }
 
-__device__ __forceinline__ int64_t greedy_token(uint64_t best) { return static_cast<uint32_t>(best >> 32) == kNone ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(best)); }
+// the first of the largest logits, in its chunk
+template <typename T> __device__ __forceinline__ int64_t greedy_token(const Row<T>& x, uint64_t best) {
+    const uint32_t key = static_cast<uint32_t>(best >> 32);
+    if (key == kNone) return -1;
+    const int c = static_cast<int>(~static_cast<uint32_t>(best));
+    float v[Row<T>::kValues];
+    Row<T>::values_of(x.load(c, c + 1), v);
+    int at = 0;
+#pragma unroll
+    for (int i = Row<T>::kValues - 1; i >= 0; --i) at = order_key(v[i]) == key ? i : at;
+    return x.first_of(c) + at;
+}
 
 // ---- few rows: slices ---------------------------------------------------------------------------------------------------
 
@@ -867,18 +962,19 @@ __global__ __launch_bounds__(kThreads) void sample_histogram_kernel(const Sample
     __shared__ uint64_t mass[kBins];
     __shared__ uint32_t count[kBins];
     const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
+    const Row<T> x(a, row);
+    const int begin = slice * a.slice_chunks, end = min(begin + a.slice_chunks, x.chunks());
+    const Ahead<T, kThreads, kAhead> ahead(x, begin, end);                    // (on their way beside the parameters)
     const Params p = slices_params(a, row, asked_of(a, row));
     if (p.greedy || !p.cut) return;
     for (int i = tid; i < kBins; i += kThreads) { mass[i] = 0; count[i] = 0; }
     __syncthreads();
-    const Row<T> x(a, row);
-    fill<T, kThreads>(x, p, slice * a.slice_chunks, min((slice + 1) * a.slice_chunks, x.chunks()), mass, count);
+    fill<T, kThreads>(x, ahead, p, begin, end, mass, count);
     __syncthreads();
-    for (int i = tid; i < kBins; i += kThreads)
-        if (count[i]) {
-            if (!p.few) add_to(a.mass + static_cast<size_t>(row) * kBins + i, mass[i]);
-            atomicAdd(a.count + static_cast<size_t>(row) * kBins + i, count[i]);
-        }
+    for (int i = tid; i < kBins; i += kThreads) {
+        if (mass[i]) add_to(a.mass + static_cast<size_t>(row) * kBins + i, mass[i]);
+        if (count[i]) atomicAdd(a.count + static_cast<size_t>(row) * kBins + i, count[i]);
+    }
 }
 
 template <typename T>
@@ -887,20 +983,22 @@ __global__ __launch_bounds__(kThreads) void sample_masses_kernel(const SampleArg
     __shared__ Cuts cuts;
     __shared__ uint32_t listed, at;
     const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x;
+    const Row<T> x(a, row);
+    const int begin = slice * a.slice_chunks, end = min(begin + a.slice_chunks, x.chunks());
+    const Bins<kThreads> bins(a.mass + static_cast<size_t>(row) * kBins, a.count + static_cast<size_t>(row) * kBins);
+    const Ahead<T, kThreads, kAhead> ahead(x, begin, end);
     const Params p = slices_params(a, row, asked_of(a, row));
     if (p.greedy) return;
     if (tid == 0) listed = 0;
     for (int i = tid; i < kMostStretches; i += kThreads) sums[i] = 0;
     int low = kBins, high = kBins, last = -1;
     if (p.cut) {
-        find_cuts<kThreads>(a.mass + static_cast<size_t>(row) * kBins, a.count + static_cast<size_t>(row) * kBins, p, cuts, parts);
+        find_cuts<kThreads>(bins, p, cuts, parts);
         low = cuts.low; high = cuts.high; last = cuts.last;
     }
     __syncthreads();
-    const Row<T> x(a, row);
-    const int begin = slice * a.slice_chunks, end = min(begin + a.slice_chunks, x.chunks());
-    for_chunks<T, kThreads>(x, begin, end, [&](int c, const float (&v)[Row<T>::kValues]) {
-        const uint64_t sum = sort_out<T>(p, v, x.first_of(c), low, high, last, list, &listed);
+    for_chunks<T, kThreads, kAhead>(x, ahead, begin, end, [&](int c, const uint4& u) {
+        const uint64_t sum = sort_out<T>(p, u, x.first_of(c), low, high, last, list, &listed);
         if (!p.few) add_all(&sums[(c - begin) / kStretch], sum);
     });
     __syncthreads();
@@ -918,29 +1016,37 @@ template <typename T>
 __global__ __launch_bounds__(kLastThreads) void sample_token_kernel(const SampleArgs a) {
     __shared__ Choice<kLastThreads> s;
     const int row = blockIdx.x, tid = threadIdx.x;
+    // everything that may be asked for at once: one after the other each takes as long as all of them
     const Asked asked = asked_of(a, row);
+    const Bins<kLastThreads> bins(a.mass + static_cast<size_t>(row) * kBins, a.count + static_cast<size_t>(row) * kBins);
+    const int in_list = static_cast<int>(a.listed_count[row]);
+    uint64_t keys[kListed / kLastThreads];
+#pragma unroll
+    for (int i = 0; i < kListed / kLastThreads; ++i) keys[i] = a.listed[static_cast<size_t>(row) * kListed + i * kLastThreads + tid];
+    const uint64_t mass = a.masses[static_cast<size_t>(row) * a.stretches + min(tid, a.stretches - 1)];
     const Params p = slices_params(a, row, asked);
     if (p.greedy) {
-        if (tid == 0) a.tokens[row] = greedy_token(p.best);
+        if (tid == 0) a.tokens[row] = greedy_token(Row<T>(a, row), p.best);
         return;
     }
     int listed = 0;
     if (p.cut) {
-        listed = static_cast<int>(a.listed_count[row]);
-        for (int i = tid; i < min(listed, kListed); i += kLastThreads) s.list[i] = a.listed[static_cast<size_t>(row) * kListed + i];
+        listed = in_list;
+#pragma unroll
+        for (int i = 0; i < kListed / kLastThreads; ++i) s.list[i * kLastThreads + tid] = keys[i];
         // (the list of a small top-k is cut by itself)
-        if (!p.few) find_cuts<kLastThreads>(a.mass + static_cast<size_t>(row) * kBins, a.count + static_cast<size_t>(row) * kBins, p, s.cuts, s.parts);
+        if (!p.few) find_cuts<kLastThreads>(bins, p, s.cuts, s.parts);
         else if (tid == 0) s.cuts = Cuts{0, kBins - 1, kBins - 1, 0, 0, 0, 0};
     }
     __syncthreads();
-    const int64_t token = choose<T, kLastThreads>(Row<T>(a, row), p, s, listed, asked.uniform, [&](int i) { return a.masses[static_cast<size_t>(row) * a.stretches + i]; });
+    const int64_t token = choose<T, kLastThreads>(Row<T>(a, row), p, s, listed, asked.uniform, [&](int i) { return i == tid ? mass : a.masses[static_cast<size_t>(row) * a.stretches + i]; });
     if (tid == 0) a.tokens[row] = token;
 }
 
 // ---- many rows: a workgroup each ----------------------------------------------------------------------------------------
 
 template <typename T>
-__global__ __launch_bounds__(kRowThreads, 5) void sample_row_kernel(const SampleArgs a) {
+__global__ __launch_bounds__(kRowThreads, 4) void sample_row_kernel(const SampleArgs a) {
     __shared__ Choice<kRowThreads> s;
     __shared__ uint32_t count[kBins], leasts[kRowThreads / 64], listed;
     __shared__ uint64_t sums[kMostStretches];
@@ -964,19 +1070,19 @@ __global__ __launch_bounds__(kRowThreads, 5) void sample_row_kernel(const Sample
     }
     const Params p = params_of(asked, a.vocab, best, least);
     if (p.greedy) {
-        if (tid == 0) a.tokens[row] = greedy_token(p.best);
+        if (tid == 0) a.tokens[row] = greedy_token(x, p.best);
         return;
     }
     int low = kBins, high = kBins, last = -1;
     __syncthreads();
     if (p.cut) {
-        fill<T, kRowThreads>(x, p, 0, chunks, s.sums, count);
+        fill<T, kRowThreads>(x, Ahead<T, kRowThreads, kAhead>(x, 0, chunks), p, 0, chunks, s.sums, count);
         __syncthreads();
-        find_cuts<kRowThreads>(s.sums, count, p, s.cuts, s.parts);
+        find_cuts<kRowThreads>(Bins<kRowThreads>(s.sums, count), p, s.cuts, s.parts);
         low = s.cuts.low; high = s.cuts.high; last = s.cuts.last;
     }
-    for_chunks<T, kRowThreads>(x, 0, chunks, [&](int c, const float (&v)[Row<T>::kValues]) {
-        const uint64_t sum = sort_out<T>(p, v, x.first_of(c), low, high, last, s.list, &listed);
+    for_chunks<T, kRowThreads, kAhead>(x, Ahead<T, kRowThreads, kAhead>(x, 0, chunks), 0, chunks, [&](int c, const uint4& u) {
+        const uint64_t sum = sort_out<T>(p, u, x.first_of(c), low, high, last, s.list, &listed);
         if (!p.few) add_all(&sums[c / kStretch], sum);
     });
     __syncthreads();
@@ -1002,14 +1108,17 @@ struct Layout { int slices, slice_chunks, stretches; size_t best, least, masses,
 Layout layout_of(int64_t rows, int64_t vocab, int dtype) {
     const int values = dtype == PLLM_F32 ? 4 : 8;
     const int64_t chunks = (vocab + 2 * values - 2) / values;                 // (a row may begin inside a chunk)
-    // A workgroup per row where there are more rows than compute units, or rows of a few chunks per thread.  Otherwise as many slices as give the machine about four workgroups
-    // per compute unit, none of fewer than two chunks per thread.
+    // A workgroup per row for rows of a few chunks per thread, and where there are more rows than compute units, if the last of them do not leave too many units idle: otherwise
+    // slices, which take a little longer for the same work and 25 us more (top-p, 300 rows of 200064 in slices 199 us, by rows 279; 832 of 32000 about 107 by the same
+    // figures, 103).  As many slices as give the machine about eight workgroups per compute unit (four: 96 rows of 200064, mixed, 81 -> 71 us), none of fewer
+    // than two chunks per thread.
     Layout l{};
-    if (rows >= compute_units() || chunks <= 2 * kRowThreads) {
+    const int64_t units = compute_units(), rounds = (rows + units - 1) / units;
+    if (chunks <= 1024 || (rows >= units && 11 * rows + 10 * 12000000 / vocab > 10 * rounds * units)) {
         l.bytes = 256;
         return l;
     }
-    const int64_t stretches = (chunks + kStretch - 1) / kStretch, slices = std::min(stretches, (4 * compute_units() + rows - 1) / rows), each = (stretches + slices - 1) / slices;
+    const int64_t stretches = (chunks + kStretch - 1) / kStretch, slices = std::min(stretches, (8 * compute_units() + rows - 1) / rows), each = (stretches + slices - 1) / slices;
     l.stretches = static_cast<int>(stretches);
     l.slice_chunks = static_cast<int>(each * kStretch);
     l.slices = static_cast<int>((stretches + each - 1) / each);
