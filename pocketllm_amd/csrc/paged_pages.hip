@@ -14,12 +14,13 @@ struct Layers { Layer layer[kLayers]; };
 
 // ---- the accepted path ------------------------------------------------------------------------------------------------
 //
-// Token `first` + kept[j] of a sequence becomes token `first` + j, first = length - n.  kept rises, so every destination is at or before its source, and pages are
-// done one after the other in the order of destinations: what a page takes lies in it or behind it.  The new scale of a page is the largest of the scales that its
+// Token `first` + kept[j] of a sequence becomes token `first` + j, first = length - n.  kept rises, so every destination is at or before its source, and what a stretch
+// of the path is written over is no later stretch's source.  The new scale of a page is the largest of the scales that its
 // content had (its own, where it keeps older tokens or a token moves within it): codes are scaled down to it by a power of two, exact but for those that get below E4M3's
 // normal values, which are rounded again.
-// A workgroup has a sequence's keys, or values, of one head and layer.  Bound: the chain of loads (path, table, scales, codes) of a page after the other, 12.7 us for 32 sequences of up to
-// 26 nodes, eight layers of 8 heads in pages of 16, whose codes would take 1; a value's token is one byte in each of D rows, so its sector is read and written for it.
+// A workgroup has a sequence's keys, or values, of one head and layer.  Bound: a value's token is one byte in each of D rows, so whatever it is, the lines of whole pages are
+// read and written for it: 32 sequences of up to 26 nodes, eight layers of 8 heads in pages of 16, 12.5 us for about 20 MB of lines (4 us), and of the chain of loads (path, table,
+// scales, codes) of a workgroup 5 us.
 
 struct CompactArgs {
     const int32_t* table; size_t table_stride;
@@ -27,17 +28,23 @@ struct CompactArgs {
     int even, most, kv_heads, pool, width, page_shift;
 };
 
-constexpr int kCompactThreads = 128;
+constexpr int kCompactThreads = 128, kCompactStretch = 64;                    // tokens whose codes are on their way together
 template <int D>
 __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const Layers layers, const CompactArgs a) {
-    constexpr int kThreads = kCompactThreads;
-    // of token j of the path: its node; pages and scales of its source and its destination.  All of them at once (a page's own is not changed before its turn, and no later
-    // page's source): one after the other each page waits for its own loads
-    __shared__ int nodes[kTreeNodes], source_page[kTreeNodes], target_page[kTreeNodes];
-    __shared__ float ratio[kTreeNodes], target_scale[kTreeNodes];
-    extern __shared__ __align__(16) uint8_t rows[];                           // [tokens that a page takes of a path][D]
+    constexpr int kThreads = kCompactThreads, kWaves = kThreads / 64;
+    // of token j of the path: where it comes from and goes to, from the layer's first code on, or -1; its node; the scales of the two pages; what its codes are multiplied
+    // by, negative where it stays as it is.  All of them, and all codes of a stretch, at once: one page after the other each waits for its own loads
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int room = a.most;
+    int64_t* const sources = reinterpret_cast<int64_t*>(smem);
+    int64_t* const targets = sources + room;
+    int* const nodes = reinterpret_cast<int*>(targets + room);
+    float* const ratio = reinterpret_cast<float*>(nodes + room);
+    float* const target_scale = ratio + room;
+    float* const factors = target_scale + room;
+    uint8_t* const rows = reinterpret_cast<uint8_t*>(factors + room);         // [tokens of a stretch][D] (on 16 bytes: 32 for a token are in front of it)
     __shared__ int good;
-    const int tid = threadIdx.x, kind = blockIdx.x & 1, head = blockIdx.x >> 1, s = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), kind = blockIdx.x & 1, head = blockIdx.x >> 1, s = blockIdx.y;
     const Layer& layer = layers.layer[blockIdx.z];
     uint8_t* const pages = kind ? layer.value_pages : layer.key_pages;
     float* const scales = kind ? layer.value_scales : layer.key_scales;
@@ -61,73 +68,92 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const La
             continue;
         }
         const int source = paged_page(table, first + node, a.width, a.page_shift, a.pool), target = paged_page(table, first + j, a.width, a.page_shift, a.pool);
+        auto place = [&](int page, int position) {
+            const int slot = position & (page_tokens - 1);
+            return page < 0 ? int64_t{-1} : (static_cast<int64_t>(page) * a.kv_heads + head) * (static_cast<int64_t>(D) << a.page_shift) + (kind ? slot : slot * D);
+        };
         nodes[j] = node;
-        source_page[j] = source;
-        target_page[j] = target;
+        sources[j] = place(source, first + node);
+        targets[j] = place(target, first + j);
         ratio[j] = source < 0 ? 0.0f : scales[static_cast<size_t>(source) * a.kv_heads + head];
         target_scale[j] = target < 0 ? 0.0f : scales[static_cast<size_t>(target) * a.kv_heads + head];
     }
     __syncthreads();
     const int count = good;
     if (count == 0) return;
-    const size_t head_bytes = static_cast<size_t>(D) << a.page_shift;
     const int last_page = (first + count - 1) >> a.page_shift;
-    for (int p = max(first, 0) >> a.page_shift; p <= last_page && p < a.width; ++p) {
+    const int page_first = max(first, 0) >> a.page_shift, held = max(first, 0) & (page_tokens - 1);           // slots of the first page that it keeps
+    float held_factor = 1.0f;                                                 // what they are multiplied by
+    bool moved = false;
+    for (int j = tid; j < count; j += kThreads) factors[j] = -1.0f;
+    __syncthreads();
+    // every page's new scale
+    for (int p = page_first; p <= last_page && p < a.width; ++p) {
         const int page0 = p << a.page_shift, from = max(max(first, 0), page0), to = min(first + count, page0 + page_tokens);
-        const int tokens = to - from, j0 = from - first, held = from - page0; // nodes[j0 ..] go to slots `held` ..
+        const int tokens = to - from, j0 = from - first;
         if (tokens <= 0 || nodes[j0 + tokens - 1] == j0 + tokens - 1) continue;              // (all of them where they are)
-        const int page = target_page[j0];
-        if (page < 0) continue;
+        if (targets[j0] < 0) continue;
+        const bool keeps = p == page_first && held > 0;
         const float own = target_scale[j0];
         bool moves = false;
-        float most = held > 0 ? own : 0.0f;
+        float most = keeps ? own : 0.0f;
         for (int t = tid & 63; t < tokens; t += 64) {                         // (every wave for itself)
-            moves |= source_page[j0 + t] >= 0;
+            moves |= sources[j0 + t] >= 0;
             most = fmaxf(most, ratio[j0 + t]);
         }
         if (!__any(moves)) continue;
+        moved = true;
         most = group_max<64>(most);
-        const float old_ratio = own == most ? 1.0f : own / most;
-        const size_t at = static_cast<size_t>(page) * a.kv_heads + head;
-        uint8_t* const codes = pages + at * head_bytes;
-        auto factor = [&](int t) { return ratio[j0 + t] == most ? 1.0f : ratio[j0 + t] / most; };
+        if (keeps && own != most) held_factor = own / most;
+        if (tid >= 64) continue;
+        for (int t = tid; t < tokens; t += 64)
+            if (sources[j0 + t] >= 0) factors[j0 + t] = ratio[j0 + t] == most ? 1.0f : ratio[j0 + t] / most;
+        if (tid == 0) scales[static_cast<size_t>(targets[j0] >> (a.page_shift + (D == 128 ? 7 : 6)))] = most;
+    }
+    if (!moved) return;                                                       // (all waves alike)
+    __syncthreads();
+    for (int j0 = 0; j0 < count; j0 += kCompactStretch) {
+        const int tokens = min(count - j0, kCompactStretch);
         // the rows, scaled, to LDS: [token][D]
         if (!kind) {
             for (int i = tid; i < tokens * (D / 16); i += kThreads) {
-                const int t = i / (D / 16), piece = i % (D / 16), source = source_page[j0 + t];
-                if (source < 0) continue;
-                const int slot = (first + nodes[j0 + t]) & (page_tokens - 1);
-                uint4 w = *reinterpret_cast<const uint4*>(pages + (static_cast<size_t>(source) * a.kv_heads + head) * head_bytes + static_cast<size_t>(slot) * D + 16 * piece);
-                const float r = factor(t);
+                const int t = i / (D / 16), piece = i % (D / 16);
+                const float r = factors[j0 + t];
+                if (r < 0.0f) continue;
+                uint4 w = *reinterpret_cast<const uint4*>(pages + sources[j0 + t] + 16 * piece);
                 if (r != 1.0f) w = make_uint4(scaled_codes(w.x, r), scaled_codes(w.y, r), scaled_codes(w.z, r), scaled_codes(w.w, r));
                 *reinterpret_cast<uint4*>(rows + t * D + 16 * piece) = w;
             }
         } else {
-            constexpr int kAtOnce = 8;                                        // requests on their way
-            for (int i0 = tid; i0 < tokens * D; i0 += kAtOnce * kThreads) {
-                uint32_t w[kAtOnce];
-                float r[kAtOnce];
+            // a wave takes every kWaves-th token, a lane its codes of dimensions lane, lane + 64
+            constexpr int kAtOnce = 4, kPer = D / 64;                         // requests on their way: of so many tokens
+            for (int t0 = wave; t0 < tokens; t0 += kAtOnce * kWaves) {
+                uint32_t w[kAtOnce][kPer];
 #pragma unroll
                 for (int u = 0; u < kAtOnce; ++u) {
-                    const int i = min(i0 + u * kThreads, tokens * D - 1), t = i / D, d = i % D, source = max(source_page[j0 + t], 0);
-                    const int slot = (first + nodes[j0 + t]) & (page_tokens - 1);
-                    r[u] = factor(t);
-                    w[u] = pages[(static_cast<size_t>(source) * a.kv_heads + head) * head_bytes + (static_cast<size_t>(d) << a.page_shift) + slot];
+                    const int t = j0 + min(t0 + u * kWaves, tokens - 1);
+                    const int64_t from = factors[t] < 0.0f ? 0 : sources[t];  // (what stays: any place of the pool)
+#pragma unroll
+                    for (int h = 0; h < kPer; ++h) w[u][h] = pages[from + ((64 * h + lane) << a.page_shift)];
                 }
 #pragma unroll
                 for (int u = 0; u < kAtOnce; ++u) {
-                    const int i = i0 + u * kThreads;
-                    if (i < tokens * D) rows[i] = static_cast<uint8_t>(r[u] != 1.0f ? scaled_codes(w[u], r[u]) : w[u]);
+                    const int t = t0 + u * kWaves;
+                    if (t >= tokens) break;
+                    const float r = factors[j0 + t];
+#pragma unroll
+                    for (int h = 0; h < kPer; ++h) rows[t * D + 64 * h + lane] = static_cast<uint8_t>(r != 1.0f ? scaled_codes(w[u][h], r) : w[u][h]);
                 }
             }
         }
         __syncthreads();
-        if (held > 0 && old_ratio != 1.0f) {                                  // what the page keeps, on the larger scale
-            const float r = old_ratio;
+        if (j0 == 0 && held_factor != 1.0f) {                                 // what the first page keeps, on the larger scale
+            uint8_t* const codes = pages + (targets[0] - (kind ? held : held * D));           // (the path's first token goes behind what it keeps)
             const int across = (held + 15) / 16, pieces = kind ? D * across : held * (D / 16);
             for (int i = tid; i < pieces; i += kThreads) {
                 uint4* piece = reinterpret_cast<uint4*>(kind ? codes + (static_cast<size_t>(i / across) << a.page_shift) + 16 * (i % across) : codes + 16 * i);
                 const int keep = kind ? held - 16 * (i % across) : 16;
+                const float r = held_factor;
                 const uint4 w = *piece;
                 const uint32_t m[4] = {first_bytes(keep), first_bytes(keep - 4), first_bytes(keep - 8), first_bytes(keep - 12)};
                 *piece = make_uint4((scaled_codes(w.x, r) & m[0]) | (w.x & ~m[0]), (scaled_codes(w.y, r) & m[1]) | (w.y & ~m[1]), (scaled_codes(w.z, r) & m[2]) | (w.z & ~m[2]),
@@ -135,14 +161,32 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const La
             }
             __syncthreads();                                                  // (older and new values share 16 bytes)
         }
-        if (tid == 0) scales[at] = most;
         if (!kind) {
-            for (int i = tid; i < tokens * (D / 16); i += kThreads)
-                if (source_page[j0 + i / (D / 16)] >= 0) *reinterpret_cast<uint4*>(codes + held * D + 16 * i) = *reinterpret_cast<const uint4*>(rows + 16 * i);
+            for (int i = tid; i < tokens * (D / 16); i += kThreads) {
+                const int t = i / (D / 16);
+                if (!(factors[j0 + t] < 0.0f)) *reinterpret_cast<uint4*>(pages + targets[j0 + t] + 16 * (i % (D / 16))) = *reinterpret_cast<const uint4*>(rows + 16 * i);
+            }
         } else {
-            for (int i = tid; i < tokens * D; i += kThreads) {
-                const int t = i % tokens, d = i / tokens;
-                if (source_page[j0 + t] >= 0) codes[(static_cast<size_t>(d) << a.page_shift) + held + t] = rows[t * D + d];
+            // 16 values of a dimension at a time, what else is among them as it was (32 sequences of ten tokens, eight layers, pages of 16: code by code, page after page 18.6 us,
+            // so 15.3)
+            const int chunk0 = max(first + j0, 0) >> 4, chunks = ((first + j0 + tokens - 1) >> 4) - chunk0 + 1;
+            for (int i = wave; i < chunks * (D / 64); i += kWaves) {
+                const int at = 16 * (chunk0 + i / (D / 64)), d = 64 * (i % (D / 64)) + lane;
+                const int from = max(at - first, j0), to = min(at + 16 - first, j0 + tokens);           // tokens that go there
+                bool any = false;
+                for (int t = from; t < to; ++t) any |= !(factors[t] < 0.0f);
+                if (!any || targets[from] < 0) continue;
+                uint4* const piece = reinterpret_cast<uint4*>(pages + (targets[from] - ((first + from) & 15)) + (static_cast<int64_t>(d) << a.page_shift));
+                const uint4 old = *piece;
+                uint64_t low = static_cast<uint64_t>(old.y) << 32 | old.x, high = static_cast<uint64_t>(old.w) << 32 | old.z;
+                for (int t = from; t < to; ++t) {
+                    if (factors[t] < 0.0f) continue;
+                    const int b = (first + t) & 15, shift = 8 * (b & 7);
+                    const uint64_t code = static_cast<uint64_t>(rows[(t - j0) * D + d]) << shift, keep = ~(uint64_t{0xff} << shift);
+                    low = b < 8 ? (low & keep) | code : low;
+                    high = b < 8 ? high : (high & keep) | code;
+                }
+                *piece = make_uint4(static_cast<uint32_t>(low), static_cast<uint32_t>(low >> 32), static_cast<uint32_t>(high), static_cast<uint32_t>(high >> 32));
             }
         }
         __syncthreads();
@@ -491,8 +535,8 @@ int pllm_paged_cache_compact(void* const* caches, int64_t layers, int64_t pool, 
     for (int64_t from = 0; from < layers; from += kLayers) {
         const int64_t count = std::min<int64_t>(layers - from, kLayers);
         const dim3 grid(static_cast<unsigned>(2 * kv_heads), static_cast<unsigned>(seqs), static_cast<unsigned>(count));
-        // (LDS for what a path can take of a page, so that many workgroups fit a compute unit)
-        const size_t lds = static_cast<size_t>(std::min(most, page_tokens) * head_dim);
+        // (LDS for as much of a path as there can be, so that many workgroups fit a compute unit)
+        const size_t lds = static_cast<size_t>(32 * most + std::min<int64_t>(most, kCompactStretch) * head_dim);
         if (head_dim == 128) hipLaunchKernelGGL((paged_compact_kernel<128>), grid, dim3(kCompactThreads), lds, static_cast<hipStream_t>(stream), some_layers(caches, from, count), a);
         else hipLaunchKernelGGL((paged_compact_kernel<64>), grid, dim3(kCompactThreads), lds, static_cast<hipStream_t>(stream), some_layers(caches, from, count), a);
     }

@@ -120,6 +120,15 @@ def test_even_trees_and_paths_that_stay(past):
     check_compact([cache], [[0, 1, 3, 4, 18, 19], [1, 2, 5, 9, -1, -1]], [6, 4], [20, 20])
 
 
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (128, 128)])
+def test_paths_of_several_stretches(dim, page):
+    """Long paths, whole or with one node or every few left out, at borders of 64 tokens, behind pasts that end anywhere in a page."""
+    kept = [list(range(1, 65)), [0] + list(range(2, 66)), list(range(100, 228)), [*range(63), *range(64, 130)], list(range(1, 256)), list(range(256)), list(range(0, 256, 3)), list(range(191, 256))]
+    pasts = [0, 7, 16, 61, 64, 100, 129, 15]
+    cache = Cache([p + 256 for p in pasts], 2, dim, page, seed=page, scale_exponents=(-9, -2))
+    check_compact([cache], [k + [-1] * (256 - len(k)) for k in kept], [len(k) for k in kept], [256] * 8)
+
+
 def test_paths_that_are_none_and_places_without_a_page():
     cache = Cache([60, 60, 60, 60], 1, 64, 16, seed=3)
     cache.table[1, 2], cache.table[2, 1], cache.table[3, 3] = -1, 2**30, cache.pool
