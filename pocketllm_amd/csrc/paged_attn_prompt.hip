@@ -11,7 +11,8 @@
 // 16-byte pieces of a row lie permuted in LDS (key rows by row % 16, value rows by row / 2 % 8), so 16 neighbouring rows read at one piece meet no
 // bank twice.  Rows behind the last sequence get zeros.
 //
-// SPLIT, for calls of few blocks: 128 rows, waves 4 to 7 have those of 0 to 3 and the other 32 keys of every tile, and what they leave meets in LDS at the end.
+// For calls of few blocks, 128 rows: waves 4 to 7 have those of 0 to 3 and the other 32 keys of every tile, and what they leave meets in LDS at the end.  For trees whose rows leave
+// much of whole blocks empty, 192: waves 0 to 3 as they are, 4 and 5, 6 and 7 with 32 rows and half of a tile's keys each, so that every SIMD has as much to do.
 //
 // Bound: 4 D operations per row and key.  8192 tokens of 48 and 8 heads, 825 G operations: 777 us, 1060 T/s, where a large matrix product of the library
 // reaches 1155; what is between is the softmax's vector instructions (48 % of the cycles, the matrix unit 47 %: the two waves of a SIMD overlap them in
@@ -19,8 +20,8 @@
 //
 // TREE: the new tokens are nodes of a drafted tree.  A node's ancestors are four 64-bit masks, walked up once per workgroup; tiles before the tree go as they do for prompts,
 // those that hold a node's key are masked by 64 bits of them per row.  Keys are cut in runs by units, below.  32 trees of 26 nodes of 48 and 8 heads behind up to 8191 positions,
-// 82 G operations, 170 us; five of up to 200 nodes of 64 and 8 heads behind up to 30000, 402 G, 508 us (790 T/s).  What is between that and prompts' rate: rows that do not fill
-// their block (156 of 256 at 26 nodes), about 12 us of a unit before its first and around its masked tiles, and 6 to 14 for the runs' sums.
+// 82 G operations, 159 us; five of up to 200 nodes of 64 and 8 heads behind up to 30000, 402 G, 505 us (800 T/s).  What is between that and prompts' rate: rows that do not fill
+// their block (156 of 192 at 26 nodes, whose blocks take 7/8 of a whole one's time), about 12 us of a unit before its first and around its masked tiles, and 6 to 14 for the runs' sums.
 #include "paged_attention.h"
 #include "paged_device.h"
 
@@ -31,7 +32,7 @@
 namespace pllm {
 namespace {
 
-constexpr int kWaves = 8, kThreads = 64 * kWaves, kBlockRows = 32 * kWaves;
+constexpr int kWaves = 8, kThreads = 64 * kWaves, kBlockRows = 32 * kWaves, kMixedRows = 192;
 constexpr int kTile = 64;                       // keys per step
 
 // Softmax weights are 2^(score - m), m what the row's largest score is compared with.  They are rounded to 16 bits for the second product (matrix instructions on
@@ -193,23 +194,19 @@ __device__ __forceinline__ bool find_unit(const PagedPromptArgs& a, int index, i
     return true;
 }
 
+// A wave's part of a workgroup's work.  SPLIT: it has 32 keys of every tile, another wave the others.
 // TREE: the new tokens are nodes of a tree; the tiles that hold some of their keys are masked by the nodes' ancestors
-template <bool BF16, int D, bool RUNS, bool SPLIT, bool TREE>
-__global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPromptArgs a) {
+template <bool BF16, int D, bool RUNS, int ROWS, bool TREE, bool SPLIT>
+__device__ __forceinline__ void prompt_rows(const PagedPromptArgs& a, unsigned char* smem, float (&factors)[4][8], int (&nan_values)[4], float (&unread)[64 + 4 * 8], float2* halves,
+                                            uint16_t (&nan_keys)[2][D][4], int* parents, uint64_t (*nodes)[kTreeWords]) {
     constexpr int kKeyBytes = kTile * D * 2, kTileBytes = 2 * kKeyBytes;      // keys [64][D], values [D][64]
     constexpr int kDimTiles = D / 32, kSteps = D / 16;
-    constexpr int kRows = SPLIT ? kBlockRows / 2 : kBlockRows, kSets = SPLIT ? 1 : 2;         // of a workgroup; 32 keys of a tile that a wave takes
-    extern __shared__ __align__(1024) unsigned char smem[];                   // [2][kTileBytes]
-    __shared__ __align__(16) float factors[4][8];                             // of tile t at t % 4: per chunk the keys' scale times `scale`, and 0 or -inf
-    __shared__ int nan_values[4];                                             // of tile t at t % 4 (masked tiles): some value code is NaN,
-    __shared__ float unread[64 + 4 * 8];
-    __shared__ float2 halves[SPLIT ? kBlockRows / 2 : 1];
-    __shared__ __align__(8) uint16_t nan_keys[2][D][4];                       // which ones: a bit per key and dimension, in the tile's half
-    __shared__ int parents[TREE ? kTreeNodes : 1];
-    __shared__ uint64_t nodes[TREE ? kRows : 1][kTreeWords];                  // what the nodes of the workgroup's rows see of the tree, from the first row's on
+    constexpr int kRows = ROWS, kSets = SPLIT ? 1 : 2;                        // of a workgroup; 32 keys of a tile that a wave takes
+    constexpr bool kMixed = ROWS == kMixedRows;                               // some waves share rows, others don't
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int place = SPLIT ? wave & 3 : wave, second = SPLIT ? wave >> 2 : 0;                // the wave's rows, the half of a tile's keys
+    // the wave's rows, the half of a tile's keys; of the rows that are shared
+    const int place = !SPLIT ? wave : kMixed ? 4 + (wave - 4) / 2 : wave & 3, second = !SPLIT ? 0 : kMixed ? wave & 1 : wave >> 2, shared_place = kMixed ? place - 4 : place;
     const int kvh = blockIdx.x, group = a.heads / a.kv_heads;
     // rows of one key/value head: token * group + head in the group; the tokens behind the last sequence are one more, without keys
     constexpr bool kDealt = TREE && RUNS;
@@ -500,6 +497,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
             for (int c = 0; c < 2 * kSets; ++c) { f[c] = 1.0f; b[c] = 0.0f; }
         }
         copies();
+        // (the requests of the copies go out before the products: left to the compiler they come last, and the next step waits for them; 8192 tokens 853 -> 797 us)
+        __builtin_amdgcn_sched_barrier(0);
         scores(half ^ 1, next);
         uint4 p[2 * kSets];
 #pragma unroll
@@ -575,11 +574,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     float lower, upper;
     swapped_pair<32>(l, lower, upper);
     float den = lower + upper;
+    // a wave's own part of LDS: 32 rows of 16 bits, of 32 where two waves bring them together
+    unsigned char* const own = smem + (kMixed && SPLIT ? 4 * 32 * D * 2 : 0) + (SPLIT ? shared_place * (32 * D * 4) : place * (32 * D * 2));
+    if constexpr (kMixed && !SPLIT) __syncthreads();                          // (the other waves' below)
     if constexpr (SPLIT) {
         // the two halves of the keys together, lane by lane
-        float4* other = reinterpret_cast<float4*>(smem + place * (32 * D * 4)) + lane;
+        float4* other = reinterpret_cast<float4*>(own) + lane;
         if (second) {
-            if (h == 0) halves[32 * place + r] = make_float2(m, den);
+            if (h == 0) halves[32 * shared_place + r] = make_float2(m, den);
 #pragma unroll
             for (int u = 0; u < kDimTiles; ++u)
 #pragma unroll
@@ -587,7 +589,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
         }
         __syncthreads();
         if (second) return;
-        const float2 theirs = halves[32 * place + r];
+        const float2 theirs = halves[32 * shared_place + r];
         const float most = fmaxf(m, theirs.x), mine_by = __builtin_amdgcn_exp2f(m - most), theirs_by = __builtin_amdgcn_exp2f(theirs.x - most);
         den = __builtin_fmaf(den, mine_by, theirs.y * theirs_by);
         m = most;
@@ -617,7 +619,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
     }
     const float inv = den == 0.0f ? 0.0f : 2.0f / den;                        // (twice: the values went in halved)
     // lane: query r, dimensions 32 u + 8 (v / 4) + 4 h + v % 4; through the wave's own part of LDS to whole rows
-    unsigned char* turn = smem + place * (32 * D * (SPLIT ? 4 : 2));
+    unsigned char* turn = own;
 #pragma unroll
     for (int u = 0; u < kDimTiles; ++u)
 #pragma unroll
@@ -633,6 +635,24 @@ __global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPr
         const int at = w0 + row;
         if (at < rows) *reinterpret_cast<uint4*>(a.out + ((static_cast<size_t>(offset) + at / group) * a.heads + kvh * group + at % group) * D + 8 * piece) = v;
     }
+}
+
+// ROWS query rows of a key/value head: 256, 32 of each wave; 128, which two waves share the keys of; 192, of which waves 4 to 7 share the last 64.
+template <bool BF16, int D, bool RUNS, int ROWS, bool TREE>
+__global__ __launch_bounds__(kThreads, 2) void paged_prompt_kernel(const PagedPromptArgs a) {
+    extern __shared__ __align__(1024) unsigned char smem[];                   // [2][kTileBytes]
+    __shared__ __align__(16) float factors[4][8];                             // of tile t at t % 4: per chunk the keys' scale times `scale`, and 0 or -inf
+    __shared__ int nan_values[4];                                             // of tile t at t % 4 (masked tiles): some value code is NaN,
+    __shared__ float unread[64 + 4 * 8];
+    __shared__ float2 halves[ROWS == kBlockRows ? 1 : ROWS == kMixedRows ? 64 : ROWS];        // m and sum of the rows whose keys two waves share
+    __shared__ __align__(8) uint16_t nan_keys[2][D][4];                       // which ones: a bit per key and dimension, in the tile's half
+    __shared__ int parents[TREE ? kTreeNodes : 1];
+    __shared__ uint64_t nodes[TREE ? ROWS : 1][kTreeWords];                   // what the nodes of the workgroup's rows see of the tree, from the first row's on
+#define PLLM_ROWS(split) prompt_rows<BF16, D, RUNS, ROWS, TREE, split>(a, smem, factors, nan_values, unread, halves, nan_keys, parents, nodes)
+    if constexpr (ROWS != kMixedRows) PLLM_ROWS(ROWS != kBlockRows);
+    else if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) < 4) PLLM_ROWS(false);          // (both have the same barriers)
+    else PLLM_ROWS(true);
+#undef PLLM_ROWS
 }
 
 // A wave per query row: its runs together, in their order.
@@ -711,14 +731,16 @@ __global__ __launch_bounds__(256) void paged_tree_merge_kernel(const PagedPrompt
 }
 
 template <bool BF16, int D, bool TREE>
-int launch(const PagedPromptArgs& a, bool split, hipStream_t stream) {
-    static SmemGrant granted[4];
+int launch(const PagedPromptArgs& a, int block_rows, hipStream_t stream) {
+    static SmemGrant granted[6];
     const size_t smem = 2 * 2 * kTile * D * 2;
     const bool runs = a.sums != nullptr;
-    const auto kernel = runs ? (split ? paged_prompt_kernel<BF16, D, true, true, TREE> : paged_prompt_kernel<BF16, D, true, false, TREE>)
-                             : (split ? paged_prompt_kernel<BF16, D, false, true, TREE> : paged_prompt_kernel<BF16, D, false, false, TREE>);
+    constexpr int kHalf = kBlockRows / 2, kMost = TREE ? kMixedRows : kBlockRows;             // (prompts have no mixed blocks)
+    const auto kernel = block_rows == kHalf        ? (runs ? paged_prompt_kernel<BF16, D, true, kHalf, TREE> : paged_prompt_kernel<BF16, D, false, kHalf, TREE>)
+                        : block_rows == kMixedRows ? (runs ? paged_prompt_kernel<BF16, D, true, kMost, TREE> : paged_prompt_kernel<BF16, D, false, kMost, TREE>)
+                                                   : (runs ? paged_prompt_kernel<BF16, D, true, kBlockRows, TREE> : paged_prompt_kernel<BF16, D, false, kBlockRows, TREE>);
     // (with the kernel's own arrays beside it, 128-wide heads pass 64 KB)
-    if (!grant_dynamic_smem(reinterpret_cast<const void*>(kernel), smem + (TREE ? 18432 : 8192), granted[2 * runs + split])) return PLLM_ERR_LAUNCH;
+    if (!grant_dynamic_smem(reinterpret_cast<const void*>(kernel), smem + (TREE ? 18432 : 8192), granted[3 * runs + (block_rows == kHalf ? 0 : block_rows == kMixedRows ? 1 : 2)])) return PLLM_ERR_LAUNCH;
     // Runs before blocks: indexes without a block come last.  Workgroups go to the shader engines in turn, those that end at once too, and an engine that got more
     // of the others than it has compute units works a second round (128 tokens behind 30000 positions in blocks of half the rows 213 -> 117 us).
     hipLaunchKernelGGL(kernel, dim3(a.kv_heads, TREE ? 1 : a.runs, a.slots), dim3(kThreads), smem, stream, a);
@@ -727,7 +749,8 @@ int launch(const PagedPromptArgs& a, bool split, hipStream_t stream) {
         const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
         const dim3 row_grid(static_cast<unsigned>((rows + 3) / 4));
         if constexpr (TREE) {
-            if (split) hipLaunchKernelGGL((paged_tree_merge_kernel<BF16, D, kBlockRows / 2>), row_grid, dim3(256), 0, stream, a);
+            if (block_rows == kHalf) hipLaunchKernelGGL((paged_tree_merge_kernel<BF16, D, kHalf>), row_grid, dim3(256), 0, stream, a);
+            else if (block_rows == kMixedRows) hipLaunchKernelGGL((paged_tree_merge_kernel<BF16, D, kMixedRows>), row_grid, dim3(256), 0, stream, a);
             else hipLaunchKernelGGL((paged_tree_merge_kernel<BF16, D, kBlockRows>), row_grid, dim3(256), 0, stream, a);
         } else hipLaunchKernelGGL((paged_prompt_merge_kernel<BF16, D>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream, a);
         if (hipGetLastError() != hipSuccess) return PLLM_ERR_LAUNCH;
@@ -767,7 +790,7 @@ int few_rows(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
     return rows < group ? 0 : static_cast<int>(rows);
 }
 
-struct Parts { int runs, few; bool split; size_t run_bytes, few_bytes; int units, deal; };
+struct Parts { int runs, few, block; size_t run_bytes, few_bytes; int units, deal; };
 Parts parts_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions, int few) {
     Parts p{};
     const int64_t rows = tokens * (heads / kv_heads);
@@ -780,8 +803,9 @@ Parts parts_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, in
     const bool alone = seqs == 1 && positions <= 2 * tokens;
     const int64_t whole = blocks_of(rows, seqs, p.few, kBlockRows) * kv_heads, half = blocks_of(rows, seqs, p.few, kBlockRows / 2) * kv_heads;
     const int whole_runs = prompt_runs(whole, positions);
-    p.split = half <= (alone ? 2 : 1) * compute_units() && (whole_runs == 1 || positions < 32 * kTile * whole_runs);
-    p.runs = rows <= p.few ? 1 : (p.split ? prompt_runs(half, positions) : whole_runs);
+    const bool split = half <= (alone ? 2 : 1) * compute_units() && (whole_runs == 1 || positions < 32 * kTile * whole_runs);
+    p.block = split ? kBlockRows / 2 : kBlockRows;
+    p.runs = rows <= p.few ? 1 : (split ? prompt_runs(half, positions) : whole_runs);
     if (alone && p.runs == 2) p.runs = 1;                                     // (the second launch: 1024 tokens of 16 and 8 heads 32.0 -> 26.4)
     const size_t parts = static_cast<size_t>(p.runs) * tokens * heads;
     p.run_bytes = p.runs > 1 ? align256(parts * head_dim * sizeof(float)) + align256(parts * sizeof(float2)) : 0;
@@ -803,14 +827,18 @@ size_t unit_bytes(int64_t units, int64_t kv_heads, int64_t rows, int64_t head_di
 Parts tree_parts(int64_t tokens, int64_t seqs, bool even, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
     const int64_t group = heads / kv_heads, rows = tokens * group, each = std::max<int64_t>(rows / seqs, 1);
     Parts p{};
+    p.block = kBlockRows;
     if (even && few_nodes(tokens / seqs, seqs, heads, kv_heads, head_dim, positions)) {
         p.few = static_cast<int>(each);
         p.few_bytes = paged_decode_parts_bytes(seqs, p.few, kv_heads, head_dim, positions);
         return p;
     }
     p.runs = 1;
-    p.split = 5 * ((each + kBlockRows / 2 - 1) / (kBlockRows / 2)) <= 8 * ((each + kBlockRows - 1) / kBlockRows);
-    const int64_t block = p.split ? kBlockRows / 2 : kBlockRows;
+    // per tile a block of half the rows takes about 5/8 of a whole one's time, a mixed one 7/8 (even calls, whose blocks are all filled alike: 32 trees of 26 nodes, 156 rows, 169 -> 159 us)
+    auto cost = [&](int64_t block_rows, int64_t tile) { return (each + block_rows - 1) / block_rows * tile; };
+    const int64_t whole = cost(kBlockRows, 8), mixed = even ? cost(kMixedRows, 7) : whole;
+    p.block = cost(kBlockRows / 2, 5) <= std::min(mixed, whole) ? kBlockRows / 2 : mixed < whole ? kMixedRows : kBlockRows;
+    const int64_t block = p.block;
     if (seqs < 64) {
         const int64_t blocks = blocks_of(rows, seqs, 0, static_cast<int>(block)) + 1, deal = std::max<int64_t>(compute_units() / kv_heads, 1), units = blocks + deal + 1;
         const size_t bytes = unit_bytes(units, kv_heads, block, head_dim) + align256(units * kv_heads * block * sizeof(float2)) + align256(seqs * sizeof(int2));
@@ -847,7 +875,7 @@ int attention(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pag
     const Parts parts = tree ? tree_parts(tokens, seqs, cu_steps == nullptr, heads, kv_heads, head_dim, positions)
                              : parts_of(tokens, seqs, heads, kv_heads, head_dim, positions, few_rows(tokens, seqs, heads, kv_heads, head_dim, positions));
     // (the rows behind the last sequence: what is left of the whole blocks, and one more)
-    const int64_t rows = tokens * (heads / kv_heads), slots = parts.units > 0 ? parts.units : blocks_of(rows, seqs, parts.few, parts.split ? kBlockRows / 2 : kBlockRows) + 1;
+    const int64_t rows = tokens * (heads / kv_heads), slots = parts.units > 0 ? parts.units : blocks_of(rows, seqs, parts.few, parts.block) + 1;
     if (rows > 0x3fffffff || slots > 0xffff) return PLLM_ERR_UNSUPPORTED;
     const uintptr_t wide = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages) | reinterpret_cast<uintptr_t>(out) |
                            reinterpret_cast<uintptr_t>(workspace);
@@ -873,7 +901,7 @@ int attention(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pag
         unsigned char* const at = static_cast<unsigned char*>(workspace);
         a.sums = reinterpret_cast<float*>(at);
         if (parts.units > 0) {
-            const int64_t block = parts.split ? kBlockRows / 2 : kBlockRows;
+            const int64_t block = parts.block;
             const size_t sums = unit_bytes(parts.units, kv_heads, block, head_dim);
             a.stats = reinterpret_cast<float2*>(at + sums);
             a.plan = reinterpret_cast<int2*>(at + sums + align256(parts.units * kv_heads * block * sizeof(float2)));
@@ -882,10 +910,10 @@ int attention(const void* q, int64_t q_stride, int dtype, const uint8_t* key_pag
     }
     if (cu_steps || a.few_rows == 0) {                                        // (otherwise every row is the decode kernel's)
         int status;
-        if (tree) status = head_dim == 128 ? (bf16 ? launch<true, 128, true>(a, parts.split, st) : launch<false, 128, true>(a, parts.split, st))
-                                           : (bf16 ? launch<true, 64, true>(a, parts.split, st) : launch<false, 64, true>(a, parts.split, st));
-        else status = head_dim == 128 ? (bf16 ? launch<true, 128, false>(a, parts.split, st) : launch<false, 128, false>(a, parts.split, st))
-                                      : (bf16 ? launch<true, 64, false>(a, parts.split, st) : launch<false, 64, false>(a, parts.split, st));
+        if (tree) status = head_dim == 128 ? (bf16 ? launch<true, 128, true>(a, parts.block, st) : launch<false, 128, true>(a, parts.block, st))
+                                           : (bf16 ? launch<true, 64, true>(a, parts.block, st) : launch<false, 64, true>(a, parts.block, st));
+        else status = head_dim == 128 ? (bf16 ? launch<true, 128, false>(a, parts.block, st) : launch<false, 128, false>(a, parts.block, st))
+                                      : (bf16 ? launch<true, 64, false>(a, parts.block, st) : launch<false, 64, false>(a, parts.block, st));
         if (status != PLLM_OK || a.few_rows == 0) return status;
     }
     PagedDecodeArgs d{};

@@ -84,6 +84,23 @@ def test_keys_cut_in_runs(nodes, pasts, heads, kv_heads, dim, dtype):
     check(cache, nodes, heads, dtype, [random_tree(rng, n) if n else [] for n in nodes], tail=2)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nodes,pasts,heads,kv_heads,dim", [
+    (150, [0, 700, 63], 1, 1, 64), (129, [1000], 2, 2, 128), (100, [3000, 5, 130], 3, 1, 128), (192, [64, 64], 4, 4, 64), (64, [2500, 1], 24, 8, 128), (65, [40, 1500], 16, 2, 64),
+])
+def test_rows_that_fill_three_quarters_of_a_block(nodes, pasts, heads, kv_heads, dim, dtype):
+    """129 to 192 rows, 257 to 384, 513 to 576: some waves have rows of their own, some share them."""
+    rng = np.random.default_rng(nodes)
+    cache = Cache([p + nodes for p in pasts], kv_heads, dim, 32, seed=nodes)
+    trees = [random_tree(rng, nodes) for _ in pasts]
+    check(cache, [nodes] * len(pasts), heads, dtype, trees, ragged=False)
+    which = cache.table[0, 0]                                                 # a NaN among the keys of the past, one among the last node's values
+    cache.key_codes[which, 0, 0, 1] = 0x7f
+    last = pasts[-1] + nodes - 1
+    cache.value_codes[cache.table[len(pasts) - 1, last // 32], kv_heads - 1, 9, last % 32] = 0xff
+    check(cache, [nodes] * len(pasts), heads, dtype, trees, ragged=False, size=3.0)
+
+
 @pytest.mark.parametrize("n", [10, 70])
 def test_a_chain_is_the_causal_form(n):
     """The nodes one after the other: what the prompt and the decode form give, within both kernels' roundings against the float64 form."""
