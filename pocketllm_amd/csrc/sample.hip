@@ -14,8 +14,8 @@
 //   4. the list in order, the cuts in it, the stretch of the row that the token lies in, the token
 // Many rows: a workgroup each, one launch.  Few rows: four launches, the first three over slices of the rows.
 // Bound: where there is no small top-k, the 64-bit exponential in two passes (about 100 instructions a value in all, of 16 cycles for a wave; the vector units are busy for 60 % of the
-// time, the rest is launches, chains of loads and barriers around the cuts, and rows that do not divide among the units): 832 rows of 32000 fp16 logits, all with top-p, 103 us,
-// of mixed parameters 75, 96 rows of 200064 in four launches 71, for bytes of 10 and 7.5.  With one, the bytes and, for a single row, the launches one after the other:
+// time, the rest is launches, chains of loads and barriers around the cuts, and rows that do not divide among the units): 832 rows of 32000 fp16 logits, all with top-p, 99 us,
+// of mixed parameters 70, 96 rows of 200064 in four launches 73, for bytes of 10 and 7.5.  With one, the bytes and, for a single row, the launches one after the other:
 // 200064 fp32 logits 21 us (3.1 + 5.3 + 5.9 + 7.4 of the launches; in one workgroup the row alone takes longer).
 #include "pllm_device.h"
 #include "pllm_internal.h"
@@ -48,6 +48,7 @@ struct SampleArgs {
     uint64_t* listed; uint32_t* listed_count;   // [rows][kListed], [rows]: order key and complement of the index
     int rows, vocab, slices, slice_chunks,      // chunks of 16 bytes of a slice, whole stretches
         stretches;
+    bool ordered;                               // a workgroup per row, those that take longest first
 };
 
 // Logits in the order of their values as unsigned numbers; NaN and minus infinity are 0x007fffff, the least of any.
@@ -231,6 +232,19 @@ __device__ __forceinline__ Asked asked_of(const SampleArgs& a, int row) {
     return Asked{a.temperature ? a.temperature[row] : a.temperature_all, a.top_p ? a.top_p[row] : a.top_p_all, a.min_p ? a.min_p[row] : a.min_p_all, a.uniform[row],
                  a.top_k ? a.top_k[row] : a.top_k_all};
 }
+// one for all lanes, in scalar registers
+__device__ __forceinline__ float of_wave(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+__device__ __forceinline__ uint64_t of_wave(uint64_t v) {
+    const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v)), high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+    return static_cast<uint64_t>(high) << 32 | low;
+}
+__device__ __forceinline__ double of_wave(double v) { return __longlong_as_double(static_cast<long long>(of_wave(static_cast<uint64_t>(__double_as_longlong(v))))); }
+__device__ __forceinline__ int of_wave(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ bool of_wave(bool v) { return __builtin_amdgcn_readfirstlane(v) != 0; }
+__device__ __forceinline__ Params of_wave(const Params& p) {
+    return Params{of_wave(p.factor), of_wave(p.most), of_wave(p.per_bin), of_wave(p.near), of_wave(p.least_weight), of_wave(p.least_before), of_wave(p.temperature), of_wave(p.top_p),
+                  of_wave(p.top_k), of_wave(p.index_shift), of_wave(p.greedy), of_wave(p.cut), of_wave(p.few), of_wave(p.counts), of_wave(p.best)};
+}
 __device__ __forceinline__ Params params_of(const Asked& asked, int vocab, uint64_t best, uint32_t least);
 // the largest and least of a wave's values, for all its lanes
 __device__ __forceinline__ void wave_extremes(uint64_t& best, uint32_t& least) {
@@ -275,7 +289,7 @@ __device__ __forceinline__ Params params_of(const Asked& asked, int vocab, uint6
     p.near = static_cast<float>(fmin((kUnit + 1.5) / p.factor, static_cast<double>(FLT_MAX)));
     const float span = fmaxf(fminf(distance(p, of_key(least)), p.near), FLT_MIN);
     p.per_bin = fminf(kBins / span, FLT_MAX);
-    return p;
+    return of_wave(p);
 }
 
 __device__ __forceinline__ void add_to(uint64_t* at, uint64_t v) { atomicAdd(reinterpret_cast<unsigned long long*>(at), static_cast<unsigned long long>(v)); }
@@ -1045,12 +1059,39 @@ __global__ __launch_bounds__(kLastThreads) void sample_token_kernel(const Sample
 
 // ---- many rows: a workgroup each ----------------------------------------------------------------------------------------
 
+// Where long rows have parameters of their own and there are more of them than compute units, those that take longest come first (no small top-k, then one, then the largest
+// logit alone): left in their order a long one may begin when the others end (of 32000, mixed: 832 rows 77 -> 67 us, 1600 110 -> 99; 3000 of 8000 89 -> 90, so not for
+// short ones).  Each workgroup finds the row of its place.
+constexpr int kOrdered = 8 * kRowThreads;
+__device__ __forceinline__ int ordered_row(const SampleArgs& a, uint64_t* parts, int& found) {
+    const int tid = threadIdx.x, each = (a.rows + kRowThreads - 1) / kRowThreads, begin = min(tid * each, a.rows), end = min(begin + each, a.rows);
+    auto kind = [&](int row) {
+        const float temperature = a.temperature ? a.temperature[row] : a.temperature_all;
+        const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
+        return !(temperature > 0.0f) || top_k == 1 ? 2 : top_k > 0 && top_k <= kFew ? 1 : 0;
+    };
+    auto of_kind = [](uint64_t counts, int k) { return static_cast<int>(counts >> (21 * k) & 0x1fffff); };
+    uint64_t counts = 0, all;
+    for (int row = begin; row < end; ++row) counts += uint64_t{1} << (21 * kind(row));
+    const uint64_t before = threads_until<kRowThreads>(counts, parts, all) - counts;
+    int place = blockIdx.x, k = 0;
+    while (k < 2 && place >= of_kind(all, k)) place -= of_kind(all, k++);
+    place -= of_kind(before, k);
+    if (place >= 0 && place < of_kind(counts, k))
+        for (int row = begin; row < end; ++row)
+            if (kind(row) == k && place-- == 0) found = row;
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(found);
+}
+
 template <typename T>
-__global__ __launch_bounds__(kRowThreads, 4) void sample_row_kernel(const SampleArgs a) {
+// (three workgroups a compute unit, which costs a few registers kept in memory: 832 rows with top-p 104 -> 99 us)
+__global__ __launch_bounds__(kRowThreads, 6) void sample_row_kernel(const SampleArgs a) {
     __shared__ Choice<kRowThreads> s;
     __shared__ uint32_t count[kBins], leasts[kRowThreads / 64], listed;
     __shared__ uint64_t sums[kMostStretches];
-    const int row = blockIdx.x, tid = threadIdx.x;
+    __shared__ int found;
+    const int row = a.ordered ? ordered_row(a, s.parts, found) : static_cast<int>(blockIdx.x), tid = threadIdx.x;
     const Row<T> x(a, row);
     const Asked asked = asked_of(a, row);                                     // (on its way beside the row)
     const int chunks = x.chunks();
@@ -1110,7 +1151,7 @@ Layout layout_of(int64_t rows, int64_t vocab, int dtype) {
     const int64_t chunks = (vocab + 2 * values - 2) / values;                 // (a row may begin inside a chunk)
     // A workgroup per row for rows of a few chunks per thread, and where there are more rows than compute units, if the last of them do not leave too many units idle: otherwise
     // slices, which take a little longer for the same work and 25 us more (top-p, 300 rows of 200064 in slices 199 us, by rows 279; 832 of 32000 about 107 by the same
-    // figures, 103).  As many slices as give the machine about eight workgroups per compute unit (four: 96 rows of 200064, mixed, 81 -> 71 us), none of fewer
+    // figures, 99).  As many slices as give the machine about eight workgroups per compute unit (four: 96 rows of 200064, mixed, 81 -> 71 us), none of fewer
     // than two chunks per thread.
     Layout l{};
     const int64_t units = compute_units(), rounds = (rows + units - 1) / units;
@@ -1169,6 +1210,7 @@ int pllm_sample_tokens(const void* logits, int64_t stride, int dtype, const floa
     a.mass = reinterpret_cast<uint64_t*>(ws + l.mass); a.count = reinterpret_cast<uint32_t*>(ws + l.count);
     a.listed = reinterpret_cast<uint64_t*>(ws + l.listed); a.listed_count = reinterpret_cast<uint32_t*>(ws + l.listed_count);
     a.rows = static_cast<int>(rows); a.vocab = static_cast<int>(vocab); a.slices = l.slices; a.slice_chunks = l.slice_chunks; a.stretches = l.stretches;
+    a.ordered = l.slices == 0 && (temperature || top_k) && rows > compute_units() && rows <= kOrdered && vocab * static_cast<int64_t>(value) / 16 > 2 * kRowThreads;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == PLLM_F32) return launch<float>(a, st);
     return dtype == PLLM_F16 ? launch<F16>(a, st) : launch<B16>(a, st);

@@ -217,3 +217,23 @@ def test_cuts_among_neighbouring_floats(count, levels):
     check(x[:1].repeat(2, 1), u, top_p=float((w[:3].sum() + (count // 2 + 0.4) * np.exp(-5.0)) / w.sum()))
     check(x, u, top_k=3 + count // 2)
     check(x, u, top_k=3 + count // 2, top_p=0.9, temperature=1.5)
+
+
+def test_more_rows_than_compute_units_with_parameters_of_their_own():
+    """Long rows of mixed parameters are taken in another order than they stand in; more of them than that is done for are not."""
+    g = torch.Generator().manual_seed(8)
+    rows, vocab = 270, 9000
+    x = (torch.randn(rows, vocab, generator=g) * 2).to(torch.float16)
+    pick = lambda *v: [v[int(i)] for i in torch.randint(len(v), (rows,), generator=g)]
+    given = dict(temperature=pick(0.0, 0.5, 1.0, 2.0, -1.0), top_k=pick(0, 1, 30, 1000, 2000, -3), top_p=pick(1.0, 0.9, 0.5), min_p=pick(0.0, 0.05))
+    check(x, uniforms(rows, 9), **given)
+    check(x, uniforms(rows, 9), top_k=given["top_k"])
+    big = 4100
+    x = (torch.randn(big, vocab, generator=g) * 2).to(torch.bfloat16).to(DEV)
+    u = torch.tensor(uniforms(big, 10), device=DEV)
+    k = torch.randint(0, 3, (big,), generator=g).int().to(DEV) * 20
+    t = torch.randint(0, 3, (big,), generator=g).float().to(DEV)
+    whole = K.sample_tokens_forward(x, u, temperature=t, top_k=k, top_p=0.95)
+    for n in (4096, 1000, 300):
+        parts = [K.sample_tokens_forward(x[i:i + n], u[i:i + n], temperature=t[i:i + n], top_k=k[i:i + n], top_p=0.95) for i in range(0, big, n)]
+        assert torch.equal(torch.cat(parts), whole)
