@@ -1,5 +1,6 @@
 // New keys and values into a paged E4M3 cache, the rotary phases on the way, and the new queries turned beside them: one launch.
-//     k' = k cos_p + swap(k) sin_p (the halves of the rotary part swapped; for keys in 64 bits), p = lengths[s] - n_s + i for token i of sequence s
+//     k' = k cos_p + swap(k) sin_p (the halves of the rotary part swapped; for keys in 64 bits), p = lengths[s] - n_s + i for token i of sequence s, or what `positions`
+//     say of it (nodes of a drafted tree: the past plus their depth)
 //     scale of a page and head: the least power of two with amax / scale <= 448 over what the page holds;  code = E4M3(k' / scale)
 // A page that a call continues keeps its scale unless the new tokens need a larger one; then its older codes are scaled down by the ratio, a power
 // of two: exact, but for codes that get below E4M3's normal values, which are rounded again.  A page that a call begins forgets what it held.
