@@ -600,19 +600,20 @@ template <int THREADS> __device__ __forceinline__ int reach(Choice<THREADS>& s, 
     return static_cast<int>(s.found[0]);
 }
 
+// a value's bin, and its part of it
+__device__ __forceinline__ int part_of(const Params& p, float x, int& part) {
+    const int bin = bin_of(p, x);
+    // (fused by name: left to the compiler, one loop had the product rounded and the other not, and looked for a value in the neighbouring part)
+    const float inside = __builtin_fmaf(distance(p, x), p.per_bin, -static_cast<float>(bin));
+    part = static_cast<int>(fminf(fmaxf(inside * kBins, 0.0f), kBins - 1.0f));
+    return bin;
+}
 // Of the listed values of a bin, in falling order of their places: the first one at which the sum (of weights, or of ones) reaches `least`.  The bin is cut in kBins parts
 // once more; what is left in a part is equal values mostly.
 template <int THREADS, typename Weight>
 __device__ __forceinline__ uint64_t resolve(Choice<THREADS>& s, const Params& p, int listed, int bin, uint64_t least, const Weight& weight) {
     const int tid = threadIdx.x;
-    auto place_of = [&](uint64_t key, int& part) {                             // its bin, and its part of it
-        const float x = of_key(static_cast<uint32_t>(key >> 32));
-        const int b = bin_of(p, x);
-        // (fused by name: left to the compiler, one loop had the product rounded and the other not, and looked for a value in the neighbouring part)
-        const float inside = __builtin_fmaf(distance(p, x), p.per_bin, -static_cast<float>(b));
-        part = static_cast<int>(fminf(fmaxf(inside * kBins, 0.0f), kBins - 1.0f));
-        return b;
-    };
+    auto place_of = [&](uint64_t key, int& part) { return part_of(p, of_key(static_cast<uint32_t>(key >> 32)), part); };
     __syncthreads();
     for (int i = tid; i < kBins; i += THREADS) s.sums[i] = 0;
     if (tid == 0) s.fews = 0;
@@ -793,35 +794,83 @@ __device__ __forceinline__ int64_t choose(const Row<T>& x, const Params& p, Choi
     }
     if (bounded && !ordered) {
         last_kept = 0;
-        // more values at the cuts than the list holds, many of them equal: by the digits of their places, from the first on, a pass over the row for each of eight
-        auto reached = [&](uint64_t least, bool counts) {                      // the place of the value at which the sum reaches `least`
-            uint64_t place = 0;
-            for (int shift = 56; shift >= 0; shift -= 8) {
-                __syncthreads();
-                for (int i = tid; i < 256; i += THREADS) s.sums[i] = 0;
+        // More values at the cuts than the list holds.  Sums go to s.sums by a number per value, below zero for none: neighbours mostly have one, and theirs goes there in one addition.
+        auto spread = [&](const auto& number, bool counts) {
+            __syncthreads();
+            for (int i = tid; i < kBins; i += THREADS) s.sums[i] = 0;
+            __syncthreads();
+            for_chunks<T, THREADS>(x, 0, x.chunks(), [&](int c, const uint4& u) {
+                float v[kValues];
+                Row<T>::values_of(u, v);
+                uint64_t sum = 0;
+                int at = 0;
+#pragma unroll
+                for (int i = 0; i < kValues; ++i) {
+                    const uint64_t w = weight_of(p, v[i]);
+                    const int its = w ? number(v[i], x.first_of(c) + i) : -1;
+                    if (its < 0) continue;
+                    if (sum && its != at) { add_to(&s.sums[at], sum); sum = 0; }
+                    at = its;
+                    sum += counts ? 1 : w;
+                }
+                const int first = __builtin_amdgcn_readfirstlane(at);
+                if (__ballot(at == first) == ~0ull) {                         // (all 64 lanes)
+                    sum = lanes_sum(sum);
+                    if (sum && (tid & 63) == 0) add_to(&s.sums[first], sum);
+                } else if (sum) add_to(&s.sums[at], sum);
+            });
+            __syncthreads();
+        };
+        if (cuts.last < 0 && !p.few) {
+            // top-p alone: by the parts of its bin, the values of one of them to the list; if these are too many and equal, as they are in 16 bits, by stretches of their indexes
+            // (96 rows of 200064, most values around 12 below the largest: in fp32 322 us, by digits 1320; in bf16 495, by digits 1210)
+            const uint64_t share = share_up(p_fraction, cuts.total);
+            uint64_t least = (share > 0 ? share : 1) - cuts.before_low, before;
+            auto part_in_bin = [&](float value) { int part; return part_of(p, value, part) == cuts.low ? part : -1; };
+            auto gather = [&](const auto& taken) {                            // to the list; how many there are
+                if (tid == 0) s.fews = 0;
                 __syncthreads();
                 for_chunks<T, THREADS>(x, 0, x.chunks(), [&](int c, const uint4& u) {
                     float v[kValues];
                     Row<T>::values_of(u, v);
-                    // (neighbours mostly have one digit: their sum in one addition)
-                    uint64_t sum = 0;
-                    int digit = 0;
 #pragma unroll
-                    for (int i = 0; i < kValues; ++i) {
-                        const uint64_t key = place_key(order_key(v[i]), x.first_of(c) + i), w = weight_of(p, v[i]);
-                        if (w == 0 || (shift < 56 && (key >> shift >> 8) != (place >> shift >> 8))) continue;
-                        const int its = 255 - static_cast<int>(key >> shift & 255);          // falling
-                        if (sum && its != digit) { add_to(&s.sums[digit], sum); sum = 0; }
-                        digit = its;
-                        sum += counts ? 1 : w;
-                    }
-                    const int first = __builtin_amdgcn_readfirstlane(digit);
-                    if (__ballot(digit == first) == ~0ull) {                  // (all 64 lanes)
-                        sum = lanes_sum(sum);
-                        if (sum && (tid & 63) == 0) add_to(&s.sums[first], sum);
-                    } else if (sum) add_to(&s.sums[digit], sum);
+                    for (int i = 0; i < kValues; ++i)
+                        if (weighs(p, v[i]) && taken(v[i], x.first_of(c) + i)) {
+                            const uint32_t at = atomicAdd(&s.fews, 1u);
+                            if (at < kListed) s.list[at] = place_key(order_key(v[i]), x.first_of(c) + i);
+                        }
                 });
                 __syncthreads();
+                return static_cast<int>(s.fews);
+            };
+            spread([&](float value, int) { return part_in_bin(value); }, false);
+            const int of = reach<THREADS>(s, kBins, least, before);
+            least -= before;
+            int n = gather([&](float value, int) { return part_in_bin(value) == of; });
+            if (n > kListed) {
+                const uint32_t key = static_cast<uint32_t>(s.list[0] >> 32);
+                bool others = false;
+                spread([&](float value, int index) {
+                    if (part_in_bin(value) != of) return -1;
+                    others |= order_key(value) != key;
+                    return index >> p.index_shift;                            // (below kBins, rising where places fall)
+                }, false);
+                if (!__syncthreads_or(others)) {
+                    const int span = reach<THREADS>(s, kBins, least, before);
+                    least -= before;
+                    n = gather([&](float value, int index) { return order_key(value) == key && index >> p.index_shift == span; });
+                }
+            }
+            if (n <= kListed) last_kept = resolve<THREADS>(s, p, n, cuts.low, least, weight_key);
+        }
+        // many of them equal: by the digits of their places, from the first on, a pass over the row for each of eight
+        auto reached = [&](uint64_t least, bool counts) {                      // the place of the value at which the sum reaches `least`
+            uint64_t place = 0;
+            for (int shift = 56; shift >= 0; shift -= 8) {
+                spread([&](float value, int index) {
+                    const uint64_t key = place_key(order_key(value), index);
+                    return shift < 56 && (key >> shift >> 8) != (place >> shift >> 8) ? -1 : 255 - static_cast<int>(key >> shift & 255);        // falling
+                }, counts);
                 uint64_t before;
                 const int its = reach<THREADS>(s, 256, least, before);
                 least -= before;
@@ -842,8 +891,9 @@ Row<T>::values_of(u, v);
             });
             return all_sum<THREADS>(sum, s.parts);
         };
-        if (p.top_k > 0 && whole(0, true) > static_cast<uint64_t>(p.top_k)) last_kept = reached(p.top_k, true);
-        if (p.top_p < 1.0f) {
+        const bool found = last_kept != 0;
+        if (!found && p.top_k > 0 && whole(0, true) > static_cast<uint64_t>(p.top_k)) last_kept = reached(p.top_k, true);
+        if (!found && p.top_p < 1.0f) {
             const uint64_t share = share_up(p_fraction, whole(last_kept, false));
             last_kept = reached(share > 0 ? share : 1, false);
         }

@@ -237,3 +237,18 @@ def test_more_rows_than_compute_units_with_parameters_of_their_own():
     for n in (4096, 1000, 300):
         parts = [K.sample_tokens_forward(x[i:i + n], u[i:i + n], temperature=t[i:i + n], top_k=k[i:i + n], top_p=0.95) for i in range(0, big, n)]
         assert torch.equal(torch.cat(parts), whole)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("vocab", [4000, 30000])
+def test_cuts_inside_a_crowd(vocab, dtype):
+    """Most values close together far below the largest: more of them in the bin of the cut than the list holds, different ones and (in fp16) equal ones too."""
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randn(4, vocab, generator=g) * 0.003 - 6
+    x[:, 17], x[:, 40], x[:, 41] = 0.0, -1.0, -35.0
+    x = x.to(dtype)
+    u = uniforms(4, vocab)
+    check(x, u, top_p=0.99)
+    check(x, u, top_p=[0.5, 0.9, 0.97, 0.995], min_p=0.0005)
+    check(x, u, top_p=0.98, temperature=2.0, top_k=vocab - 1)
+    check(x, u, top_p=0.9, top_k=vocab // 2 + 500)
