@@ -685,7 +685,7 @@ __device__ __forceinline__ uint64_t resolve(Choice<THREADS>& s, const Params& p,
     return s.few[at];
 }
 
-// The last step, by a workgroup: the token.  The listed values are in s.list, unordered, `listed` of them (more than the list holds: bisection); certain(i) is what is
+// The last step, by a workgroup: the token.  The listed values are in s.list, unordered, `listed` of them (more than the list holds: passes over the row); certain(i) is what is
 // kept for certain of stretch i (kStretch chunks).
 template <typename T, int THREADS, typename Certain>
 __device__ __forceinline__ int64_t choose(const Row<T>& x, const Params& p, Choice<THREADS>& s, int listed, float u, const Certain& certain) {
@@ -1122,6 +1122,7 @@ __device__ __forceinline__ int ordered_row(const SampleArgs& a, uint64_t* parts,
     };
     auto of_kind = [](uint64_t counts, int k) { return static_cast<int>(counts >> (21 * k) & 0x1fffff); };
     uint64_t counts = 0, all;
+    if (tid == 0) found = blockIdx.x;                                         // (parameters that change under the call: some row)
     for (int row = begin; row < end; ++row) counts += uint64_t{1} << (21 * kind(row));
     const uint64_t before = threads_until<kRowThreads>(counts, parts, all) - counts;
     int place = blockIdx.x, k = 0;
