@@ -15,8 +15,8 @@
 // Many rows: a workgroup each, one launch.  Few rows: four launches, the first three over slices of the rows.
 // Bound: where there is no small top-k, the 64-bit exponential in two passes (about 100 instructions a value in all, of 16 cycles for a wave; the vector units are busy for 60 % of the
 // time, the rest is launches, chains of loads and barriers around the cuts, and rows that do not divide among the units): 832 rows of 32000 fp16 logits, all with top-p, 99 us,
-// of mixed parameters 70, 96 rows of 200064 in four launches 73, for bytes of 10 and 7.5.  With one, the bytes and, for a single row, the launches one after the other:
-// 200064 fp32 logits 21 us (3.1 + 5.3 + 5.9 + 7.4 of the launches; in one workgroup the row alone takes longer).
+// of mixed parameters 67, 96 rows of 200064 in four launches 71, for bytes of 10 and 7.5.  With one, the bytes and, for a single row, the launches one after the other:
+// 200064 fp32 logits 21 us (2.8 + 5.3 + 5.7 + 7.6 of the launches).
 #include "pllm_device.h"
 #include "pllm_internal.h"
 
@@ -246,14 +246,26 @@ __device__ __forceinline__ Params of_wave(const Params& p) {
                   of_wave(p.top_k), of_wave(p.index_shift), of_wave(p.greedy), of_wave(p.cut), of_wave(p.few), of_wave(p.counts), of_wave(p.best)};
 }
 __device__ __forceinline__ Params params_of(const Asked& asked, int vocab, uint64_t best, uint32_t least);
-// the largest and least of a wave's values, for all its lanes
+// the largest and least of a wave's values, for all its lanes: shifts within 16 lanes, then the ends of 16 and of 32 lanes to those behind, then the last lane's
 __device__ __forceinline__ void wave_extremes(uint64_t& best, uint32_t& least) {
-#pragma unroll
-    for (int i = 32; i > 0; i /= 2) {
-        const uint64_t b = __shfl_xor(static_cast<unsigned long long>(best), i);
-        best = b > best ? b : best;
-        least = min(least, static_cast<uint32_t>(__shfl_xor(static_cast<int>(least), i)));
+#define PLLM_STEP(ctrl, rows)                                                                                                                          \
+    {                                                                                                                                                  \
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(best), ctrl, rows, 0xf, false);                                       \
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<uint32_t>(best >> 32), ctrl, rows, 0xf, false);                                 \
+        const uint64_t b = static_cast<uint64_t>(hi) << 32 | lo;                                                                                       \
+        best = b > best ? b : best;                                                                                                                    \
+        least = min(least, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(-1, static_cast<int>(least), ctrl, rows, 0xf, false)));                   \
     }
+    PLLM_STEP(0x111, 0xf)
+    PLLM_STEP(0x112, 0xf)
+    PLLM_STEP(0x114, 0xf)
+    PLLM_STEP(0x118, 0xf)
+    PLLM_STEP(0x142, 0xa)
+    PLLM_STEP(0x143, 0xc)
+#undef PLLM_STEP
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(best), 63), hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(best >> 32), 63);
+    best = static_cast<uint64_t>(hi) << 32 | lo;
+    least = __builtin_amdgcn_readlane(least, 63);
 }
 // the row's parameters, by a wave from what the slices left
 __device__ __forceinline__ Params slices_params(const SampleArgs& a, int row, const Asked& asked) {
@@ -1190,8 +1202,9 @@ template <typename T> int launch(const SampleArgs& a, hipStream_t stream) {
     }
     hipLaunchKernelGGL((sample_extremes_kernel<T>), grid, dim3(kThreads), 0, stream, a);
     const bool cut = a.top_k || a.top_p || (a.top_k_all > 0 && a.top_k_all < a.vocab) || a.top_p_all < 1.0f;
-    if (cut) hipLaunchKernelGGL((sample_histogram_kernel<T>), grid, dim3(kThreads), 0, stream, a);
-    hipLaunchKernelGGL((sample_masses_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+    const bool drawn = (a.temperature || a.temperature_all > 0.0f) && (a.top_k || a.top_k_all != 1);                  // (otherwise every row's largest)
+    if (drawn && cut) hipLaunchKernelGGL((sample_histogram_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+    if (drawn) hipLaunchKernelGGL((sample_masses_kernel<T>), grid, dim3(kThreads), 0, stream, a);
     hipLaunchKernelGGL((sample_token_kernel<T>), dim3(a.rows), dim3(kLastThreads), 0, stream, a);
     return hipGetLastError() == hipSuccess ? PLLM_OK : PLLM_ERR_LAUNCH;
 }
