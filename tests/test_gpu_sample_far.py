@@ -1,0 +1,58 @@
+"""sample_tokens_forward where distances from the largest logit leave float32's range as numbers of bins: a few allowed tokens beside masked ones."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import tree_oracle as T
+from test_gpu_sample import check
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def both_sides(row, **given):
+    """Numbers on both sides of every border between the tokens that are kept of a row, and in the middle between borders."""
+    x, params = row.double().numpy(), {n: float(np.float32(v)) for n, v in given.items()}
+    params = {n: int(v) if n == "top_k" else v for n, v in params.items()}
+    tokens, borders = [], []
+    for u in (np.arange(256) + 0.5) / 256:                                    # (no allowed token below has less than 1/256)
+        token, _ = T.sample(x, u, **params)
+        if not tokens or token != tokens[-1]:
+            low, high = (u - 1 / 256, u) if tokens else (0.0, 0.0)
+            for _ in range(20 if tokens else 0):
+                middle = (low + high) / 2
+                low, high = (middle, high) if T.sample(x, middle, **params)[0] != token else (low, middle)
+            tokens.append(token)
+            borders.append(high)
+    borders.append(1.0)
+    return sorted({float(np.float32(u)) for a, b in zip(borders, borders[1:]) for u in (a + 1e-5, (a + b) / 2, b - 1e-5)})
+
+
+PARAMETERS = [dict(), dict(top_p=0.99), dict(top_p=0.6), dict(top_k=1500), dict(top_k=1500, top_p=0.9), dict(min_p=0.05), dict(temperature=0.7, min_p=0.01), dict(top_k=40),
+              dict(temperature=3.0, top_p=0.97)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [3200, 40000])
+@pytest.mark.parametrize("allowed", [{40: 10.0, 41: 8.0}, {40: 2.0, 41: 0.0, 42: -1.0}, {41: -3.0, 42: 1.0, 43: 0.5}, {40: 5.0, 41: 3.0, 800: 5.0, 802: 2.5},
+                                     {8: 0.0, 9: -1.75, 1600: 0.0, 1601: -2.0, 3192: 0.0, 3194: -2.5}])
+def test_a_few_allowed_tokens(allowed, vocab, dtype):
+    """All else is masked: every chunk of 16 bytes that has an allowed token has a masked one too, and the largest of each such chunk is the same."""
+    row = torch.full((vocab,), -float("inf"))
+    for i, v in allowed.items():
+        row[i] = v
+    for given in PARAMETERS:
+        u = both_sides(row[:3200], **given)
+        check(row.to(dtype).repeat(len(u), 1), u, **given)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [3200, 40000])
+def test_masks_in_every_chunk(vocab, dtype):
+    """Of every four neighbours one is masked, one has the largest value, the others anything below it: tens of thousands of values beyond where bins end."""
+    g = torch.Generator().manual_seed(vocab)
+    row = 4 - 12 * torch.rand(vocab, generator=g)
+    row[::4], row[2::4] = 4.0, -float("inf")
+    u = torch.rand(6, generator=g).tolist()
+    for given in (dict(), dict(top_p=0.9), dict(top_p=0.9999), dict(min_p=0.01), dict(top_k=vocab // 2), dict(top_k=1024), dict(temperature=2.5, top_p=0.98)):
+        check(row.to(dtype).repeat(6, 1), u, **given)
