@@ -115,34 +115,38 @@ template <typename T> struct Row {
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
-    // the largest of a chunk's values (NaN or minus infinity if there is none)
+    // its values, minus infinity for NaN
+    static __device__ __forceinline__ void values_of(const uint4& u, float (&v)[kValues]) {
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) v[i] = fmaxf(Chunk<T>::at(u, i), -INFINITY);
+    }
+    // The largest of them; the least, minus infinity among them.  (Of float32 after NaN became minus infinity: a maximum hands a signalling NaN on as a quiet one, and the
+    // compiler brings two maxima together in one instruction, in which that takes the other value's place.)
     static __device__ __forceinline__ float most_of(const uint4& u) {
         if constexpr (std::is_same_v<T, F16>) {
             const Half2 m = __builtin_elementwise_max(__builtin_elementwise_max(half2_of(u.x), half2_of(u.y)), __builtin_elementwise_max(half2_of(u.z), half2_of(u.w)));
             return fmaxf(static_cast<float>(m[0]), static_cast<float>(m[1]));
         } else {
-            float m = Chunk<T>::at(u, 0);
+            float v[kValues];
+            values_of(u, v);
+            float m = v[0];
 #pragma unroll
-            for (int i = 1; i < kValues; ++i) m = fmaxf(m, Chunk<T>::at(u, i));
+            for (int i = 1; i < kValues; ++i) m = fmaxf(m, v[i]);
             return m;
         }
     }
-    // the least, minus infinity among them
     static __device__ __forceinline__ float least_of(const uint4& u) {
         if constexpr (std::is_same_v<T, F16>) {
             const Half2 m = __builtin_elementwise_min(__builtin_elementwise_min(half2_of(u.x), half2_of(u.y)), __builtin_elementwise_min(half2_of(u.z), half2_of(u.w)));
             return fminf(static_cast<float>(m[0]), static_cast<float>(m[1]));
         } else {
-            float m = Chunk<T>::at(u, 0);
+            float v[kValues];
+            values_of(u, v);
+            float m = v[0];
 #pragma unroll
-            for (int i = 1; i < kValues; ++i) m = fminf(m, Chunk<T>::at(u, i));
+            for (int i = 1; i < kValues; ++i) m = fminf(m, v[i]);
             return m;
         }
-    }
-    // its values, minus infinity for NaN
-    static __device__ __forceinline__ void values_of(const uint4& u, float (&v)[kValues]) {
-#pragma unroll
-        for (int i = 0; i < kValues; ++i) v[i] = fmaxf(Chunk<T>::at(u, i), -INFINITY);
     }
 };
 // The next chunks of a thread, every STEP-th, on their way.

@@ -1,4 +1,4 @@
-"""sample_tokens_forward where distances from the largest logit leave float32's range as numbers of bins: a few allowed tokens beside masked ones."""
+"""sample_tokens_forward where distances from the largest logit leave float32's range as numbers of bins: a few allowed tokens beside masked ones; NaN of any kind."""
 import numpy as np
 import pytest
 import torch
@@ -56,3 +56,30 @@ def test_masks_in_every_chunk(vocab, dtype):
     u = torch.rand(6, generator=g).tolist()
     for given in (dict(), dict(top_p=0.9), dict(top_p=0.9999), dict(min_p=0.01), dict(top_k=vocab // 2), dict(top_k=1024), dict(temperature=2.5, top_p=0.98)):
         check(row.to(dtype).repeat(6, 1), u, **given)
+
+
+NANS = {torch.float32: (torch.int32, (0x7fc00000, 0x7f800001, 0x7fbfffff, -0x400000, -0x7fffff)), torch.float16: (torch.int16, (0x7e00, 0x7c01, 0x7dff, -0x200, -0x3ff)),
+        torch.bfloat16: (torch.int16, (0x7fc0, 0x7f81, 0x7fbf, -0x40, -0x7f))}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [1000, 40000])
+def test_nan_of_any_kind_is_never_a_token(vocab, dtype):
+    """Quiet and signalling NaN of both signs among the logits, and in a row of few others."""
+    x = (torch.randn(4, vocab, generator=torch.Generator().manual_seed(vocab)) * 2).to(dtype)
+    holder, codes = NANS[dtype]
+    for i, code in enumerate(codes):
+        x.view(holder)[:, i::11] = code
+    x.view(holder)[3, 100:] = codes[1]
+    assert int(x[:3].isnan().sum()) == 3 * sum(len(range(i, vocab, 11)) for i in range(5)) and not torch.isfinite(x[3, 100:]).any()
+    u = [0.02, 0.35, 0.66, 0.97]
+    for given in (dict(), dict(top_p=0.9), dict(top_k=20), dict(min_p=0.05), dict(temperature=0.0)):
+        check(x, u, **given)
+    # the largest beside signalling ones in its 16 bytes, at each of their places
+    for at in range(8):
+        row = torch.zeros(2, vocab, dtype=dtype)
+        row.view(holder)[:, 8:16] = codes[1]
+        row[0, 8 + at] = 3.0
+        row[1, 8 + at] = row[1, 8 + (at + 3) % 8] = 3.0
+        check(row, [0.5, 0.5], temperature=0.0)
+        check(row, [0.004, 0.004])
