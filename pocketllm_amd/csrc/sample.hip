@@ -225,9 +225,7 @@ __device__ __forceinline__ uint64_t only(bool v) { return ~(static_cast<uint64_t
 // (plus infinity as the largest: it has no distance from itself, the others an infinite one; a difference that is no number is none)
 __device__ __forceinline__ float distance(const Params& p, float x) { return fmaxf(p.most - x, 0.0f); }
 __device__ __forceinline__ bool weighs(const Params& p, float x) { return distance(p, x) <= p.near; }
-// a distance in bins: the last bin takes all from its beginning on, also where masks left so little to measure bins by that a distance in them is no float
-__device__ __forceinline__ float in_bins(const Params& p, float distance) { return fminf(distance * p.per_bin, kBins - 1.0f); }
-__device__ __forceinline__ int bin_of(const Params& p, float x) { return static_cast<int>(in_bins(p, distance(p, x))); }
+__device__ __forceinline__ int bin_of(const Params& p, float x) { return static_cast<int>(fminf(distance(p, x) * p.per_bin, kBins - 1.0f)); }
 __device__ __forceinline__ double weight_before(const Params& p, float x) {                   // (anything where x does not weigh)
     return exponential(fmin(static_cast<double>(x) - static_cast<double>(p.most), 0.0) * p.factor);
 }
@@ -306,7 +304,9 @@ __device__ __forceinline__ Params params_of(const Asked& asked, int vocab, uint6
     // (weights below 2^-44 are none; in the last step of a float's more)
     p.near = static_cast<float>(fmin((kUnit + 1.5) / p.factor, static_cast<double>(FLT_MAX)));
     const float span = fmaxf(fminf(distance(p, of_key(least)), p.near), FLT_MIN);
-    p.per_bin = fminf(kBins / span, FLT_MAX);
+    // (Masks can leave next to nothing between the largest value and the least.  Counted in bins of that width what is farther away would be at infinity, in none of them: no
+    // bin is so narrow that `near` is not a float number of them.)
+    p.per_bin = fminf(fminf(kBins / span, FLT_MAX), 0.5f * FLT_MAX / p.near);
     return of_wave(p);
 }
 
@@ -534,7 +534,7 @@ __device__ __forceinline__ uint64_t sort_out(const Params& p, const uint4& u, in
     bool above[Row<T>::kValues], inside[Row<T>::kValues];
 #pragma unroll
     for (int i = 0; i < Row<T>::kValues; ++i) {
-        const float d = distance(p, v[i]), place = in_bins(p, d);
+        const float d = distance(p, v[i]), place = d * p.per_bin;
         const bool here = d <= p.near;
         above[i] = here && place < from;
         inside[i] = here && ((place >= from && place < to) || (place >= last_from && place < last_to));
