@@ -212,7 +212,7 @@ __device__ __forceinline__ uint64_t share_up(uint64_t fraction, uint64_t of) {  
 
 struct Params {
     double factor;                              // base-2 exponent per unit of distance from the largest logit
-    float most, per_bin, near;                  // the largest logit; bins per unit of distance; distance behind which weights are none
+    float most, per_bin, near;                  // the largest logit; bins per unit of distance (half of it, below); distance behind which weights are none
     uint64_t least_weight;                      // of min_p
     double least_before;                        // of a weight that rounds to no less
     float temperature, top_p;
@@ -222,8 +222,9 @@ struct Params {
 };
 // all bits or none: a mask where a choice would be a branch around what is chosen, and a chunk's values would go one after the other
 __device__ __forceinline__ uint64_t only(bool v) { return ~(static_cast<uint64_t>(v) - 1); }
-// (plus infinity as the largest: it has no distance from itself, the others an infinite one; a difference that is no number is none)
-__device__ __forceinline__ float distance(const Params& p, float x) { return fmaxf(p.most - x, 0.0f); }
+// Half the distance from the largest logit, all of which may be more than the largest float.  (Plus infinity as the largest: it has no distance from itself, the others an infinite one;
+// a difference that is no number is none.)
+__device__ __forceinline__ float distance(const Params& p, float x) { return fmaxf(__builtin_fmaf(x, -0.5f, 0.5f * p.most), 0.0f); }
 __device__ __forceinline__ bool weighs(const Params& p, float x) { return distance(p, x) <= p.near; }
 __device__ __forceinline__ int bin_of(const Params& p, float x) { return static_cast<int>(fminf(distance(p, x) * p.per_bin, kBins - 1.0f)); }
 __device__ __forceinline__ double weight_before(const Params& p, float x) {                   // (anything where x does not weigh)
@@ -302,7 +303,7 @@ __device__ __forceinline__ Params params_of(const Asked& asked, int vocab, uint6
     p.cut = (p.top_k > 0 && p.top_k < vocab) || p.top_p < 1.0f;
     p.factor = 1.44269504088896340736 / static_cast<double>(p.temperature);
     // (weights below 2^-44 are none; in the last step of a float's more)
-    p.near = static_cast<float>(fmin((kUnit + 1.5) / p.factor, static_cast<double>(FLT_MAX)));
+    p.near = static_cast<float>(fmin(0.5 * (kUnit + 1.5) / p.factor, static_cast<double>(FLT_MAX)));
     const float span = fmaxf(fminf(distance(p, of_key(least)), p.near), FLT_MIN);
     // (Masks can leave next to nothing between the largest value and the least.  Counted in bins of that width what is farther away would be at infinity, in none of them: no
     // bin is so narrow that `near` is not a float number of them.)

@@ -1,10 +1,11 @@
-"""sample_tokens_forward where distances from the largest logit leave float32's range as numbers of bins: a few allowed tokens beside masked ones; NaN of any kind."""
+"""sample_tokens_forward where distances from the largest logit leave float32's range, as logits or as numbers of bins: a few allowed tokens beside masked ones, finite logits
+farther apart than the largest float32, NaN of any kind."""
 import numpy as np
 import pytest
 import torch
 
 from oracle import tree_oracle as T
-from test_gpu_sample import check
+from test_gpu_sample import check, sampled
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -56,6 +57,32 @@ def test_masks_in_every_chunk(vocab, dtype):
     u = torch.rand(6, generator=g).tolist()
     for given in (dict(), dict(top_p=0.9), dict(top_p=0.9999), dict(min_p=0.01), dict(top_k=vocab // 2), dict(top_k=1024), dict(temperature=2.5, top_p=0.98)):
         check(row.to(dtype).repeat(6, 1), u, **given)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1e37, 1e38, 3e38, float("inf")])
+def test_finite_logits_farther_apart_than_the_largest_number(temperature, dtype):
+    """3e38 and -3e38: the difference is no float32, and the weight is exp(-6e38 / temperature)."""
+    inf = float("inf")
+    row = torch.full((3200,), -inf)
+    row[9], row[20], row[30], row[31] = -3.0e38, 3.0e38, 0.0, -inf
+    u = [0.05, 0.1, 0.3, 0.4, 0.6, 0.7, 0.97]
+    for vocab in (3200, 40000):
+        x = torch.cat([row, torch.full((vocab - 3200,), -inf)]).to(dtype).repeat(len(u), 1)
+        for given in (dict(), dict(top_p=0.9), dict(top_k=2), dict(top_k=1500), dict(min_p=0.3)):
+            check(x, u, temperature=temperature, **given)
+    g = torch.Generator().manual_seed(9)
+    x = ((torch.rand(5, 3000, generator=g) * 2 - 1) * 3.3e38).to(dtype)
+    for given in (dict(), dict(top_p=0.8), dict(top_k=1200), dict(top_k=30, top_p=0.7)):
+        check(x, [0.03, 0.2, 0.47, 0.8, 0.99], temperature=temperature, **given)
+
+
+def test_the_share_of_a_far_logit():
+    """By hand: exp(-2) / (1 + exp(-2)) = 0.119 at a temperature of 3e38, one half without end."""
+    x = torch.full((4, 300), -float("inf"))
+    x[:, 9], x[:, 20] = -3.0e38, 3.0e38
+    assert sampled(x, [0.05, 0.11, 0.13, 0.4], temperature=3e38) == [9, 9, 20, 20]
+    assert sampled(x, [0.05, 0.4, 0.49, 0.51], temperature=float("inf")) == [9, 9, 9, 20]
 
 
 NANS = {torch.float32: (torch.int32, (0x7fc00000, 0x7f800001, 0x7fbfffff, -0x400000, -0x7fffff)), torch.float16: (torch.int16, (0x7e00, 0x7c01, 0x7dff, -0x200, -0x3ff)),
