@@ -222,7 +222,8 @@ __device__ __forceinline__ void prompt_rows(const PagedPromptArgs& a, unsigned c
         unit.s = __builtin_amdgcn_readfirstlane(unit.s);
         s = unit.s;
         row0 = unit.block * kRows;
-        if (kvh == 0 && unit.block == 0 && unit.run == 0 && tid == 0) a.plan[s] = make_int2(unit.first, unit.runs);
+        // (the rows behind the last sequence have no place in the plan: nothing of theirs is joined)
+        if (kvh == 0 && unit.block == 0 && unit.run == 0 && tid == 0 && s < a.seqs) a.plan[s] = make_int2(unit.first, unit.runs);
     } else if (!find_block<kRows, TREE>(a, blockIdx.z, group, s, row0)) return;
     const bool tail = s == a.seqs;
     const int offset = offset_of<TREE>(a, s), n = (tail ? a.tokens : offset_of<TREE>(a, s + 1)) - offset;
