@@ -564,11 +564,13 @@ int pllm_paged_cache_compact(void* const* caches, int64_t layers, int64_t pool, 
 
 /*
  * The sequences of the next step out of the present ones (no counterpart in the reference).  Row r of new_table [rows, table_width] goes on with the first kept[r] tokens of row sources[r] of block_table
- * [seqs, table_width] (any other source: with none) and has pages for reserve[r] tokens.
+ * [seqs, table_width] (any other source: with none) and has pages for reserve[r] tokens, of kept and reserve as many as table_width pages hold: what is asked for beyond them is
+ * cut off and not reported.
  *   uses    [pool] int32: holders of every page, the entries of block_table among them (a page is free at 0); entries outside the pool (-1) hold nothing
  * Whole kept pages are shared.  A page that is kept in part stays the row's if no other new row and no holder outside block_table has it (of rows that keep it in part
- * the first has it), the others get a copy in every layer.  Free pages go lowest first to the rows in their order; missing [rows] int32 says how many pages a
- * row lacks (their entries are -1).  new_uses [pool]: the holders afterwards; block_table's rows hold nothing any more.  caches as above.
+ * the first has it), the others get a copy in every layer.  Free pages go lowest first to the rows in their order; missing [rows] int32 says how many pages that it is to
+ * write to a row lacks (their entries are -1): those that the pool has no more of, and one kept in part that the source has not.  Whole kept pages that the source has not are
+ * -1 here too and not counted.  new_uses [pool]: the holders afterwards; block_table's rows hold nothing any more.  caches as above.
  */
 size_t pllm_paged_cache_fork_workspace_bytes(int64_t rows, int64_t pool);
 int pllm_paged_cache_fork(void* const* caches, int64_t layers, int64_t pool, int64_t page_tokens, const int32_t* block_table, int64_t table_stride, int64_t table_width,

@@ -154,7 +154,8 @@ def compact(key_codes, value_codes, key_scales, value_scales, table, lengths, ke
 
 
 def fork(table, uses, sources, kept, reserve, page: int):
-    """New table, uses, missing pages per row and the copies [(from, to)]."""
+    """New table, uses, missing pages per row and the copies [(from, to)].  Room ends with the table; of it a row lacks what the pool has no page for, and a page kept in part that the
+    source has not."""
     seqs, width = table.shape
     pool = len(uses)
     uses = [int(n) for n in uses]
@@ -192,6 +193,7 @@ def fork(table, uses, sources, kept, reserve, page: int):
         if begun is not None:
             if begun < 0 or r in stay:
                 pages.append(begun)
+                lacks += begun < 0
             else:
                 copied = begun
         while len(pages) < last:

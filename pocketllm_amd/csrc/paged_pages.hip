@@ -198,7 +198,8 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(const La
 // Row r of the new table goes on with the first kept[r] tokens of row sources[r] and has room for reserve[r].  Whole pages are shared.  A page that is kept in part, which
 // the row goes on to fill, stays the row's if no other new row and no holder outside the table has it (of several rows that keep it in part the first); the others get a
 // copy.  Then come free pages: those without a holder, lowest numbers first, to the rows in their order.  Holders are counted, free pages dealt out (by one workgroup, so
-// that the order is fixed), then tables and copies made.  Integer atomics only: their order changes nothing.
+// that the order is fixed), then tables and copies made.  Integer atomics only: their order changes nothing.  What a row is to write to and has no page for is missing: what the
+// pool has no more of, and a page kept in part that its source has not.  A row's room ends with the table.
 // Bound: the chain of dependent loads (row, table, count) and the second launch, not the bytes: 64 sequences of up to 4000 tokens in pages of 64, four layers, 15 us, of them 8.9 and
 // 6.1 in the two launches; 16 beams of 4 prompts 12.
 
@@ -440,7 +441,11 @@ __global__ __launch_bounds__(256) void paged_fork_rows_kernel(const Layers layer
     if (block < table_blocks) {
         const ForkRow f = fork_row(a, r);
         const int at = 256 * block + tid, fresh_from = f.full + (f.some && copied < 0 ? 1 : 0);
-        if (block == 0 && tid == 0) a.missing[r] = max(f.last - fresh_from, 0) - clamp_int(given - start, 0, max(f.last - fresh_from, 0));
+        if (block == 0 && tid == 0) {
+            const int wants = max(f.last - fresh_from, 0);
+            const bool nowhere = f.some && copied < 0 && fork_entry(a, f.source, f.full) < 0;                // (kept in part, and the source has no page there)
+            a.missing[r] = wants - clamp_int(given - start, 0, wants) + nowhere;
+        }
         if (at >= a.width) return;
         int page = -1;
         if (at < fresh_from) page = fork_entry(a, f.source, at);

@@ -1003,13 +1003,15 @@ def paged_cache_compact_forward(layers, block_table: torch.Tensor, lengths: torc
 
 def paged_cache_fork_forward(layers, block_table: torch.Tensor, page_uses: torch.Tensor, sources: torch.Tensor, kept: torch.Tensor, reserve: torch.Tensor):
     """The sequences of the next step out of the present ones: row r goes on with the first kept[r] tokens of row sources[r] of block_table (any source outside it: with
-    none, a new sequence) and has pages for reserve[r] tokens; all int32 [rows].  A row that no other goes on with ends, and its pages are free.
+    none, a new sequence) and has pages for reserve[r] tokens; all int32 [rows].  A row that no other goes on with ends, and its pages are free.  Both numbers are cut at what a row
+    of the table holds, without a word in `missing`: a caller that may ask for more compares them with pages * page_tokens.
 
     block_table int32 [seqs, pages], -1 where a row has no page; page_uses int32 [pool]: how many holders every page has, the table's entries among them, free at 0.
     Whole kept pages are shared.  A page that is kept in part, which the row will write to, stays the row's where no other new row and no holder outside the table has it (of
     rows that keep it in part the first has it); the others get a copy in every layer (layers as in paged_cache_compact_forward).  Free pages go to the rows in
     their order, lowest numbers first.
-    Returns (block_table [rows, pages], page_uses [pool], missing int32 [rows]: pages that a row did not get, -1 in its table); the old table holds nothing any more."""
+    Returns (block_table [rows, pages], page_uses [pool], missing int32 [rows]: pages that a row is to write to and did not get, -1 in its table, because no more are free or its
+    source has none for what it keeps in part); the old table holds nothing any more.  Whole kept pages that the source has not stay -1, uncounted."""
     what = "paged_cache_fork"
     made = _bindings.paged_cache_fork("paged_cache_fork_forward", layers, block_table, page_uses, sources, kept, reserve)
     if made is not None:
