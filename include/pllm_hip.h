@@ -534,7 +534,8 @@ int pllm_paged_kv_append_at(const void* q, int64_t q_stride, const void* k_new, 
  * counted within the sequence: an earlier one, or -1 (as is anything else) for a node that follows the past.
  *
  * Attention of all nodes over the cache that already holds them: every node sees the positions before the tree, its ancestors and itself.  Otherwise as
- * pllm_paged_attention_prompt; cu_steps may be null.  A sequence with more than 256 new tokens gets zeros.
+ * pllm_paged_attention_prompt; cu_steps may be null.  A sequence with more than 256 new tokens gets zeros.  A call repeated gives the same bits; the order of a row's sums, and so its last
+ * bits, can depend on the call's other sequences where trees have more than 64 query rows (nodes times heads / kv_heads) or cu_steps is given.
  * workspace: pllm_paged_attention_tree_workspace_bytes(..., even: no cu_steps, ..., table_width * page_tokens) bytes, 16-byte aligned.
  */
 size_t pllm_paged_attention_tree_workspace_bytes(int64_t tokens, int64_t seqs, int even, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions);

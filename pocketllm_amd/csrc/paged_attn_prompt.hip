@@ -20,7 +20,7 @@
 //
 // TREE: the new tokens are nodes of a drafted tree.  A node's ancestors are four 64-bit masks, walked up once per workgroup; tiles before the tree go as they do for prompts,
 // those that hold a node's key are masked by 64 bits of them per row.  Keys are cut in runs by units, below.  32 trees of 26 nodes of 48 and 8 heads behind up to 8191 positions,
-// 82 G operations, 159 us; five of up to 200 nodes of 64 and 8 heads behind up to 30000, 402 G, 505 us (800 T/s).  What is between that and prompts' rate: rows that do not fill
+// 82 G operations, 159 us; five of up to 200 nodes of 64 and 8 heads behind up to 30000, 402 G, 510 us (790 T/s).  What is between that and prompts' rate: rows that do not fill
 // their block (156 of 192 at 26 nodes, whose blocks take 7/8 of a whole one's time), about 12 us of a unit before its first and around its masked tiles, and 6 to 14 for the runs' sums.
 #include "paged_attention.h"
 #include "paged_device.h"
@@ -814,7 +814,8 @@ Parts parts_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, in
 }
 
 // Whether the decode kernel takes trees, all of the same number of nodes: few rows, or so few keys before them that its shorter way to the first product counts (one
-// tree of 26 nodes of 48 and 8 heads behind 4000 positions 18.6 us, by units 28; behind 100000 positions 16 nodes 90, by units 82).
+// tree of 26 nodes of 48 and 8 heads behind 4000 positions 18.6 us, by units 28; behind 100000 positions 16 nodes 90, by units 82).  By the table's width, which the
+// host knows, for the lengths, which it does not: with a table of 131072 positions that tree goes by units and takes 31.
 constexpr int kTreeFewRows = 64, kTreeFewKeys = 1 << 18;
 bool few_nodes(int64_t nodes, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t positions) {
     const int64_t rows = nodes * (heads / kv_heads);

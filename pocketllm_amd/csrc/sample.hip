@@ -13,10 +13,10 @@
 //      to kFew everything above the cut goes to the list, and no other value's weight is ever formed
 //   4. the list in order, the cuts in it, the stretch of the row that the token lies in, the token
 // Many rows: a workgroup each, one launch.  Few rows: four launches, the first three over slices of the rows.
-// Bound: where there is no small top-k, the 64-bit exponential in two passes (about 100 instructions a value in all, of 16 cycles for a wave; the vector units are busy for 60 % of the
+// Bound: where there is no small top-k, the 64-bit exponential in two passes (about 100 instructions a value in all; the vector units are busy for 60 % of the
 // time, the rest is launches, chains of loads and barriers around the cuts, and rows that do not divide among the units): 832 rows of 32000 fp16 logits, all with top-p, 99 us,
-// of mixed parameters 67, 96 rows of 200064 in four launches 71, for bytes of 10 and 7.5.  With one, the bytes and, for a single row, the launches one after the other:
-// 200064 fp32 logits 21 us (2.8 + 5.3 + 5.7 + 7.6 of the launches).
+// of mixed parameters 70, 96 rows of 200064 in four launches 72, for bytes of 10 and 7.5.  With one, the bytes and, for a single row, the launches one after the other:
+// 200064 fp32 logits 21 us (3.0 + 5.4 + 5.8 + 7.6 of the launches).
 #include "pllm_device.h"
 #include "pllm_internal.h"
 
@@ -900,8 +900,8 @@ __device__ __forceinline__ int64_t choose(const Row<T>& x, const Params& p, Choi
         auto whole = [&](uint64_t from, bool counts) {
             uint64_t sum = 0;
             for_chunks<T, THREADS>(x, 0, x.chunks(), [&](int c, const uint4& u) {
-float v[kValues];
-Row<T>::values_of(u, v);
+                float v[kValues];
+                Row<T>::values_of(u, v);
 #pragma unroll
                 for (int i = 0; i < kValues; ++i) {
                     const uint64_t w = place_key(order_key(v[i]), x.first_of(c) + i) < from ? 0 : weight_of(p, v[i]);
@@ -1129,7 +1129,7 @@ __global__ __launch_bounds__(kLastThreads) void sample_token_kernel(const Sample
 // ---- many rows: a workgroup each ----------------------------------------------------------------------------------------
 
 // Where long rows have parameters of their own and there are more of them than compute units, those that take longest come first (no small top-k, then one, then the largest
-// logit alone): left in their order a long one may begin when the others end (of 32000, mixed: 832 rows 77 -> 67 us, 1600 110 -> 99; 3000 of 8000 89 -> 90, so not for
+// logit alone): left in their order a long one may begin when the others end (of 32000, mixed: 832 rows 77 -> 70 us, 1600 110 -> 99; 3000 of 8000 89 -> 90, so not for
 // short ones).  Each workgroup finds the row of its place.
 constexpr int kOrdered = 8 * kRowThreads;
 __device__ __forceinline__ int ordered_row(const SampleArgs& a, uint64_t* parts, int& found) {

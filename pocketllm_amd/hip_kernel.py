@@ -846,7 +846,8 @@ def paged_attention_tree_forward(q: torch.Tensor, key_pages: torch.Tensor, value
     itself.  q [tokens, heads * head_dim], the nodes of sequence s in rows cu_steps[s] .. cu_steps[s + 1] - 1 (None: tokens / seqs each) and in the last positions
     of the cache in the same order; parents int32 [tokens]: the node that each hangs from, counted within its sequence, an earlier one, or -1 (as is anything else)
     for one that follows the past.  At most 256 nodes per sequence (with cu_steps, rows of a sequence with more are zeros).  Rows behind the last
-    sequence are zeros."""
+    sequence are zeros.  A call repeated gives the same bits; the order of a row's sums, and so its last bits, can depend on the call's other sequences where trees have more than 64
+    query rows (nodes times heads / kv_heads) or cu_steps is given."""
     what = "paged_attention_tree"
     out = _bindings.paged_attention_tree("paged_attention_tree_forward", q, key_pages, value_pages, key_scales, value_scales, block_table, lengths, parents, cu_steps, scale)
     if out is not None:
